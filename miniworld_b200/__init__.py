@@ -2,12 +2,17 @@
 module in :mod:`miniworld_b200.training`).
 
 Public surface: the module classes (drop-in for ``miniworld_engine.modules.TriangleMultiplication`` as
-MiniWorld's blocks use it), the functional entry points over the C ABI, and the row-sharded /
+MiniWorld's blocks use it), the functional entry points over the C ABI, the
+block operators of any width (:mod:`miniworld_b200.blocks` and their modules), and the row-sharded /
 batch-parallel multi-GPU wrappers.
 """
 
 from .modules import (  # noqa: F401
     BidirectionalTriangleMultiplication,
+    BlockJoin,
+    BlockNorm,
+    GatedFeedForward,
+    SandwichTransition,
     Transition,
     TriangleMultiplication,
     TriangleMultiplicationIncoming,
@@ -20,6 +25,10 @@ __all__ = [
     "TriangleMultiplication",
     "BidirectionalTriangleMultiplication",
     "Transition",
+    "BlockNorm",
+    "BlockJoin",
+    "GatedFeedForward",
+    "SandwichTransition",
     "TriangleMultiplicationOutgoing",
     "TriangleMultiplicationIncoming",
     "to_openfold_state_dict",

@@ -1,4 +1,4 @@
-"""ctypes binding of ``libb200_trimul.so`` (the C ABI declared in ``include/b200_trimul.h``).
+"""ctypes binding of ``libb200_trimul.so`` (the C ABI declared in ``include/b200_trimul.h`` and ``include/b200_blocks.h``).
 
 There is no fallback: if the library is missing or a call fails, a ``RuntimeError`` is raised.
 """
@@ -141,6 +141,18 @@ SIGNATURES["b200_trimul_backward_any"] = SIGNATURES["b200_trimul_backward"]
 SIGNATURES["b200_trimul_forward_lines"] = SIGNATURES["b200_trimul_forward_ex"]
 SIGNATURES["b200_trimul_backward_lines"] = SIGNATURES["b200_trimul_backward"]
 
+# name -> (restype, argtypes) of include/b200_blocks.h
+_L = ctypes.c_longlong
+BLOCKS_SIGNATURES = {
+    "b200_block_join_forward": (c_int, [c_void_p] * 13 + [_L, c_int, _L, c_int, c_int, c_int, c_float, c_float, c_void_p]),
+    "b200_block_join_workspace_bytes": (c_int, [_L, c_int, _L, POINTER(c_size_t)]),
+    "b200_block_join_backward": (c_int, [c_void_p] * 22 + [c_size_t, _L, c_int, _L, c_int, c_int, c_int, c_void_p]),
+    "b200_ff_workspace_bytes": (c_int, [_L, c_int, c_int, c_int, c_int, POINTER(c_size_t)]),
+    "b200_ff_forward": (c_int, [c_void_p] * 6 + [c_size_t, _L, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "b200_ff_backward": (c_int, [c_void_p] * 10 + [c_size_t, _L, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "b200_blocks_read_status": (c_int, [c_void_p, POINTER(c_int)]),
+}
+
 _lib = None
 
 
@@ -155,7 +167,7 @@ def load() -> ctypes.CDLL:
             "(there is no CPU or PyTorch fallback for this path)"
         )
     lib = ctypes.CDLL(str(LIB_PATH))
-    for name, (restype, argtypes) in SIGNATURES.items():
+    for name, (restype, argtypes) in {**SIGNATURES, **BLOCKS_SIGNATURES}.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is not exported
         fn.restype = restype
         fn.argtypes = argtypes

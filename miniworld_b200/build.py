@@ -1,4 +1,4 @@
-"""Build recipe of the two in-tree libraries: the kernels behind the C ABI (one ``nvcc`` call, sm_100a only) and the native
+"""Build recipe of the two in-tree libraries: the kernels behind the C ABI (``nvcc``, sm_100a only) and the native
 host side of the module calls (``csrc/host.cpp``, one ``g++`` call against PyTorch's headers, linked to the first)."""
 
 from __future__ import annotations
@@ -6,6 +6,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -16,6 +17,8 @@ NATIVE_PATH = PKG_DIR / "_native.so"
 NATIVE_TAG_PATH = PKG_DIR / "_native.tag"  # what NATIVE_PATH was built against
 HOST_SOURCE = CSRC / "host.cpp"
 HEADER = PKG_DIR.parent / "include" / "b200_trimul.h"
+BLOCKS_HEADER = PKG_DIR.parent / "include" / "b200_blocks.h"
+BLOCKS_HOST = CSRC / "host_blocks.inc"  # part of HOST_SOURCE
 
 NVCC_FLAGS = [
     "-gencode",
@@ -23,14 +26,13 @@ NVCC_FLAGS = [
     "-lineinfo",
     "-O3",
     "-std=c++17",
-    "-shared",
     "-Xcompiler",
     "-fPIC",
 ]
 
 
 def _sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.inc")) + [HEADER]
+    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [p for p in sorted(CSRC.glob("*.inc")) if p != BLOCKS_HOST] + [HEADER, BLOCKS_HEADER]
 
 
 def is_stale() -> bool:
@@ -53,7 +55,7 @@ def native_is_stale() -> bool:
     if not NATIVE_PATH.exists() or not NATIVE_TAG_PATH.exists() or NATIVE_TAG_PATH.read_text() != native_tag():
         return True
     built = NATIVE_PATH.stat().st_mtime
-    return any(src.stat().st_mtime > built for src in (HOST_SOURCE, HEADER, Path(__file__)))
+    return any(src.stat().st_mtime > built for src in (HOST_SOURCE, HEADER, BLOCKS_HOST, BLOCKS_HEADER, Path(__file__)))
 
 
 def find_nvcc() -> str:
@@ -91,17 +93,31 @@ def build_native(force: bool = False) -> Path:
     return NATIVE_PATH
 
 
+def _compile(source: Path, force: bool, verbose: bool) -> Path:
+    """Object file of one ``.cu`` file, kept beside the package and made again when a file that it includes is newer."""
+    obj, deps = PKG_DIR / f"{source.stem}.o", PKG_DIR / f"{source.stem}.tag"
+    if not force and obj.exists() and deps.exists():
+        used = [Path(w) for w in deps.read_text().replace("\\\n", " ").split()[1:]]
+        built = obj.stat().st_mtime
+        if used and all(p.exists() and p.stat().st_mtime <= built for p in used):
+            return obj
+    cmd = [find_nvcc(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-MD", "-MF", str(deps)]
+    proc = _run(cmd + ["-c", "-o", str(obj), str(source)])
+    if verbose:
+        print(proc.stderr)
+    return obj
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile ``csrc/trimul_abi.cu`` into ``libb200_trimul.so`` beside the package (no GPU needed), then ``_native.so``."""
+    """Compile ``csrc/*.cu`` side by side and link them to ``libb200_trimul.so`` beside the package (no GPU needed), then
+    ``_native.so``."""
     if force or is_stale():
-        cmd = [find_nvcc(), *NVCC_FLAGS]
-        if verbose:
-            cmd += ["-Xptxas", "-v"]
+        sources = sorted(CSRC.glob("*.cu"))
+        with ThreadPoolExecutor(len(sources)) as pool:
+            objects = list(pool.map(lambda source: _compile(source, force, verbose), sources))
         tmp = LIB_PATH.with_suffix(".so.tmp")
-        proc = _run(cmd + ["-o", str(tmp), str(CSRC / "trimul_abi.cu")])
+        _run([find_nvcc(), *NVCC_FLAGS, "-shared", "-o", str(tmp), *map(str, objects)])
         os.replace(tmp, LIB_PATH)
-        if verbose:
-            print(proc.stderr)
     build_native(force)
     return LIB_PATH
 

@@ -1,0 +1,545 @@
+// C-ABI entry points of the block operators (see include/b200_blocks.h): argument checks, tensor maps, the choice of a variant and
+// launches; all arithmetic is in the kernels.
+#include "../../include/b200_blocks.h"
+
+#include <algorithm>
+#include <utility>
+
+#include "feed_forward.cuh"
+#include "host_util.cuh"
+#include "join.cuh"
+
+namespace trimul {
+
+static size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+// ---------------------------------------------------------------- join
+// Threads of a row and 8-element pieces of each (NV): the fewest idle lanes, then the fewest pieces. Up to 32 threads reduce by
+// shuffles alone; wider rows take several warps.
+struct JoinShape {
+  int team, nv;
+};
+static JoinShape join_forward_shape(int d) {
+  JoinShape best{0, 0};
+  int waste = 0;
+  for (int nv = 1; nv <= 4; ++nv)
+    for (int team : {1, 2, 4, 8, 16, 32, 64, 128}) {
+      const int have = team * nv * 8;
+      if (have < d || (team > 32 && nv < 4)) continue;
+      if (best.team == 0 || have - d < waste) {
+        best = {team, nv};
+        waste = have - d;
+      }
+      break;
+    }
+  return best;
+}
+static int join_backward_team(int d) {
+  int team = 1;
+  while (team < 32 && team * 8 < d) team *= 2;
+  if (team * 8 < d) team = (d + 255) / 256 * 32;
+  return team;
+}
+struct JoinGrid {
+  int team, teams, blocks;
+  long long rows_per_team;  // with a shared gate
+};
+static JoinGrid join_backward_grid(long long rows, int d, bool shared_gate, int sms) {
+  JoinGrid g;
+  g.team = join_backward_team(d);
+  g.teams = kJoinBackwardThreads / g.team;
+  g.blocks = static_cast<int>(std::min<long long>(sms, (rows + g.teams - 1) / g.teams));
+  g.rows_per_team = 0;
+  if (shared_gate) g.rows_per_team = (rows + static_cast<long long>(g.blocks) * g.teams - 1) / (static_cast<long long>(g.blocks) * g.teams);
+  return g;
+}
+constexpr int kMaxSms = 160;
+
+static int check_join(long long rows, int d, long long gate_rows, int dtype, int post_kind, int pre_kind) {
+  if (rows < 0 || d < 1 || gate_rows < 1) return B200_TRIMUL_E_SHAPE;
+  if (rows > (1ll << 40) / d || rows % gate_rows != 0) return B200_TRIMUL_E_SHAPE;
+  if (d > B200_NORM_MAX_WIDTH || dtype < 0 || dtype > 2 || post_kind < 0 || post_kind > 2 || pre_kind < 0 || pre_kind > 2)
+    return B200_TRIMUL_E_UNSUPPORTED;
+  return B200_TRIMUL_OK;
+}
+static bool all_aligned16(std::initializer_list<const void*> ps) {
+  for (const void* q : ps)
+    if (!aligned(q, 16)) return false;
+  return true;
+}
+
+template <typename T>
+static int launch_join_forward(const JoinParams& p0, bool wide, int sms, cudaStream_t stream) {
+  JoinParams p = p0;
+  const JoinShape s = join_forward_shape(p.d);
+  p.team = s.team;
+  const int teams = kJoinForwardThreads / s.team;
+  const int blocks = static_cast<int>(std::min<long long>((p.rows + teams - 1) / teams, 8ll * sms));
+  void (*kernel)(JoinParams) = nullptr;
+  switch (s.nv) {
+    case 1: kernel = wide ? join_forward_kernel<T, true, 1> : join_forward_kernel<T, false, 1>; break;
+    case 2: kernel = wide ? join_forward_kernel<T, true, 2> : join_forward_kernel<T, false, 2>; break;
+    case 3: kernel = wide ? join_forward_kernel<T, true, 3> : join_forward_kernel<T, false, 3>; break;
+    default: kernel = wide ? join_forward_kernel<T, true, 4> : join_forward_kernel<T, false, 4>; break;
+  }
+  TRIMUL_CUDA(launch_overlapped(kernel, dim3(blocks), kJoinForwardThreads, 0, stream, p));
+  return B200_TRIMUL_OK;
+}
+
+template <typename T>
+static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& g, const JoinSums& sums, cudaStream_t stream) {
+  const int smem = p.sums != nullptr ? g.teams * p.d * 4 : 0;
+  TRIMUL_CUDA(launch_overlapped(wide ? join_backward_kernel<T, true> : join_backward_kernel<T, false>, dim3(g.blocks), g.team * g.teams, smem,
+                                stream, p));
+  if (p.sums != nullptr) TRIMUL_CUDA(launch_overlapped(join_sums_kernel, dim3((p.d + 31) / 32, 5), 256, 0, stream, sums));
+  if (p.dgate != nullptr && p.gate_rows > 1) {
+    const int blocks = static_cast<int>(std::min<long long>(p.rows / p.gate_rows, 1024));
+    TRIMUL_CUDA(launch_overlapped(wide ? join_gate_kernel<T, true> : join_gate_kernel<T, false>, dim3(blocks), 256, 0, stream, p));
+  }
+  return B200_TRIMUL_OK;
+}
+
+static size_t join_sums_bytes(int d) { return up(static_cast<size_t>(kMaxSms) * 5 * d * 4, 1024); }
+
+// ---------------------------------------------------------------- feed-forward
+// The current device, whose context is then the calling thread's: a thread that has not used the GPU yet (autograd's, on its first
+// backward) has none, and tensor maps are made by the driver.
+static int ff_device(DeviceInfo* info) {
+  const int rc = device_info(info);
+  if (rc != 0) return rc;
+  TRIMUL_CUDA(cudaSetDevice(info->device));
+  return B200_TRIMUL_OK;
+}
+
+static int ff_ld(int hidden) { return static_cast<int>(up(hidden, 64)); }  // rows of h, da and db: whole 128-byte lines
+
+// Rows [rows][cols] of 16-bit elements, `ld` elements apart, in boxes of 64 columns by `box` rows
+static int ff_map(CUtensorMap* m, const void* base, long long rows, int cols, long long ld, int box) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(ld) * 2};
+  const uint32_t b[2] = {64, static_cast<uint32_t>(box)};
+  return make_map(m, base, 2, dims, strides, b);
+}
+
+template <int OP, bool PAIR, bool F16>
+static int ff_launch_kernel(const FfMaps& maps, const FfParams& p, const DeviceInfo& info, cudaStream_t stream) {
+  const int rc = set_smem(ff_kernel<OP, PAIR, F16>, kFfSmemBytes, info.device);
+  if (rc != B200_TRIMUL_OK) return rc;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * p.splits * (OP == kFfWeights ? 3 : 1);
+  const int units = PAIR ? info.sms / 2 : info.sms;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, units)) * (PAIR ? 2 : 1));
+  cfg.blockDim = dim3(kFfThreads);
+  cfg.dynamicSmemBytes = kFfSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  TRIMUL_CUDA(cudaLaunchKernelEx(&cfg, ff_kernel<OP, PAIR, F16>, maps, p));
+  return B200_TRIMUL_OK;
+}
+template <int OP>
+static int ff_launch(const FfMaps& maps, const FfParams& p, bool pair, bool f16, const DeviceInfo& info, cudaStream_t stream) {
+  if (pair) return f16 ? ff_launch_kernel<OP, true, true>(maps, p, info, stream) : ff_launch_kernel<OP, true, false>(maps, p, info, stream);
+  return f16 ? ff_launch_kernel<OP, false, true>(maps, p, info, stream) : ff_launch_kernel<OP, false, false>(maps, p, info, stream);
+}
+
+static int blocks_of(long long n, int b) { return static_cast<int>((n + b - 1) / b); }
+
+// CTA pairs where their 256-row tiles still occupy most of the GPU, single CTAs below
+static bool ff_pair(long long rows, long long n_tiles, int sms) { return rows > 128 && blocks_of(rows, 256) * n_tiles >= sms / 2 * 3 / 4; }
+
+struct FfProblem {
+  long long rows;
+  int d, hidden, ld;
+  bool f16;
+  int act;
+  const void *w_a, *w_b, *w_s;  // operands, in the type of x
+  DeviceInfo info;
+  cudaStream_t stream;
+};
+
+// h = act(x W_a^T) * (x W_b^T), or with dy the backward's da, db, h
+static int ff_hidden(const FfProblem& f, const void* x, const void* dy, void* const out[3]) {
+  const bool pair = ff_pair(f.rows, blocks_of(f.hidden, 128), f.info.sms);
+  const int units = pair ? 128 : 64;
+  FfMaps maps = {};
+  int rc = ff_map(&maps.a[dy != nullptr ? 1 : 0], x, f.rows, f.d, f.d, 128);
+  if (rc == 0) rc = ff_map(&maps.b[0], f.w_a, f.hidden, f.d, f.d, units);
+  if (rc == 0) rc = ff_map(&maps.b[1], f.w_b, f.hidden, f.d, f.d, units);
+  if (rc == 0 && dy != nullptr) rc = ff_map(&maps.a[0], dy, f.rows, f.d, f.d, 128);
+  if (rc == 0 && dy != nullptr) rc = ff_map(&maps.b[2], f.w_s, f.d, f.hidden, f.hidden, 64);
+  if (rc != 0) return rc;
+  FfParams p = {};
+  for (int i = 0; i < 3; ++i) p.out[i] = out[i];
+  p.ld = f.ld;
+  p.rows = static_cast<int>(f.rows);
+  p.cols = f.hidden;
+  p.m_tiles = blocks_of(f.rows, pair ? 256 : 128);
+  p.n_tiles = blocks_of(f.hidden, units);
+  p.kb = p.kb_second = blocks_of(f.d, 64);
+  p.bn = 2 * units;
+  p.splits = 1;
+  p.act = f.act;
+  return dy != nullptr ? ff_launch<kFfHidden>(maps, p, pair, f.f16, f.info, f.stream) : ff_launch<kFfUp>(maps, p, pair, f.f16, f.info, f.stream);
+}
+
+// y = h W_s^T, or (two operands) dx = da W_a + db W_b
+static int ff_project(const FfProblem& f, const void* first, const void* second, void* out) {
+  const bool input = second != nullptr;
+  const bool pair = ff_pair(f.rows, blocks_of(f.d, 256), f.info.sms);
+  int bn = pair ? 256 : 128;
+  while (bn > (pair && input ? 128 : 64) && blocks_of(f.d, bn / 2) * (bn / 2) < blocks_of(f.d, bn) * bn) bn /= 2;
+  FfMaps maps = {};
+  int rc = ff_map(&maps.a[0], first, f.rows, f.hidden, f.ld, 128);
+  if (input) {
+    if (rc == 0) rc = ff_map(&maps.a[1], second, f.rows, f.hidden, f.ld, 128);
+    if (rc == 0) rc = ff_map(&maps.b[0], f.w_a, f.hidden, f.d, f.d, 64);
+    if (rc == 0) rc = ff_map(&maps.b[1], f.w_b, f.hidden, f.d, f.d, 64);
+  } else if (rc == 0) {
+    rc = ff_map(&maps.b[0], f.w_s, f.d, f.hidden, f.hidden, pair ? bn / 2 : bn);
+  }
+  if (rc != 0) return rc;
+  FfParams p = {};
+  p.out[0] = out;
+  p.ld = f.d;
+  p.rows = static_cast<int>(f.rows);
+  p.cols = f.d;
+  p.m_tiles = blocks_of(f.rows, pair ? 256 : 128);
+  p.n_tiles = blocks_of(f.d, bn);
+  p.kb = p.kb_second = blocks_of(f.hidden, 64);
+  p.bn = bn;
+  p.splits = 1;
+  return input ? ff_launch<kFfInput>(maps, p, pair, f.f16, f.info, f.stream) : ff_launch<kFfDown>(maps, p, pair, f.f16, f.info, f.stream);
+}
+
+// Tiles and parts of the weight gradients' products [hidden, d]: about two rounds of tiles for the whole GPU, but parts of at least
+// eight k blocks
+struct FfSplit {
+  bool pair;
+  int bn, m_tiles, n_tiles, kb, splits, kb_split;
+};
+static FfSplit ff_split(long long rows, int d, int hidden, int sms) {
+  FfSplit s;
+  s.kb = std::max(1, blocks_of(rows, 64));
+  s.pair = hidden > 128 && d > 64 && static_cast<long long>(hidden) * d >= 512 * 128;
+  s.bn = s.pair ? 256 : 128;
+  while (s.bn > (s.pair ? 128 : 64) && blocks_of(d, s.bn / 2) * (s.bn / 2) < blocks_of(d, s.bn) * s.bn) s.bn /= 2;
+  s.m_tiles = blocks_of(hidden, s.pair ? 256 : 128);
+  s.n_tiles = blocks_of(d, s.bn);
+  const long long tiles = 3ll * s.m_tiles * s.n_tiles, units = s.pair ? sms / 2 : sms;
+  long long parts = tiles >= units ? 1 : (units + tiles - 1) / tiles;
+  parts = std::max<long long>(1, std::min<long long>(parts, s.kb / 8));
+  s.kb_split = blocks_of(s.kb, static_cast<int>(parts));
+  s.splits = blocks_of(s.kb, s.kb_split);
+  return s;
+}
+
+static int ff_weight_gradients(const FfProblem& f, const void* x, const void* dy, void* const hidden3[3], float* partial, void* dw_a,
+                               void* dw_b, void* dw_s, int weight_dtype) {
+  const FfSplit s = ff_split(f.rows, f.d, f.hidden, f.info.sms);
+  FfMaps maps = {};
+  int rc = 0;
+  for (int i = 0; i < 3 && rc == 0; ++i) rc = ff_map(&maps.a[i], hidden3[i], f.rows, f.hidden, f.ld, 64);
+  if (rc == 0) rc = ff_map(&maps.b[0], x, f.rows, f.d, f.d, 64);
+  if (rc == 0) rc = ff_map(&maps.b[1], dy, f.rows, f.d, f.d, 64);
+  if (rc != 0) return rc;
+  FfParams p = {};
+  p.partial = partial;
+  p.rows = f.hidden;
+  p.cols = f.d;
+  p.m_tiles = s.m_tiles;
+  p.n_tiles = s.n_tiles;
+  p.kb = s.kb;
+  p.bn = s.bn;
+  p.splits = s.splits;
+  p.kb_split = s.kb_split;
+  rc = ff_launch<kFfWeights>(maps, p, s.pair, f.f16, f.info, f.stream);
+  if (rc != 0) return rc;
+  FfReduce r = {};
+  r.partial = partial;
+  r.out[0] = dw_a;
+  r.out[1] = dw_b;
+  r.out[2] = dw_s;
+  r.splits = s.splits;
+  r.H = f.hidden;
+  r.D = f.d;
+  r.type = weight_dtype;
+  TRIMUL_CUDA(launch_overlapped(ff_reduce_kernel, dim3(blocks_of(f.d, 32), blocks_of(f.hidden, 32), 3), 256, 0, f.stream, r));
+  return 0;
+}
+
+static int check_ff(long long rows, int d, int hidden, int weight_dtype, int dtype = 0) {
+  if (rows < 0 || rows > 0x7FFFFFFFll - 256 || d < 1 || hidden < 1) return B200_TRIMUL_E_SHAPE;
+  if (d % 8 != 0 || hidden % 8 != 0 || d > (1 << 20) || hidden > (1 << 20)) return B200_TRIMUL_E_UNSUPPORTED;
+  if (dtype != B200_BLOCKS_BF16 && dtype != B200_BLOCKS_F16) return B200_TRIMUL_E_UNSUPPORTED;
+  if (weight_dtype < 0 || weight_dtype > 2) return B200_TRIMUL_E_UNSUPPORTED;
+  return B200_TRIMUL_OK;
+}
+
+struct FfRegions {
+  size_t weights, hidden[3], partial, total;
+};
+static FfRegions ff_regions(long long rows, int d, int hidden, int weight_dtype, bool backward, int sms) {
+  FfRegions r = {};
+  size_t at = 0;
+  r.weights = at;
+  if (weight_dtype == B200_BLOCKS_F32) at += up(static_cast<size_t>(3) * hidden * d * 2, 1024);
+  for (int i = 0; i < (backward ? 3 : 1); ++i) {
+    r.hidden[i] = at;
+    at += up(static_cast<size_t>(rows) * ff_ld(hidden) * 2, 1024);
+  }
+  r.partial = at;
+  if (backward) at += up(static_cast<size_t>(ff_split(rows, d, hidden, sms).splits) * 3 * hidden * d * 4, 1024);
+  r.total = at;
+  return r;
+}
+
+// The problem of a call, its weights cast if they are fp32
+static int ff_problem(FfProblem* f, const void* w_a, const void* w_b, const void* w_s, long long rows, int d, int hidden, int dtype,
+                      int weight_dtype, int activation, uint8_t* cast_to, void* cuda_stream) {
+  f->rows = rows;
+  f->d = d;
+  f->hidden = hidden;
+  f->ld = ff_ld(hidden);
+  f->f16 = dtype == B200_BLOCKS_F16;
+  f->act = activation;
+  f->stream = static_cast<cudaStream_t>(cuda_stream);
+  f->w_a = w_a;
+  f->w_b = w_b;
+  f->w_s = w_s;
+  if (weight_dtype != B200_BLOCKS_F32) return 0;
+  const long long n = static_cast<long long>(hidden) * d;
+  f->w_a = cast_to;
+  f->w_b = cast_to + n * 2;
+  f->w_s = cast_to + n * 4;
+  const int blocks = static_cast<int>(std::min<long long>((3 * n / 8 + 255) / 256, 8 * f->info.sms));
+  TRIMUL_CUDA(launch_overlapped(ff_cast_kernel, dim3(blocks), 256, 0, f->stream, static_cast<const float*>(w_a), static_cast<const float*>(w_b),
+                                static_cast<const float*>(w_s), reinterpret_cast<uint4*>(cast_to), n / 8, static_cast<int>(f->f16)));
+  return 0;
+}
+
+}  // namespace trimul
+
+using namespace trimul;
+
+extern "C" {
+
+int b200_block_join_forward(const void* x, const void* u, const void* gate, const uint8_t* mask, const float* scale, const float* post_w,
+                            const float* post_b, const float* pre_w, const float* pre_b, void* y, void* h, float* post_stats,
+                            float* pre_stats, long long rows, int d, long long gate_rows, int dtype, int post_kind, int pre_kind,
+                            float post_eps, float pre_eps, void* cuda_stream) {
+  int rc = check_join(rows, d, gate_rows, dtype, post_kind, pre_kind);
+  if (rc != 0) return rc;
+  if (rows == 0) return B200_TRIMUL_OK;
+  if (x == nullptr || (u != nullptr) != (y != nullptr) || (pre_kind != kNormNone) != (h != nullptr)) return B200_TRIMUL_E_NULL;
+  if (u == nullptr && (pre_kind == kNormNone || post_kind != kNormNone || gate != nullptr || mask != nullptr || scale != nullptr))
+    return B200_TRIMUL_E_NULL;
+  DeviceInfo info;
+  rc = device_info(&info);
+  if (rc != 0) return rc;
+  JoinParams p = {};
+  p.x = x;
+  p.u = u;
+  p.gate = gate;
+  p.mask = mask;
+  p.scale = scale;
+  p.post_w = post_w;
+  p.post_b = post_b;
+  p.pre_w = pre_w;
+  p.pre_b = pre_b;
+  p.y = y;
+  p.h = h;
+  p.post_stats = reinterpret_cast<float2*>(post_stats);
+  p.pre_stats = reinterpret_cast<float2*>(pre_stats);
+  p.rows = rows;
+  p.gate_rows = gate_rows;
+  p.d = d;
+  p.post_kind = post_kind;
+  p.pre_kind = pre_kind;
+  p.post_eps = post_eps;
+  p.pre_eps = pre_eps;
+  const int size = dtype == B200_BLOCKS_F32 ? 4 : 2;
+  if (!aligned(x, size) || !aligned(u, size) || !aligned(gate, size) || !aligned(y, size) || !aligned(h, size) ||
+      !aligned(post_stats, 8) || !aligned(pre_stats, 8))
+    return B200_TRIMUL_E_ALIGN;
+  const bool wide = d % 8 == 0 && all_aligned16({x, u, gate, y, h});
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  if (dtype == B200_BLOCKS_BF16) return launch_join_forward<__nv_bfloat16>(p, wide, info.sms, stream);
+  if (dtype == B200_BLOCKS_F16) return launch_join_forward<__half>(p, wide, info.sms, stream);
+  return launch_join_forward<float>(p, wide, info.sms, stream);
+}
+
+int b200_block_join_workspace_bytes(long long rows, int d, long long gate_rows, size_t* out_bytes) {
+  if (out_bytes == nullptr) return B200_TRIMUL_E_NULL;
+  const int rc = check_join(rows, d, gate_rows, 0, 0, 0);
+  if (rc != 0) return rc;
+  *out_bytes = join_sums_bytes(d);
+  if (gate_rows > 1) {
+    const int team = join_backward_team(d);
+    *out_bytes += static_cast<size_t>(kMaxSms) * (kJoinBackwardThreads / team) * 2 * 8 * team * 4;
+  }
+  return B200_TRIMUL_OK;
+}
+
+int b200_block_join_backward(const void* dy, const void* dh, const void* x, const void* u, const void* gate, const uint8_t* mask,
+                             const float* scale, const float* post_w, const float* post_b, const float* pre_w, const float* pre_b,
+                             const float* post_stats, const float* pre_stats, void* dx, void* du, void* dgate, float* d_scale,
+                             float* d_post_w, float* d_post_b, float* d_pre_w, float* d_pre_b, void* workspace, size_t workspace_bytes,
+                             long long rows, int d, long long gate_rows, int dtype, int post_kind, int pre_kind, void* cuda_stream) {
+  int rc = check_join(rows, d, gate_rows, dtype, post_kind, pre_kind);
+  if (rc != 0) return rc;
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  if (rows == 0) {
+    for (float* s : {d_scale, d_post_w, d_post_b, d_pre_w, d_pre_b})
+      if (s != nullptr) TRIMUL_CUDA(cudaMemsetAsync(s, 0, static_cast<size_t>(d) * 4, stream));
+    return B200_TRIMUL_OK;
+  }
+  if (x == nullptr || workspace == nullptr || (post_kind != kNormNone && post_stats == nullptr) || (pre_kind != kNormNone && pre_stats == nullptr))
+    return B200_TRIMUL_E_NULL;
+  if (u == nullptr && (pre_kind == kNormNone || post_kind != kNormNone || gate != nullptr || mask != nullptr || scale != nullptr))
+    return B200_TRIMUL_E_NULL;
+  if ((pre_kind == kNormNone && dh != nullptr) || (u == nullptr && (dy != nullptr || du != nullptr)) || (gate == nullptr && dgate != nullptr))
+    return B200_TRIMUL_E_NULL;
+  if (!aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;
+  size_t need = 0;
+  rc = b200_block_join_workspace_bytes(rows, d, gate_rows, &need);
+  if (rc != 0) return rc;
+  if (workspace_bytes < need) return B200_TRIMUL_E_WORKSPACE;
+  DeviceInfo info;
+  rc = device_info(&info);
+  if (rc != 0) return rc;
+  const JoinGrid g = join_backward_grid(rows, d, gate != nullptr && gate_rows > 1, std::min(info.sms, kMaxSms));
+  JoinParams p = {};
+  p.x = x;
+  p.u = u;
+  p.gate = gate;
+  p.mask = mask;
+  p.scale = scale;
+  p.post_w = post_w;
+  p.post_b = post_b;
+  p.pre_w = pre_w;
+  p.pre_b = pre_b;
+  p.post_stats = reinterpret_cast<float2*>(const_cast<float*>(post_stats));
+  p.pre_stats = reinterpret_cast<float2*>(const_cast<float*>(pre_stats));
+  p.dy = dy;
+  p.dh = dh;
+  p.dx = dx;
+  p.du = du;
+  p.dgate = dgate;
+  p.rows = rows;
+  p.gate_rows = gate_rows;
+  p.rows_per_team = g.rows_per_team;
+  p.d = d;
+  p.team = g.team;
+  p.post_kind = post_kind;
+  p.pre_kind = pre_kind;
+  JoinSums sums = {};
+  float* const outs[5] = {d_scale, d_post_w, d_post_b, d_pre_w, d_pre_b};
+  bool any = false;
+  for (int i = 0; i < 5; ++i) {
+    sums.out[i] = outs[i];
+    any = any || outs[i] != nullptr;
+  }
+  p.sums = any ? static_cast<float*>(workspace) : nullptr;
+  p.gate_part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + join_sums_bytes(d));
+  sums.sums = p.sums;
+  sums.blocks = g.blocks;
+  sums.d = d;
+  const int size = dtype == B200_BLOCKS_F32 ? 4 : 2;
+  for (const void* q : {x, u, gate, dy, dh, static_cast<const void*>(dx), static_cast<const void*>(du), static_cast<const void*>(dgate)})
+    if (!aligned(q, size)) return B200_TRIMUL_E_ALIGN;
+  if (!aligned(post_stats, 8) || !aligned(pre_stats, 8)) return B200_TRIMUL_E_ALIGN;
+  const bool wide = d % 8 == 0 && all_aligned16({x, u, gate, dy, dh, dx, du, dgate});
+  if (dtype == B200_BLOCKS_BF16) return launch_join_backward<__nv_bfloat16>(p, wide, g, sums, stream);
+  if (dtype == B200_BLOCKS_F16) return launch_join_backward<__half>(p, wide, g, sums, stream);
+  return launch_join_backward<float>(p, wide, g, sums, stream);
+}
+
+int b200_ff_workspace_bytes(long long rows, int d, int hidden, int weight_dtype, int backward, size_t* out_bytes) {
+  if (out_bytes == nullptr) return B200_TRIMUL_E_NULL;
+  const int rc = check_ff(rows, d, hidden, weight_dtype);
+  if (rc != 0) return rc;
+  // (no GPU is needed to ask: the largest number of parts that ff_split gives for any SM count up to kMaxSms)
+  size_t most = 0;
+  if (backward != 0)
+    for (int sms = 2; sms <= kMaxSms; sms += 2) most = std::max(most, ff_regions(rows, d, hidden, weight_dtype, true, sms).total);
+  else
+    most = ff_regions(rows, d, hidden, weight_dtype, false, kMaxSms).total;
+  *out_bytes = std::max<size_t>(most, 1024);
+  return B200_TRIMUL_OK;
+}
+
+int b200_ff_forward(const void* x, const void* w_a, const void* w_b, const void* w_s, void* y, void* workspace, size_t workspace_bytes,
+                    long long rows, int d, int hidden, int dtype, int weight_dtype, int activation, void* cuda_stream) {
+  int rc = check_ff(rows, d, hidden, weight_dtype, dtype);
+  if (rc != 0) return rc;
+  if (weight_dtype != B200_BLOCKS_F32 && weight_dtype != dtype) return B200_TRIMUL_E_UNSUPPORTED;
+  if (activation != B200_ACT_SILU && activation != B200_ACT_GELU) return B200_TRIMUL_E_UNSUPPORTED;
+  if (rows == 0) return B200_TRIMUL_OK;
+  if (x == nullptr || w_a == nullptr || w_b == nullptr || w_s == nullptr || y == nullptr || workspace == nullptr) return B200_TRIMUL_E_NULL;
+  if (!all_aligned16({x, w_a, w_b, w_s, y}) || !aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;
+  FfProblem f;
+  rc = ff_device(&f.info);
+  if (rc != 0) return rc;
+  const FfRegions r = ff_regions(rows, d, hidden, weight_dtype, false, f.info.sms);
+  if (workspace_bytes < r.total) return B200_TRIMUL_E_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  rc = ff_problem(&f, w_a, w_b, w_s, rows, d, hidden, dtype, weight_dtype, activation, ws + r.weights, cuda_stream);
+  if (rc != 0) return rc;
+  void* const out[3] = {ws + r.hidden[0], nullptr, nullptr};
+  rc = ff_hidden(f, x, nullptr, out);
+  return rc != 0 ? rc : ff_project(f, out[0], nullptr, y);
+}
+
+int b200_ff_backward(const void* dy, const void* x, const void* w_a, const void* w_b, const void* w_s, void* dx, void* dw_a, void* dw_b,
+                     void* dw_s, void* workspace, size_t workspace_bytes, long long rows, int d, int hidden, int dtype, int weight_dtype,
+                     int activation, void* cuda_stream) {
+  int rc = check_ff(rows, d, hidden, weight_dtype, dtype);
+  if (rc != 0) return rc;
+  if (weight_dtype != B200_BLOCKS_F32 && weight_dtype != dtype) return B200_TRIMUL_E_UNSUPPORTED;
+  if (activation != B200_ACT_SILU && activation != B200_ACT_GELU) return B200_TRIMUL_E_UNSUPPORTED;
+  const size_t weight_bytes = static_cast<size_t>(hidden) * d * (weight_dtype == B200_BLOCKS_F32 ? 4 : 2);
+  if (rows == 0) {
+    for (void* w : {dw_a, dw_b, dw_s})
+      if (w != nullptr) TRIMUL_CUDA(cudaMemsetAsync(w, 0, weight_bytes, static_cast<cudaStream_t>(cuda_stream)));
+    return B200_TRIMUL_OK;
+  }
+  if (dy == nullptr || x == nullptr || w_a == nullptr || w_b == nullptr || w_s == nullptr || workspace == nullptr) return B200_TRIMUL_E_NULL;
+  if (!all_aligned16({dy, x, w_a, w_b, w_s, dx, dw_a, dw_b, dw_s}) || !aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;
+  FfProblem f;
+  rc = ff_device(&f.info);
+  if (rc != 0) return rc;
+  const FfRegions r = ff_regions(rows, d, hidden, weight_dtype, true, f.info.sms);
+  if (workspace_bytes < r.total) return B200_TRIMUL_E_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  rc = ff_problem(&f, w_a, w_b, w_s, rows, d, hidden, dtype, weight_dtype, activation, ws + r.weights, cuda_stream);
+  if (rc != 0) return rc;
+  void* const hidden3[3] = {ws + r.hidden[0], ws + r.hidden[1], ws + r.hidden[2]};
+  rc = ff_hidden(f, x, dy, hidden3);
+  if (rc == 0 && dx != nullptr) rc = ff_project(f, hidden3[0], hidden3[1], dx);
+  if (rc == 0 && (dw_a != nullptr || dw_b != nullptr || dw_s != nullptr))
+    rc = ff_weight_gradients(f, x, dy, hidden3, reinterpret_cast<float*>(ws + r.partial), dw_a, dw_b, dw_s, weight_dtype);
+  return rc;
+}
+
+int b200_blocks_read_status(void* cuda_stream, int* code) {
+  if (code == nullptr) return B200_TRIMUL_E_NULL;
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  *code = 0;
+  TRIMUL_CUDA(cudaMemcpyFromSymbolAsync(code, ff_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream));
+  TRIMUL_CUDA(cudaStreamSynchronize(stream));
+  if (*code != 0) {
+    const int zero = 0;
+    TRIMUL_CUDA(cudaMemcpyToSymbolAsync(ff_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream));
+    TRIMUL_CUDA(cudaStreamSynchronize(stream));
+  }
+  return B200_TRIMUL_OK;
+}
+
+}  // extern "C"

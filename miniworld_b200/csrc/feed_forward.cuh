@@ -1,0 +1,470 @@
+// The gated feed-forward of any width (multiples of eight), x [M, D], W_a and W_b [H, D], W_s [D, H]:
+//
+//   a = x W_a^T,  b = x W_b^T,  h = act(a) b,  y = h W_s^T                        (act: SiLU, or GELU with the error function)
+//   dh = dy W_s,  da = dh b act'(a),  db = dh act(a),  dx = da W_a + db W_b,  dW_a = da^T x,  dW_b = db^T x,  dW_s = dy^T h
+//
+// Nothing but x is kept for the backward: a and b are formed again (16 M D H multiply-adds in all instead of 12, against two
+// tensors [M, H] written and read, and their rounding). Five products on the tensor cores (fp32 accumulators in tensor memory), by
+// one kernel template; what is between two products of a row is done in the first one's epilogue, on the accumulators:
+//
+//   kFfUp       a | b side by side in one accumulator, h leaves              K = D
+//   kFfDown     y = h W_s^T                                                   K = H
+//   kFfHidden   dh, and a | b again: da, db and h leave                       K = D, D
+//   kFfInput    dx = da W_a + db W_b, one accumulator over both               K = H, H
+//   kFfWeights  dW_a, dW_b and dW_s^T = h^T dy: three products of one shape, the rows (K = M) split over the CTAs; fp32 partials
+//
+// Operands as they lie in memory: the weights' other orientation and the rows-as-K operands are read MN-major, so nothing is
+// transposed. h, da and db are rounded to the type of x (saturating for fp16), each once, as operands of 16-bit products have to be.
+// The structure is the contraction's: persistent CTAs (pairs for large products: 256-row tiles, each CTA supplies its rows of the
+// first operand and half of the second), one warp loads through TMA, one issues the MMAs, the others are the epilogue of the tile
+// before. All waits are bounded; one that gives up leaves a code in ff_status.
+#pragma once
+
+#include "ptx.cuh"
+
+namespace trimul {
+
+__device__ int ff_status;  // 0, or the code of the first wait that gave up (it stays until the host has read it)
+
+enum FfOp : int { kFfUp = 0, kFfDown = 1, kFfHidden = 2, kFfInput = 3, kFfWeights = 4 };
+enum FfAct : int { kFfSilu = 0, kFfGelu = 1 };
+
+struct FfMaps {
+  CUtensorMap a[3];
+  CUtensorMap b[3];
+};
+
+struct FfParams {
+  void* out[3];        // h | y | da, db, h | dx | (kFfWeights: not used)
+  float* partial;      // kFfWeights: [splits][3][rows][cols]
+  long long ld;        // elements from one row of `out` to the next
+  int rows, cols;      // of the output
+  int m_tiles, n_tiles;
+  int kb, kb_second;   // 64-deep k blocks of the first and of the second segment
+  int bn;              // accumulator columns of an output tile (kFfUp and kFfHidden: of its a | b part)
+  int splits, kb_split;  // kFfWeights: parts of the k range, k blocks of each
+  int act;
+};
+
+constexpr int kFfStages = 6;
+constexpr int kFfStageBytes = 32768;  // 128 rows of the first operand, up to 128 of the second, 64 deep
+constexpr int kFfThreads = 64 + 256;
+constexpr int kFfSmemBytes = kFfStages * kFfStageBytes + 256 + 1024;
+
+template <bool F16>
+__device__ __forceinline__ uint32_t ff_pack(float a, float b) {
+  return F16 ? pack_f16x2_sat(make_float2(a, b)) : pack_bf16x2(a, b);
+}
+
+// act(a) and its derivative
+__device__ __forceinline__ float ff_act(float a, int act) {
+  if (act == kFfSilu) return __fdividef(a, 1.0f + __expf(-a));
+  return 0.5f * a * (1.0f + erff(a * 0.70710678f));
+}
+__device__ __forceinline__ float2 ff_act_slope(float a, int act) {
+  if (act == kFfSilu) {
+    const float s = __fdividef(1.0f, 1.0f + __expf(-a));
+    return make_float2(a * s, s * fmaf(a, 1.0f - s, 1.0f));
+  }
+  const float cdf = 0.5f * (1.0f + erff(a * 0.70710678f));
+  return make_float2(a * cdf, fmaf(a * 0.39894228f, __expf(-0.5f * a * a), cdf));
+}
+
+template <int OP, bool PAIR, bool F16>
+__global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
+  constexpr int S = kFfStages;
+  constexpr bool A_MN = OP == kFfWeights;
+  constexpr bool SECOND = OP == kFfHidden || OP == kFfInput;  // two segments of k
+  constexpr int G = PAIR ? 2 : 1;                              // CTAs of a tile
+  constexpr int kUnits = PAIR ? 128 : 64;                      // hidden units of a tile (kFfUp, kFfHidden)
+  constexpr uint32_t kAcc = OP == kFfHidden ? kUnits : (PAIR ? 256 : 128);  // columns from one of the two accumulators to the other
+  constexpr uint32_t kAcc0 = OP == kFfHidden ? 2 * kUnits : 0;  // (kFfHidden: a | b first, then dh of even and odd tiles)
+  constexpr uint32_t kTmemCols = PAIR ? 512 : 256;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bar_base = base + S * kFfStageBytes;
+  auto full = [&](int s) { return bar_base + 8u * s; };
+  auto empty = [&](int s) { return bar_base + 8u * (S + s); };
+  auto acc_full = [&](int a) { return bar_base + 8u * (2 * S + a); };
+  auto acc_empty = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
+  const uint32_t ab_empty = bar_base + 8u * (2 * S + 4);  // kFfHidden: a | b are in registers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_base - smem_u32(smem_raw)) + 8 * (2 * S + 5));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), 8 * G);
+    }
+    mbar_init(ab_empty, 8 * G);
+    *abort_flag = 0;
+    fence_mbar_init();
+    for (int i = 0; i < 3; ++i) {
+      if (i == 0 || OP == kFfWeights || (i == 1 && SECOND)) prefetch_tmap(&maps.a[i]);
+      if (i == 0 || OP == kFfHidden || (i == 1 && OP != kFfDown)) prefetch_tmap(&maps.b[i]);
+    }
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  grid_dependency_wait();
+  grid_dependents_launch();
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // barriers of both CTAs are initialised before any signal crosses
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int per_split = p.m_tiles * p.n_tiles * (OP == kFfWeights ? 3 : 1);
+  const int tiles = per_split * p.splits;
+  struct Tile {
+    int split, product, m, n, kb0, kb1;
+  };
+  // the second operand's tiles run fastest (they share the rows of the first), the parts of a split k range slowest (tiles in
+  // flight read the same rows)
+  auto tile_at = [&](int i) {
+    Tile t;
+    t.split = OP == kFfWeights ? i / per_split : 0;
+    i -= t.split * per_split;
+    t.n = i % p.n_tiles;
+    i /= p.n_tiles;
+    t.m = i % p.m_tiles;
+    t.product = i / p.m_tiles;
+    t.kb0 = OP == kFfWeights ? t.split * p.kb_split : 0;
+    t.kb1 = OP == kFfWeights ? min(p.kb, t.kb0 + p.kb_split) : p.kb + (SECOND ? p.kb_second : 0);
+    return t;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads (both CTAs of a pair)
+    if (lane == 0) {
+      int s = 0, issued = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      const int bn_cta = p.bn / G;
+      for (int i = first; ok && i < tiles; i += step) {
+        const Tile t = tile_at(i);
+        const int m0 = (t.m * G + static_cast<int>(rank)) * 128;
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, &ff_status, kDevTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const bool second = SECOND && kb >= p.kb;
+          const int k0 = (second ? kb - p.kb : kb) * 64;
+          // kFfHidden: first dh (half as many columns), then a | b
+          const int cols = OP == kFfHidden && !second ? bn_cta / 2 : bn_cta;
+          if (rank == 0) mbar_arrive_expect_tx(full(s), G * (16384u + cols * 128u));
+          const uint32_t sa = base + s * kFfStageBytes, sb = sa + 16384;
+          auto load = [&](uint32_t dst, const CUtensorMap* m, int c0, int c1) {
+            if constexpr (PAIR)
+              tma_load_2d_pair(dst, m, map_to_cta(full(s), 0), c0, c1);
+            else
+              tma_load_2d(dst, m, full(s), c0, c1);
+          };
+          if constexpr (A_MN) {
+            load(sa, &maps.a[t.product], m0, k0);
+            load(sa + 8192, &maps.a[t.product], m0 + 64, k0);
+          } else {
+            load(sa, &maps.a[second ? 1 : 0], k0, m0);
+          }
+          if constexpr (OP == kFfUp) {
+            if constexpr (PAIR) {
+              load(sb, &maps.b[rank], k0, t.n * kUnits);
+            } else {
+              load(sb, &maps.b[0], k0, t.n * kUnits);
+              load(sb + 8192, &maps.b[1], k0, t.n * kUnits);
+            }
+          } else if constexpr (OP == kFfDown) {
+            load(sb, &maps.b[0], k0, t.n * p.bn + static_cast<int>(rank) * bn_cta);
+          } else if constexpr (OP == kFfHidden) {
+            if (!second) {
+              load(sb, &maps.b[2], t.n * kUnits + static_cast<int>(rank) * 64, k0);
+            } else if constexpr (PAIR) {
+              load(sb, &maps.b[rank], k0, t.n * kUnits);
+            } else {
+              load(sb, &maps.b[0], k0, t.n * kUnits);
+              load(sb + 8192, &maps.b[1], k0, t.n * kUnits);
+            }
+          } else {
+            const CUtensorMap* m = OP == kFfInput ? &maps.b[second ? 1 : 0] : &maps.b[t.product == 2 ? 1 : 0];
+            const int n0 = t.n * p.bn + static_cast<int>(rank) * bn_cta;
+            for (int c = 0; c < bn_cta; c += 64) load(sb + c * 128, m, n0 + c, k0);
+          }
+          ++issued;
+          if (++s == S) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // every copy that was started lands before the CTA may exit (a pair's leader counts the bytes of both CTAs; the closing
+      // cluster barrier keeps the other one)
+      if (rank == 0) {
+        const int pending = issued < S ? issued : S;
+        for (int q = 0; q < pending; ++q) {
+          if (s == 0) {
+            s = S;
+            ph ^= 1u;
+          }
+          --s;
+          const long long t0 = clock64();
+          while (!mbar_try_wait(full(s), ph)) {
+            if (*abort_flag != 0 || clock64() - t0 > kWaitLimitCycles) {
+              atomicCAS(&ff_status, 0, kDevTimeoutDrain);
+              break;
+            }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMAs (the pair's leader)
+    if (rank == 0 && elect_one()) {
+      int s = 0, it = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      const uint32_t fmt = F16 ? kFmtF16 : kFmtBF16;
+      for (int i = first; ok && i < tiles; i += step, ++it) {
+        const Tile t = tile_at(i);
+        const int acc = it & 1;
+        if (!mbar_wait(acc_empty(acc), ((it >> 1) & 1) ^ 1u, abort_flag, &ff_status, kDevTimeoutMma)) break;
+        tc_fence_after();
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          const bool second = SECOND && kb >= p.kb;
+          if (OP == kFfHidden && kb == p.kb) {
+            if (!mbar_wait(ab_empty, (it & 1) ^ 1u, abort_flag, &ff_status, kDevTimeoutMma)) {
+              ok = false;
+              break;
+            }
+          }
+          if (!mbar_wait(full(s), ph, abort_flag, &ff_status, kDevTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = base + s * kFfStageBytes, sb = sa + 16384;
+          const bool b_mn = OP == kFfInput || OP == kFfWeights || (OP == kFfHidden && !second);
+          const int n = OP == kFfHidden && !second ? p.bn / 2 : p.bn;
+          const uint32_t idesc = umma_idesc(128 * G, n, A_MN, b_mn, fmt, fmt);
+          const uint32_t d = OP == kFfHidden && second ? tmem : tmem + kAcc0 + acc * kAcc;
+          const uint64_t da = A_MN ? umma_desc_mnmajor(sa, 8192) : umma_desc_kmajor(sa);
+          const uint64_t db = b_mn ? umma_desc_mnmajor(sb, 8192) : umma_desc_kmajor(sb);
+          const uint32_t ka = A_MN ? 128 : 2, kn = b_mn ? 128 : 2;  // 16-byte units per 16 of k
+          const bool fresh = OP == kFfHidden ? kb == 0 || kb == p.kb : kb == t.kb0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t more = fresh && k == 0 ? 0u : 1u;
+            if constexpr (PAIR)
+              umma_pair(d, da + k * ka, db + k * kn, idesc, more);
+            else
+              umma_bf16(d, da + k * ka, db + k * kn, idesc, more);
+          }
+          if constexpr (PAIR)
+            umma_commit_pair(empty(s));
+          else
+            umma_commit(empty(s));
+          if (++s == S) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) {
+          if constexpr (PAIR)
+            umma_commit_pair(acc_full(acc));
+          else
+            umma_commit(acc_full(acc));
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue: a row per thread, half of the tile's columns per group
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    int it = 0;
+    for (int i = first; i < tiles; i += step, ++it) {
+      const Tile t = tile_at(i);
+      const int acc = it & 1;
+      const int row = (t.m * G + static_cast<int>(rank)) * 128 + q * 32 + lane;
+      const bool in = row < p.rows;
+      if (!mbar_wait_warp(acc_full(acc), (it >> 1) & 1, abort_flag, &ff_status, kDevTimeoutEpilogue)) break;
+      tc_fence_after();
+      auto release = [&](uint32_t bar) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR)
+            mbar_arrive_leader(bar, rank);
+          else
+            mbar_arrive(bar);
+        }
+      };
+      // 8 neighbours of the output from 8 values
+      auto store8 = [&](void* out, int col, const float* v) {
+        if (in && col < p.cols)
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + static_cast<size_t>(row) * p.ld + col) =
+              make_uint4(ff_pack<F16>(v[0], v[1]), ff_pack<F16>(v[2], v[3]), ff_pack<F16>(v[4], v[5]), ff_pack<F16>(v[6], v[7]));
+      };
+      const uint32_t d = tmem + lanes + kAcc0 + acc * kAcc;
+      if constexpr (OP == kFfUp) {
+        constexpr int N = kUnits / 2;
+#pragma unroll 1
+        for (int c = 0; c < N; c += 16) {
+          uint32_t va[16], vb[16];
+          tmem_ld16(d + half * N + c, va);
+          tmem_ld16(d + kUnits + half * N + c, vb);
+          tmem_ld_wait();
+          if (c + 16 == N) release(acc_empty(acc));
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = ff_act(__uint_as_float(va[j]), p.act) * __uint_as_float(vb[j]);
+          const int col = t.n * kUnits + half * N + c;
+          store8(p.out[0], col, v);
+          store8(p.out[0], col + 8, v + 8);
+        }
+      } else if constexpr (OP == kFfHidden) {
+        constexpr int N = kUnits / 2;
+#pragma unroll 1
+        for (int c = 0; c < N; c += 16) {
+          uint32_t va[16], vb[16], vd[16];
+          tmem_ld16(tmem + lanes + half * N + c, va);
+          tmem_ld16(tmem + lanes + kUnits + half * N + c, vb);
+          tmem_ld16(d + half * N + c, vd);
+          tmem_ld_wait();
+          if (c + 16 == N) {
+            release(ab_empty);
+            if (lane == 0) {
+              if constexpr (PAIR)
+                mbar_arrive_leader(acc_empty(acc), rank);
+              else
+                mbar_arrive(acc_empty(acc));
+            }
+          }
+          const int col = t.n * kUnits + half * N + c;
+          float da[16], db[16], h[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float b = __uint_as_float(vb[j]), dh = __uint_as_float(vd[j]);
+            const float2 f = ff_act_slope(__uint_as_float(va[j]), p.act);
+            da[j] = dh * b * f.y;
+            db[j] = dh * f.x;
+            h[j] = f.x * b;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j += 8) {
+            store8(p.out[0], col + j, da + j);
+            store8(p.out[1], col + j, db + j);
+            store8(p.out[2], col + j, h + j);
+          }
+        }
+      } else {
+        const int n = p.bn / 2;
+#pragma unroll 1
+        for (int c = 0; c < n; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(d + half * n + c, v);
+          tmem_ld_wait();
+          if (c + 16 >= n) release(acc_empty(acc));
+          const int col = t.n * p.bn + half * n + c;
+          float f[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]);
+          if constexpr (OP != kFfWeights) {
+            store8(p.out[0], col, f);
+            store8(p.out[0], col + 8, f + 8);
+          } else if (in) {
+            float* o = p.partial + ((static_cast<size_t>(t.split) * 3 + t.product) * p.rows + row) * p.cols + col;
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              if (col + j < p.cols) *reinterpret_cast<float4*>(o + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // neither CTA leaves while the other may still signal its barriers or read its operands
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem, kTmemCols);
+    else
+      tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Sums the parts of the weight gradients in the order of the rows and rounds once: dW_a, dW_b [H, D] as they lie, dW_s [D, H] from
+// its transpose (through shared memory). A block takes 32 x 32 values of one product.
+struct FfReduce {
+  const float* partial;  // [splits][3][H][D]
+  void* out[3];
+  int splits, H, D;
+  int type;  // 0 bf16, 1 fp32, 2 fp16
+};
+__device__ __forceinline__ void ff_put(void* out, size_t i, float v, int type) {
+  if (type == 1)
+    static_cast<float*>(out)[i] = v;
+  else if (type == 0)
+    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+  else
+    static_cast<__half*>(out)[i] = __float2half_rn(v);
+}
+__global__ void __launch_bounds__(256) ff_reduce_kernel(const FfReduce p) {
+  __shared__ float tile[32][33];
+  grid_dependency_wait();
+  grid_dependents_launch();
+  void* out = p.out[blockIdx.z];
+  if (out == nullptr) return;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
+  const size_t part = static_cast<size_t>(3) * p.H * p.D;
+  for (int j = ty; j < 32; j += 8) {
+    const int r = blockIdx.y * 32 + j;
+    float a = 0.f;
+    if (r < p.H && c < p.D) {
+      const float* s = p.partial + (static_cast<size_t>(blockIdx.z) * p.H + r) * p.D + c;
+      for (int k = 0; k < p.splits; ++k) a += __ldcg(s + k * part);
+      if (blockIdx.z < 2) ff_put(out, static_cast<size_t>(r) * p.D + c, a, p.type);
+    }
+    tile[j][tx] = a;
+  }
+  if (blockIdx.z < 2) return;
+  __syncthreads();
+  for (int j = ty; j < 32; j += 8) {
+    const int d = blockIdx.x * 32 + j, h = blockIdx.y * 32 + tx;
+    if (d < p.D && h < p.H) ff_put(out, static_cast<size_t>(d) * p.H + h, tile[tx][j], p.type);
+  }
+}
+
+// fp32 master weights as operands (the type of x, saturating for fp16)
+__global__ void __launch_bounds__(256) ff_cast_kernel(const float* a, const float* b, const float* s, uint4* out, long long n8, int f16) {
+  grid_dependency_wait();
+  grid_dependents_launch();
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < 3 * n8; i += static_cast<long long>(gridDim.x) * 256) {
+    const int which = static_cast<int>(i / n8);
+    const float4* w = reinterpret_cast<const float4*>((which == 0 ? a : which == 1 ? b : s) + (i - which * n8) * 8);
+    const float4 u = __ldcg(w), v = __ldcg(w + 1);
+    out[i] = f16 ? make_uint4(ff_pack<true>(u.x, u.y), ff_pack<true>(u.z, u.w), ff_pack<true>(v.x, v.y), ff_pack<true>(v.z, v.w))
+                 : make_uint4(ff_pack<false>(u.x, u.y), ff_pack<false>(u.z, u.w), ff_pack<false>(v.x, v.y), ff_pack<false>(v.z, v.w));
+  }
+}
+
+}  // namespace trimul

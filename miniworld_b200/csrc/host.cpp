@@ -23,6 +23,7 @@
 #include <tuple>
 #include <vector>
 
+#include "../../include/b200_blocks.h"
 #include "../../include/b200_trimul.h"
 
 // The parameters of a call, in Python a list of tensors or a pair (a module's _modules, ((child, name), ...)) that names the
@@ -379,6 +380,8 @@ OptTensor transition_train(const Tensor& x, const CallParams& call, double eps, 
   return TransitionNode::apply(x, at::TensorList(params), eps, residual);
 }
 
+#include "host_blocks.inc"
+
 }  // namespace
 
 namespace pybind11::detail {
@@ -420,4 +423,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("trimul_train", torch::wrap_pybind_function_no_gil(trimul_train));
   m.def("transition_forward", torch::wrap_pybind_function_no_gil(transition_forward));
   m.def("transition_train", torch::wrap_pybind_function_no_gil(transition_train));
+  m.def("block_join", torch::wrap_pybind_function_no_gil(block_join));
+  m.def("gated_feed_forward", torch::wrap_pybind_function_no_gil(gated_feed_forward));
 }

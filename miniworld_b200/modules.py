@@ -29,6 +29,7 @@ import torch
 from torch import nn
 
 from . import _lib
+from . import blocks
 from . import functional as F_
 
 D_SUPPORTED = 128
@@ -511,3 +512,98 @@ class Transition(_Scratch):
             if self.check_status:
                 F_.check_status(status, "b200_transition_forward")
         return y if in_dtype == torch.bfloat16 else y.to(in_dtype)
+
+
+class BlockNorm(Fp32LayerNorm):
+    """The norm in front of a block, ``forward(x [..., d]) -> norm(x)``: ``kind`` "layer" or "rms" over any width up to 4096, on bf16,
+    fp16 or fp32 tensors. The affine parameters stay fp32 (:class:`Fp32LayerNorm`); ``bias`` defaults to the layer norm's only."""
+
+    def __init__(self, d: int, kind: str = "layer", eps: float = 1e-5, bias: Optional[bool] = None):
+        if kind not in ("layer", "rms"):
+            raise ValueError(f"norm kind must be 'layer' or 'rms', got {kind!r}")
+        super().__init__(d, eps=eps, bias=kind == "layer" if bias is None else bool(bias))
+        self.kind = kind
+
+    def norm(self) -> blocks.Norm:
+        """The arguments of :func:`miniworld_b200.blocks.block_join` that this module stands for."""
+        return blocks.Norm(self.kind, self.weight, self.bias, float(self.eps))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return blocks.block_norm(x, self.weight, self.bias, kind=self.kind, eps=float(self.eps))
+
+    def extra_repr(self) -> str:
+        return f"{self.normalized_shape[0]}, kind={self.kind!r}, eps={self.eps}, bias={self.bias is not None}"
+
+
+class BlockJoin(nn.Module):
+    """What closes a block and opens the next: ``forward(x, u, gate=None, mask=None, next_norm=None)`` gives
+    ``y = x + mask * scale * sigmoid(gate) * norm(u)`` and, with the next block's :class:`BlockNorm`, ``(y, next_norm(y))`` in the same
+    pass. ``kind`` None: no norm after the block; ``scale`` the initial value of a learned fp32 scale per channel, None: no scale."""
+
+    def __init__(self, d: int, kind: Optional[str] = "layer", eps: float = 1e-5, bias: Optional[bool] = None, scale: Optional[float] = None):
+        super().__init__()
+        self.d = d
+        self.norm_out = None if kind is None else BlockNorm(d, kind, eps, bias)
+        self.scale = None if scale is None else nn.Parameter(torch.full((d,), float(scale)))
+
+    def _apply(self, fn, recurse=True):
+        kept = None if self.scale is None else self.scale.data
+        super()._apply(fn, recurse)
+        if kept is not None and self.scale.dtype != kept.dtype:  # pinned to fp32 like the norms' parameters
+            self.scale.data = kept.to(self.scale.device)
+        return self
+
+    def forward(self, x: torch.Tensor, u: torch.Tensor, gate: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                next_norm: Optional[BlockNorm] = None):
+        return blocks.block_join(x, u, gate=gate, scale=self.scale, mask=mask, post=None if self.norm_out is None else self.norm_out.norm(),
+                                 pre=None if next_norm is None else next_norm.norm())
+
+
+class GatedFeedForward(nn.Module):
+    """``forward(x [..., d]) -> squeeze(act(expand_a x) * expand_b x)``, the products of :class:`Transition` for any widths that are
+    multiples of 8 (parameter names and shapes are its: ``expand_a`` / ``expand_b`` [hidden, d], ``squeeze`` [d, hidden], bias-free).
+    ``hidden`` defaults to ``n * d``; ``activation`` "silu" or "gelu"."""
+
+    def __init__(self, d: int, n: int = 4, hidden: Optional[int] = None, activation: str = "silu", implementation=None,
+                 check_status: bool = False):
+        super().__init__()
+        hidden = n * d if hidden is None else hidden
+        if d < 8 or d % 8 or hidden < 8 or hidden % 8:
+            raise NotImplementedError(f"widths that are multiples of 8 are implemented, got d = {d}, hidden = {hidden}")
+        if activation not in ("silu", "gelu"):
+            raise ValueError(f"activation must be 'silu' or 'gelu', got {activation!r}")
+        impl = getattr(implementation, "value", implementation)
+        impl = impl.lower() if isinstance(impl, str) else impl
+        if impl not in _ACCEPTED_IMPLEMENTATIONS:
+            raise ValueError(f"implementation={implementation!r}: this module has exactly one backend (B200 CUDA kernels)")
+        self.d, self.hidden, self.activation = d, hidden, activation
+        self.check_status = bool(check_status)
+        self.expand_a = nn.Linear(d, hidden, bias=False)
+        self.expand_b = nn.Linear(d, hidden, bias=False)
+        self.squeeze = nn.Linear(hidden, d, bias=False)
+        nn.init.zeros_(self.squeeze.weight)  # the reference's final linears start at zero
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = blocks.gated_feed_forward(x, self.expand_a.weight, self.expand_b.weight, self.squeeze.weight, activation=self.activation)
+        if self.check_status:
+            blocks.check_status(x.device)
+        return y
+
+
+class SandwichTransition(nn.Module):
+    """A feed-forward block of any width with norms on both sides, ``forward(x, gate=None, mask=None) -> x + update``:
+
+        update = mask * scale * sigmoid(gate) * norm_out(squeeze(act(expand_a h) * expand_b h)),   h = ln_in(x)
+
+    the :class:`Transition` of token and alignment tensors (``kind_out`` None, ``scale`` None and no gate: the same operator; its
+    parameters then have the same names, ``ln_in``, ``feed_forward.expand_a`` ... under ``feed_forward``)."""
+
+    def __init__(self, d: int, n: int = 4, hidden: Optional[int] = None, activation: str = "silu", kind: str = "layer",
+                 kind_out: Optional[str] = "layer", scale: Optional[float] = None, implementation=None, check_status: bool = False):
+        super().__init__()
+        self.ln_in = BlockNorm(d, kind)
+        self.feed_forward = GatedFeedForward(d, n, hidden, activation, implementation, check_status)
+        self.join = BlockJoin(d, kind_out, scale=scale)
+
+    def forward(self, x: torch.Tensor, gate: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return self.join(x, self.feed_forward(self.ln_in(x)), gate, mask)

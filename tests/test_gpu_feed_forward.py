@@ -1,0 +1,224 @@
+"""The gated feed-forward of any width, forward and backward, against float64.
+
+Tolerances. h, da and db are rounded to the type T of the input once, then summed: each relative rounding error lies within
+eps_T / 2 and has a standard deviation of at most eps_T / sqrt(12), so a sum of n products with the other operand is off by a
+standard deviation of eps_T / sqrt(12) * sqrt(sum of the squared products); six of these bound it (for n <= 12 they are above the
+worst case, eps_T / 2 times the sum of the magnitudes). On top come the rounding of the result, eps / 2 of it, and fp32 arithmetic:
+the products' sums and the activation (a few units of 2^-24 each, and 2^-21 for the fast exponential and division), 2^-16 of the
+sum of the magnitudes."""
+
+import math
+
+import pytest
+import torch
+
+import miniworld_b200 as mw
+from miniworld_b200 import blocks
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    assert blocks.read_status(DEV) == 0
+
+
+def _make(rows, d, hidden, type, weights=None, seed=0):
+    g = torch.Generator().manual_seed(seed + math.prod(rows if isinstance(rows, tuple) else (rows,)) * 31 + d * 7 + hidden)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    weights = type if weights is None else weights
+    rows = rows if isinstance(rows, tuple) else (rows,)
+    return {"x": r(*rows, d).to(type).to(DEV), "w_a": (r(hidden, d) * d**-0.5).to(weights).to(DEV),
+            "w_b": (r(hidden, d) * d**-0.5).to(weights).to(DEV), "w_s": (r(d, hidden) * hidden**-0.5).to(weights).to(DEV),
+            "dy": (r(*rows, d) * 0.1).to(type).to(DEV)}
+
+
+def _want(t, act, type):
+    """name -> (value, bound without the result's rounding)."""
+    d = t["x"].shape[-1]
+    x, dy = t["x"].to(type).double().reshape(-1, d), t["dy"].double().reshape(-1, d)
+    wa, wb, ws = (t[k].to(type).double() for k in ("w_a", "w_b", "w_s"))  # (fp32 weights are rounded first)
+    a, b = x @ wa.t(), x @ wb.t()
+    if act == "silu":
+        s = torch.sigmoid(a)
+        f, slope = a * s, s * (1 + a * (1 - s))
+    else:
+        c = 0.5 * torch.erfc(-a * 0.5**0.5)
+        f, slope = a * c, c + a * torch.exp(-a * a / 2) * (2 * torch.pi) ** -0.5
+    h = f * b
+    dh = dy @ ws
+    da, db = dh * b * slope, dh * f
+    eps, small = torch.finfo(type).eps, 2.0**-16
+    # what a, b, dh themselves are off by in fp32, through the following products
+    fa, fb, fd = small * (x.abs() @ wa.abs().t()), small * (x.abs() @ wb.abs().t()), small * (dy.abs() @ ws.abs())
+    eh = f.abs() * fb + 1.2 * fa * b.abs() + small * h.abs()
+    eda = fd * (b * slope).abs() + dh.abs() * (fb + b.abs() * fa) + small * da.abs()
+    edb = fd * f.abs() + 1.2 * dh.abs() * fa + small * db.abs()
+
+    def product(p, ep, q):  # p [m, k] rounded to the type and off by ep, q [k, n] as it is
+        return p @ q, 6 * eps / 12**0.5 * (p.square() @ q.square()).sqrt() + small * (p.abs() @ q.abs()) + ep @ q.abs()
+
+    dx1, dx2 = product(da, eda, wa), product(db, edb, wb)
+    shape = t["x"].shape
+    out = {"y": product(h, eh, ws.t()), "x": (dx1[0] + dx2[0], dx1[1] + dx2[1]), "w_a": product(da.t(), eda.t(), x),
+           "w_b": product(db.t(), edb.t(), x)}
+    s = product(h.t(), eh.t(), dy)
+    out["w_s"] = (s[0].t(), s[1].t())
+    for k in ("y", "x"):
+        out[k] = tuple(v.reshape(shape) for v in out[k])
+    return out
+
+
+def _run(t, act):
+    leaves = {k: v.clone().requires_grad_(True) for k, v in t.items() if k != "dy"}
+    y = blocks.gated_feed_forward(*leaves.values(), activation=act)
+    with torch.no_grad():
+        assert torch.equal(y, blocks.gated_feed_forward(*leaves.values(), activation=act))
+    g = torch.autograd.grad(y, list(leaves.values()), t["dy"], retain_graph=True)
+    for a, b in zip(g, torch.autograd.grad(y, list(leaves.values()), t["dy"])):
+        assert torch.equal(a, b)  # the same bits again
+    return {"y": y.detach(), **dict(zip(leaves, g))}
+
+
+def _compare(got, want, what):
+    for k, (ref, bound) in want.items():
+        g = got[k]
+        assert g.shape == ref.shape, (what, k)
+        assert torch.isfinite(g).all(), (what, k)
+        # (a subnormal result of a 16-bit type is rounded to a multiple of the smallest one)
+        bound = bound + torch.finfo(g.dtype).eps / 2 * ref.abs() + torch.finfo(g.dtype).smallest_normal * torch.finfo(g.dtype).eps
+        bad = (g.double() - ref).abs() / bound
+        assert float(bad.max()) <= 1.0, (what, k, float(bad.max()), int(bad.argmax()))
+
+
+@pytest.mark.parametrize("rows,d,hidden", [
+    (1, 8, 8), (1, 64, 256), (1, 768, 2048), (2, 72, 136), (3, 384, 1536), (7, 128, 512), (8, 200, 536), (9, 256, 1024), (31, 64, 64),
+    (64, 136, 72), (127, 64, 256), (128, 128, 128), (129, 384, 1536), (255, 192, 320), (257, 320, 264), (384, 384, 1536), (609, 384, 1536),
+    (1000, 64, 256), (1100, 1000, 2000), (2048, 512, 2048), (5000, 96, 384), (9001, 64, 256), (40000, 24, 40), (20011, 256, 1024),
+])
+def test_against_float64(rows, d, hidden):
+    t = _make(rows, d, hidden, torch.bfloat16)
+    _compare(_run(t, "silu"), _want(t, "silu", torch.bfloat16), (rows, d, hidden))
+
+
+@pytest.mark.parametrize("rows,d,hidden", [(1, 64, 128), (5, 384, 1536), (300, 200, 536), (2100, 256, 768), (12000, 128, 512)])
+@pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("weights", ["same", "fp32"])
+def test_types_and_activations(rows, d, hidden, type, act, weights):
+    t = _make(rows, d, hidden, type, torch.float32 if weights == "fp32" else None)
+    got = _run(t, act)
+    assert got["w_a"].dtype == t["w_a"].dtype and got["y"].dtype == type
+    _compare(got, _want(t, act, type), (rows, d, hidden, type, act, weights))
+
+
+def test_other_float_types_run_through_bf16():
+    t = _make(50, 64, 128, torch.bfloat16)
+    want = blocks.gated_feed_forward(t["x"], t["w_a"], t["w_b"], t["w_s"])
+    for type in (torch.float32, torch.float64):
+        y = blocks.gated_feed_forward(t["x"].to(type), t["w_a"], t["w_b"], t["w_s"])
+        assert y.dtype == type and torch.equal(y, want.to(type))
+    x = t["x"].float().requires_grad_(True)
+    (g,) = torch.autograd.grad(blocks.gated_feed_forward(x, t["w_a"], t["w_b"], t["w_s"]).sum(), x)
+    assert g.dtype == torch.float32
+
+
+@pytest.mark.parametrize("rows", [1, 4, 200, 3000])
+def test_large_activations(rows):
+    """Arguments of the activation far on both sides: no overflow on the way, exact zeros and identities."""
+    t = _make(rows, 64, 128, torch.bfloat16)
+    t["w_a"] *= 64
+    for act in ("silu", "gelu"):
+        _compare(_run(t, act), _want(t, act, torch.bfloat16), (rows, act))
+
+
+@pytest.mark.parametrize("rows", [2, 200])
+def test_fp16_saturates(rows):
+    x = torch.full((rows, 64), 60.0, dtype=torch.float16, device=DEV)
+    w = torch.full((64, 64), 1.0, dtype=torch.float16, device=DEV)
+    y = blocks.gated_feed_forward(x, w, w, torch.eye(64, dtype=torch.float16, device=DEV))
+    assert (y == 65504).all()  # a = b = 3840, h = 65504 instead of infinity
+
+
+@pytest.mark.parametrize("rows", [3, 150])
+def test_rows_do_not_touch_one_another(rows):
+    t = _make(rows, 128, 256, torch.bfloat16)
+    w = [t[k] for k in ("w_a", "w_b", "w_s")]
+    want = blocks.gated_feed_forward(t["x"], *w)
+    for bad in (float("nan"), float("inf")):
+        x = t["x"].clone()
+        x[1] = bad
+        got = blocks.gated_feed_forward(x, *w)
+        assert not torch.isfinite(got[1]).any()
+        keep = torch.arange(rows, device=DEV) != 1
+        assert torch.equal(got[keep], want[keep])
+
+
+def test_only_what_is_asked_for():
+    t = _make(70, 64, 128, torch.bfloat16)
+    full = _run(t, "silu")
+    names = ["x", "w_a", "w_b", "w_s"]
+    for wanted in (["x"], ["w_a"], ["w_s"], ["x", "w_b"], ["w_a", "w_b", "w_s"]):
+        leaves = {k: t[k].clone().requires_grad_(k in wanted) for k in names}
+        y = blocks.gated_feed_forward(*leaves.values())
+        for k, g in zip(wanted, torch.autograd.grad(y, [leaves[k] for k in wanted], t["dy"])):
+            assert torch.equal(g, full[k]), (wanted, k)
+
+
+def test_no_rows():
+    t = _make((2, 0), 64, 128, torch.bfloat16)
+    got = _run(t, "silu")
+    assert got["y"].shape == (2, 0, 64) and got["x"].shape == (2, 0, 64)
+    assert not got["w_a"].any() and not got["w_b"].any() and not got["w_s"].any()
+
+
+def test_layouts_are_converted():
+    t = _make((6, 50), 64, 128, torch.bfloat16)
+    w = [t[k] for k in ("w_a", "w_b", "w_s")]
+    want = blocks.gated_feed_forward(t["x"], *w)
+    swapped = t["x"].transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(blocks.gated_feed_forward(swapped, *w), want)
+    flat = torch.zeros(6 * 50 * 64 + 1, dtype=torch.bfloat16, device=DEV)
+    flat[1:] = t["x"].flatten()
+    assert torch.equal(blocks.gated_feed_forward(flat[1:].view(6, 50, 64), *w), want)
+    # gradients that arrive expanded or off a boundary
+    x = t["x"].clone().requires_grad_(True)
+    y = blocks.gated_feed_forward(x, *w)
+    (a,) = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+    (b,) = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    assert torch.equal(a, b)
+    odd = torch.zeros(y.numel() + 1, dtype=torch.bfloat16, device=DEV)
+    odd[1:] = 1
+    assert torch.equal(torch.autograd.grad(y, x, odd[1:].view_as(y))[0], a)
+
+
+def test_refusals():
+    t = _make(4, 64, 128, torch.bfloat16)
+    x, wa, wb, ws = (t[k] for k in ("x", "w_a", "w_b", "w_s"))
+    f = blocks.gated_feed_forward
+    off = torch.zeros(128 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(128, 64)
+    for call, word in [
+        (lambda: f(x.cpu(), wa, wb, ws), "CUDA"), (lambda: f(x, wa.cpu(), wb, ws), "CUDA"), (lambda: f(x.long(), wa, wb, ws), "float"),
+        (lambda: f(x, wa.half(), wb.half(), ws.half()), "weights"), (lambda: f(x, wa, wb.float(), ws), "one type"),
+        (lambda: f(x[:, :32], wa, wb, ws), "w_a must be"), (lambda: f(x, wa, wb[:64], ws), "w_b must be"), (lambda: f(x, wa, wb, ws.t()), "w_s must be"),
+        (lambda: f(x, wa, wb, ws.t().contiguous().t()), "contiguous"), (lambda: f(x, off, wb, ws), "16-byte"),
+        (lambda: f(x[:, :60], wa[:, :60].contiguous(), wb[:, :60].contiguous(), ws[:60].contiguous()), "multiples of 8"),
+        (lambda: f(x, wa[:100], wb[:100], ws[:, :100].contiguous()), "multiples of 8"), (lambda: f(x, wa[:0], wb[:0], ws[:, :0]), "multiples of 8"),
+    ]:
+        with pytest.raises(RuntimeError, match=word):
+            call()
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda r: f(r, wa, wb, ws))(x)
+
+
+def test_module_matches_the_function():
+    m = mw.GatedFeedForward(64, n=2, activation="gelu", check_status=True).to(DEV)
+    torch.nn.init.normal_(m.squeeze.weight, std=0.1)
+    x = torch.randn(3, 5, 64, device=DEV).bfloat16()
+    want = blocks.gated_feed_forward(x, m.expand_a.weight, m.expand_b.weight, m.squeeze.weight, activation="gelu")
+    y = m(x)
+    assert torch.equal(y, want)
+    y.float().square().sum().backward()
+    assert all(p.grad is not None and p.grad.dtype == torch.float32 and bool(p.grad.any()) for p in m.parameters())
