@@ -3,11 +3,13 @@
 #include "../../include/b200_blocks.h"
 
 #include <algorithm>
+#include <numeric>
 #include <utility>
 
 #include "feed_forward.cuh"
 #include "host_util.cuh"
 #include "join.cuh"
+#include "join_tiles.cuh"
 
 namespace trimul {
 
@@ -68,13 +70,78 @@ static bool all_aligned16(std::initializer_list<const void*> ps) {
   return true;
 }
 
+// Tiles of a call (see join_tiles.cuh): rows to a tile, stages and their places. False where the tensors do not start on 16 bytes
+// or a row takes more warps than there are or two stages do not fit: the kernels of join.cuh
+// then run. As many rows to a tile as the block works on at a time, fewer where that would leave SMs without one.
+static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count, int size, int nv, int params, int blocks_most) {
+  for (int i = 0; i < count; ++i)
+    if (!aligned(tensors[i], 16)) return false;
+  const JoinParams& j = p->j;
+  if (j.team > kTileWarps * 32) return false;
+  const int unit = 16 / static_cast<int>(std::gcd(16, j.d * size));  // rows whose bytes are a multiple of 16
+  const int teams = kTileWarps * 32 / j.team;
+  const long long share = (j.rows + blocks_most - 1) / blocks_most;
+  long long rows = std::min<long long>(teams, share);
+  rows = static_cast<long long>(up(static_cast<size_t>(rows), unit));
+  p->params = 8 * nv * j.team;
+  const int fixed = params * p->params * 4 + kTileScratch;
+  while (true) {
+    p->slot = static_cast<int>(up(static_cast<size_t>(rows) * j.d * size, 128));
+    p->stages = std::min(kTileMaxStages, (kTileSmem - fixed) / (p->slot * p->slots));
+    if (p->stages >= 2) break;
+    if (rows <= unit) return false;
+    rows = static_cast<long long>(up(static_cast<size_t>(rows / 2), unit));
+  }
+  p->tile_rows = static_cast<int>(rows);
+  const long long tiles = (j.rows + rows - 1) / rows;
+  if (tiles > 0x7FFFFFFF) return false;
+  p->tiles = static_cast<int>(tiles);
+  p->stages = static_cast<int>(std::min<long long>(p->stages, std::max<long long>(2, (tiles + blocks_most - 1) / blocks_most)));
+  return true;
+}
+static int tile_smem(const JoinTileParams& p, int params) {
+  // (the backward's sums pass through the stages)
+  return params * p.params * 4 + kTileScratch + std::max(p.stages * p.slots * p.slot, kTileWarps * 32 * 8 * 4);  // (at most kTileSmem)
+}
+template <typename T, int VEC>
+static auto tile_forward_kernel(int nv) {
+  switch (nv) {
+    case 1: return join_tile_forward_kernel<T, VEC, 1>;
+    case 2: return join_tile_forward_kernel<T, VEC, 2>;
+    case 3: return join_tile_forward_kernel<T, VEC, 3>;
+    default: return join_tile_forward_kernel<T, VEC, 4>;
+  }
+}
+// elements of a row that a thread reads at once
+static int join_vec(int d) { return d % 8 == 0 ? 8 : d % 2 == 0 ? 2 : 1; }
+
 template <typename T>
-static int launch_join_forward(const JoinParams& p0, bool wide, int sms, cudaStream_t stream) {
+static int launch_join_forward(const JoinParams& p0, bool wide, const DeviceInfo& info, cudaStream_t stream) {
+  JoinTileParams q = {};
+  q.j = p0;
+  const JoinShape s = join_forward_shape(p0.d);
+  q.j.team = s.team;
+  q.slot_of[0] = q.slots++;
+  q.slot_of[1] = p0.u != nullptr ? q.slots++ : -1;
+  q.slot_of[2] = p0.gate != nullptr && p0.gate_rows == 1 ? q.slots++ : -1;
+  q.slot_of[3] = q.slot_of[4] = -1;
+  q.out_slot[0] = p0.y != nullptr ? 0 : -1;
+  q.out_slot[1] = p0.h != nullptr ? (p0.u != nullptr ? 1 : 0) : -1;
+  q.out_slot[2] = -1;
+  const void* tensors[] = {p0.x, p0.u, q.slot_of[2] >= 0 ? p0.gate : nullptr, p0.y, p0.h};
+  if (plan_tiles(&q, tensors, 5, sizeof(T), s.nv, 4, info.sms)) {
+    const int vec = join_vec(p0.d);
+    auto kernel = vec == 8 ? tile_forward_kernel<T, 8>(s.nv) : vec == 2 ? tile_forward_kernel<T, 2>(s.nv) : tile_forward_kernel<T, 1>(s.nv);
+    const int rc = set_smem(kernel, kTileSmem, info.device);
+    if (rc != 0) return rc;
+    const int threads = kTileWarps * 32 / s.team * s.team + 32;
+    TRIMUL_CUDA(launch_overlapped(kernel, dim3(std::min(info.sms, q.tiles)), threads, tile_smem(q, 4), stream, q));
+    return B200_TRIMUL_OK;
+  }
   JoinParams p = p0;
-  const JoinShape s = join_forward_shape(p.d);
   p.team = s.team;
   const int teams = kJoinForwardThreads / s.team;
-  const int blocks = static_cast<int>(std::min<long long>((p.rows + teams - 1) / teams, 8ll * sms));
+  const int blocks = static_cast<int>(std::min<long long>((p.rows + teams - 1) / teams, 8ll * info.sms));
   void (*kernel)(JoinParams) = nullptr;
   switch (s.nv) {
     case 1: kernel = wide ? join_forward_kernel<T, true, 1> : join_forward_kernel<T, false, 1>; break;
@@ -86,8 +153,48 @@ static int launch_join_forward(const JoinParams& p0, bool wide, int sms, cudaStr
   return B200_TRIMUL_OK;
 }
 
+constexpr long long kSharedGateRows = 256;  // gate rows of fewer rows take the kernels of join.cuh: less scratch a gate row
+
 template <typename T>
-static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& g, const JoinSums& sums, cudaStream_t stream) {
+static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& g, const JoinSums& sums, const DeviceInfo& info,
+                                cudaStream_t stream) {
+  JoinTileParams q = {};
+  q.j = p;
+  const bool shared_gate = p.gate != nullptr && p.gate_rows > 1;
+  q.slot_of[0] = p.pre_kind != kNormNone ? q.slots++ : -1;
+  q.slot_of[1] = p.u != nullptr ? q.slots++ : -1;
+  q.slot_of[2] = p.gate != nullptr && !shared_gate ? q.slots++ : -1;
+  q.slot_of[3] = p.dy != nullptr ? q.slots++ : -1;
+  q.slot_of[4] = p.dh != nullptr ? q.slots++ : -1;
+  q.out_slot[0] = p.dx == nullptr ? -1 : q.slot_of[0] >= 0 ? q.slot_of[0] : q.slot_of[3] >= 0 ? q.slot_of[3] : q.slots++;
+  q.out_slot[1] = p.du != nullptr ? q.slot_of[1] : -1;
+  q.out_slot[2] = p.dgate != nullptr && !shared_gate ? q.slot_of[2] : -1;
+  const void* tensors[] = {p.x, p.u, q.slot_of[2] >= 0 ? p.gate : nullptr, p.dy, p.dh, p.dx, p.du, q.out_slot[2] >= 0 ? p.dgate : nullptr};
+  if (q.slots > 0 && (!shared_gate || p.gate_rows >= kSharedGateRows) && plan_tiles(&q, tensors, 8, sizeof(T), 1, 3, std::min(info.sms, kMaxSms))) {
+    int blocks = std::min(std::min(info.sms, kMaxSms), q.tiles);
+    if (shared_gate) {
+      q.block_tiles = (q.tiles + blocks - 1) / blocks;
+      q.group_slots = static_cast<int>(static_cast<long long>(q.block_tiles) * q.tile_rows / p.gate_rows) + 2;
+    }
+    const int vec = join_vec(p.d);
+    auto kernel = vec == 8 ? join_tile_backward_kernel<T, 8> : vec == 2 ? join_tile_backward_kernel<T, 2> : join_tile_backward_kernel<T, 1>;
+    const int rc = set_smem(kernel, kTileSmem, info.device);
+    if (rc != 0) return rc;
+    const int threads = kTileWarps * 32 / p.team * p.team + 32;
+    TRIMUL_CUDA(launch_overlapped(kernel, dim3(blocks), threads, tile_smem(q, 3), stream, q));
+    if (p.sums != nullptr) {
+      JoinTileSums t = {p.sums, p.scale, p.post_w, p.post_b, {}, blocks, p.d, p.post_kind};
+      for (int i = 0; i < 5; ++i) t.out[i] = sums.out[i];
+      TRIMUL_CUDA(launch_overlapped(join_tile_sums_kernel, dim3((p.d + 31) / 32, 2), 1024, 0, stream, t));
+    }
+    if (p.dgate != nullptr && shared_gate) {
+      auto last = vec == 8 ? join_tile_gate_kernel<T, 8> : vec == 2 ? join_tile_gate_kernel<T, 2> : join_tile_gate_kernel<T, 1>;
+      const long long groups = p.rows / p.gate_rows;
+      if (groups > 65535) return B200_TRIMUL_E_SHAPE;
+      TRIMUL_CUDA(launch_overlapped(last, dim3((8 * p.team + 31) / 32, static_cast<unsigned>(groups)), 256, 0, stream, q));
+    }
+    return B200_TRIMUL_OK;
+  }
   const int smem = p.sums != nullptr ? g.teams * p.d * 4 : 0;
   TRIMUL_CUDA(launch_overlapped(wide ? join_backward_kernel<T, true> : join_backward_kernel<T, false>, dim3(g.blocks), g.team * g.teams, smem,
                                 stream, p));
@@ -370,9 +477,9 @@ int b200_block_join_forward(const void* x, const void* u, const void* gate, cons
     return B200_TRIMUL_E_ALIGN;
   const bool wide = d % 8 == 0 && all_aligned16({x, u, gate, y, h});
   const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  if (dtype == B200_BLOCKS_BF16) return launch_join_forward<__nv_bfloat16>(p, wide, info.sms, stream);
-  if (dtype == B200_BLOCKS_F16) return launch_join_forward<__half>(p, wide, info.sms, stream);
-  return launch_join_forward<float>(p, wide, info.sms, stream);
+  if (dtype == B200_BLOCKS_BF16) return launch_join_forward<__nv_bfloat16>(p, wide, info, stream);
+  if (dtype == B200_BLOCKS_F16) return launch_join_forward<__half>(p, wide, info, stream);
+  return launch_join_forward<float>(p, wide, info, stream);
 }
 
 int b200_block_join_workspace_bytes(long long rows, int d, long long gate_rows, size_t* out_bytes) {
@@ -382,7 +489,10 @@ int b200_block_join_workspace_bytes(long long rows, int d, long long gate_rows, 
   *out_bytes = join_sums_bytes(d);
   if (gate_rows > 1) {
     const int team = join_backward_team(d);
-    *out_bytes += static_cast<size_t>(kMaxSms) * (kJoinBackwardThreads / team) * 2 * 8 * team * 4;
+    // the kernels of join.cuh: two gate rows a team; on tiles: the gate rows that the blocks' rows touch (see launch_join_backward)
+    const size_t plain = static_cast<size_t>(kMaxSms) * (kJoinBackwardThreads / team) * 2 * 8 * team * 4;
+    const long long most = gate_rows >= kSharedGateRows ? 2 * (rows + kTileWarps * 32 + 16) / gate_rows + 3 * kMaxSms : 0;
+    *out_bytes += std::max(plain, static_cast<size_t>(most) * (kTileWarps * 32 / team) * 8 * team * 4);
   }
   return B200_TRIMUL_OK;
 }
@@ -456,9 +566,9 @@ int b200_block_join_backward(const void* dy, const void* dh, const void* x, cons
     if (!aligned(q, size)) return B200_TRIMUL_E_ALIGN;
   if (!aligned(post_stats, 8) || !aligned(pre_stats, 8)) return B200_TRIMUL_E_ALIGN;
   const bool wide = d % 8 == 0 && all_aligned16({x, u, gate, dy, dh, dx, du, dgate});
-  if (dtype == B200_BLOCKS_BF16) return launch_join_backward<__nv_bfloat16>(p, wide, g, sums, stream);
-  if (dtype == B200_BLOCKS_F16) return launch_join_backward<__half>(p, wide, g, sums, stream);
-  return launch_join_backward<float>(p, wide, g, sums, stream);
+  if (dtype == B200_BLOCKS_BF16) return launch_join_backward<__nv_bfloat16>(p, wide, g, sums, info, stream);
+  if (dtype == B200_BLOCKS_F16) return launch_join_backward<__half>(p, wide, g, sums, info, stream);
+  return launch_join_backward<float>(p, wide, g, sums, info, stream);
 }
 
 int b200_ff_workspace_bytes(long long rows, int d, int hidden, int weight_dtype, int backward, size_t* out_bytes) {
@@ -532,11 +642,11 @@ int b200_blocks_read_status(void* cuda_stream, int* code) {
   if (code == nullptr) return B200_TRIMUL_E_NULL;
   const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   *code = 0;
-  TRIMUL_CUDA(cudaMemcpyFromSymbolAsync(code, ff_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream));
+  TRIMUL_CUDA(cudaMemcpyFromSymbolAsync(code, blocks_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream));
   TRIMUL_CUDA(cudaStreamSynchronize(stream));
   if (*code != 0) {
     const int zero = 0;
-    TRIMUL_CUDA(cudaMemcpyToSymbolAsync(ff_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream));
+    TRIMUL_CUDA(cudaMemcpyToSymbolAsync(blocks_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream));
     TRIMUL_CUDA(cudaStreamSynchronize(stream));
   }
   return B200_TRIMUL_OK;

@@ -17,14 +17,13 @@
 // transposed. h, da and db are rounded to the type of x (saturating for fp16), each once, as operands of 16-bit products have to be.
 // The structure is the contraction's: persistent CTAs (pairs for large products: 256-row tiles, each CTA supplies its rows of the
 // first operand and half of the second), one warp loads through TMA, one issues the MMAs, the others are the epilogue of the tile
-// before. All waits are bounded; one that gives up leaves a code in ff_status.
+// before. All waits are bounded; one that gives up leaves a code in blocks_status.
 #pragma once
 
+#include "blocks_status.cuh"
 #include "ptx.cuh"
 
 namespace trimul {
-
-__device__ int ff_status;  // 0, or the code of the first wait that gave up (it stays until the host has read it)
 
 enum FfOp : int { kFfUp = 0, kFfDown = 1, kFfHidden = 2, kFfInput = 3, kFfWeights = 4 };
 enum FfAct : int { kFfSilu = 0, kFfGelu = 1 };
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
         const Tile t = tile_at(i);
         const int m0 = (t.m * G + static_cast<int>(rank)) * 128;
         for (int kb = t.kb0; kb < t.kb1; ++kb) {
-          if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, &ff_status, kDevTimeoutProducer)) {
+          if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, &blocks_status, kDevTimeoutProducer)) {
             ok = false;
             break;
           }
@@ -226,7 +225,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
           const long long t0 = clock64();
           while (!mbar_try_wait(full(s), ph)) {
             if (*abort_flag != 0 || clock64() - t0 > kWaitLimitCycles) {
-              atomicCAS(&ff_status, 0, kDevTimeoutDrain);
+              atomicCAS(&blocks_status, 0, kDevTimeoutDrain);
               break;
             }
           }
@@ -243,17 +242,17 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
       for (int i = first; ok && i < tiles; i += step, ++it) {
         const Tile t = tile_at(i);
         const int acc = it & 1;
-        if (!mbar_wait(acc_empty(acc), ((it >> 1) & 1) ^ 1u, abort_flag, &ff_status, kDevTimeoutMma)) break;
+        if (!mbar_wait(acc_empty(acc), ((it >> 1) & 1) ^ 1u, abort_flag, &blocks_status, kDevTimeoutMma)) break;
         tc_fence_after();
         for (int kb = t.kb0; kb < t.kb1; ++kb) {
           const bool second = SECOND && kb >= p.kb;
           if (OP == kFfHidden && kb == p.kb) {
-            if (!mbar_wait(ab_empty, (it & 1) ^ 1u, abort_flag, &ff_status, kDevTimeoutMma)) {
+            if (!mbar_wait(ab_empty, (it & 1) ^ 1u, abort_flag, &blocks_status, kDevTimeoutMma)) {
               ok = false;
               break;
             }
           }
-          if (!mbar_wait(full(s), ph, abort_flag, &ff_status, kDevTimeoutMma)) {
+          if (!mbar_wait(full(s), ph, abort_flag, &blocks_status, kDevTimeoutMma)) {
             ok = false;
             break;
           }
@@ -302,7 +301,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
       const int acc = it & 1;
       const int row = (t.m * G + static_cast<int>(rank)) * 128 + q * 32 + lane;
       const bool in = row < p.rows;
-      if (!mbar_wait_warp(acc_full(acc), (it >> 1) & 1, abort_flag, &ff_status, kDevTimeoutEpilogue)) break;
+      if (!mbar_wait_warp(acc_full(acc), (it >> 1) & 1, abort_flag, &blocks_status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
       auto release = [&](uint32_t bar) {
         tc_fence_before();
