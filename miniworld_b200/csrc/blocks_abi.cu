@@ -73,7 +73,7 @@ static bool all_aligned16(std::initializer_list<const void*> ps) {
 // Tiles of a call (see join_tiles.cuh): rows to a tile, stages and their places. False where the tensors do not start on 16 bytes
 // or a row takes more warps than there are or two stages do not fit: the kernels of join.cuh
 // then run. As many rows to a tile as the block works on at a time, fewer where that would leave SMs without one.
-static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count, int size, int nv, int params, int blocks_most) {
+static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count, int size, int nv, int params, int blocks_most, int smem) {
   for (int i = 0; i < count; ++i)
     if (!aligned(tensors[i], 16)) return false;
   const JoinParams& j = p->j;
@@ -87,7 +87,7 @@ static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count,
   const int fixed = params * p->params * 4 + kTileScratch;
   while (true) {
     p->slot = static_cast<int>(up(static_cast<size_t>(rows) * j.d * size, 128));
-    p->stages = std::min(kTileMaxStages, (kTileSmem - fixed) / (p->slot * p->slots));
+    p->stages = std::min(kTileMaxStages, (smem - fixed) / (p->slot * p->slots));
     if (p->stages >= 2) break;
     if (rows <= unit) return false;
     rows = static_cast<long long>(up(static_cast<size_t>(rows / 2), unit));
@@ -101,15 +101,16 @@ static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count,
 }
 static int tile_smem(const JoinTileParams& p, int params) {
   // (the backward's sums pass through the stages)
-  return params * p.params * 4 + kTileScratch + std::max(p.stages * p.slots * p.slot, kTileWarps * 32 * 8 * 4);  // (at most kTileSmem)
+  return params * p.params * 4 + kTileScratch + std::max(p.stages * p.slots * p.slot, params == 3 ? kTileWarps * 32 * 8 * 4 : 0);
 }
-template <typename T, int VEC>
-static auto tile_forward_kernel(int nv) {
+using TileKernel = void (*)(JoinTileParams);
+template <typename T, int VEC, bool EXACT>
+static TileKernel tile_forward_kernel(int nv) {
   switch (nv) {
-    case 1: return join_tile_forward_kernel<T, VEC, 1>;
-    case 2: return join_tile_forward_kernel<T, VEC, 2>;
-    case 3: return join_tile_forward_kernel<T, VEC, 3>;
-    default: return join_tile_forward_kernel<T, VEC, 4>;
+    case 1: return join_tile_forward_kernel<T, VEC, 1, EXACT>;
+    case 2: return join_tile_forward_kernel<T, VEC, 2, EXACT>;
+    case 3: return join_tile_forward_kernel<T, VEC, 3, EXACT>;
+    default: return join_tile_forward_kernel<T, VEC, 4, EXACT>;
   }
 }
 // elements of a row that a thread reads at once
@@ -129,13 +130,17 @@ static int launch_join_forward(const JoinParams& p0, bool wide, const DeviceInfo
   q.out_slot[1] = p0.h != nullptr ? (p0.u != nullptr ? 1 : 0) : -1;
   q.out_slot[2] = -1;
   const void* tensors[] = {p0.x, p0.u, q.slot_of[2] >= 0 ? p0.gate : nullptr, p0.y, p0.h};
-  if (plan_tiles(&q, tensors, 5, sizeof(T), s.nv, 4, info.sms)) {
+  const int per_sm = s.nv == 1 ? 2 : 1;
+  if (plan_tiles(&q, tensors, 5, sizeof(T), s.nv, 4, per_sm * info.sms, per_sm == 2 ? kTileSmemHalf : kTileSmem)) {
     const int vec = join_vec(p0.d);
-    auto kernel = vec == 8 ? tile_forward_kernel<T, 8>(s.nv) : vec == 2 ? tile_forward_kernel<T, 2>(s.nv) : tile_forward_kernel<T, 1>(s.nv);
+    const TileKernel kernel = p0.d == 8 * s.nv * s.team ? tile_forward_kernel<T, 8, true>(s.nv)
+                              : vec == 8                ? tile_forward_kernel<T, 8, false>(s.nv)
+                              : vec == 2                ? tile_forward_kernel<T, 2, false>(s.nv)
+                                                        : tile_forward_kernel<T, 1, false>(s.nv);
     const int rc = set_smem(kernel, kTileSmem, info.device);
     if (rc != 0) return rc;
     const int threads = kTileWarps * 32 / s.team * s.team + 32;
-    TRIMUL_CUDA(launch_overlapped(kernel, dim3(std::min(info.sms, q.tiles)), threads, tile_smem(q, 4), stream, q));
+    TRIMUL_CUDA(launch_overlapped(kernel, dim3(std::min(per_sm * info.sms, q.tiles)), threads, tile_smem(q, 4), stream, q));
     return B200_TRIMUL_OK;
   }
   JoinParams p = p0;
@@ -170,14 +175,17 @@ static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& 
   q.out_slot[1] = p.du != nullptr ? q.slot_of[1] : -1;
   q.out_slot[2] = p.dgate != nullptr && !shared_gate ? q.slot_of[2] : -1;
   const void* tensors[] = {p.x, p.u, q.slot_of[2] >= 0 ? p.gate : nullptr, p.dy, p.dh, p.dx, p.du, q.out_slot[2] >= 0 ? p.dgate : nullptr};
-  if (q.slots > 0 && (!shared_gate || p.gate_rows >= kSharedGateRows) && plan_tiles(&q, tensors, 8, sizeof(T), 1, 3, std::min(info.sms, kMaxSms))) {
+  if (q.slots > 0 && (!shared_gate || p.gate_rows >= kSharedGateRows) && plan_tiles(&q, tensors, 8, sizeof(T), 1, 3, std::min(info.sms, kMaxSms), kTileSmem)) {
     int blocks = std::min(std::min(info.sms, kMaxSms), q.tiles);
     if (shared_gate) {
       q.block_tiles = (q.tiles + blocks - 1) / blocks;
       q.group_slots = static_cast<int>(static_cast<long long>(q.block_tiles) * q.tile_rows / p.gate_rows) + 2;
     }
     const int vec = join_vec(p.d);
-    auto kernel = vec == 8 ? join_tile_backward_kernel<T, 8> : vec == 2 ? join_tile_backward_kernel<T, 2> : join_tile_backward_kernel<T, 1>;
+    const TileKernel kernel = p.d == 8 * p.team ? join_tile_backward_kernel<T, 8, true>
+                              : vec == 8        ? join_tile_backward_kernel<T, 8, false>
+                              : vec == 2        ? join_tile_backward_kernel<T, 2, false>
+                                                : join_tile_backward_kernel<T, 1, false>;
     const int rc = set_smem(kernel, kTileSmem, info.device);
     if (rc != 0) return rc;
     const int threads = kTileWarps * 32 / p.team * p.team + 32;

@@ -20,7 +20,8 @@ namespace trimul {
 constexpr int kTileWarps = 15;                         // warps that compute (with the copying one four to a scheduler: 128 registers)
 constexpr int kTileThreads = kTileWarps * 32 + 32;     // ... and the one that copies
 constexpr int kTileMaxStages = 8;
-constexpr int kTileSmem = 224 * 1024;                  // of the 227 KB a block may have
+constexpr int kTileSmem = 224 * 1024;                  // of the 227 KB a block may have (the 228 KB of an SM)
+constexpr int kTileSmemHalf = 112 * 1024;              // two blocks an SM: forward, eight elements of a row a thread
 
 struct JoinTileParams {
   JoinParams j;
@@ -66,15 +67,15 @@ __device__ __forceinline__ void tile_params(const float* w, int params, int t, i
   }
 }
 
-// A row's elements of this thread from a stage; zero past the width
-template <typename T, int VEC, int NV>
+// A row's elements of this thread from a stage; zero past the width (EXACT: there is nothing past it, 8 NV elements of every thread are there)
+template <typename T, int VEC, int NV, bool EXACT>
 __device__ __forceinline__ void tile_load(const uint8_t* row, int d, int t, int team, float2 (&v)[4 * NV]) {
   const T* p = reinterpret_cast<const T*>(row);
   if constexpr (VEC == 8) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * team + t) * 8;
-      if (c < d) {
+      if (EXACT || c < d) {
         if constexpr (sizeof(T) == 2) {
           const uint4 w = *reinterpret_cast<const uint4*>(p + c);
           v[4 * j] = Io<T>::two(w.x);
@@ -113,14 +114,14 @@ __device__ __forceinline__ void tile_load(const uint8_t* row, int d, int t, int 
     }
   }
 }
-template <typename T, int VEC, int NV>
+template <typename T, int VEC, int NV, bool EXACT>
 __device__ __forceinline__ void tile_store(uint8_t* row, int d, int t, int team, const float2 (&v)[4 * NV]) {
   T* p = reinterpret_cast<T*>(row);
   if constexpr (VEC == 8) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * team + t) * 8;
-      if (c >= d) continue;
+      if (!EXACT && c >= d) continue;
       if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<uint4*>(p + c) = make_uint4(Io<T>::pack(v[4 * j].x, v[4 * j].y), Io<T>::pack(v[4 * j + 1].x, v[4 * j + 1].y),
                                                       Io<T>::pack(v[4 * j + 2].x, v[4 * j + 2].y), Io<T>::pack(v[4 * j + 3].x, v[4 * j + 3].y));
@@ -164,8 +165,23 @@ __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t byt
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
 }
 
+__device__ __forceinline__ float exp2f_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 sigmoid2(float2 g) { return make_float2(sigmoid_fast(g.x), sigmoid_fast(g.y)); }
+// 1 / (1 + 2^(-g log2 e)), two at a time
+__device__ __forceinline__ float2 sigmoid2(float2 g) {
+  const float2 n = __fmul2_rn(g, f2(-1.44269504f));
+  const float2 e = __fadd2_rn(make_float2(exp2f_fast(n.x), exp2f_fast(n.y)), f2(1.f));
+  return make_float2(reciprocal_fast(e.x), reciprocal_fast(e.y));
+}
 
 // What both directions share: barriers, the ring, the copying warp
 template <typename T>
@@ -256,54 +272,113 @@ struct TileRing {
   }
 };
 
-// Sums of two values over a team; as TeamSum
+// Sums over a team, the same bits in every thread (as TeamSum, the steps unrolled)
 struct TileSum {
   float2* scratch;
-  int warps, id, half, warp_in_team;
-  __device__ __forceinline__ float2 operator()(float2 v, int team) {
-    const int width = team < 32 ? team : 32;
-    for (int o = width >> 1; o > 0; o >>= 1) {
+  int team, warps, id, half, warp_in_team;
+  template <typename F>
+  __device__ __forceinline__ void steps(F f) const {
+    if (team >= 32) f(16);
+    if (team >= 16) f(8);
+    if (team >= 8) f(4);
+    if (team >= 4) f(2);
+    if (team >= 2) f(1);
+  }
+  // every warp's value in shared memory, ready to be read
+  __device__ __forceinline__ const float2* exchange(float2 v) {
+    float2* s = scratch + half * 16;
+    half ^= 1;
+    if ((threadIdx.x & 31) == 0) s[warp_in_team] = v;
+    named_bar_sync(1 + id, team);
+    return s;
+  }
+  __device__ __forceinline__ float one(float v) {
+    steps([&](int o) { v += __shfl_xor_sync(0xFFFFFFFFu, v, o); });
+    if (warps > 1) {
+      const float2* s = exchange(make_float2(v, 0.f));
+      v = 0.f;
+      for (int i = 0; i < warps; ++i) v += s[i].x;
+    }
+    return v;
+  }
+  __device__ __forceinline__ float2 two(float2 v) {
+    steps([&](int o) {
       const float a = __shfl_xor_sync(0xFFFFFFFFu, v.x, o), b = __shfl_xor_sync(0xFFFFFFFFu, v.y, o);
       v = __fadd2_rn(v, make_float2(a, b));
-    }
+    });
     if (warps > 1) {
-      float2* s = scratch + half * 16;
-      half ^= 1;
-      if ((threadIdx.x & 31) == 0) s[warp_in_team] = v;
-      named_bar_sync(1 + id, team);
+      const float2* s = exchange(v);
       v = f2(0.f);
       for (int i = 0; i < warps; ++i) v = __fadd2_rn(v, s[i]);
     }
     return v;
   }
+  // Mean and sum of squared deviations of a row from those of each thread's `n` values, merged pairwise (the deviations of two
+  // equal parts add (difference of the means)^2 n / 2): one exchange instead of one for the mean and one for the deviations
+  __device__ __forceinline__ float2 merge(float mean, float dev, float n) {
+    steps([&](int o) {
+      const float m = __shfl_xor_sync(0xFFFFFFFFu, mean, o), q = __shfl_xor_sync(0xFFFFFFFFu, dev, o);
+      const float delta = m - mean;
+      mean = 0.5f * (mean + m);
+      dev = fmaf(delta * delta, 0.5f * n, dev + q);
+      n += n;
+    });
+    if (warps > 1) {
+      const float2* s = exchange(make_float2(mean, dev));
+      mean = dev = 0.f;
+      for (int i = 0; i < warps; ++i) mean += s[i].x;
+      mean = __fdividef(mean, static_cast<float>(warps));
+      for (int i = 0; i < warps; ++i) {
+        const float delta = s[i].x - mean;
+        dev += fmaf(delta * delta, n, s[i].y);
+      }
+    }
+    return make_float2(mean, dev);
+  }
 };
 
-template <int VEC, int NV>
+// mean and 1 / sigma of a row
+template <int VEC, int NV, bool EXACT>
 __device__ __forceinline__ float2 tile_stats(const float2 (&v)[4 * NV], int kind, float eps, int d, float inv, int t, int team, TileSum& sum) {
-  float mean = 0.f;
-  if (kind == kNormLayer) {
-    float2 a = f2(0.f);
+  float mean = 0.f, dev;
+  if (EXACT && kind == kNormLayer) {
+    float2 a = v[0], q = f2(0.f);
 #pragma unroll
-    for (int i = 0; i < 4 * NV; ++i) a = __fadd2_rn(a, v[i]);
-    mean = sum(make_float2(a.x + a.y, 0.f), team).x * inv;
-  }
-  float2 q = f2(0.f);
+    for (int i = 1; i < 4 * NV; ++i) a = __fadd2_rn(a, v[i]);
+    mean = (a.x + a.y) * (1.0f / (8 * NV));
 #pragma unroll
-  for (int i = 0; i < 4 * NV; ++i) {
-    float2 c = __fadd2_rn(v[i], f2(-mean));
-    if (tile_col<VEC>(2 * i, t, team) >= d) c.x = 0.f;
-    if (tile_col<VEC>(2 * i + 1, t, team) >= d) c.y = 0.f;
-    q = __ffma2_rn(c, c, q);
+    for (int i = 0; i < 4 * NV; ++i) {
+      const float2 c = __fadd2_rn(v[i], f2(-mean));
+      q = __ffma2_rn(c, c, q);
+    }
+    const float2 all = sum.merge(mean, q.x + q.y, 8 * NV);
+    mean = all.x;
+    dev = all.y;
+  } else {
+    if (kind == kNormLayer) {
+      float2 a = f2(0.f);
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) a = __fadd2_rn(a, v[i]);
+      mean = sum.one(a.x + a.y) * inv;
+    }
+    float2 q = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) {
+      float2 c = __fadd2_rn(v[i], f2(-mean));
+      if (!EXACT && tile_col<VEC>(2 * i, t, team) >= d) c.x = 0.f;
+      if (!EXACT && tile_col<VEC>(2 * i + 1, t, team) >= d) c.y = 0.f;
+      q = __ffma2_rn(c, c, q);
+    }
+    dev = sum.one(q.x + q.y);
   }
-  const float var = sum(make_float2(q.x + q.y, 0.f), team).x * inv;
-  return make_float2(mean, 1.0f / sqrtf(var + eps));
+  return make_float2(mean, rsqrtf(fmaf(dev, inv, eps)));
 }
 
 // Shared memory: parameters | scratch of the sums | barriers | stages
 constexpr int kTileScratch = 8 * 32 * 8 + 2 * kTileMaxStages * 8 + 16;
 
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(kTileThreads, 1) join_tile_forward_kernel(const JoinTileParams p) {
+template <typename T, int VEC, int NV, bool EXACT>
+__global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forward_kernel(const JoinTileParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   float* par = reinterpret_cast<float*>(smem);  // w_s, b_s, w_pre, b_pre
   uint8_t* at = smem + 4 * p.params * 4;
@@ -341,33 +416,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_forward_kernel(cons
     return;
   }
   const int d = j.d, team = j.team, t = threadIdx.x % team, id = threadIdx.x / team, teams = workers / team;
-  TileSum sum{scratch + (team > 32 ? id : 0) * 32, (team + 31) / 32, id, 0, t >> 5};
+  TileSum sum{scratch + (team > 32 ? id : 0) * 32, team, (team + 31) / 32, id, 0, t >> 5};
   const float inv = 1.0f / static_cast<float>(d);
-  const size_t row_bytes = static_cast<size_t>(d) * sizeof(T);
+  const int row_bytes = d * static_cast<int>(sizeof(T));
   const int n = ring.count();
   for (int k = 0; k < n; ++k) {
     const int s = k % p.stages;
     if (!mbar_wait_warp(ring.full(s), (k / p.stages) & 1, abort_flag, &blocks_status, kDevTimeoutStats)) break;
     uint8_t* stage = ring.stage(s);
+    const long long r0 = static_cast<long long>(ring.first() + k * ring.step()) * p.tile_rows;
+    const int rows = j.rows - r0 < p.tile_rows ? static_cast<int>(j.rows - r0) : p.tile_rows;
     for (int r = id; r - id < p.tile_rows; r += teams) {
-      const long long row = static_cast<long long>(ring.first() + k * ring.step()) * p.tile_rows + r;
-      const bool on = r < p.tile_rows && row < j.rows;
-      const size_t off = on ? r * row_bytes : 0;
+      const long long row = r0 + r;
+      const bool on = r < rows;
+      const int off = on ? r * row_bytes : 0;
       float2 x[4 * NV], w[4 * NV];
-      tile_load<T, VEC, NV>(stage + p.slot_of[0] * p.slot + off, d, t, team, x);
+      tile_load<T, VEC, NV, EXACT>(stage + p.slot_of[0] * p.slot + off, d, t, team, x);
       if (j.u != nullptr) {
         const bool valid = on && (j.mask == nullptr || __ldcg(j.mask + row) != 0);
         float2 u[4 * NV];
-        tile_load<T, VEC, NV>(stage + p.slot_of[1] * p.slot + off, d, t, team, u);
+        tile_load<T, VEC, NV, EXACT>(stage + p.slot_of[1] * p.slot + off, d, t, team, u);
         if (j.post_kind != kNormNone) {
-          const float2 st = tile_stats<VEC, NV>(u, j.post_kind, j.post_eps, d, inv, t, team, sum);
+          const float2 st = tile_stats<VEC, NV, EXACT>(u, j.post_kind, j.post_eps, d, inv, t, team, sum);
           if (on && t == 0 && j.post_stats != nullptr) j.post_stats[row] = st;
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) u[i] = __fmul2_rn(__fadd2_rn(u[i], f2(-st.x)), f2(st.y));
         }
-        tile_params<VEC, NV>(par, p.params, t, team, w);
+        if (j.post_w != nullptr || j.scale != nullptr) {
+          tile_params<VEC, NV>(par, p.params, t, team, w);
 #pragma unroll
-        for (int i = 0; i < 4 * NV; ++i) u[i] = __fmul2_rn(u[i], w[i]);
+          for (int i = 0; i < 4 * NV; ++i) u[i] = __fmul2_rn(u[i], w[i]);
+        }
         if (j.post_b != nullptr) {
           tile_params<VEC, NV>(par + p.params, p.params, t, team, w);
 #pragma unroll
@@ -375,7 +454,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_forward_kernel(cons
         }
         if (j.gate != nullptr) {
           if (p.slot_of[2] >= 0) {
-            tile_load<T, VEC, NV>(stage + p.slot_of[2] * p.slot + off, d, t, team, w);
+            tile_load<T, VEC, NV, EXACT>(stage + p.slot_of[2] * p.slot + off, d, t, team, w);
           } else {
             const long long g = on ? row / j.gate_rows : 0;
 #pragma unroll
@@ -388,10 +467,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_forward_kernel(cons
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) x[i] = __fadd2_rn(x[i], u[i]);
         }
-        if (on) tile_store<T, VEC, NV>(stage + p.out_slot[0] * p.slot + off, d, t, team, x);
+        if (on) tile_store<T, VEC, NV, EXACT>(stage + p.out_slot[0] * p.slot + off, d, t, team, x);
       }
       if (j.pre_kind != kNormNone) {
-        const float2 st = tile_stats<VEC, NV>(x, j.pre_kind, j.pre_eps, d, inv, t, team, sum);
+        const float2 st = tile_stats<VEC, NV, EXACT>(x, j.pre_kind, j.pre_eps, d, inv, t, team, sum);
         if (on && t == 0 && j.pre_stats != nullptr) j.pre_stats[row] = st;
         tile_params<VEC, NV>(par + 2 * p.params, p.params, t, team, w);
 #pragma unroll
@@ -401,7 +480,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_forward_kernel(cons
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) x[i] = __fadd2_rn(x[i], w[i]);
         }
-        if (on) tile_store<T, VEC, NV>(stage + p.out_slot[1] * p.slot + off, d, t, team, x);
+        if (on) tile_store<T, VEC, NV, EXACT>(stage + p.out_slot[1] * p.slot + off, d, t, team, x);
       }
     }
     fence_proxy_async_smem();
@@ -413,7 +492,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_forward_kernel(cons
 // A shared gate's gradient: a team adds up its rows of the current gate row in registers and leaves them in fp32 when the gate row
 // changes, in a place of its own for each gate row that the block's tiles touch ([blocks][group_slots][teams][8 team]);
 // join_tile_gate_kernel adds them up in the order of the blocks and teams.
-template <typename T, int VEC>
+template <typename T, int VEC, bool EXACT>
 __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(const JoinTileParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   float* par = reinterpret_cast<float*>(smem);  // w_s, b_s, w_pre
@@ -454,9 +533,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
     void* const out[3] = {j.dx, j.du, j.dgate};
     ring.copy(in, out, lane);
   } else {
-    TileSum sum{scratch + (team > 32 ? id : 0) * 32, (team + 31) / 32, id, 0, t >> 5};
+    TileSum sum{scratch + (team > 32 ? id : 0) * 32, team, (team + 31) / 32, id, 0, t >> 5};
     const float inv = 1.0f / static_cast<float>(d);
-    const size_t row_bytes = static_cast<size_t>(d) * sizeof(T);
+    const int row_bytes = d * static_cast<int>(sizeof(T));
     const bool shared_gate = p.block_tiles != 0;
     float2 sg_sum[4];
 #pragma unroll
@@ -479,9 +558,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
       // (statistics and mask of the first round: asked for before the wait)
       float2 post = f2(0.f), pre = f2(0.f);
       bool valid = false;
+      const int rows = j.rows - r0 < p.tile_rows ? static_cast<int>(j.rows - r0) : p.tile_rows;
       auto row_facts = [&](int r) {
         const long long row = r0 + r;
-        const bool on = r < p.tile_rows && row < j.rows;
+        const bool on = r < rows;
         valid = j.u != nullptr && on && (j.mask == nullptr || __ldcg(j.mask + row) != 0);
         if (on && j.post_kind != kNormNone) post = __ldcg(j.post_stats + row);
         if (on && j.pre_kind != kNormNone) pre = __ldcg(j.pre_stats + row);
@@ -493,17 +573,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
       for (int r = id; r - id < p.tile_rows; r += teams) {
         if (r != id) on = row_facts(r);
         const long long row = r0 + r;
-        const size_t off = on ? r * row_bytes : 0;
+        const int off = on ? r * row_bytes : 0;
         float2 x[4], e[4], q[4], u[4], g[4], w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = e[i] = u[i] = f2(0.f), g[i] = f2(1.f);
-        if (j.pre_kind != kNormNone && on) tile_load<T, VEC, 1>(stage + p.slot_of[0] * p.slot + off, d, t, team, x);
-        if (j.dy != nullptr && on) tile_load<T, VEC, 1>(stage + p.slot_of[3] * p.slot + off, d, t, team, e);
+        if (j.pre_kind != kNormNone && on) tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[0] * p.slot + off, d, t, team, x);
+        if (j.dy != nullptr && on) tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[3] * p.slot + off, d, t, team, e);
         if (valid) {
-          tile_load<T, VEC, 1>(stage + p.slot_of[1] * p.slot + off, d, t, team, u);
+          tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[1] * p.slot + off, d, t, team, u);
           if (j.gate != nullptr) {
             if (!shared_gate) {
-              tile_load<T, VEC, 1>(stage + p.slot_of[2] * p.slot + off, d, t, team, g);
+              tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[2] * p.slot + off, d, t, team, g);
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i) tile_gate<T, VEC>(j.gate, row / j.gate_rows, d, t, team, i, g[i]);
@@ -529,7 +609,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
             }
           }
           if (j.dh != nullptr && on) {
-            tile_load<T, VEC, 1>(stage + p.slot_of[4] * p.slot + off, d, t, team, q);
+            tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[4] * p.slot + off, d, t, team, q);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) q[i] = f2(0.f);
@@ -545,12 +625,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
             c1 = __fadd2_rn(c1, q[i]);
             c2 = __ffma2_rn(q[i], x[i], c2);
           }
-          const float2 c = sum(make_float2(c1.x + c1.y, c2.x + c2.y), team);
+          const float2 c = sum.two(make_float2(c1.x + c1.y, c2.x + c2.y));
           const float m1 = j.pre_kind == kNormLayer ? -c.x * inv : 0.f, m2 = -c.y * inv;
 #pragma unroll
           for (int i = 0; i < 4; ++i) e[i] = __ffma2_rn(f2(pre.y), __ffma2_rn(x[i], f2(m2), __fadd2_rn(q[i], f2(m1))), e[i]);
         }
-        if (on && p.out_slot[0] >= 0) tile_store<T, VEC, 1>(stage + p.out_slot[0] * p.slot + off, d, t, team, e);
+        if (on && p.out_slot[0] >= 0) tile_store<T, VEC, 1, EXACT>(stage + p.out_slot[0] * p.slot + off, d, t, team, e);
         if (j.u == nullptr) continue;
         float2 a1 = f2(0.f), a2 = f2(0.f);
         tile_params<VEC, 1>(par, p.params, t, team, w);
@@ -576,7 +656,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
           for (int i = 0; i < 4; ++i)
             g[i] = __fmul2_rn(__fmul2_rn(e[i], __ffma2_rn(u[i], w[i], b[i])), __fadd2_rn(f2(1.f), make_float2(-g[i].x, -g[i].y)));
           if (!shared_gate) {
-            if (on) tile_store<T, VEC, 1>(stage + p.out_slot[2] * p.slot + off, d, t, team, g);
+            if (on) tile_store<T, VEC, 1, EXACT>(stage + p.out_slot[2] * p.slot + off, d, t, team, g);
           } else if (on) {
             const long long now = row / j.gate_rows;
             if (now != group) {
@@ -588,7 +668,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
           }
         }
         if (j.post_kind != kNormNone) {
-          const float2 c = sum(make_float2(a1.x + a1.y, a2.x + a2.y), team);
+          const float2 c = sum.two(make_float2(a1.x + a1.y, a2.x + a2.y));
           const float m1 = j.post_kind == kNormLayer ? -c.x * inv : 0.f, m2 = -c.y * inv;
 #pragma unroll
           for (int i = 0; i < 4; ++i) q[i] = __fmul2_rn(f2(post.y), __ffma2_rn(u[i], f2(m2), __fadd2_rn(q[i], f2(m1))));
@@ -597,7 +677,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
 #pragma unroll
           for (int i = 0; i < 4; ++i) q[i] = f2(0.f);
         }
-        if (on && p.out_slot[1] >= 0) tile_store<T, VEC, 1>(stage + p.out_slot[1] * p.slot + off, d, t, team, q);
+        if (on && p.out_slot[1] >= 0) tile_store<T, VEC, 1, EXACT>(stage + p.out_slot[1] * p.slot + off, d, t, team, q);
       }
       fence_proxy_async_smem();
       __syncwarp();
