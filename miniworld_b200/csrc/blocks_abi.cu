@@ -365,7 +365,11 @@ static int ff_weight_gradients(const FfProblem& f, const void* x, const void* dy
   if (rc == 0) rc = ff_map(&maps.b[1], dy, f.rows, f.d, f.d, 64);
   if (rc != 0) return rc;
   FfParams p = {};
-  p.partial = partial;
+  if (s.splits > 1) p.partial = partial;
+  p.out[0] = dw_a;
+  p.out[1] = dw_b;
+  p.out[2] = dw_s;
+  p.type = weight_dtype;
   p.rows = f.hidden;
   p.cols = f.d;
   p.m_tiles = s.m_tiles;
@@ -375,7 +379,7 @@ static int ff_weight_gradients(const FfProblem& f, const void* x, const void* dy
   p.splits = s.splits;
   p.kb_split = s.kb_split;
   rc = ff_launch<kFfWeights>(maps, p, s.pair, f.f16, f.info, f.stream);
-  if (rc != 0) return rc;
+  if (rc != 0 || s.splits == 1) return rc;
   FfReduce r = {};
   r.partial = partial;
   r.out[0] = dw_a;
@@ -385,7 +389,7 @@ static int ff_weight_gradients(const FfProblem& f, const void* x, const void* dy
   r.H = f.hidden;
   r.D = f.d;
   r.type = weight_dtype;
-  TRIMUL_CUDA(launch_overlapped(ff_reduce_kernel, dim3(blocks_of(f.d, 32), blocks_of(f.hidden, 32), 3), 256, 0, f.stream, r));
+  TRIMUL_CUDA(launch_overlapped(ff_reduce_kernel, dim3(blocks_of(f.d, 128), blocks_of(f.hidden, 32), 3), 256, 0, f.stream, r));
   return 0;
 }
 
@@ -410,7 +414,8 @@ static FfRegions ff_regions(long long rows, int d, int hidden, int weight_dtype,
     at += up(static_cast<size_t>(rows) * ff_ld(hidden) * 2, 1024);
   }
   r.partial = at;
-  if (backward) at += up(static_cast<size_t>(ff_split(rows, d, hidden, sms).splits) * 3 * hidden * d * 4, 1024);
+  const int splits = backward ? ff_split(rows, d, hidden, sms).splits : 0;
+  if (splits > 1) at += up(static_cast<size_t>(splits) * 3 * hidden * d * 4, 1024);
   r.total = at;
   return r;
 }

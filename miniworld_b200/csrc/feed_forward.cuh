@@ -34,8 +34,8 @@ struct FfMaps {
 };
 
 struct FfParams {
-  void* out[3];        // h | y | da, db, h | dx | (kFfWeights: not used)
-  float* partial;      // kFfWeights: [splits][3][rows][cols]
+  void* out[3];        // h | y | da, db, h | dx | dW_a, dW_b, dW_s (kFfWeights with one part; null: not asked for)
+  float* partial;      // kFfWeights with several: [splits][3][rows][cols]
   long long ld;        // elements from one row of `out` to the next
   int rows, cols;      // of the output
   int m_tiles, n_tiles;
@@ -43,11 +43,13 @@ struct FfParams {
   int bn;              // accumulator columns of an output tile (kFfUp and kFfHidden: of its a | b part)
   int splits, kb_split;  // kFfWeights: parts of the k range, k blocks of each
   int act;
+  int type;            // kFfWeights: of `out`, 0 bf16, 1 fp32, 2 fp16
 };
 
 constexpr int kFfStages = 6;
 constexpr int kFfStageBytes = 32768;  // 128 rows of the first operand, up to 128 of the second, 64 deep
-constexpr int kFfThreads = 64 + 256;
+constexpr int kFfEpilogueWarps = 16;
+constexpr int kFfThreads = 64 + 32 * kFfEpilogueWarps;
 constexpr int kFfSmemBytes = kFfStages * kFfStageBytes + 256 + 1024;
 
 template <bool F16>
@@ -67,6 +69,44 @@ __device__ __forceinline__ float2 ff_act_slope(float a, int act) {
   }
   const float cdf = 0.5f * (1.0f + erff(a * 0.70710678f));
   return make_float2(a * cdf, fmaf(a * 0.39894228f, __expf(-0.5f * a * a), cdf));
+}
+
+// 32 bytes in one request where the address allows: whole sectors of L2 (in halves a tile's stores took twice as long)
+__device__ __forceinline__ void ff_store32(void* p, const uint32_t (&w)[8]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 31u) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+__device__ __forceinline__ void ff_put(void* out, size_t i, float v, int type) {
+  if (type == 1)
+    static_cast<float*>(out)[i] = v;
+  else if (type == 0)
+    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+  else
+    static_cast<__half*>(out)[i] = __float2half_rn(v);
+}
+// 16 neighbours of a row, those before `left` (a multiple of 8)
+__device__ __forceinline__ void ff_put16(void* out, size_t i, const float (&v)[16], int left, int type) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 8) {
+    if (j >= left) break;
+    if (type == 1) {
+      uint32_t w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(v[j + k]);
+      ff_store32(static_cast<float*>(out) + i + j, w);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = type == 0 ? pack_bf16x2(v[j + 2 * k], v[j + 2 * k + 1]) : pack_f16x2(make_float2(v[j + 2 * k], v[j + 2 * k + 1]));
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + i + j) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
 }
 
 template <int OP, bool PAIR, bool F16>
@@ -102,9 +142,9 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full(a), 1);
-      mbar_init(acc_empty(a), 8 * G);
+      mbar_init(acc_empty(a), kFfEpilogueWarps * G);
     }
-    mbar_init(ab_empty, 8 * G);
+    mbar_init(ab_empty, kFfEpilogueWarps * G);
     *abort_flag = 0;
     fence_mbar_init();
     for (int i = 0; i < 3; ++i) {
@@ -292,8 +332,10 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue: a row per thread, half of the tile's columns per group
-    const int q = warp & 3, half = (warp - 2) >> 2;
+    // ------------------------------------------------------------ epilogue: a row per thread, a quarter of the tile's columns per
+    // group of four warps. All of a thread's accumulators are read at once and handed back before the arithmetic (kFfHidden: those
+    // of a and b, of which there is one set; dh has two).
+    const int q = warp & 3, part = (warp - 2) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     int it = 0;
     for (int i = first; i < tiles; i += step, ++it) {
@@ -313,84 +355,84 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
             mbar_arrive(bar);
         }
       };
-      // 8 neighbours of the output from 8 values
-      auto store8 = [&](void* out, int col, const float* v) {
-        if (in && col < p.cols)
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + static_cast<size_t>(row) * p.ld + col) =
-              make_uint4(ff_pack<F16>(v[0], v[1]), ff_pack<F16>(v[2], v[3]), ff_pack<F16>(v[4], v[5]), ff_pack<F16>(v[6], v[7]));
+      // 16 neighbours of a row of the output (multiples of 8 of them within the width)
+      auto store16 = [&](void* out, int col, const float (&v)[16]) {
+        if (!in || col >= p.cols) return;
+        uint16_t* o = static_cast<uint16_t*>(out) + static_cast<size_t>(row) * p.ld + col;
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = ff_pack<F16>(v[2 * j], v[2 * j + 1]);
+        if (col + 16 <= p.cols)
+          ff_store32(o, w);
+        else
+          *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
       };
       const uint32_t d = tmem + lanes + kAcc0 + acc * kAcc;
-      if constexpr (OP == kFfUp) {
-        constexpr int N = kUnits / 2;
-#pragma unroll 1
-        for (int c = 0; c < N; c += 16) {
-          uint32_t va[16], vb[16];
-          tmem_ld16(d + half * N + c, va);
-          tmem_ld16(d + kUnits + half * N + c, vb);
-          tmem_ld_wait();
-          if (c + 16 == N) release(acc_empty(acc));
-          float v[16];
+      if constexpr (OP == kFfUp || OP == kFfHidden) {
+        constexpr int N = kUnits / 4;
+        const uint32_t ab = (OP == kFfUp ? d : tmem + lanes) + part * N;
+        uint32_t va[N / 16][16], vb[N / 16][16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = ff_act(__uint_as_float(va[j]), p.act) * __uint_as_float(vb[j]);
-          const int col = t.n * kUnits + half * N + c;
-          store8(p.out[0], col, v);
-          store8(p.out[0], col + 8, v + 8);
+        for (int c = 0; c < N / 16; ++c) {
+          tmem_ld16(ab + c * 16, va[c]);
+          tmem_ld16(ab + kUnits + c * 16, vb[c]);
         }
-      } else if constexpr (OP == kFfHidden) {
-        constexpr int N = kUnits / 2;
-#pragma unroll 1
-        for (int c = 0; c < N; c += 16) {
-          uint32_t va[16], vb[16], vd[16];
-          tmem_ld16(tmem + lanes + half * N + c, va);
-          tmem_ld16(tmem + lanes + kUnits + half * N + c, vb);
-          tmem_ld16(d + half * N + c, vd);
-          tmem_ld_wait();
-          if (c + 16 == N) {
-            release(ab_empty);
-            if (lane == 0) {
-              if constexpr (PAIR)
-                mbar_arrive_leader(acc_empty(acc), rank);
-              else
-                mbar_arrive(acc_empty(acc));
+        tmem_ld_wait();
+        release(OP == kFfUp ? acc_empty(acc) : ab_empty);
+#pragma unroll
+        for (int c = 0; c < N / 16; ++c) {
+          const int col = t.n * kUnits + part * N + c * 16;
+          if constexpr (OP == kFfUp) {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = ff_act(__uint_as_float(va[c][j]), p.act) * __uint_as_float(vb[c][j]);
+            store16(p.out[0], col, v);
+          } else {
+            uint32_t vd[16];
+            tmem_ld16(d + part * N + c * 16, vd);
+            tmem_ld_wait();
+            if (c == N / 16 - 1) release(acc_empty(acc));
+            float da[16], db[16], h[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float b = __uint_as_float(vb[c][j]), dh = __uint_as_float(vd[j]);
+              const float2 f = ff_act_slope(__uint_as_float(va[c][j]), p.act);
+              da[j] = dh * b * f.y;
+              db[j] = dh * f.x;
+              h[j] = f.x * b;
             }
-          }
-          const int col = t.n * kUnits + half * N + c;
-          float da[16], db[16], h[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float b = __uint_as_float(vb[j]), dh = __uint_as_float(vd[j]);
-            const float2 f = ff_act_slope(__uint_as_float(va[j]), p.act);
-            da[j] = dh * b * f.y;
-            db[j] = dh * f.x;
-            h[j] = f.x * b;
-          }
-#pragma unroll
-          for (int j = 0; j < 16; j += 8) {
-            store8(p.out[0], col + j, da + j);
-            store8(p.out[1], col + j, db + j);
-            store8(p.out[2], col + j, h + j);
+            store16(p.out[0], col, da);
+            store16(p.out[1], col, db);
+            store16(p.out[2], col, h);
           }
         }
       } else {
-        const int n = p.bn / 2;
+        const int n = p.bn / 4;
 #pragma unroll 1
         for (int c = 0; c < n; c += 16) {
           uint32_t v[16];
-          tmem_ld16(d + half * n + c, v);
+          tmem_ld16(d + part * n + c, v);
           tmem_ld_wait();
           if (c + 16 >= n) release(acc_empty(acc));
-          const int col = t.n * p.bn + half * n + c;
+          const int col = t.n * p.bn + part * n + c;
           float f[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]);
           if constexpr (OP != kFfWeights) {
-            store8(p.out[0], col, f);
-            store8(p.out[0], col + 8, f + 8);
-          } else if (in) {
-            float* o = p.partial + ((static_cast<size_t>(t.split) * 3 + t.product) * p.rows + row) * p.cols + col;
+            store16(p.out[0], col, f);
+          } else if (in && col < p.cols) {
+            const int left = p.cols - col;
+            if (p.partial != nullptr) {
+              ff_put16(p.partial, ((static_cast<size_t>(t.split) * 3 + t.product) * p.rows + row) * p.cols + col, f, left, 1);
+            } else if (void* const o = t.product == 0 ? p.out[0] : t.product == 1 ? p.out[1] : p.out[2]; o != nullptr) {
+              if (t.product < 2) {
+                ff_put16(o, static_cast<size_t>(row) * p.cols + col, f, left, p.type);
+              } else {  // dW_s [D, H]: neighbouring lanes are neighbours in memory
 #pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              if (col + j < p.cols) *reinterpret_cast<float4*>(o + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+                for (int j = 0; j < 16; ++j)
+                  if (j < left) ff_put(o, static_cast<size_t>(col + j) * p.rows + row, f[j], p.type);
+              }
+            }
           }
         }
       }
@@ -411,44 +453,63 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
 }
 
 // Sums the parts of the weight gradients in the order of the rows and rounds once: dW_a, dW_b [H, D] as they lie, dW_s [D, H] from
-// its transpose (through shared memory). A block takes 32 x 32 values of one product.
+// its transpose (through shared memory). A block takes 32 x 128 values of one product.
 struct FfReduce {
   const float* partial;  // [splits][3][H][D]
   void* out[3];
   int splits, H, D;
   int type;  // 0 bf16, 1 fp32, 2 fp16
 };
-__device__ __forceinline__ void ff_put(void* out, size_t i, float v, int type) {
-  if (type == 1)
-    static_cast<float*>(out)[i] = v;
-  else if (type == 0)
-    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
-  else
-    static_cast<__half*>(out)[i] = __float2half_rn(v);
-}
 __global__ void __launch_bounds__(256) ff_reduce_kernel(const FfReduce p) {
-  __shared__ float tile[32][33];
+  __shared__ float tile[32][129];
   grid_dependency_wait();
   grid_dependents_launch();
-  void* out = p.out[blockIdx.z];
+  void* out = blockIdx.z == 0 ? p.out[0] : blockIdx.z == 1 ? p.out[1] : p.out[2];
   if (out == nullptr) return;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + tx;
+  const int c = blockIdx.x * 128 + tx * 4;
   const size_t part = static_cast<size_t>(3) * p.H * p.D;
-  for (int j = ty; j < 32; j += 8) {
-    const int r = blockIdx.y * 32 + j;
-    float a = 0.f;
-    if (r < p.H && c < p.D) {
-      const float* s = p.partial + (static_cast<size_t>(blockIdx.z) * p.H + r) * p.D + c;
-      for (int k = 0; k < p.splits; ++k) a += __ldcg(s + k * part);
-      if (blockIdx.z < 2) ff_put(out, static_cast<size_t>(r) * p.D + c, a, p.type);
+  float4 a[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < p.splits; ++k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = blockIdx.y * 32 + ty + 8 * j;
+      if (r >= p.H || c >= p.D) continue;
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partial + k * part + (static_cast<size_t>(blockIdx.z) * p.H + r) * p.D + c));
+      a[j].x += v.x;
+      a[j].y += v.y;
+      a[j].z += v.z;
+      a[j].w += v.w;
     }
-    tile[j][tx] = a;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = blockIdx.y * 32 + ty + 8 * j;
+    if (blockIdx.z < 2) {
+      if (r >= p.H || c >= p.D) continue;
+      const size_t i = static_cast<size_t>(r) * p.D + c;
+      if (p.type == 1)
+        reinterpret_cast<float4*>(static_cast<float*>(out) + i)[0] = a[j];
+      else if (p.type == 0)
+        reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i)[0] = make_uint2(pack_bf16x2(a[j].x, a[j].y), pack_bf16x2(a[j].z, a[j].w));
+      else
+        reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i)[0] =
+            make_uint2(pack_f16x2(make_float2(a[j].x, a[j].y)), pack_f16x2(make_float2(a[j].z, a[j].w)));
+    } else {
+      float* s = &tile[ty + 8 * j][tx * 4];
+      s[0] = a[j].x;
+      s[1] = a[j].y;
+      s[2] = a[j].z;
+      s[3] = a[j].w;
+    }
   }
   if (blockIdx.z < 2) return;
   __syncthreads();
-  for (int j = ty; j < 32; j += 8) {
-    const int d = blockIdx.x * 32 + j, h = blockIdx.y * 32 + tx;
+  const int h = blockIdx.y * 32 + tx;
+  for (int j = ty; j < 128; j += 8) {
+    const int d = blockIdx.x * 128 + j;
     if (d < p.D && h < p.H) ff_put(out, static_cast<size_t>(d) * p.H + h, tile[tx][j], p.type);
   }
 }
