@@ -236,9 +236,19 @@ static int ff_map(CUtensorMap* m, const void* base, long long rows, int cols, lo
   return make_map(m, base, 2, dims, strides, b);
 }
 
-template <int OP, bool PAIR, bool F16>
+struct FfProblem {
+  long long rows;
+  int d, hidden, ld;
+  bool f16;
+  int act;
+  const void *w_a, *w_b, *w_s;  // operands, in the type of x
+  DeviceInfo info;
+  cudaStream_t stream;
+};
+
+template <int OP, bool PAIR, bool F16, int ACT>
 static int ff_launch_kernel(const FfMaps& maps, const FfParams& p, const DeviceInfo& info, cudaStream_t stream) {
-  const int rc = set_smem(ff_kernel<OP, PAIR, F16>, kFfSmemBytes, info.device);
+  const int rc = set_smem(ff_kernel<OP, PAIR, F16, ACT>, kFfSmemBytes, info.device);
   if (rc != B200_TRIMUL_OK) return rc;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * p.splits * (OP == kFfWeights ? 3 : 1);
   const int units = PAIR ? info.sms / 2 : info.sms;
@@ -255,29 +265,25 @@ static int ff_launch_kernel(const FfMaps& maps, const FfParams& p, const DeviceI
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  TRIMUL_CUDA(cudaLaunchKernelEx(&cfg, ff_kernel<OP, PAIR, F16>, maps, p));
+  TRIMUL_CUDA(cudaLaunchKernelEx(&cfg, ff_kernel<OP, PAIR, F16, ACT>, maps, p));
   return B200_TRIMUL_OK;
 }
+template <int OP, bool PAIR, bool F16>
+static int ff_launch_act(const FfMaps& maps, const FfParams& p, int act, const DeviceInfo& info, cudaStream_t stream) {
+  if constexpr (OP == kFfUp || OP == kFfHidden)
+    if (act == kFfGelu) return ff_launch_kernel<OP, PAIR, F16, kFfGelu>(maps, p, info, stream);
+  return ff_launch_kernel<OP, PAIR, F16, kFfSilu>(maps, p, info, stream);
+}
 template <int OP>
-static int ff_launch(const FfMaps& maps, const FfParams& p, bool pair, bool f16, const DeviceInfo& info, cudaStream_t stream) {
-  if (pair) return f16 ? ff_launch_kernel<OP, true, true>(maps, p, info, stream) : ff_launch_kernel<OP, true, false>(maps, p, info, stream);
-  return f16 ? ff_launch_kernel<OP, false, true>(maps, p, info, stream) : ff_launch_kernel<OP, false, false>(maps, p, info, stream);
+static int ff_launch(const FfMaps& maps, const FfParams& p, bool pair, const FfProblem& f) {
+  if (pair) return f.f16 ? ff_launch_act<OP, true, true>(maps, p, f.act, f.info, f.stream) : ff_launch_act<OP, true, false>(maps, p, f.act, f.info, f.stream);
+  return f.f16 ? ff_launch_act<OP, false, true>(maps, p, f.act, f.info, f.stream) : ff_launch_act<OP, false, false>(maps, p, f.act, f.info, f.stream);
 }
 
 static int blocks_of(long long n, int b) { return static_cast<int>((n + b - 1) / b); }
 
 // CTA pairs where their 256-row tiles still occupy most of the GPU, single CTAs below
 static bool ff_pair(long long rows, long long n_tiles, int sms) { return rows > 128 && blocks_of(rows, 256) * n_tiles >= sms / 2 * 3 / 4; }
-
-struct FfProblem {
-  long long rows;
-  int d, hidden, ld;
-  bool f16;
-  int act;
-  const void *w_a, *w_b, *w_s;  // operands, in the type of x
-  DeviceInfo info;
-  cudaStream_t stream;
-};
 
 // h = act(x W_a^T) * (x W_b^T), or with dy the backward's da, db, h
 static int ff_hidden(const FfProblem& f, const void* x, const void* dy, void* const out[3]) {
@@ -300,8 +306,7 @@ static int ff_hidden(const FfProblem& f, const void* x, const void* dy, void* co
   p.kb = p.kb_second = blocks_of(f.d, 64);
   p.bn = 2 * units;
   p.splits = 1;
-  p.act = f.act;
-  return dy != nullptr ? ff_launch<kFfHidden>(maps, p, pair, f.f16, f.info, f.stream) : ff_launch<kFfUp>(maps, p, pair, f.f16, f.info, f.stream);
+  return dy != nullptr ? ff_launch<kFfHidden>(maps, p, pair, f) : ff_launch<kFfUp>(maps, p, pair, f);
 }
 
 // y = h W_s^T, or (two operands) dx = da W_a + db W_b
@@ -330,7 +335,7 @@ static int ff_project(const FfProblem& f, const void* first, const void* second,
   p.kb = p.kb_second = blocks_of(f.hidden, 64);
   p.bn = bn;
   p.splits = 1;
-  return input ? ff_launch<kFfInput>(maps, p, pair, f.f16, f.info, f.stream) : ff_launch<kFfDown>(maps, p, pair, f.f16, f.info, f.stream);
+  return input ? ff_launch<kFfInput>(maps, p, pair, f) : ff_launch<kFfDown>(maps, p, pair, f);
 }
 
 // Tiles and parts of the weight gradients' products [hidden, d]: about two rounds of tiles for the whole GPU, but parts of at least
@@ -378,7 +383,7 @@ static int ff_weight_gradients(const FfProblem& f, const void* x, const void* dy
   p.bn = s.bn;
   p.splits = s.splits;
   p.kb_split = s.kb_split;
-  rc = ff_launch<kFfWeights>(maps, p, s.pair, f.f16, f.info, f.stream);
+  rc = ff_launch<kFfWeights>(maps, p, s.pair, f);
   if (rc != 0 || s.splits == 1) return rc;
   FfReduce r = {};
   r.partial = partial;

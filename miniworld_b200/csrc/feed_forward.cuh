@@ -42,7 +42,6 @@ struct FfParams {
   int kb, kb_second;   // 64-deep k blocks of the first and of the second segment
   int bn;              // accumulator columns of an output tile (kFfUp and kFfHidden: of its a | b part)
   int splits, kb_split;  // kFfWeights: parts of the k range, k blocks of each
-  int act;
   int type;            // kFfWeights: of `out`, 0 bf16, 1 fp32, 2 fp16
 };
 
@@ -57,18 +56,63 @@ __device__ __forceinline__ uint32_t ff_pack(float a, float b) {
   return F16 ? pack_f16x2_sat(make_float2(a, b)) : pack_bf16x2(a, b);
 }
 
-// act(a) and its derivative
-__device__ __forceinline__ float ff_act(float a, int act) {
-  if (act == kFfSilu) return __fdividef(a, 1.0f + __expf(-a));
-  return 0.5f * a * (1.0f + erff(a * 0.70710678f));
+__device__ __forceinline__ float2 ff_f2(float v) { return make_float2(v, v); }
+// 1 / (1 + 2^(-a log2 e)) of two values with one reciprocal, of the product of the two denominators (the special-function unit, four
+// lanes a clock, is what an epilogue of few products waits for). The exponent is held below 64, so that the product stays finite:
+// sigmoid(a) is 2^-63 for a < -43, off by less than 1e-19.
+__device__ __forceinline__ float2 ff_sigmoid2(float2 a) {
+  const float2 n = __fmul2_rn(a, ff_f2(-1.44269504f));
+  float2 x;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.x) : "f"(fminf(n.x, 63.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.y) : "f"(fminf(n.y, 63.f)));
+  x = __fadd2_rn(x, ff_f2(1.f));
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x.x * x.y));
+  return __fmul2_rn(ff_f2(r), make_float2(x.y, x.x));
 }
-__device__ __forceinline__ float2 ff_act_slope(float a, int act) {
+// Values of 16 neighbouring units: act(a) b
+__device__ __forceinline__ void ff_gate16(const uint32_t (&a)[16], const uint32_t (&b)[16], int act, float (&h)[16]) {
   if (act == kFfSilu) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-a));
-    return make_float2(a * s, s * fmaf(a, 1.0f - s, 1.0f));
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float2 va = make_float2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), vb = make_float2(__uint_as_float(b[j]), __uint_as_float(b[j + 1]));
+      const float2 r = __fmul2_rn(__fmul2_rn(va, ff_sigmoid2(va)), vb);
+      h[j] = r.x;
+      h[j + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float v = __uint_as_float(a[j]);
+      h[j] = 0.5f * v * (1.0f + erff(v * 0.70710678f)) * __uint_as_float(b[j]);
+    }
   }
-  const float cdf = 0.5f * (1.0f + erff(a * 0.70710678f));
-  return make_float2(a * cdf, fmaf(a * 0.39894228f, __expf(-0.5f * a * a), cdf));
+}
+// ... and of the backward: dh b act'(a), dh act(a), act(a) b
+__device__ __forceinline__ void ff_gate_back16(const uint32_t (&a)[16], const uint32_t (&b)[16], const uint32_t (&d)[16], int act, float (&da)[16],
+                                               float (&db)[16], float (&h)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 2) {
+    const float2 va = make_float2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), vb = make_float2(__uint_as_float(b[j]), __uint_as_float(b[j + 1]));
+    const float2 vd = make_float2(__uint_as_float(d[j]), __uint_as_float(d[j + 1]));
+    float2 f, slope;
+    if (act == kFfSilu) {
+      const float2 s = ff_sigmoid2(va);
+      f = __fmul2_rn(va, s);
+      slope = __ffma2_rn(f, __fadd2_rn(ff_f2(1.f), make_float2(-s.x, -s.y)), s);  // s (1 + a (1 - s))
+    } else {
+      const float2 cdf = make_float2(0.5f * (1.0f + erff(va.x * 0.70710678f)), 0.5f * (1.0f + erff(va.y * 0.70710678f)));
+      f = __fmul2_rn(va, cdf);
+      slope = make_float2(fmaf(va.x * 0.39894228f, __expf(-0.5f * va.x * va.x), cdf.x), fmaf(va.y * 0.39894228f, __expf(-0.5f * va.y * va.y), cdf.y));
+    }
+    const float2 x = __fmul2_rn(__fmul2_rn(vd, vb), slope), y = __fmul2_rn(vd, f), z = __fmul2_rn(f, vb);
+    da[j] = x.x;
+    da[j + 1] = x.y;
+    db[j] = y.x;
+    db[j + 1] = y.y;
+    h[j] = z.x;
+    h[j + 1] = z.y;
+  }
 }
 
 // 32 bytes in one request where the address allows: whole sectors of L2 (in halves a tile's stores took twice as long)
@@ -109,7 +153,7 @@ __device__ __forceinline__ void ff_put16(void* out, size_t i, const float (&v)[1
   }
 }
 
-template <int OP, bool PAIR, bool F16>
+template <int OP, bool PAIR, bool F16, int ACT>
 __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
   constexpr int S = kFfStages;
   constexpr bool A_MN = OP == kFfWeights;
@@ -384,8 +428,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
           const int col = t.n * kUnits + part * N + c * 16;
           if constexpr (OP == kFfUp) {
             float v[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = ff_act(__uint_as_float(va[c][j]), p.act) * __uint_as_float(vb[c][j]);
+            ff_gate16(va[c], vb[c], ACT, v);
             store16(p.out[0], col, v);
           } else {
             uint32_t vd[16];
@@ -393,14 +436,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
             tmem_ld_wait();
             if (c == N / 16 - 1) release(acc_empty(acc));
             float da[16], db[16], h[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float b = __uint_as_float(vb[c][j]), dh = __uint_as_float(vd[j]);
-              const float2 f = ff_act_slope(__uint_as_float(va[c][j]), p.act);
-              da[j] = dh * b * f.y;
-              db[j] = dh * f.x;
-              h[j] = f.x * b;
-            }
+            ff_gate_back16(va[c], vb[c], vd, ACT, da, db, h);
             store16(p.out[0], col, da);
             store16(p.out[1], col, db);
             store16(p.out[2], col, h);
