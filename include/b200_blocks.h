@@ -68,14 +68,17 @@ int b200_block_join_backward(const void* dy, const void* dh, const void* x, cons
  * in each call). Workspaces: 1024-byte aligned, b200_ff_workspace_bytes of the same sizes (backward 0 or 1).
  */
 int b200_ff_workspace_bytes(long long rows, int d, int hidden, int weight_dtype, int backward, size_t* out_bytes);
-int b200_ff_forward(const void* x, const void* w_a, const void* w_b, const void* w_s, void* y, void* workspace,
+/* For a backward: bytes that the forward of these sizes keeps (h, and both expanded inputs in fp16), 0 where the backward forms them
+ * again faster. A forward and its backward get the same buffer as `kept` (1024-byte aligned), or both null. */
+int b200_ff_kept_bytes(long long rows, int d, int hidden, size_t* out_bytes);
+int b200_ff_forward(const void* x, const void* w_a, const void* w_b, const void* w_s, void* y, void* kept, void* workspace,
                     size_t workspace_bytes, long long rows, int d, int hidden, int dtype, int weight_dtype, int activation,
                     void* cuda_stream);
 
 /* Gradients from dy [rows, d] and the forward's inputs: dx (dtype), dw_a, dw_b, dw_s (weight_dtype, the weights' shapes). Null
  * outputs are left out, the others overwritten. */
-int b200_ff_backward(const void* dy, const void* x, const void* w_a, const void* w_b, const void* w_s, void* dx, void* dw_a,
-                     void* dw_b, void* dw_s, void* workspace, size_t workspace_bytes, long long rows, int d, int hidden, int dtype,
+int b200_ff_backward(const void* dy, const void* x, const void* w_a, const void* w_b, const void* w_s, const void* kept, void* dx,
+                     void* dw_a, void* dw_b, void* dw_s, void* workspace, size_t workspace_bytes, long long rows, int d, int hidden, int dtype,
                      int weight_dtype, int activation, void* cuda_stream);
 
 /* Synchronises `cuda_stream`; *code: 0, or the code of the first wait of a feed-forward kernel on the current device that gave up

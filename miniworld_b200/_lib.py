@@ -148,8 +148,9 @@ BLOCKS_SIGNATURES = {
     "b200_block_join_workspace_bytes": (c_int, [_L, c_int, _L, POINTER(c_size_t)]),
     "b200_block_join_backward": (c_int, [c_void_p] * 22 + [c_size_t, _L, c_int, _L, c_int, c_int, c_int, c_void_p]),
     "b200_ff_workspace_bytes": (c_int, [_L, c_int, c_int, c_int, c_int, POINTER(c_size_t)]),
-    "b200_ff_forward": (c_int, [c_void_p] * 6 + [c_size_t, _L, c_int, c_int, c_int, c_int, c_int, c_void_p]),
-    "b200_ff_backward": (c_int, [c_void_p] * 10 + [c_size_t, _L, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "b200_ff_kept_bytes": (c_int, [_L, c_int, c_int, POINTER(c_size_t)]),
+    "b200_ff_forward": (c_int, [c_void_p] * 7 + [c_size_t, _L, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "b200_ff_backward": (c_int, [c_void_p] * 11 + [c_size_t, _L, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "b200_blocks_read_status": (c_int, [c_void_p, POINTER(c_int)]),
 }
 

@@ -15,6 +15,8 @@ namespace trimul {
 
 static size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
+constexpr int kMaxSms = 160;
+
 // ---------------------------------------------------------------- join
 // Threads of a row and 8-element pieces of each (NV): the fewest idle lanes, then the fewest pieces. Up to 32 threads reduce by
 // shuffles alone; wider rows take several warps.
@@ -55,7 +57,6 @@ static JoinGrid join_backward_grid(long long rows, int d, bool shared_gate, int 
   if (shared_gate) g.rows_per_team = (rows + static_cast<long long>(g.blocks) * g.teams - 1) / (static_cast<long long>(g.blocks) * g.teams);
   return g;
 }
-constexpr int kMaxSms = 160;
 
 static int check_join(long long rows, int d, long long gate_rows, int dtype, int post_kind, int pre_kind) {
   if (rows < 0 || d < 1 || gate_rows < 1) return B200_TRIMUL_E_SHAPE;
@@ -246,14 +247,15 @@ struct FfProblem {
   cudaStream_t stream;
 };
 
-template <int OP, bool PAIR, bool F16, int ACT>
+template <int OP, bool PAIR, bool F16, int ACT, bool SPLIT>
 static int ff_launch_kernel(const FfMaps& maps, const FfParams& p, const DeviceInfo& info, cudaStream_t stream) {
-  const int rc = set_smem(ff_kernel<OP, PAIR, F16, ACT>, kFfSmemBytes, info.device);
+  const auto kernel = ff_kernel<OP, PAIR, F16, ACT, SPLIT>;
+  const int rc = set_smem(kernel, kFfSmemBytes, info.device);
   if (rc != B200_TRIMUL_OK) return rc;
-  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * p.splits * (OP == kFfWeights ? 3 : 1);
-  const int units = PAIR ? info.sms / 2 : info.sms;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * (OP == kFfWeights ? 3 * p.splits : 1);
+  const int cluster = (PAIR ? 2 : 1) * (SPLIT ? p.splits : 1);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, units)) * (PAIR ? 2 : 1));
+  cfg.gridDim = dim3(static_cast<unsigned>(SPLIT ? tiles : std::min<long long>(tiles, info.sms / cluster)) * cluster);
   cfg.blockDim = dim3(kFfThreads);
   cfg.dynamicSmemBytes = kFfSmemBytes;
   cfg.stream = stream;
@@ -261,23 +263,25 @@ static int ff_launch_kernel(const FfMaps& maps, const FfParams& p, const DeviceI
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  TRIMUL_CUDA(cudaLaunchKernelEx(&cfg, ff_kernel<OP, PAIR, F16, ACT>, maps, p));
+  TRIMUL_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, p));
   return B200_TRIMUL_OK;
 }
 template <int OP, bool PAIR, bool F16>
-static int ff_launch_act(const FfMaps& maps, const FfParams& p, int act, const DeviceInfo& info, cudaStream_t stream) {
-  if constexpr (OP == kFfUp || OP == kFfHidden)
-    if (act == kFfGelu) return ff_launch_kernel<OP, PAIR, F16, kFfGelu>(maps, p, info, stream);
-  return ff_launch_kernel<OP, PAIR, F16, kFfSilu>(maps, p, info, stream);
+static int ff_launch_variant(const FfMaps& maps, const FfParams& p, int act, const DeviceInfo& info, cudaStream_t stream) {
+  if constexpr (OP == kFfUp || OP == kFfHidden || OP == kFfGrad)
+    if (act == kFfGelu) return ff_launch_kernel<OP, PAIR, F16, kFfGelu, false>(maps, p, info, stream);
+  if constexpr (OP == kFfDown || OP == kFfInput)
+    if (p.splits > 1) return ff_launch_kernel<OP, PAIR, F16, kFfSilu, true>(maps, p, info, stream);
+  return ff_launch_kernel<OP, PAIR, F16, kFfSilu, false>(maps, p, info, stream);
 }
 template <int OP>
 static int ff_launch(const FfMaps& maps, const FfParams& p, bool pair, const FfProblem& f) {
-  if (pair) return f.f16 ? ff_launch_act<OP, true, true>(maps, p, f.act, f.info, f.stream) : ff_launch_act<OP, true, false>(maps, p, f.act, f.info, f.stream);
-  return f.f16 ? ff_launch_act<OP, false, true>(maps, p, f.act, f.info, f.stream) : ff_launch_act<OP, false, false>(maps, p, f.act, f.info, f.stream);
+  if (pair) return f.f16 ? ff_launch_variant<OP, true, true>(maps, p, f.act, f.info, f.stream) : ff_launch_variant<OP, true, false>(maps, p, f.act, f.info, f.stream);
+  return f.f16 ? ff_launch_variant<OP, false, true>(maps, p, f.act, f.info, f.stream) : ff_launch_variant<OP, false, false>(maps, p, f.act, f.info, f.stream);
 }
 
 static int blocks_of(long long n, int b) { return static_cast<int>((n + b - 1) / b); }
@@ -286,7 +290,7 @@ static int blocks_of(long long n, int b) { return static_cast<int>((n + b - 1) /
 static bool ff_pair(long long rows, long long n_tiles, int sms) { return rows > 128 && blocks_of(rows, 256) * n_tiles >= sms / 2 * 3 / 4; }
 
 // h = act(x W_a^T) * (x W_b^T), or with dy the backward's da, db, h
-static int ff_hidden(const FfProblem& f, const void* x, const void* dy, void* const out[3]) {
+static int ff_hidden(const FfProblem& f, const void* x, const void* dy, void* const out[3], void* const keep[2] = nullptr) {
   const bool pair = ff_pair(f.rows, blocks_of(f.hidden, 128), f.info.sms);
   const int units = pair ? 128 : 64;
   FfMaps maps = {};
@@ -298,6 +302,7 @@ static int ff_hidden(const FfProblem& f, const void* x, const void* dy, void* co
   if (rc != 0) return rc;
   FfParams p = {};
   for (int i = 0; i < 3; ++i) p.out[i] = out[i];
+  if (keep != nullptr) p.keep[0] = keep[0], p.keep[1] = keep[1];
   p.ld = f.ld;
   p.rows = static_cast<int>(f.rows);
   p.cols = f.hidden;
@@ -309,12 +314,76 @@ static int ff_hidden(const FfProblem& f, const void* x, const void* dy, void* co
   return dy != nullptr ? ff_launch<kFfHidden>(maps, p, pair, f) : ff_launch<kFfUp>(maps, p, pair, f);
 }
 
+// da and db from dy with the forward's a and b
+static int ff_grad(const FfProblem& f, const void* dy, const void* const kept[2], void* da, void* db) {
+  const bool pair = ff_pair(f.rows, blocks_of(f.hidden, 256), f.info.sms);
+  const int bn = pair ? 256 : 128;
+  FfMaps maps = {};
+  int rc = ff_map(&maps.a[0], dy, f.rows, f.d, f.d, 128);
+  if (rc == 0) rc = ff_map(&maps.b[0], f.w_s, f.d, f.hidden, f.hidden, 64);
+  if (rc != 0) return rc;
+  FfParams p = {};
+  p.out[0] = da;
+  p.out[1] = db;
+  p.kept[0] = kept[0];
+  p.kept[1] = kept[1];
+  p.ld = f.ld;
+  p.rows = static_cast<int>(f.rows);
+  p.cols = f.hidden;
+  p.m_tiles = blocks_of(f.rows, pair ? 256 : 128);
+  p.n_tiles = blocks_of(f.hidden, bn);
+  p.kb = blocks_of(f.d, 64);
+  p.bn = bn;
+  p.splits = 1;
+  return ff_launch<kFfGrad>(maps, p, pair, f);
+}
+
+// Tiles of y = h W_s^T or dx = da W_a + db W_b (`input`): k blocks are far more than tiles where there are few rows. Pairs (tiles of 256
+// rows) read half as much of the second operand a product as single CTAs do, and what a single CTA's smaller tile reads from L2 is
+// what bounds it, so pairs are taken where, with their k range split over a cluster of up to eight CTAs, they still occupy half the GPU.
+// CTAs (pairs) that clusters of `splits` of them occupy at a time: a cluster lies within one of the GPU's processing clusters, of
+// which clusters of four leave a ninth and clusters of eight a fifth of the SMs idle (33 and 15 of them on 148 SMs).
+static long long ff_split_units(bool pair, int splits, int sms) {
+  const int cluster = splits * (pair ? 2 : 1);
+  const int ctas = cluster <= 2 ? sms : cluster == 4 ? sms * 33 / 37 : sms * 30 / 37;
+  return ctas / (pair ? 2 : 1);
+}
+struct FfProject {
+  bool pair;
+  int bn, m_tiles, n_tiles, kb, splits, kb_split;
+};
+static FfProject ff_project_plan(long long rows, int d, int hidden, bool input, int sms) {
+  FfProject best = {};
+  const int kb_all = blocks_of(hidden, 64) * (input ? 2 : 1);
+  for (int pair = 1; pair >= 0; --pair) {
+    if (pair && rows <= 128) continue;
+    FfProject q = {};
+    q.pair = pair != 0;
+    q.bn = pair ? 256 : 128;
+    while (q.bn > (pair && input ? 128 : 64) && blocks_of(d, q.bn / 2) * (q.bn / 2) < blocks_of(d, q.bn) * q.bn) q.bn /= 2;
+    const int units = pair ? sms / 2 : sms;
+    q.m_tiles = blocks_of(rows, pair ? 256 : 128);
+    while (q.bn > (pair && input ? 128 : 64) && static_cast<long long>(q.m_tiles) * blocks_of(d, q.bn) * (pair ? 4 : 8) < units) q.bn /= 2;
+    q.n_tiles = blocks_of(d, q.bn);
+    q.kb = blocks_of(hidden, 64);
+    const long long tiles = static_cast<long long>(q.m_tiles) * q.n_tiles;
+    // parts of at least two k blocks, a power of two of them, in one round of tiles
+    q.splits = 1;
+    while (q.splits < (pair ? 4 : 8) && tiles * q.splits * 2 <= ff_split_units(pair != 0, q.splits * 2, sms) && kb_all >= q.splits * 4) q.splits *= 2;
+    q.kb_split = blocks_of(kb_all, q.splits);
+    while ((q.splits - 1) * q.kb_split >= kb_all) q.splits /= 2, q.kb_split = blocks_of(kb_all, q.splits);  // (no part empty)
+    best = q;
+    if (tiles * q.splits * 2 >= units) break;
+  }
+  return best;
+}
+
 // y = h W_s^T, or (two operands) dx = da W_a + db W_b
 static int ff_project(const FfProblem& f, const void* first, const void* second, void* out) {
   const bool input = second != nullptr;
-  const bool pair = ff_pair(f.rows, blocks_of(f.d, 256), f.info.sms);
-  int bn = pair ? 256 : 128;
-  while (bn > (pair && input ? 128 : 64) && blocks_of(f.d, bn / 2) * (bn / 2) < blocks_of(f.d, bn) * bn) bn /= 2;
+  const FfProject plan = ff_project_plan(f.rows, f.d, f.hidden, input, f.info.sms);
+  const bool pair = plan.pair;
+  const int bn = plan.bn;
   FfMaps maps = {};
   int rc = ff_map(&maps.a[0], first, f.rows, f.hidden, f.ld, 128);
   if (input) {
@@ -330,19 +399,45 @@ static int ff_project(const FfProblem& f, const void* first, const void* second,
   p.ld = f.d;
   p.rows = static_cast<int>(f.rows);
   p.cols = f.d;
-  p.m_tiles = blocks_of(f.rows, pair ? 256 : 128);
-  p.n_tiles = blocks_of(f.d, bn);
-  p.kb = p.kb_second = blocks_of(f.hidden, 64);
+  p.m_tiles = plan.m_tiles;
+  p.n_tiles = plan.n_tiles;
+  p.kb = p.kb_second = plan.kb;
   p.bn = bn;
-  p.splits = 1;
+  p.splits = plan.splits;
+  p.kb_split = plan.kb_split;
   return input ? ff_launch<kFfInput>(maps, p, pair, f) : ff_launch<kFfDown>(maps, p, pair, f);
 }
 
-// Tiles and parts of the weight gradients' products [hidden, d]: about two rounds of tiles for the whole GPU, but parts of at least
-// eight k blocks
+template <bool F16, int R>
+static int ff_vec_launch(const FfProblem& f, FfVec v) {
+  const int rc0 = set_smem(ff_vec_up_kernel<F16, R>, kFfVecSmem, f.info.device);
+  if (rc0 != 0) return rc0;
+  const int rc1 = set_smem(ff_vec_down_kernel<F16, R>, kFfVecSmem, f.info.device);
+  if (rc1 != 0) return rc1;
+  const int warps = kFfVecThreads / 32;
+  TRIMUL_CUDA(launch_overlapped(ff_vec_up_kernel<F16, R>, dim3(blocks_of(f.hidden, warps)), kFfVecThreads, R * f.d * 4, f.stream, v));
+  v.part = std::min(f.hidden, kFfVecSmem / (R * 4) / 256 * 256);
+  TRIMUL_CUDA(launch_overlapped(ff_vec_down_kernel<F16, R>, dim3(blocks_of(f.d, warps)), kFfVecThreads, R * v.part * 4, f.stream, v));
+  return 0;
+}
+static int ff_vec_rows_up(long long rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : 4; }
+static bool ff_vec(long long rows, int d) { return rows <= kFfVecRows && ff_vec_rows_up(rows) * static_cast<long long>(d) * 4 <= kFfVecSmem; }
+template <bool F16>
+static int ff_vec_forward(const FfProblem& f, const void* x, void* h, void* y) {
+  const FfVec v = {x, f.w_a, f.w_b, f.w_s, h, y, static_cast<int>(f.rows), f.d, f.hidden, f.act, 0};
+  switch (ff_vec_rows_up(f.rows)) {
+    case 1: return ff_vec_launch<F16, 1>(f, v);
+    case 2: return ff_vec_launch<F16, 2>(f, v);
+    default: return ff_vec_launch<F16, 4>(f, v);
+  }
+}
+
+// Tiles and parts of the weight gradients' products [hidden, d]: as many parts as fill the GPU in one round of tiles (more parts would
+// take more rounds and cost the fp32 partials' traffic), of at least eight k blocks
 struct FfSplit {
   bool pair;
   int bn, m_tiles, n_tiles, kb, splits, kb_split;
+  int most;  // parts before they are made equal: no fewer than `splits` for any smaller number of SMs
 };
 static FfSplit ff_split(long long rows, int d, int hidden, int sms) {
   FfSplit s;
@@ -353,8 +448,9 @@ static FfSplit ff_split(long long rows, int d, int hidden, int sms) {
   s.m_tiles = blocks_of(hidden, s.pair ? 256 : 128);
   s.n_tiles = blocks_of(d, s.bn);
   const long long tiles = 3ll * s.m_tiles * s.n_tiles, units = s.pair ? sms / 2 : sms;
-  long long parts = tiles >= units ? 1 : (units + tiles - 1) / tiles;
+  long long parts = units / tiles;
   parts = std::max<long long>(1, std::min<long long>(parts, s.kb / 8));
+  s.most = static_cast<int>(parts);
   s.kb_split = blocks_of(s.kb, static_cast<int>(parts));
   s.splits = blocks_of(s.kb, s.kb_split);
   return s;
@@ -394,7 +490,7 @@ static int ff_weight_gradients(const FfProblem& f, const void* x, const void* dy
   r.H = f.hidden;
   r.D = f.d;
   r.type = weight_dtype;
-  TRIMUL_CUDA(launch_overlapped(ff_reduce_kernel, dim3(blocks_of(f.d, 128), blocks_of(f.hidden, 32), 3), 256, 0, f.stream, r));
+  TRIMUL_CUDA(launch_overlapped(ff_reduce_kernel, dim3(blocks_of(f.d, 128), blocks_of(f.hidden, 32), 3), 1024, 0, f.stream, r));
   return 0;
 }
 
@@ -406,10 +502,19 @@ static int check_ff(long long rows, int d, int hidden, int weight_dtype, int dty
   return B200_TRIMUL_OK;
 }
 
+// What the forward keeps for the backward: h in x's type, a and b in fp16, [rows][ld] each; nothing where forming a and b again is
+// cheaper. Writing and reading them costs 8 bytes a value, forming them 4 D operations: 0.0012 against 0.0027 D picoseconds at
+// 6.5 TB/s and 1.5 PFLOP/s, equal at D = 460; calls of few rows are bound by latency either way and keep nothing.
+// (16384 x 1024 x 4096: training step 1207 -> 1000 us.)
+static size_t ff_kept_bytes(long long rows, int d, int hidden) {
+  if (d < 512 || rows < 1024) return 0;
+  return 3 * up(static_cast<size_t>(rows) * ff_ld(hidden) * 2, 1024);
+}
+
 struct FfRegions {
   size_t weights, hidden[3], partial, total;
 };
-static FfRegions ff_regions(long long rows, int d, int hidden, int weight_dtype, bool backward, int sms) {
+static FfRegions ff_regions(long long rows, int d, int hidden, int weight_dtype, bool backward) {
   FfRegions r = {};
   size_t at = 0;
   r.weights = at;
@@ -419,8 +524,8 @@ static FfRegions ff_regions(long long rows, int d, int hidden, int weight_dtype,
     at += up(static_cast<size_t>(rows) * ff_ld(hidden) * 2, 1024);
   }
   r.partial = at;
-  const int splits = backward ? ff_split(rows, d, hidden, sms).splits : 0;
-  if (splits > 1) at += up(static_cast<size_t>(splits) * 3 * hidden * d * 4, 1024);
+  const int parts = backward ? ff_split(rows, d, hidden, kMaxSms).most : 0;
+  if (parts > 1) at += up(static_cast<size_t>(parts) * 3 * hidden * d * 4, 1024);
   r.total = at;
   return r;
 }
@@ -593,39 +698,50 @@ int b200_ff_workspace_bytes(long long rows, int d, int hidden, int weight_dtype,
   if (out_bytes == nullptr) return B200_TRIMUL_E_NULL;
   const int rc = check_ff(rows, d, hidden, weight_dtype);
   if (rc != 0) return rc;
-  // (no GPU is needed to ask: the largest number of parts that ff_split gives for any SM count up to kMaxSms)
-  size_t most = 0;
-  if (backward != 0)
-    for (int sms = 2; sms <= kMaxSms; sms += 2) most = std::max(most, ff_regions(rows, d, hidden, weight_dtype, true, sms).total);
-  else
-    most = ff_regions(rows, d, hidden, weight_dtype, false, kMaxSms).total;
-  *out_bytes = std::max<size_t>(most, 1024);
+  *out_bytes = std::max<size_t>(ff_regions(rows, d, hidden, weight_dtype, backward != 0).total, 1024);
   return B200_TRIMUL_OK;
 }
 
-int b200_ff_forward(const void* x, const void* w_a, const void* w_b, const void* w_s, void* y, void* workspace, size_t workspace_bytes,
-                    long long rows, int d, int hidden, int dtype, int weight_dtype, int activation, void* cuda_stream) {
+int b200_ff_kept_bytes(long long rows, int d, int hidden, size_t* out_bytes) {
+  if (out_bytes == nullptr) return B200_TRIMUL_E_NULL;
+  const int rc = check_ff(rows, d, hidden, 0);
+  if (rc != 0) return rc;
+  *out_bytes = ff_kept_bytes(rows, d, hidden);
+  return B200_TRIMUL_OK;
+}
+
+int b200_ff_forward(const void* x, const void* w_a, const void* w_b, const void* w_s, void* y, void* kept, void* workspace,
+                    size_t workspace_bytes, long long rows, int d, int hidden, int dtype, int weight_dtype, int activation, void* cuda_stream) {
   int rc = check_ff(rows, d, hidden, weight_dtype, dtype);
   if (rc != 0) return rc;
   if (weight_dtype != B200_BLOCKS_F32 && weight_dtype != dtype) return B200_TRIMUL_E_UNSUPPORTED;
   if (activation != B200_ACT_SILU && activation != B200_ACT_GELU) return B200_TRIMUL_E_UNSUPPORTED;
   if (rows == 0) return B200_TRIMUL_OK;
   if (x == nullptr || w_a == nullptr || w_b == nullptr || w_s == nullptr || y == nullptr || workspace == nullptr) return B200_TRIMUL_E_NULL;
-  if (!all_aligned16({x, w_a, w_b, w_s, y}) || !aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;
+  if (!all_aligned16({x, w_a, w_b, w_s, y}) || !aligned(workspace, 1024) || !aligned(kept, 1024)) return B200_TRIMUL_E_ALIGN;
   FfProblem f;
   rc = ff_device(&f.info);
   if (rc != 0) return rc;
-  const FfRegions r = ff_regions(rows, d, hidden, weight_dtype, false, f.info.sms);
+  const FfRegions r = ff_regions(rows, d, hidden, weight_dtype, false);
   if (workspace_bytes < r.total) return B200_TRIMUL_E_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   rc = ff_problem(&f, w_a, w_b, w_s, rows, d, hidden, dtype, weight_dtype, activation, ws + r.weights, cuda_stream);
   if (rc != 0) return rc;
+  const size_t keep = kept != nullptr ? ff_kept_bytes(rows, d, hidden) / 3 : 0;
+  if (keep != 0) {
+    uint8_t* k = static_cast<uint8_t*>(kept);
+    void* const all[3] = {k, nullptr, nullptr};
+    void* const ab[2] = {k + keep, k + 2 * keep};
+    rc = ff_hidden(f, x, nullptr, all, ab);
+    return rc != 0 ? rc : ff_project(f, k, nullptr, y);
+  }
   void* const out[3] = {ws + r.hidden[0], nullptr, nullptr};
+  if (ff_vec(rows, d)) return f.f16 ? ff_vec_forward<true>(f, x, out[0], y) : ff_vec_forward<false>(f, x, out[0], y);
   rc = ff_hidden(f, x, nullptr, out);
   return rc != 0 ? rc : ff_project(f, out[0], nullptr, y);
 }
 
-int b200_ff_backward(const void* dy, const void* x, const void* w_a, const void* w_b, const void* w_s, void* dx, void* dw_a, void* dw_b,
+int b200_ff_backward(const void* dy, const void* x, const void* w_a, const void* w_b, const void* w_s, const void* kept, void* dx, void* dw_a, void* dw_b,
                      void* dw_s, void* workspace, size_t workspace_bytes, long long rows, int d, int hidden, int dtype, int weight_dtype,
                      int activation, void* cuda_stream) {
   int rc = check_ff(rows, d, hidden, weight_dtype, dtype);
@@ -639,17 +755,25 @@ int b200_ff_backward(const void* dy, const void* x, const void* w_a, const void*
     return B200_TRIMUL_OK;
   }
   if (dy == nullptr || x == nullptr || w_a == nullptr || w_b == nullptr || w_s == nullptr || workspace == nullptr) return B200_TRIMUL_E_NULL;
-  if (!all_aligned16({dy, x, w_a, w_b, w_s, dx, dw_a, dw_b, dw_s}) || !aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;
+  if (!all_aligned16({dy, x, w_a, w_b, w_s, dx, dw_a, dw_b, dw_s}) || !aligned(workspace, 1024) || !aligned(kept, 1024)) return B200_TRIMUL_E_ALIGN;
   FfProblem f;
   rc = ff_device(&f.info);
   if (rc != 0) return rc;
-  const FfRegions r = ff_regions(rows, d, hidden, weight_dtype, true, f.info.sms);
+  const FfRegions r = ff_regions(rows, d, hidden, weight_dtype, true);
   if (workspace_bytes < r.total) return B200_TRIMUL_E_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   rc = ff_problem(&f, w_a, w_b, w_s, rows, d, hidden, dtype, weight_dtype, activation, ws + r.weights, cuda_stream);
   if (rc != 0) return rc;
-  void* const hidden3[3] = {ws + r.hidden[0], ws + r.hidden[1], ws + r.hidden[2]};
-  rc = ff_hidden(f, x, dy, hidden3);
+  void* hidden3[3] = {ws + r.hidden[0], ws + r.hidden[1], ws + r.hidden[2]};
+  const size_t keep = kept != nullptr ? ff_kept_bytes(rows, d, hidden) / 3 : 0;
+  if (keep != 0) {
+    uint8_t* k = static_cast<uint8_t*>(const_cast<void*>(kept));
+    const void* const ab[2] = {k + keep, k + 2 * keep};
+    hidden3[2] = k;
+    rc = ff_grad(f, dy, ab, hidden3[0], hidden3[1]);
+  } else {
+    rc = ff_hidden(f, x, dy, hidden3);
+  }
   if (rc == 0 && dx != nullptr) rc = ff_project(f, hidden3[0], hidden3[1], dx);
   if (rc == 0 && (dw_a != nullptr || dw_b != nullptr || dw_s != nullptr))
     rc = ff_weight_gradients(f, x, dy, hidden3, reinterpret_cast<float*>(ws + r.partial), dw_a, dw_b, dw_s, weight_dtype);

@@ -3,14 +3,16 @@
 //   a = x W_a^T,  b = x W_b^T,  h = act(a) b,  y = h W_s^T                        (act: SiLU, or GELU with the error function)
 //   dh = dy W_s,  da = dh b act'(a),  db = dh act(a),  dx = da W_a + db W_b,  dW_a = da^T x,  dW_b = db^T x,  dW_s = dy^T h
 //
-// Nothing but x is kept for the backward: a and b are formed again (16 M D H multiply-adds in all instead of 12, against two
-// tensors [M, H] written and read, and their rounding). Five products on the tensor cores (fp32 accumulators in tensor memory), by
+// The backward forms a and b again from x (16 M D H multiply-adds in all instead of 12), or, where that costs more than writing and
+// reading them (D >= 512 and many rows: the caller then keeps a buffer), takes them from the forward, as fp16 for either type of x
+// (11 bits of their values, saturating: kept in bf16 they would add more to the gradients' error than all other roundings). Products on the tensor cores (fp32 accumulators in tensor memory), by
 // one kernel template; what is between two products of a row is done in the first one's epilogue, on the accumulators:
 //
 //   kFfUp       a | b side by side in one accumulator, h leaves              K = D
 //   kFfDown     y = h W_s^T                                                   K = H
 //   kFfHidden   dh, and a | b again: da, db and h leave                       K = D, D
 //   kFfInput    dx = da W_a + db W_b, one accumulator over both               K = H, H
+//   kFfGrad     dh with a and b from the forward: da and db leave             K = D
 //   kFfWeights  dW_a, dW_b and dW_s^T = h^T dy: three products of one shape, the rows (K = M) split over the CTAs; fp32 partials
 //
 // Operands as they lie in memory: the weights' other orientation and the rows-as-K operands are read MN-major, so nothing is
@@ -25,7 +27,7 @@
 
 namespace trimul {
 
-enum FfOp : int { kFfUp = 0, kFfDown = 1, kFfHidden = 2, kFfInput = 3, kFfWeights = 4 };
+enum FfOp : int { kFfUp = 0, kFfDown = 1, kFfHidden = 2, kFfInput = 3, kFfWeights = 4, kFfGrad = 5 };
 enum FfAct : int { kFfSilu = 0, kFfGelu = 1 };
 
 struct FfMaps {
@@ -41,7 +43,9 @@ struct FfParams {
   int m_tiles, n_tiles;
   int kb, kb_second;   // 64-deep k blocks of the first and of the second segment
   int bn;              // accumulator columns of an output tile (kFfUp and kFfHidden: of its a | b part)
-  int splits, kb_split;  // kFfWeights: parts of the k range, k blocks of each
+  int splits, kb_split;  // kFfWeights, SPLIT: parts of the k range, k blocks of each
+  const void* kept[2]; // kFfGrad: a and b of the forward, fp16, rows `ld` apart
+  void* keep[2];       // kFfUp: where to leave them, or null
   int type;            // kFfWeights: of `out`, 0 bf16, 1 fp32, 2 fp16
 };
 
@@ -153,7 +157,29 @@ __device__ __forceinline__ void ff_put16(void* out, size_t i, const float (&v)[1
   }
 }
 
-template <int OP, bool PAIR, bool F16, int ACT>
+// 16 values as fp16, saturating; p on a 32-byte boundary
+__device__ __forceinline__ void ff_keep16(__half* p, const uint32_t (&v)[16]) {
+  uint32_t w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = pack_f16x2_sat(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])));
+  ff_store32(p, w);
+}
+__device__ __forceinline__ void ff_kept16(const uint4 (&w)[2], uint32_t (&v)[16]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t q[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = f16x2_to_float2(q[k]);
+      v[8 * j + 2 * k] = __float_as_uint(f.x);
+      v[8 * j + 2 * k + 1] = __float_as_uint(f.y);
+    }
+  }
+}
+
+// SPLIT: the k range of an output tile over the CTAs (pairs) of a cluster, for products of few tiles and a long k. Each leaves its fp32
+// tile in the (by then idle) stages, and each adds up its share of the rows over the cluster's shared memory, in the order of k.
+template <int OP, bool PAIR, bool F16, int ACT, bool SPLIT>
 __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant__ FfMaps maps, const FfParams p) {
   constexpr int S = kFfStages;
   constexpr bool A_MN = OP == kFfWeights;
@@ -176,8 +202,11 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
-  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const uint32_t cluster_rank = PAIR || SPLIT ? cluster_ctarank() : 0;
+  const uint32_t rank = PAIR ? cluster_rank & 1u : 0;   // in the pair; 0 leads
+  const uint32_t leader = PAIR ? cluster_rank & ~1u : cluster_rank;
+  const int ctas = SPLIT ? G * p.splits : G;            // of a tile
+  const int first = blockIdx.x / ctas, step = gridDim.x / ctas;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -209,12 +238,24 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
   grid_dependents_launch();
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync_all();  // barriers of both CTAs are initialised before any signal crosses
+  if constexpr (PAIR || SPLIT) cluster_sync_all();  // barriers of both CTAs are initialised before any signal crosses
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  auto commit = [&](uint32_t bar) {
+    if constexpr (PAIR)
+      umma_commit_mask(bar, static_cast<uint16_t>(3u << leader));
+    else
+      umma_commit(bar);
+  };
+  auto arrive = [&](uint32_t bar) {  // (a barrier of the leader's)
+    if (PAIR && rank != 0)
+      mbar_arrive_cluster(map_to_cta(bar, leader));
+    else
+      mbar_arrive(bar);
+  };
 
   const int per_split = p.m_tiles * p.n_tiles * (OP == kFfWeights ? 3 : 1);
-  const int tiles = per_split * p.splits;
+  const int tiles = SPLIT ? per_split : per_split * p.splits;
   struct Tile {
     int split, product, m, n, kb0, kb1;
   };
@@ -228,8 +269,9 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     i /= p.n_tiles;
     t.m = i % p.m_tiles;
     t.product = i / p.m_tiles;
-    t.kb0 = OP == kFfWeights ? t.split * p.kb_split : 0;
-    t.kb1 = OP == kFfWeights ? min(p.kb, t.kb0 + p.kb_split) : p.kb + (SECOND ? p.kb_second : 0);
+    const int kb = p.kb + (SECOND ? p.kb_second : 0);
+    t.kb0 = OP == kFfWeights ? t.split * p.kb_split : SPLIT ? static_cast<int>(cluster_rank) / G * p.kb_split : 0;
+    t.kb1 = OP == kFfWeights || SPLIT ? min(kb, t.kb0 + p.kb_split) : kb;
     return t;
   };
 
@@ -256,7 +298,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
           const uint32_t sa = base + s * kFfStageBytes, sb = sa + 16384;
           auto load = [&](uint32_t dst, const CUtensorMap* m, int c0, int c1) {
             if constexpr (PAIR)
-              tma_load_2d_pair(dst, m, map_to_cta(full(s), 0), c0, c1);
+              tma_load_2d_pair(dst, m, map_to_cta(full(s), leader), c0, c1);
             else
               tma_load_2d(dst, m, full(s), c0, c1);
           };
@@ -342,7 +384,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
           }
           tc_fence_after();
           const uint32_t sa = base + s * kFfStageBytes, sb = sa + 16384;
-          const bool b_mn = OP == kFfInput || OP == kFfWeights || (OP == kFfHidden && !second);
+          const bool b_mn = OP == kFfInput || OP == kFfWeights || OP == kFfGrad || (OP == kFfHidden && !second);
           const int n = OP == kFfHidden && !second ? p.bn / 2 : p.bn;
           const uint32_t idesc = umma_idesc(128 * G, n, A_MN, b_mn, fmt, fmt);
           const uint32_t d = OP == kFfHidden && second ? tmem : tmem + kAcc0 + acc * kAcc;
@@ -358,21 +400,13 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
             else
               umma_bf16(d, da + k * ka, db + k * kn, idesc, more);
           }
-          if constexpr (PAIR)
-            umma_commit_pair(empty(s));
-          else
-            umma_commit(empty(s));
+          commit(empty(s));
           if (++s == S) {
             s = 0;
             ph ^= 1u;
           }
         }
-        if (ok) {
-          if constexpr (PAIR)
-            umma_commit_pair(acc_full(acc));
-          else
-            umma_commit(acc_full(acc));
-        }
+        if (ok) commit(acc_full(acc));
       }
     }
   } else {
@@ -387,17 +421,22 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
       const int acc = it & 1;
       const int row = (t.m * G + static_cast<int>(rank)) * 128 + q * 32 + lane;
       const bool in = row < p.rows;
+      // kFfGrad: the forward's a and b, a piece ahead of the accumulators
+      uint4 ka[2], kb[2];
+      auto kept = [&](int col) {
+        ka[0] = ka[1] = kb[0] = kb[1] = make_uint4(0u, 0u, 0u, 0u);
+        if (!in || col >= p.cols) return;
+        const size_t at = (static_cast<size_t>(row) * p.ld + col) * 2;
+        ld_gpu_chunks(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.kept[0]) + at), true, ka);
+        ld_gpu_chunks(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.kept[1]) + at), true, kb);
+      };
+      if constexpr (OP == kFfGrad) kept(t.n * p.bn + part * (p.bn / 4));
       if (!mbar_wait_warp(acc_full(acc), (it >> 1) & 1, abort_flag, &blocks_status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
       auto release = [&](uint32_t bar) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR)
-            mbar_arrive_leader(bar, rank);
-          else
-            mbar_arrive(bar);
-        }
+        if (lane == 0) arrive(bar);
       };
       // 16 neighbours of a row of the output (multiples of 8 of them within the width)
       auto store16 = [&](void* out, int col, const float (&v)[16]) {
@@ -430,6 +469,11 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
             float v[16];
             ff_gate16(va[c], vb[c], ACT, v);
             store16(p.out[0], col, v);
+            if (p.keep[0] != nullptr && in && col < p.cols) {
+              const size_t at = static_cast<size_t>(row) * p.ld + col;  // (rows of the buffer are whole lines: past the width there is room)
+              ff_keep16(static_cast<__half*>(p.keep[0]) + at, va[c]);
+              ff_keep16(static_cast<__half*>(p.keep[1]) + at, vb[c]);
+            }
           } else {
             uint32_t vd[16];
             tmem_ld16(d + part * N + c * 16, vd);
@@ -449,12 +493,32 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
           uint32_t v[16];
           tmem_ld16(d + part * n + c, v);
           tmem_ld_wait();
-          if (c + 16 >= n) release(acc_empty(acc));
+          if (!SPLIT && c + 16 >= n) release(acc_empty(acc));
           const int col = t.n * p.bn + part * n + c;
+          if constexpr (SPLIT) {
+            // fp32 rows of bn columns, 16-byte pieces in an order that spreads a column over the banks
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t piece = static_cast<uint32_t>(part * n + c) / 4 + j;
+              const uint32_t at = base + static_cast<uint32_t>(q * 32 + lane) * p.bn * 4 + ((piece ^ (lane & 7u)) << 4);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[4 * j]), "r"(v[4 * j + 1]), "r"(v[4 * j + 2]), "r"(v[4 * j + 3])
+                           : "memory");
+            }
+            continue;
+          }
           float f[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]);
-          if constexpr (OP != kFfWeights) {
+          if constexpr (OP == kFfGrad) {
+            uint32_t va[16], vb[16];
+            ff_kept16(ka, va);
+            ff_kept16(kb, vb);
+            if (c + 16 < n) kept(col + 16);
+            float da[16], db[16];
+            ff_gate_back16(va, vb, v, ACT, da, db, f);  // (h is the forward's)
+            store16(p.out[0], col, da);
+            store16(p.out[1], col, db);
+          } else if constexpr (OP != kFfWeights) {
             store16(p.out[0], col, f);
           } else if (in && col < p.cols) {
             const int left = p.cols - col;
@@ -475,9 +539,42 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     }
   }
 
+  if constexpr (SPLIT) {
+    __syncwarp();
+    cluster_sync_all();  // every CTA's tile is in its shared memory
+    const Tile t = tile_at(first);
+    const int share = 128 / p.splits;  // rows of this CTA
+    const int r0 = static_cast<int>(cluster_rank) / G * share;
+    const int pieces = p.bn / 8;
+    for (int e = threadIdx.x; e < share * pieces; e += kFfThreads) {
+      const int r = r0 + e / pieces, c = e % pieces;
+      const int row = (t.m * G + static_cast<int>(rank)) * 128 + r, col = t.n * p.bn + c * 8;
+      if (row >= p.rows || col >= p.cols) continue;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = 0.f;
+      for (int k = 0; k < p.splits; ++k) {
+        const uint32_t tile = map_to_cta(base, k * G + rank) + static_cast<uint32_t>(r) * p.bn * 4;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float4 v;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                       : "r"(tile + (((2u * c + j) ^ (r & 7u)) << 4)));
+          f[4 * j] += v.x;
+          f[4 * j + 1] += v.y;
+          f[4 * j + 2] += v.z;
+          f[4 * j + 3] += v.w;
+        }
+      }
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out[0]) + static_cast<size_t>(row) * p.ld + col) =
+          make_uint4(ff_pack<F16>(f[0], f[1]), ff_pack<F16>(f[2], f[3]), ff_pack<F16>(f[4], f[5]), ff_pack<F16>(f[6], f[7]));
+    }
+  }
+
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync_all();  // neither CTA leaves while the other may still signal its barriers or read its operands
+  if constexpr (PAIR || SPLIT) cluster_sync_all();  // no CTA leaves while another may still signal its barriers or read its memory
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -496,57 +593,160 @@ struct FfReduce {
   int splits, H, D;
   int type;  // 0 bf16, 1 fp32, 2 fp16
 };
-__global__ void __launch_bounds__(256) ff_reduce_kernel(const FfReduce p) {
+__global__ void __launch_bounds__(1024) ff_reduce_kernel(const FfReduce p) {
   __shared__ float tile[32][129];
   grid_dependency_wait();
   grid_dependents_launch();
   void* out = blockIdx.z == 0 ? p.out[0] : blockIdx.z == 1 ? p.out[1] : p.out[2];
   if (out == nullptr) return;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c = blockIdx.x * 128 + tx * 4;
+  const int c = blockIdx.x * 128 + tx * 4, r = blockIdx.y * 32 + ty;
+  const bool in = r < p.H && c < p.D;
   const size_t part = static_cast<size_t>(3) * p.H * p.D;
-  float4 a[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < p.splits; ++k) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = blockIdx.y * 32 + ty + 8 * j;
-      if (r >= p.H || c >= p.D) continue;
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partial + k * part + (static_cast<size_t>(blockIdx.z) * p.H + r) * p.D + c));
-      a[j].x += v.x;
-      a[j].y += v.y;
-      a[j].z += v.z;
-      a[j].w += v.w;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (in) {
+    const float* s = p.partial + (static_cast<size_t>(blockIdx.z) * p.H + r) * p.D + c;
+#pragma unroll 8
+    for (int k = 0; k < p.splits; ++k) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(s + k * part));
+      a.x += v.x;
+      a.y += v.y;
+      a.z += v.z;
+      a.w += v.w;
     }
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = blockIdx.y * 32 + ty + 8 * j;
-    if (blockIdx.z < 2) {
-      if (r >= p.H || c >= p.D) continue;
-      const size_t i = static_cast<size_t>(r) * p.D + c;
-      if (p.type == 1)
-        reinterpret_cast<float4*>(static_cast<float*>(out) + i)[0] = a[j];
-      else if (p.type == 0)
-        reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i)[0] = make_uint2(pack_bf16x2(a[j].x, a[j].y), pack_bf16x2(a[j].z, a[j].w));
-      else
-        reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i)[0] =
-            make_uint2(pack_f16x2(make_float2(a[j].x, a[j].y)), pack_f16x2(make_float2(a[j].z, a[j].w)));
-    } else {
-      float* s = &tile[ty + 8 * j][tx * 4];
-      s[0] = a[j].x;
-      s[1] = a[j].y;
-      s[2] = a[j].z;
-      s[3] = a[j].w;
-    }
+  if (blockIdx.z < 2) {
+    if (!in) return;
+    const size_t i = static_cast<size_t>(r) * p.D + c;
+    if (p.type == 1)
+      *reinterpret_cast<float4*>(static_cast<float*>(out) + i) = a;
+    else if (p.type == 0)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+    else
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = make_uint2(pack_f16x2(make_float2(a.x, a.y)), pack_f16x2(make_float2(a.z, a.w)));
+    return;
   }
-  if (blockIdx.z < 2) return;
+  float* s = &tile[ty][tx * 4];
+  s[0] = a.x;
+  s[1] = a.y;
+  s[2] = a.z;
+  s[3] = a.w;
   __syncthreads();
   const int h = blockIdx.y * 32 + tx;
-  for (int j = ty; j < 128; j += 8) {
+#pragma unroll
+  for (int j = ty; j < 128; j += 32) {
     const int d = blockIdx.x * 128 + j;
     if (d < p.D && h < p.H) ff_put(out, static_cast<size_t>(d) * p.H + h, tile[tx][j], p.type);
+  }
+}
+
+// A few rows (the single tokens of serving): every weight is read once and meets all rows, so the bytes of the weights bound it and
+// tensor cores would idle on tiles of 128 rows. A warp takes a hidden unit (its rows of W_a and W_b) or a column of y (a row of W_s), a
+// lane every 32nd piece of eight weights; the rows lie in shared memory in fp32. R: rows, rounded up to a power of two.
+constexpr int kFfVecRows = 4;  // (768 x 2048, both kernels: one row 6.0 us, four 8.8, eight 18.9; tiles of tensor cores 15.7)
+constexpr int kFfVecThreads = 256;
+constexpr int kFfVecSmem = 96 * 1024;  // rows of the second product pass through it in parts
+
+template <bool F16>
+__device__ __forceinline__ float2 ff_two(uint32_t w) {
+  return F16 ? f16x2_to_float2(w) : bf16x2_to_float2(w);
+}
+// rows [0, R) x columns [k0, k0 + n) of a 16-bit matrix to fp32 [R][n], the halves of each piece of eight n / 2 apart (16-byte reads of
+// a warp without bank conflicts); rows past `rows` are zero
+template <bool F16, int R>
+__device__ __forceinline__ void ff_vec_rows(float* to, const void* from, int rows, int ld, int k0, int n) {
+  const int pieces = n / 8;
+  for (int e = threadIdx.x; e < R * pieces; e += kFfVecThreads) {
+    const int r = e / pieces, c = (e - r * pieces) * 8;
+    const uint4 w = r < rows ? __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(from) + static_cast<size_t>(r) * ld + k0 + c)) : make_uint4(0, 0, 0, 0);
+    const float2 a = ff_two<F16>(w.x), b = ff_two<F16>(w.y), d = ff_two<F16>(w.z), f = ff_two<F16>(w.w);
+    float* o = to + r * n + c / 2;
+    *reinterpret_cast<float4*>(o) = make_float4(a.x, a.y, b.x, b.y);
+    *reinterpret_cast<float4*>(o + n / 2) = make_float4(d.x, d.y, f.x, f.y);
+  }
+}
+// acc[r] += the products of eight weights with the rows' eight values
+template <bool F16, int R>
+__device__ __forceinline__ void ff_vec_step(float2 (&acc)[R], const float* rows, int n, int c, const uint4& w) {
+  const float2 v[4] = {ff_two<F16>(w.x), ff_two<F16>(w.y), ff_two<F16>(w.z), ff_two<F16>(w.w)};
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float4 a = *reinterpret_cast<const float4*>(rows + r * n + c / 2);
+    const float4 b = *reinterpret_cast<const float4*>(rows + r * n + n / 2 + c / 2);
+    acc[r] = __ffma2_rn(make_float2(a.x, a.y), v[0], acc[r]);
+    acc[r] = __ffma2_rn(make_float2(a.z, a.w), v[1], acc[r]);
+    acc[r] = __ffma2_rn(make_float2(b.x, b.y), v[2], acc[r]);
+    acc[r] = __ffma2_rn(make_float2(b.z, b.w), v[3], acc[r]);
+  }
+}
+__device__ __forceinline__ float ff_warp_sum(float2 v) {
+  float s = v.x + v.y;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  return s;
+}
+
+struct FfVec {
+  const void *x, *w_a, *w_b, *w_s;
+  void *h, *y;  // h [rows][hidden]
+  int rows, d, hidden, act;
+  int part;     // columns of h that are in shared memory at a time
+};
+template <bool F16, int R>
+__global__ void __launch_bounds__(kFfVecThreads) ff_vec_up_kernel(const FfVec p) {
+  extern __shared__ __align__(16) float vec_rows[];
+  grid_dependency_wait();
+  grid_dependents_launch();
+  ff_vec_rows<F16, R>(vec_rows, p.x, p.rows, p.d, 0, p.d);
+  __syncthreads();
+  const int unit = blockIdx.x * (kFfVecThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (unit >= p.hidden) return;
+  const uint16_t* wa = static_cast<const uint16_t*>(p.w_a) + static_cast<size_t>(unit) * p.d;
+  const uint16_t* wb = static_cast<const uint16_t*>(p.w_b) + static_cast<size_t>(unit) * p.d;
+  float2 a[R], b[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) a[r] = b[r] = make_float2(0.f, 0.f);
+#pragma unroll 2
+  for (int c = lane * 8; c < p.d; c += 256) {
+    const uint4 va = __ldcg(reinterpret_cast<const uint4*>(wa + c)), vb = __ldcg(reinterpret_cast<const uint4*>(wb + c));
+    ff_vec_step<F16, R>(a, vec_rows, p.d, c, va);
+    ff_vec_step<F16, R>(b, vec_rows, p.d, c, vb);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float sa = ff_warp_sum(a[r]), sb = ff_warp_sum(b[r]);
+    if (lane == r % 32 && r < p.rows) {
+      const float f = p.act == kFfSilu ? __fdividef(sa, 1.0f + __expf(-sa)) : 0.5f * sa * (1.0f + erff(sa * 0.70710678f));
+      static_cast<uint16_t*>(p.h)[static_cast<size_t>(r) * p.hidden + unit] = static_cast<uint16_t>(ff_pack<F16>(f * sb, 0.f));
+    }
+  }
+}
+template <bool F16, int R>
+__global__ void __launch_bounds__(kFfVecThreads) ff_vec_down_kernel(const FfVec p) {
+  extern __shared__ __align__(16) float vec_rows[];
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int col = blockIdx.x * (kFfVecThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const uint16_t* w = static_cast<const uint16_t*>(p.w_s) + static_cast<size_t>(col < p.d ? col : 0) * p.hidden;
+  float2 acc[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) acc[r] = make_float2(0.f, 0.f);
+  for (int k0 = 0; k0 < p.hidden; k0 += p.part) {
+    const int n = min(p.part, p.hidden - k0);
+    if (k0 != 0) __syncthreads();
+    ff_vec_rows<F16, R>(vec_rows, p.h, p.rows, p.hidden, k0, n);
+    __syncthreads();
+#pragma unroll 4
+    for (int c = lane * 8; c < n; c += 256) {
+      const uint4 v = __ldcg(reinterpret_cast<const uint4*>(w + k0 + c));
+      ff_vec_step<F16, R>(acc, vec_rows, n, c, v);
+    }
+  }
+  if (col >= p.d) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float s = ff_warp_sum(acc[r]);
+    if (lane == r % 32 && r < p.rows) static_cast<uint16_t*>(p.y)[static_cast<size_t>(r) * p.d + col] = static_cast<uint16_t>(ff_pack<F16>(s, 0.f));
   }
 }
 

@@ -463,6 +463,14 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
       : "memory");
 }
 
+// The same for a pair inside a larger cluster: `mask` has the bits of its two CTAs.
+__device__ __forceinline__ void umma_commit_mask(uint32_t bar, uint16_t mask) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(mask)
+      : "memory");
+}
+
 // ------------------------------------------------------------------ small math
 __device__ __forceinline__ float tanh_approx(float x) {
   float y;

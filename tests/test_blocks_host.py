@@ -86,16 +86,20 @@ def test_feed_forward_refuses(lib, p):
     assert sizes(100, 64, 256, 1, 0, ctypes.byref(need)) == 0 and need.value >= forward + 3 * 64 * 256 * 2
     assert sizes(100, 64, 256, 0, 1, ctypes.byref(need)) == 0 and need.value >= 3 * 100 * 256 * 2
 
-    def call(x=p, w=p, y=p, ws=p, n=1 << 40, rows=10, d=64, hidden=256, dtype=0, weights=0, act=0):
-        return lib.b200_ff_forward(x, w, p, p, y, ws, n, rows, d, hidden, dtype, weights, act, None)
+    def call(x=p, w=p, y=p, kept=None, ws=p, n=1 << 40, rows=10, d=64, hidden=256, dtype=0, weights=0, act=0):
+        return lib.b200_ff_forward(x, w, p, p, y, kept, ws, n, rows, d, hidden, dtype, weights, act, None)
 
     assert call(dtype=1) == -3 and call(dtype=2, weights=0) == -3 and call(act=2) == -3 and call(d=12) == -3 and call(rows=-1) == -2
     assert call(x=None) == -1 and call(w=None) == -1 and call(y=None) == -1 and call(ws=None) == -1
-    assert call(x=p + 8) == -4 and call(w=p + 2) == -4 and call(ws=p + 16) == -4
+    assert call(x=p + 8) == -4 and call(w=p + 2) == -4 and call(ws=p + 16) == -4 and call(kept=p + 16) == -4
     assert call(rows=0, x=None) == 0
+    assert lib.b200_ff_kept_bytes(4096, 1024, 4096, ctypes.byref(need)) == 0 and need.value == 3 * 4096 * 4096 * 2
+    assert lib.b200_ff_kept_bytes(4096, 384, 1536, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.b200_ff_kept_bytes(64, 1024, 4096, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.b200_ff_kept_bytes(64, 1020, 4096, ctypes.byref(need)) == -3 and lib.b200_ff_kept_bytes(64, 1024, 4096, None) == -1
 
     def back(dy=p, dx=p, dw=p, ws=p, d=64, dtype=0, act=0):
-        return lib.b200_ff_backward(dy, p, p, p, p, dx, dw, p, p, ws, 1 << 40, 10, d, 256, dtype, 0, act, None)
+        return lib.b200_ff_backward(dy, p, p, p, p, None, dx, dw, p, p, ws, 1 << 40, 10, d, 256, dtype, 0, act, None)
 
     assert back(dy=None) == -1 and back(ws=None) == -1 and back(dx=p + 8) == -4 and back(dw=p + 4) == -4 and back(d=4) == -3
     assert back(dtype=1) == -3 and back(act=-1) == -3
