@@ -7,6 +7,7 @@
 #include <utility>
 
 #include "feed_forward.cuh"
+#include "feed_forward_narrow.cuh"
 #include "host_util.cuh"
 #include "join.cuh"
 #include "join_tiles.cuh"
@@ -80,7 +81,8 @@ static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count,
   const JoinParams& j = p->j;
   if (j.team > kTileWarps * 32) return false;
   const int unit = 16 / static_cast<int>(std::gcd(16, j.d * size));  // rows whose bytes are a multiple of 16
-  const int teams = kTileWarps * 32 / j.team;
+  const int teams = j.team > 32 ? std::min(kTileTeams, kTileWarps * 32 / j.team) : kTileWarps * 32 / j.team;
+  p->workers = teams * j.team;
   const long long share = (j.rows + blocks_most - 1) / blocks_most;
   long long rows = std::min<long long>(teams, share);
   rows = static_cast<long long>(up(static_cast<size_t>(rows), unit));
@@ -102,7 +104,7 @@ static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count,
 }
 static int tile_smem(const JoinTileParams& p, int params) {
   // (the backward's sums pass through the stages)
-  return params * p.params * 4 + kTileScratch + std::max(p.stages * p.slots * p.slot, params == 3 ? kTileWarps * 32 * 8 * 4 : 0);
+  return params * p.params * 4 + kTileScratch + std::max(p.stages * p.slots * p.slot, params == 3 ? p.workers * 8 * 4 : 0);
 }
 using TileKernel = void (*)(JoinTileParams);
 template <typename T, int VEC, bool EXACT>
@@ -113,6 +115,11 @@ static TileKernel tile_forward_kernel(int nv) {
     case 3: return join_tile_forward_kernel<T, VEC, 3, EXACT>;
     default: return join_tile_forward_kernel<T, VEC, 4, EXACT>;
   }
+}
+template <typename T, bool JOIN>
+static TileKernel tile_backward_kernel(int vec, bool exact) {
+  if (exact) return join_tile_backward_kernel<T, 8, true, JOIN>;
+  return vec == 8 ? join_tile_backward_kernel<T, 8, false, JOIN> : vec == 2 ? join_tile_backward_kernel<T, 2, false, JOIN> : join_tile_backward_kernel<T, 1, false, JOIN>;
 }
 // elements of a row that a thread reads at once
 static int join_vec(int d) { return d % 8 == 0 ? 8 : d % 2 == 0 ? 2 : 1; }
@@ -140,8 +147,7 @@ static int launch_join_forward(const JoinParams& p0, bool wide, const DeviceInfo
                                                         : tile_forward_kernel<T, 1, false>(s.nv);
     const int rc = set_smem(kernel, kTileSmem, info.device);
     if (rc != 0) return rc;
-    const int threads = kTileWarps * 32 / s.team * s.team + 32;
-    TRIMUL_CUDA(launch_overlapped(kernel, dim3(std::min(per_sm * info.sms, q.tiles)), threads, tile_smem(q, 4), stream, q));
+    TRIMUL_CUDA(launch_overlapped(kernel, dim3(std::min(per_sm * info.sms, q.tiles)), q.workers + 32, tile_smem(q, 4), stream, q));
     return B200_TRIMUL_OK;
   }
   JoinParams p = p0;
@@ -175,22 +181,20 @@ static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& 
   q.out_slot[0] = p.dx == nullptr ? -1 : q.slot_of[0] >= 0 ? q.slot_of[0] : q.slot_of[3] >= 0 ? q.slot_of[3] : q.slots++;
   q.out_slot[1] = p.du != nullptr ? q.slot_of[1] : -1;
   q.out_slot[2] = p.dgate != nullptr && !shared_gate ? q.slot_of[2] : -1;
+  const bool join = p.u != nullptr;
+  const int most = std::min(info.sms, kMaxSms) * (join ? 1 : 2);
   const void* tensors[] = {p.x, p.u, q.slot_of[2] >= 0 ? p.gate : nullptr, p.dy, p.dh, p.dx, p.du, q.out_slot[2] >= 0 ? p.dgate : nullptr};
-  if (q.slots > 0 && (!shared_gate || p.gate_rows >= kSharedGateRows) && plan_tiles(&q, tensors, 8, sizeof(T), 1, 3, std::min(info.sms, kMaxSms), kTileSmem)) {
-    int blocks = std::min(std::min(info.sms, kMaxSms), q.tiles);
+  if (q.slots > 0 && (!shared_gate || p.gate_rows >= kSharedGateRows) && plan_tiles(&q, tensors, 8, sizeof(T), 1, 3, most, join ? kTileSmem : kTileSmemHalf)) {
+    const int blocks = std::min(most, q.tiles);
     if (shared_gate) {
       q.block_tiles = (q.tiles + blocks - 1) / blocks;
       q.group_slots = static_cast<int>(static_cast<long long>(q.block_tiles) * q.tile_rows / p.gate_rows) + 2;
     }
     const int vec = join_vec(p.d);
-    const TileKernel kernel = p.d == 8 * p.team ? join_tile_backward_kernel<T, 8, true>
-                              : vec == 8        ? join_tile_backward_kernel<T, 8, false>
-                              : vec == 2        ? join_tile_backward_kernel<T, 2, false>
-                                                : join_tile_backward_kernel<T, 1, false>;
+    const TileKernel kernel = join ? tile_backward_kernel<T, true>(vec, p.d == 8 * p.team) : tile_backward_kernel<T, false>(vec, p.d == 8 * p.team);
     const int rc = set_smem(kernel, kTileSmem, info.device);
     if (rc != 0) return rc;
-    const int threads = kTileWarps * 32 / p.team * p.team + 32;
-    TRIMUL_CUDA(launch_overlapped(kernel, dim3(blocks), threads, tile_smem(q, 3), stream, q));
+    TRIMUL_CUDA(launch_overlapped(kernel, dim3(blocks), q.workers + 32, tile_smem(q, 3), stream, q));
     if (p.sums != nullptr) {
       JoinTileSums t = {p.sums, p.scale, p.post_w, p.post_b, {}, blocks, p.d, p.post_kind};
       for (int i = 0; i < 5; ++i) t.out[i] = sums.out[i];
@@ -200,7 +204,7 @@ static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& 
       auto last = vec == 8 ? join_tile_gate_kernel<T, 8> : vec == 2 ? join_tile_gate_kernel<T, 2> : join_tile_gate_kernel<T, 1>;
       const long long groups = p.rows / p.gate_rows;
       if (groups > 65535) return B200_TRIMUL_E_SHAPE;
-      TRIMUL_CUDA(launch_overlapped(last, dim3((8 * p.team + 31) / 32, static_cast<unsigned>(groups)), 256, 0, stream, q));
+      TRIMUL_CUDA(launch_overlapped(last, dim3((8 * p.team + 31) / 32, static_cast<unsigned>(groups)), 1024, 0, stream, q));
     }
     return B200_TRIMUL_OK;
   }
@@ -215,7 +219,8 @@ static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& 
   return B200_TRIMUL_OK;
 }
 
-static size_t join_sums_bytes(int d) { return up(static_cast<size_t>(kMaxSms) * 5 * d * 4, 1024); }
+// (a norm's two blocks an SM leave two of the four sums: up to eight in all)
+static size_t join_sums_bytes(int d) { return up(static_cast<size_t>(kMaxSms) * 8 * d * 4, 1024); }
 
 // ---------------------------------------------------------------- feed-forward
 // The current device, whose context is then the calling thread's: a thread that has not used the GPU yet (autograd's, on its first
@@ -406,6 +411,32 @@ static int ff_project(const FfProblem& f, const void* first, const void* second,
   p.splits = plan.splits;
   p.kb_split = plan.kb_split;
   return input ? ff_launch<kFfInput>(maps, p, pair, f) : ff_launch<kFfDown>(maps, p, pair, f);
+}
+
+// Narrow tensors in one kernel, where its tiles of 256 rows occupy most of the GPU
+static bool ff_narrow(long long rows, int d, int sms) { return d <= 128 && blocks_of(rows, 256) >= sms / 2 * 3 / 4; }
+template <bool F16, int ACT, int HALVES>
+static int ff_narrow_launch(const FfProblem& f, const void* x, void* y) {
+  const auto kernel = ff_narrow_kernel<F16, ACT, HALVES>;
+  int rc = set_smem(kernel, kNwSmemBytes, f.info.device);
+  FfMaps maps = {};
+  if (rc == 0) rc = ff_map(&maps.a[0], x, f.rows, f.d, f.d, 128);
+  if (rc == 0) rc = ff_map(&maps.b[0], f.w_a, f.hidden, f.d, f.d, 64);
+  if (rc == 0) rc = ff_map(&maps.b[1], f.w_b, f.hidden, f.d, f.d, 64);
+  if (rc == 0) rc = ff_map(&maps.b[2], f.w_s, f.d, f.hidden, f.hidden, 32 * HALVES);
+  if (rc != 0) return rc;
+  const FfNarrowParams p = {y, f.rows, f.d, blocks_of(f.rows, 256), blocks_of(f.hidden, 64)};
+  TRIMUL_CUDA(launch_overlapped(kernel, dim3(2 * std::min(p.num_tiles, f.info.sms / 2)), kNwThreads, kNwSmemBytes, f.stream, maps, p));
+  return 0;
+}
+static int ff_narrow_forward(const FfProblem& f, const void* x, void* y) {
+  const bool wide = f.d > 64, gelu = f.act == kFfGelu;
+  if (f.f16) {
+    if (gelu) return wide ? ff_narrow_launch<true, kFfGelu, 2>(f, x, y) : ff_narrow_launch<true, kFfGelu, 1>(f, x, y);
+    return wide ? ff_narrow_launch<true, kFfSilu, 2>(f, x, y) : ff_narrow_launch<true, kFfSilu, 1>(f, x, y);
+  }
+  if (gelu) return wide ? ff_narrow_launch<false, kFfGelu, 2>(f, x, y) : ff_narrow_launch<false, kFfGelu, 1>(f, x, y);
+  return wide ? ff_narrow_launch<false, kFfSilu, 2>(f, x, y) : ff_narrow_launch<false, kFfSilu, 1>(f, x, y);
 }
 
 template <bool F16, int R>
@@ -736,6 +767,7 @@ int b200_ff_forward(const void* x, const void* w_a, const void* w_b, const void*
     return rc != 0 ? rc : ff_project(f, k, nullptr, y);
   }
   void* const out[3] = {ws + r.hidden[0], nullptr, nullptr};
+  if (ff_narrow(rows, d, f.info.sms)) return ff_narrow_forward(f, x, y);
   if (ff_vec(rows, d)) return f.f16 ? ff_vec_forward<true>(f, x, out[0], y) : ff_vec_forward<false>(f, x, out[0], y);
   rc = ff_hidden(f, x, nullptr, out);
   return rc != 0 ? rc : ff_project(f, out[0], nullptr, y);

@@ -17,8 +17,11 @@
 
 namespace trimul {
 
-constexpr int kTileWarps = 15;                         // warps that compute (with the copying one four to a scheduler: 128 registers)
-constexpr int kTileThreads = kTileWarps * 32 + 32;     // ... and the one that copies
+// Warps that compute; one more copies: four to a scheduler with 128 registers a thread, or two such blocks an SM with 64 (the
+// forward with eight elements of a row a thread, the backward of a norm alone).
+constexpr int kTileWarps = 15;
+constexpr int kTileThreads = kTileWarps * 32 + 32;
+constexpr int kTileTeams = 7;                          // most teams of several warps
 constexpr int kTileMaxStages = 8;
 constexpr int kTileSmem = 224 * 1024;                  // of the 227 KB a block may have (the 228 KB of an SM)
 constexpr int kTileSmemHalf = 112 * 1024;              // two blocks an SM: forward, eight elements of a row a thread
@@ -33,9 +36,22 @@ struct JoinTileParams {
   int slot_of[5];      // x, u, gate, dy, dh: place in a stage, -1: not there
   int out_slot[3];     // forward: y, h; backward: dx, du, dgate; -1: not asked for
   int params;          // floats of one parameter vector in shared memory (the width of all threads of a row)
+  int workers;         // threads that compute
   int block_tiles;     // backward with a shared gate: consecutive tiles of a block (0: every grid-th tile)
   int group_slots;     // ... and the gate rows that they can touch
 };
+
+// Shared memory by its 32-bit address: the compiler keeps no 64-bit pointers for it
+__device__ __forceinline__ uint4 lds4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ float2 as_f2(uint32_t x, uint32_t y) { return make_float2(__uint_as_float(x), __uint_as_float(y)); }
+__device__ __forceinline__ uint32_t bits(float v) { return __float_as_uint(v); }
 
 // offset of parameter c in shared memory: pieces of four of eight neighbours apart, so that a warp's 16-byte reads are conflict-free
 template <int VEC>
@@ -47,47 +63,70 @@ __device__ __forceinline__ int tile_col(int i, int t, int team) {
   return ((i / VEC) * team + t) * VEC + i % VEC;
 }
 template <int VEC, int NV>
-__device__ __forceinline__ void tile_params(const float* w, int params, int t, int team, float2 (&v)[4 * NV]) {
+__device__ __forceinline__ void tile_params(uint32_t w, int params, int t, int team, float2 (&v)[4 * NV]) {
   if constexpr (VEC == 8) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const float4 a = *reinterpret_cast<const float4*>(w + (j * team + t) * 4);
-      const float4 b = *reinterpret_cast<const float4*>(w + (params >> 1) + (j * team + t) * 4);
-      v[4 * j] = make_float2(a.x, a.y);
-      v[4 * j + 1] = make_float2(a.z, a.w);
-      v[4 * j + 2] = make_float2(b.x, b.y);
-      v[4 * j + 3] = make_float2(b.z, b.w);
+      const uint32_t at = w + (j * team + t) * 16;
+      const uint4 a = lds4(at), b = lds4(at + params * 2);
+      v[4 * j] = as_f2(a.x, a.y);
+      v[4 * j + 1] = as_f2(a.z, a.w);
+      v[4 * j + 2] = as_f2(b.x, b.y);
+      v[4 * j + 3] = as_f2(b.z, b.w);
     }
-  } else if constexpr (VEC == 2) {
-#pragma unroll
-    for (int i = 0; i < 4 * NV; ++i) v[i] = *reinterpret_cast<const float2*>(w + (i * team + t) * 2);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4 * NV; ++i) v[i] = make_float2(w[2 * i * team + t], w[(2 * i + 1) * team + t]);
+    for (int i = 0; i < 4 * NV; ++i) {
+      if constexpr (VEC == 2) {
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[i].x), "=f"(v[i].y) : "r"(w + (i * team + t) * 8) : "memory");
+      } else {
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i].x) : "r"(w + (2 * i * team + t) * 4) : "memory");
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i].y) : "r"(w + ((2 * i + 1) * team + t) * 4) : "memory");
+      }
+    }
   }
+}
+
+template <typename T>
+__device__ __forceinline__ float lds_one(uint32_t a) {
+  if constexpr (sizeof(T) == 4) {
+    float f;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+    return f;
+  } else {
+    unsigned short w;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(a) : "memory");
+    return Io<T>::one(w);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void sts_one(uint32_t a, float v) {
+  if constexpr (sizeof(T) == 4)
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+  else
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(static_cast<unsigned short>(Io<T>::pack(v, 0.f))) : "memory");
 }
 
 // A row's elements of this thread from a stage; zero past the width (EXACT: there is nothing past it, 8 NV elements of every thread are there)
 template <typename T, int VEC, int NV, bool EXACT>
-__device__ __forceinline__ void tile_load(const uint8_t* row, int d, int t, int team, float2 (&v)[4 * NV]) {
-  const T* p = reinterpret_cast<const T*>(row);
+__device__ __forceinline__ void tile_load(uint32_t p, int d, int t, int team, float2 (&v)[4 * NV]) {
   if constexpr (VEC == 8) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * team + t) * 8;
       if (EXACT || c < d) {
         if constexpr (sizeof(T) == 2) {
-          const uint4 w = *reinterpret_cast<const uint4*>(p + c);
+          const uint4 w = lds4(p + c * 2);
           v[4 * j] = Io<T>::two(w.x);
           v[4 * j + 1] = Io<T>::two(w.y);
           v[4 * j + 2] = Io<T>::two(w.z);
           v[4 * j + 3] = Io<T>::two(w.w);
         } else {
-          const float4 a = *reinterpret_cast<const float4*>(p + c), b = *reinterpret_cast<const float4*>(p + c + 4);
-          v[4 * j] = make_float2(a.x, a.y);
-          v[4 * j + 1] = make_float2(a.z, a.w);
-          v[4 * j + 2] = make_float2(b.x, b.y);
-          v[4 * j + 3] = make_float2(b.z, b.w);
+          const uint4 a = lds4(p + c * 4), b = lds4(p + c * 4 + 16);
+          v[4 * j] = as_f2(a.x, a.y);
+          v[4 * j + 1] = as_f2(a.z, a.w);
+          v[4 * j + 2] = as_f2(b.x, b.y);
+          v[4 * j + 3] = as_f2(b.z, b.w);
         }
       } else {
 #pragma unroll
@@ -100,34 +139,38 @@ __device__ __forceinline__ void tile_load(const uint8_t* row, int d, int t, int 
       const int c = (i * team + t) * 2;
       v[i] = make_float2(0.f, 0.f);
       if (c < d) {
-        if constexpr (sizeof(T) == 2)
-          v[i] = Io<T>::two(*reinterpret_cast<const uint32_t*>(p + c));
-        else
-          v[i] = *reinterpret_cast<const float2*>(p + c);
+        if constexpr (sizeof(T) == 2) {
+          uint32_t w;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(p + c * 2) : "memory");
+          v[i] = Io<T>::two(w);
+        } else {
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[i].x), "=f"(v[i].y) : "r"(p + c * 4) : "memory");
+        }
       }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NV; ++i) {
       const int a = 2 * i * team + t, b = a + team;
-      v[i] = make_float2(a < d ? static_cast<float>(p[a]) : 0.f, b < d ? static_cast<float>(p[b]) : 0.f);
+      v[i] = make_float2(0.f, 0.f);
+      if (a < d) v[i].x = lds_one<T>(p + a * static_cast<int>(sizeof(T)));
+      if (b < d) v[i].y = lds_one<T>(p + b * static_cast<int>(sizeof(T)));
     }
   }
 }
 template <typename T, int VEC, int NV, bool EXACT>
-__device__ __forceinline__ void tile_store(uint8_t* row, int d, int t, int team, const float2 (&v)[4 * NV]) {
-  T* p = reinterpret_cast<T*>(row);
+__device__ __forceinline__ void tile_store(uint32_t p, int d, int t, int team, const float2 (&v)[4 * NV]) {
   if constexpr (VEC == 8) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * team + t) * 8;
       if (!EXACT && c >= d) continue;
       if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(p + c) = make_uint4(Io<T>::pack(v[4 * j].x, v[4 * j].y), Io<T>::pack(v[4 * j + 1].x, v[4 * j + 1].y),
-                                                      Io<T>::pack(v[4 * j + 2].x, v[4 * j + 2].y), Io<T>::pack(v[4 * j + 3].x, v[4 * j + 3].y));
+        sts4(p + c * 2, Io<T>::pack(v[4 * j].x, v[4 * j].y), Io<T>::pack(v[4 * j + 1].x, v[4 * j + 1].y), Io<T>::pack(v[4 * j + 2].x, v[4 * j + 2].y),
+             Io<T>::pack(v[4 * j + 3].x, v[4 * j + 3].y));
       } else {
-        *reinterpret_cast<float4*>(p + c) = make_float4(v[4 * j].x, v[4 * j].y, v[4 * j + 1].x, v[4 * j + 1].y);
-        *reinterpret_cast<float4*>(p + c + 4) = make_float4(v[4 * j + 2].x, v[4 * j + 2].y, v[4 * j + 3].x, v[4 * j + 3].y);
+        sts4(p + c * 4, bits(v[4 * j].x), bits(v[4 * j].y), bits(v[4 * j + 1].x), bits(v[4 * j + 1].y));
+        sts4(p + c * 4 + 16, bits(v[4 * j + 2].x), bits(v[4 * j + 2].y), bits(v[4 * j + 3].x), bits(v[4 * j + 3].y));
       }
     }
   } else if constexpr (VEC == 2) {
@@ -136,16 +179,16 @@ __device__ __forceinline__ void tile_store(uint8_t* row, int d, int t, int team,
       const int c = (i * team + t) * 2;
       if (c >= d) continue;
       if constexpr (sizeof(T) == 2)
-        *reinterpret_cast<uint32_t*>(p + c) = Io<T>::pack(v[i].x, v[i].y);
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(p + c * 2), "r"(Io<T>::pack(v[i].x, v[i].y)) : "memory");
       else
-        *reinterpret_cast<float2*>(p + c) = v[i];
+        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(p + c * 4), "f"(v[i].x), "f"(v[i].y) : "memory");
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NV; ++i) {
       const int a = 2 * i * team + t, b = a + team;
-      if (a < d) Io<T>::put(p + a, v[i].x);
-      if (b < d) Io<T>::put(p + b, v[i].y);
+      if (a < d) sts_one<T>(p + a * static_cast<int>(sizeof(T)), v[i].x);
+      if (b < d) sts_one<T>(p + b * static_cast<int>(sizeof(T)), v[i].y);
     }
   }
 }
@@ -375,19 +418,20 @@ __device__ __forceinline__ float2 tile_stats(const float2 (&v)[4 * NV], int kind
 }
 
 // Shared memory: parameters | scratch of the sums | barriers | stages
-constexpr int kTileScratch = 8 * 32 * 8 + 2 * kTileMaxStages * 8 + 16;
+constexpr int kTileScratch = kTileTeams * 32 * 8 + 2 * kTileMaxStages * 8 + 16;
 
 template <typename T, int VEC, int NV, bool EXACT>
 __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forward_kernel(const JoinTileParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   float* par = reinterpret_cast<float*>(smem);  // w_s, b_s, w_pre, b_pre
+  const uint32_t par_at = smem_u32(smem);
   uint8_t* at = smem + 4 * p.params * 4;
   float2* scratch = reinterpret_cast<float2*>(at);
-  const uint32_t bars = smem_u32(at + 8 * 32 * 8);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(at + 8 * 32 * 8 + 2 * kTileMaxStages * 8);
+  const uint32_t bars = smem_u32(at + kTileTeams * 32 * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(at + kTileTeams * 32 * 8 + 2 * kTileMaxStages * 8);
   const TileRing<T> ring{p, at + kTileScratch, bars, abort_flag};
   const JoinParams& j = p.j;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   const int workers = blockDim.x - 32;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -423,7 +467,7 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
   for (int k = 0; k < n; ++k) {
     const int s = k % p.stages;
     if (!mbar_wait_warp(ring.full(s), (k / p.stages) & 1, abort_flag, &blocks_status, kDevTimeoutStats)) break;
-    uint8_t* stage = ring.stage(s);
+    const uint32_t stage = smem_u32(ring.stage(s));
     const long long r0 = static_cast<long long>(ring.first() + k * ring.step()) * p.tile_rows;
     const int rows = j.rows - r0 < p.tile_rows ? static_cast<int>(j.rows - r0) : p.tile_rows;
     for (int r = id; r - id < p.tile_rows; r += teams) {
@@ -443,12 +487,12 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
           for (int i = 0; i < 4 * NV; ++i) u[i] = __fmul2_rn(__fadd2_rn(u[i], f2(-st.x)), f2(st.y));
         }
         if (j.post_w != nullptr || j.scale != nullptr) {
-          tile_params<VEC, NV>(par, p.params, t, team, w);
+          tile_params<VEC, NV>(par_at, p.params, t, team, w);
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) u[i] = __fmul2_rn(u[i], w[i]);
         }
         if (j.post_b != nullptr) {
-          tile_params<VEC, NV>(par + p.params, p.params, t, team, w);
+          tile_params<VEC, NV>(par_at + 4 * p.params, p.params, t, team, w);
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) u[i] = __fadd2_rn(u[i], w[i]);
         }
@@ -472,11 +516,11 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
       if (j.pre_kind != kNormNone) {
         const float2 st = tile_stats<VEC, NV, EXACT>(x, j.pre_kind, j.pre_eps, d, inv, t, team, sum);
         if (on && t == 0 && j.pre_stats != nullptr) j.pre_stats[row] = st;
-        tile_params<VEC, NV>(par + 2 * p.params, p.params, t, team, w);
+        tile_params<VEC, NV>(par_at + 4 * 2 * p.params, p.params, t, team, w);
 #pragma unroll
         for (int i = 0; i < 4 * NV; ++i) x[i] = __fmul2_rn(__fmul2_rn(__fadd2_rn(x[i], f2(-st.x)), f2(st.y)), w[i]);
         if (j.pre_b != nullptr) {
-          tile_params<VEC, NV>(par + 3 * p.params, p.params, t, team, w);
+          tile_params<VEC, NV>(par_at + 4 * 3 * p.params, p.params, t, team, w);
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) x[i] = __fadd2_rn(x[i], w[i]);
         }
@@ -492,14 +536,15 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
 // A shared gate's gradient: a team adds up its rows of the current gate row in registers and leaves them in fp32 when the gate row
 // changes, in a place of its own for each gate row that the block's tiles touch ([blocks][group_slots][teams][8 team]);
 // join_tile_gate_kernel adds them up in the order of the blocks and teams.
-template <typename T, int VEC, bool EXACT>
-__global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(const JoinTileParams p) {
+template <typename T, int VEC, bool EXACT, bool JOIN>
+__global__ void __launch_bounds__(kTileThreads, JOIN ? 1 : 2) join_tile_backward_kernel(const JoinTileParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   float* par = reinterpret_cast<float*>(smem);  // w_s, b_s, w_pre
+  const uint32_t par_at = smem_u32(smem);
   uint8_t* at = smem + 3 * p.params * 4;
   float2* scratch = reinterpret_cast<float2*>(at);
-  const uint32_t bars = smem_u32(at + 8 * 32 * 8);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(at + 8 * 32 * 8 + 2 * kTileMaxStages * 8);
+  const uint32_t bars = smem_u32(at + kTileTeams * 32 * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(at + kTileTeams * 32 * 8 + 2 * kTileMaxStages * 8);
   const TileRing<T> ring{p, at + kTileScratch, bars, abort_flag};
   const JoinParams& j = p.j;
   const int lane = threadIdx.x & 31;
@@ -536,7 +581,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
     TileSum sum{scratch + (team > 32 ? id : 0) * 32, team, (team + 31) / 32, id, 0, t >> 5};
     const float inv = 1.0f / static_cast<float>(d);
     const int row_bytes = d * static_cast<int>(sizeof(T));
-    const bool shared_gate = p.block_tiles != 0;
+    const bool shared_gate = JOIN && p.block_tiles != 0;
     float2 sg_sum[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) sg_sum[i] = f2(0.f);
@@ -552,34 +597,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
         sg_sum[i] = f2(0.f);
       }
     };
+    // statistics and mask of the team's next row, asked for while this one is worked on
+    float2 next_post = f2(0.f), next_pre = f2(0.f);
+    int next_valid = 0;
+    auto row_facts = [&](int k, int r) {
+      const long long row = static_cast<long long>(ring.first() + k * ring.step()) * p.tile_rows + r;
+      next_valid = 0;
+      if (k >= n || r >= p.tile_rows || row >= j.rows) return;
+      if (JOIN) next_valid = j.mask == nullptr ? 1 : __ldcg(j.mask + row);
+      if (JOIN && j.post_kind != kNormNone) next_post = __ldcg(j.post_stats + row);
+      if (j.pre_kind != kNormNone) next_pre = __ldcg(j.pre_stats + row);
+    };
+    row_facts(0, id);
     for (int k = 0; k < n; ++k) {
       const int s = k % p.stages;
       const long long r0 = static_cast<long long>(ring.first() + k * ring.step()) * p.tile_rows;
-      // (statistics and mask of the first round: asked for before the wait)
-      float2 post = f2(0.f), pre = f2(0.f);
-      bool valid = false;
       const int rows = j.rows - r0 < p.tile_rows ? static_cast<int>(j.rows - r0) : p.tile_rows;
-      auto row_facts = [&](int r) {
-        const long long row = r0 + r;
-        const bool on = r < rows;
-        valid = j.u != nullptr && on && (j.mask == nullptr || __ldcg(j.mask + row) != 0);
-        if (on && j.post_kind != kNormNone) post = __ldcg(j.post_stats + row);
-        if (on && j.pre_kind != kNormNone) pre = __ldcg(j.pre_stats + row);
-        return on;
-      };
-      bool on = row_facts(id);
       if (!mbar_wait_warp(ring.full(s), (k / p.stages) & 1, abort_flag, &blocks_status, kDevTimeoutStats)) break;
-      uint8_t* stage = ring.stage(s);
+      const uint32_t stage = smem_u32(ring.stage(s));
       for (int r = id; r - id < p.tile_rows; r += teams) {
-        if (r != id) on = row_facts(r);
+        const bool on = r < rows;
+        const bool valid = next_valid != 0;
+        const float2 post = next_post, pre = next_pre;
+        if (r - id + teams < p.tile_rows)
+          row_facts(k, r + teams);
+        else
+          row_facts(k + 1, id);
         const long long row = r0 + r;
         const int off = on ? r * row_bytes : 0;
         float2 x[4], e[4], q[4], u[4], g[4], w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = e[i] = u[i] = f2(0.f), g[i] = f2(1.f);
         if (j.pre_kind != kNormNone && on) tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[0] * p.slot + off, d, t, team, x);
-        if (j.dy != nullptr && on) tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[3] * p.slot + off, d, t, team, e);
-        if (valid) {
+        if (JOIN && j.dy != nullptr && on) tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[3] * p.slot + off, d, t, team, e);
+        if (JOIN && valid) {
           tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[1] * p.slot + off, d, t, team, u);
           if (j.gate != nullptr) {
             if (!shared_gate) {
@@ -597,10 +648,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
           }
         }
         if (j.pre_kind != kNormNone) {
-          if (valid) {
-            tile_params<VEC, 1>(par, p.params, t, team, w);
+          if (JOIN && valid) {
+            tile_params<VEC, 1>(par_at, p.params, t, team, w);
             if (j.post_b != nullptr) {
-              tile_params<VEC, 1>(par + p.params, p.params, t, team, q);
+              tile_params<VEC, 1>(par_at + 4 * p.params, p.params, t, team, q);
 #pragma unroll
               for (int i = 0; i < 4; ++i) x[i] = __ffma2_rn(__ffma2_rn(u[i], w[i], q[i]), g[i], x[i]);
             } else {
@@ -614,7 +665,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
 #pragma unroll
             for (int i = 0; i < 4; ++i) q[i] = f2(0.f);
           }
-          tile_params<VEC, 1>(par + 2 * p.params, p.params, t, team, w);
+          tile_params<VEC, 1>(par_at + 4 * 2 * p.params, p.params, t, team, w);
           float2 c1 = f2(0.f), c2 = f2(0.f);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -631,9 +682,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
           for (int i = 0; i < 4; ++i) e[i] = __ffma2_rn(f2(pre.y), __ffma2_rn(x[i], f2(m2), __fadd2_rn(q[i], f2(m1))), e[i]);
         }
         if (on && p.out_slot[0] >= 0) tile_store<T, VEC, 1, EXACT>(stage + p.out_slot[0] * p.slot + off, d, t, team, e);
-        if (j.u == nullptr) continue;
+        if constexpr (!JOIN) continue;
         float2 a1 = f2(0.f), a2 = f2(0.f);
-        tile_params<VEC, 1>(par, p.params, t, team, w);
+        tile_params<VEC, 1>(par_at, p.params, t, team, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           e[i] = valid ? __fmul2_rn(e[i], g[i]) : f2(0.f);  // z
@@ -647,7 +698,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
           // gradient of the logits: z (n w_s + b_s) (1 - sigmoid)
           float2 b[4];
           if (j.post_b != nullptr) {
-            tile_params<VEC, 1>(par + p.params, p.params, t, team, b);
+            tile_params<VEC, 1>(par_at + 4 * p.params, p.params, t, team, b);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) b[i] = f2(0.f);
@@ -695,7 +746,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) join_tile_backward_kernel(con
   float* buf = reinterpret_cast<float*>(ring.stage0);
   const bool worker = static_cast<int>(threadIdx.x) < workers;
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
+  for (int s = JOIN ? 0 : 2; s < 4; ++s) {
     const float2(&v)[4] = s == 0 ? s1 : s == 1 ? s2 : s == 2 ? s3 : s4;
     __syncthreads();
     if (worker) {
@@ -757,30 +808,34 @@ __global__ void __launch_bounds__(1024) join_tile_sums_kernel(const JoinTileSums
   if (p.out[2] != nullptr) p.out[2][c] = scale * b;
 }
 
-// Gradient of the shared gate rows: the teams of every block that has rows of one, eight chains a column
+// Gradient of the shared gate rows: the teams of every block that has rows of one, 32 chains a column
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) join_tile_gate_kernel(const JoinTileParams p) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) join_tile_gate_kernel(const JoinTileParams p) {
+  __shared__ float part[32][33];
   grid_dependency_wait();
   grid_dependents_launch();
   const JoinParams& j = p.j;
   const int x = threadIdx.x & 31, chain = threadIdx.x >> 5;
-  const int team = j.team, teams = kTileWarps * 32 / team;
+  const int team = j.team, teams = p.workers / team;
   const long long block_rows = static_cast<long long>(p.block_tiles) * p.tile_rows;
   const long long group = blockIdx.y, begin = group * j.gate_rows, end = begin + j.gate_rows;
   const int b0 = static_cast<int>(begin / block_rows), b1 = static_cast<int>((end - 1) / block_rows);
   const int c = blockIdx.x * 32 + x;  // element of the teams' order
   float a = 0.f;
-  for (int k = chain; c < 8 * team && k < (b1 - b0 + 1) * teams; k += 8) {
-    const int block = b0 + k / teams;
-    const long long slot = group - block * block_rows / j.gate_rows;
-    a += __ldcg(j.gate_part + ((static_cast<long long>(block) * p.group_slots + slot) * teams + k % teams) * (8 * team) + c);
+  if (c < 8 * team) {
+    const long long step = static_cast<long long>(8) * team;
+    for (int block = b0; block <= b1; ++block) {
+      const long long slot = group - block * block_rows / j.gate_rows;
+      const float* from = j.gate_part + ((static_cast<long long>(block) * p.group_slots + slot) * teams) * step + c;
+      // (teams of a block and chains: block after block continues where the last one stopped)
+      for (int k = (chain + 32 - (block - b0) * teams % 32) % 32; k < teams; k += 32) a += __ldcg(from + k * step);
+    }
   }
   part[chain][x] = a;
   __syncthreads();
   if (chain != 0) return;
   a = 0.f;
-  for (int k = 0; k < 8; ++k) a += part[k][x];
+  for (int k = 0; k < 32; ++k) a += part[k][x];
   const int col = tile_col<VEC>(c / team, c % team, team);
   if (c < 8 * team && col < j.d) Io<T>::put(static_cast<T*>(j.dgate) + group * j.d + col, a);
 }

@@ -103,6 +103,28 @@ def test_against_float64(rows, d, hidden):
     _compare(_run(t, "silu"), _want(t, "silu", torch.bfloat16), (rows, d, hidden))
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("rows,d,hidden", [(7200, 64, 64), (9473, 8, 8), (9473, 128, 64), (100001, 16, 64), (120000, 8, 136), (60003, 64, 256), (19000, 72, 72),
+                                           (40001, 120, 320), (30000, 128, 512), (7169, 56, 1000), (70007, 24, 192)])
+def test_narrow_tensors_of_many_rows(rows, d, hidden, act):
+    """Several tiles a CTA pair, one to sixteen blocks of hidden units, odd numbers of them among these."""
+    type = torch.float16 if hidden % 3 == 0 else torch.bfloat16
+    t = _make(rows, d, hidden, type)
+    _compare(_run(t, act), _want(t, act, type), (rows, d, hidden, act))
+
+
+def test_narrow_rows_do_not_touch_one_another():
+    t = _make(20000, 64, 128, torch.bfloat16)
+    w = [t[k] for k in ("w_a", "w_b", "w_s")]
+    want = blocks.gated_feed_forward(t["x"], *w)
+    x = t["x"].clone()
+    x[777::1000] = float("nan")
+    got = blocks.gated_feed_forward(x, *w)
+    keep = torch.ones(20000, dtype=torch.bool, device=DEV)
+    keep[777::1000] = False
+    assert torch.equal(got[keep], want[keep]) and not torch.isfinite(got[~keep]).any()
+
+
 @pytest.mark.parametrize("rows,d,hidden", [(1, 64, 128), (5, 384, 1536), (300, 200, 536), (2100, 256, 768), (12000, 128, 512)])
 @pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
