@@ -61,28 +61,37 @@ __device__ __forceinline__ uint32_t ff_pack(float a, float b) {
 }
 
 __device__ __forceinline__ float2 ff_f2(float v) { return make_float2(v, v); }
-// 1 / (1 + 2^(-a log2 e)) of two values with one reciprocal, of the product of the two denominators (the special-function unit, four
-// lanes a clock, is what an epilogue of few products waits for). The exponent is held below 64, so that the product stays finite:
-// sigmoid(a) is 2^-63 for a < -43, off by less than 1e-19.
-__device__ __forceinline__ float2 ff_sigmoid2(float2 a) {
-  const float2 n = __fmul2_rn(a, ff_f2(-1.44269504f));
-  float2 x;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.x) : "f"(fminf(n.x, 63.f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.y) : "f"(fminf(n.y, 63.f)));
+// 1 / (1 + 2^(-a log2 e)) of four values with one reciprocal, of the product of the four denominators (the special-function unit, four
+// lanes a clock and scheduler, is what an epilogue of few products waits for). The exponent is held below 31, so that the product stays
+// finite: sigmoid(a) is 2^-31 for a < -21, off by less than 5e-10.
+__device__ __forceinline__ void ff_sigmoid4(float2 a, float2 b, float2& sa, float2& sb) {
+  float2 x = __fmul2_rn(a, ff_f2(-1.44269504f)), y = __fmul2_rn(b, ff_f2(-1.44269504f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.x) : "f"(fminf(x.x, 31.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.y) : "f"(fminf(x.y, 31.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(fminf(y.x, 31.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(fminf(y.y, 31.f)));
   x = __fadd2_rn(x, ff_f2(1.f));
+  y = __fadd2_rn(y, ff_f2(1.f));
+  const float px = x.x * x.y, py = y.x * y.y;
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x.x * x.y));
-  return __fmul2_rn(ff_f2(r), make_float2(x.y, x.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(px * py));
+  sa = __fmul2_rn(ff_f2(r * py), make_float2(x.y, x.x));
+  sb = __fmul2_rn(ff_f2(r * px), make_float2(y.y, y.x));
 }
+__device__ __forceinline__ float2 ff_at(const uint32_t (&v)[16], int j) { return make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); }
 // Values of 16 neighbouring units: act(a) b
 __device__ __forceinline__ void ff_gate16(const uint32_t (&a)[16], const uint32_t (&b)[16], int act, float (&h)[16]) {
   if (act == kFfSilu) {
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-      const float2 va = make_float2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), vb = make_float2(__uint_as_float(b[j]), __uint_as_float(b[j + 1]));
-      const float2 r = __fmul2_rn(__fmul2_rn(va, ff_sigmoid2(va)), vb);
+    for (int j = 0; j < 16; j += 4) {
+      const float2 u = ff_at(a, j), v = ff_at(a, j + 2);
+      float2 su, sv;
+      ff_sigmoid4(u, v, su, sv);
+      const float2 r = __fmul2_rn(__fmul2_rn(u, su), ff_at(b, j)), q = __fmul2_rn(__fmul2_rn(v, sv), ff_at(b, j + 2));
       h[j] = r.x;
       h[j + 1] = r.y;
+      h[j + 2] = q.x;
+      h[j + 3] = q.y;
     }
   } else {
 #pragma unroll
@@ -96,26 +105,30 @@ __device__ __forceinline__ void ff_gate16(const uint32_t (&a)[16], const uint32_
 __device__ __forceinline__ void ff_gate_back16(const uint32_t (&a)[16], const uint32_t (&b)[16], const uint32_t (&d)[16], int act, float (&da)[16],
                                                float (&db)[16], float (&h)[16]) {
 #pragma unroll
-  for (int j = 0; j < 16; j += 2) {
-    const float2 va = make_float2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), vb = make_float2(__uint_as_float(b[j]), __uint_as_float(b[j + 1]));
-    const float2 vd = make_float2(__uint_as_float(d[j]), __uint_as_float(d[j + 1]));
-    float2 f, slope;
-    if (act == kFfSilu) {
-      const float2 s = ff_sigmoid2(va);
-      f = __fmul2_rn(va, s);
-      slope = __ffma2_rn(f, __fadd2_rn(ff_f2(1.f), make_float2(-s.x, -s.y)), s);  // s (1 + a (1 - s))
-    } else {
-      const float2 cdf = make_float2(0.5f * (1.0f + erff(va.x * 0.70710678f)), 0.5f * (1.0f + erff(va.y * 0.70710678f)));
-      f = __fmul2_rn(va, cdf);
-      slope = make_float2(fmaf(va.x * 0.39894228f, __expf(-0.5f * va.x * va.x), cdf.x), fmaf(va.y * 0.39894228f, __expf(-0.5f * va.y * va.y), cdf.y));
+  for (int i = 0; i < 16; i += 4) {
+    float2 s[2];
+    if (act == kFfSilu) ff_sigmoid4(ff_at(a, i), ff_at(a, i + 2), s[0], s[1]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int j = i + 2 * k;
+      const float2 va = ff_at(a, j), vb = ff_at(b, j), vd = ff_at(d, j);
+      float2 f, slope;
+      if (act == kFfSilu) {
+        f = __fmul2_rn(va, s[k]);
+        slope = __ffma2_rn(f, __fadd2_rn(ff_f2(1.f), make_float2(-s[k].x, -s[k].y)), s[k]);  // s (1 + a (1 - s))
+      } else {
+        const float2 cdf = make_float2(0.5f * (1.0f + erff(va.x * 0.70710678f)), 0.5f * (1.0f + erff(va.y * 0.70710678f)));
+        f = __fmul2_rn(va, cdf);
+        slope = make_float2(fmaf(va.x * 0.39894228f, __expf(-0.5f * va.x * va.x), cdf.x), fmaf(va.y * 0.39894228f, __expf(-0.5f * va.y * va.y), cdf.y));
+      }
+      const float2 x = __fmul2_rn(__fmul2_rn(vd, vb), slope), y = __fmul2_rn(vd, f), z = __fmul2_rn(f, vb);
+      da[j] = x.x;
+      da[j + 1] = x.y;
+      db[j] = y.x;
+      db[j + 1] = y.y;
+      h[j] = z.x;
+      h[j + 1] = z.y;
     }
-    const float2 x = __fmul2_rn(__fmul2_rn(vd, vb), slope), y = __fmul2_rn(vd, f), z = __fmul2_rn(f, vb);
-    da[j] = x.x;
-    da[j + 1] = x.y;
-    db[j] = y.x;
-    db[j + 1] = y.y;
-    h[j] = z.x;
-    h[j + 1] = z.y;
   }
 }
 

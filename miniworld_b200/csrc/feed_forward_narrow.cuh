@@ -8,11 +8,13 @@
 //   gate     : h[row, u] = act(D1[row, u]) * D1[row, 64 + u]  -> 16 bits, into tensor memory
 //   G2(block): D2[row, :] += h[row, 0:64] * W_s[:, block]^T                            (M 256, N 64 or 128, A operand from tensor memory)
 //
-// CTA 0 loads the block's rows of W_a, CTA 1 those of W_b, each its half of the rows of W_s. Tensor memory: D1[0], D1[1], D2[0], D2[1]
-// (128 columns each); a tile's h borrows the D2 buffer that does not accumulate. Blocks alternate between D1's buffers and between two
-// groups of eight warps by their running number gb (tiles may have an odd number of blocks). What bounds it is the gate's arithmetic:
-// 64 x 128 values a block and group against 256 + 128 cycles of products.
-// Warps: 0 weights, 1 G1, 2 input tiles, 3 G2, 4-19 the gate's groups, 20-23 output. All waits are bounded.
+// CTA 0 loads the block's rows of W_a, CTA 1 those of W_b, each its half of the rows of W_s. Tensor memory: D1[0..2] (128 columns each)
+// and D2 (two of 64 for D <= 64, one of 128). Blocks go round three groups of eight warps by their running number gb; a group reads its
+// D1 into registers and leaves h in the same columns, which are free again once G2 of the block is complete.
+// What bounds it is the special-function unit: an exponential a unit and a reciprocal for four, 1.25 x 64 x 128 / 16 = 640 cycles a
+// block and SM, so the groups are there to keep it busy while others wait for products, tensor memory and barriers: 196608 x 64 x 256
+// with two groups (h in the idle D2, a reciprocal for two) 42 us, of which that unit was busy half of the time; now XX us.
+// Warps: 0 weights, 1 G1, 2 input tiles, 3 G2, 4-27 the gate's groups, 28-31 output. All waits are bounded.
 #pragma once
 
 #include "feed_forward.cuh"
@@ -27,19 +29,20 @@ struct FfNarrowParams {
   int blocks;     // of 64 hidden units
 };
 
-constexpr int kNwThreads = 768;
-constexpr int kNwWStages = 5;  // (the order of waits below relies on it: see blk_done)
+constexpr int kNwThreads = 1024;
+constexpr int kNwGroups = 3;
+constexpr int kNwWStages = 5;
 constexpr int kNwXStages = 3;
 constexpr int kNwWStageBytes = 24576;  // 64 rows of W_a or W_b, up to 64 of W_s
 constexpr int kNwXBytes = 32768;
 constexpr int kNwSmemBytes = kNwXStages * kNwXBytes + kNwWStages * kNwWStageBytes + 256 + 1024;
-constexpr uint32_t kNwColD2 = 256;
+constexpr uint32_t kNwColD2 = 128 * kNwGroups;
 
 // HALVES: 64-wide parts of D
 template <bool F16, int ACT, int HALVES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNwThreads, 1)
 ff_narrow_kernel(const __grid_constant__ FfMaps maps, const FfNarrowParams p) {
-  constexpr int WS = kNwWStages, XS = kNwXStages;
+  constexpr int WS = kNwWStages, XS = kNwXStages, G = kNwGroups;
   constexpr int kN2 = 64 * HALVES;  // columns of D2
   constexpr uint32_t kWBytes = HALVES * 8192 + (kN2 / 2) * 128;
   extern __shared__ uint8_t smem_raw[];
@@ -52,13 +55,17 @@ ff_narrow_kernel(const __grid_constant__ FfMaps maps, const FfNarrowParams p) {
   constexpr int B0 = 2 * XS;
   auto w_full = [&](int s) { return bar_base + 8u * (B0 + s); };         // leader: bytes of both CTAs
   auto blk_done = [&](int s) { return bar_base + 8u * (B0 + WS + s); };  // both: G2 of the block in weight stage s is complete
-  auto d1_full = [&](int b) { return bar_base + 8u * (B0 + 2 * WS + b); };       // both
-  auto d1_empty = [&](int b) { return bar_base + 8u * (B0 + 2 * WS + 2 + b); };  // leader: 8 warps of each CTA
-  auto h_full = [&](int b) { return bar_base + 8u * (B0 + 2 * WS + 4 + b); };    // leader: 8 warps of each CTA
-  auto d2_full = [&](int b) { return bar_base + 8u * (B0 + 2 * WS + 6 + b); };   // both
-  auto d2_empty = [&](int b) { return bar_base + 8u * (B0 + 2 * WS + 8 + b); };  // leader: 4 warps of each CTA
-  auto d2_read = [&](int b) { return bar_base + 8u * (B0 + 2 * WS + 10 + b); };  // own: this CTA has read D2[b]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_base - smem_u32(smem_raw)) + 8 * (B0 + 2 * WS + 12));
+  auto d1_full = [&](int g) { return bar_base + 8u * (B0 + 2 * WS + g); };          // both
+  auto d1_free = [&](int g) { return bar_base + 8u * (B0 + 2 * WS + G + g); };      // both: G2 has read h out of it
+  auto h_full = [&](int g) { return bar_base + 8u * (B0 + 2 * WS + 2 * G + g); };   // leader: 8 warps of each CTA
+  constexpr int B1 = B0 + 2 * WS + 3 * G;
+  auto d2_full = [&](int b) { return bar_base + 8u * (B1 + b); };        // both
+  auto d2_empty = [&](int b) { return bar_base + 8u * (B1 + 2 + b); };   // leader: 4 warps of each CTA
+  // the D2 buffer of tile t and how often it has been used before
+  auto d2_of = [&](int t) { return HALVES == 1 ? t & 1 : 0; };
+  auto d2_use = [&](int t) { return HALVES == 1 ? t >> 1 : t; };
+  auto d2_col = [&](int t) { return kNwColD2 + (HALVES == 1 ? (t & 1) * 64u : 0u); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_base - smem_u32(smem_raw)) + 8 * (B1 + 4));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* const status = &blocks_status;
 
@@ -74,13 +81,14 @@ ff_narrow_kernel(const __grid_constant__ FfMaps maps, const FfNarrowParams p) {
       mbar_init(w_full(s), 1);
       mbar_init(blk_done(s), 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(d1_full(s), 1);
-      mbar_init(d1_empty(s), 16);
-      mbar_init(h_full(s), 16);
-      mbar_init(d2_full(s), 1);
-      mbar_init(d2_empty(s), 8);
-      mbar_init(d2_read(s), 4);
+    for (int g = 0; g < G; ++g) {
+      mbar_init(d1_full(g), 1);
+      mbar_init(d1_free(g), 1);
+      mbar_init(h_full(g), 16);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(d2_full(b), 1);
+      mbar_init(d2_empty(b), 8);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -151,17 +159,17 @@ ff_narrow_kernel(const __grid_constant__ FfMaps maps, const FfNarrowParams p) {
       constexpr uint32_t idesc = umma_idesc(256, 128, false, false, F16 ? kFmtF16 : kFmtBF16, F16 ? kFmtF16 : kFmtBF16);
       int t = 0, hb = 0;
       for (int gb = 0; gb < total; ++gb) {
-        const int s = t % XS, slot = gb % WS, b = gb & 1;
+        const int s = t % XS, slot = gb % WS, g = gb % G;
         if (hb == 0 && !mbar_wait(x_full(s), (t / XS) & 1, abort_flag, status, kDevTimeoutMma)) break;
         if (!mbar_wait(w_full(slot), static_cast<uint32_t>((gb / WS) & 1), abort_flag, status, kDevTimeoutMma)) break;
-        if (!mbar_wait(d1_empty(b), static_cast<uint32_t>(((gb >> 1) & 1) ^ 1), abort_flag, status, kDevTimeoutMma)) break;
+        if (!mbar_wait(d1_free(g), static_cast<uint32_t>(((gb / G) & 1) ^ 1), abort_flag, status, kDevTimeoutMma)) break;
         tc_fence_after();
         const uint32_t xs = x_base + s * kNwXBytes, ws = w_base + slot * kNwWStageBytes;
 #pragma unroll
         for (int ks = 0; ks < 4 * HALVES; ++ks)
-          umma_pair(tmem + b * 128, umma_desc_kmajor(xs + (ks >> 2) * 16384) + static_cast<uint64_t>((ks & 3) * 2),
+          umma_pair(tmem + g * 128, umma_desc_kmajor(xs + (ks >> 2) * 16384) + static_cast<uint64_t>((ks & 3) * 2),
                     umma_desc_kmajor(ws + (ks >> 2) * 8192) + static_cast<uint64_t>((ks & 3) * 2), idesc, ks != 0 ? 1u : 0u);
-        umma_commit_pair(d1_full(b));
+        umma_commit_pair(d1_full(g));
         if (++hb == nb) {
           umma_commit_pair(x_empty(s));
           hb = 0;
@@ -176,60 +184,46 @@ ff_narrow_kernel(const __grid_constant__ FfMaps maps, const FfNarrowParams p) {
       constexpr uint32_t idesc = umma_idesc(256, kN2, false, false, F16 ? kFmtF16 : kFmtBF16, F16 ? kFmtF16 : kFmtBF16);
       int t = 0, hb = 0;
       for (int gb = 0; gb < total; ++gb) {
-        const int slot = gb % WS, b = gb & 1;
-        // D2[t & 1] last held tile t - 2 (and lent columns to h during tile t - 1, whose G2s this thread has issued before)
-        if (hb == 0 && !mbar_wait(d2_empty(t & 1), ((t >> 1) & 1) ^ 1u, abort_flag, status, kDevTimeoutMma)) break;
-        if (!mbar_wait(h_full(b), static_cast<uint32_t>((gb >> 1) & 1), abort_flag, status, kDevTimeoutMma)) break;
+        const int slot = gb % WS, g = gb % G;
+        if (hb == 0 && !mbar_wait(d2_empty(d2_of(t)), (d2_use(t) & 1) ^ 1u, abort_flag, status, kDevTimeoutMma)) break;
+        if (!mbar_wait(h_full(g), static_cast<uint32_t>((gb / G) & 1), abort_flag, status, kDevTimeoutMma)) break;
         tc_fence_after();
         const uint32_t ws = w_base + slot * kNwWStageBytes + 16384;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          umma_pair_ta(tmem + kNwColD2 + (t & 1) * 128, tmem + kNwColD2 + ((t + 1) & 1) * 128 + ((gb >> 1) & 1) * 64 + b * 32 + ks * 8,
-                       umma_desc_kmajor(ws) + static_cast<uint64_t>(ks * 2), idesc, (hb | ks) != 0 ? 1u : 0u);
+        for (int ks = 0; ks < 4; ++ks)  // (h of units 0-31 and of units 32-63: see the gate)
+          umma_pair_ta(tmem + d2_col(t), tmem + g * 128 + (ks >> 1) * 32 + (ks & 1) * 8, umma_desc_kmajor(ws) + static_cast<uint64_t>(ks * 2), idesc,
+                       (hb | ks) != 0 ? 1u : 0u);
         umma_commit_pair(blk_done(slot));
+        umma_commit_pair(d1_free(g));
         if (++hb == nb) {
-          umma_commit_pair(d2_full(t & 1));
+          umma_commit_pair(d2_full(d2_of(t)));
           hb = 0;
           ++t;
         }
       }
     }
-  } else if (warp < 20) {
-    // ------------------------------------------------------------ gate: a row and 32 of the block's 64 units a thread
+  } else if (warp < 4 + 8 * G) {
+    // ------------------------------------------------------------ gate: a row and 32 of the block's 64 units a thread, 16 at a time.
+    // h (16 columns) replaces the thread's own values of a, which no other thread reads.
     const int grp = (warp - 4) >> 3, uh = ((warp - 4) >> 2) & 1;
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_d1 = tmem + lanes + grp * 128 + uh * 32;
-    int read_tile = -1;  // the last tile before which this group has waited for D2 to be read
-    for (int gb = grp; gb < total; gb += 2) {
-      const int t = gb / nb;
-      if (!mbar_wait_warp(d1_full(grp), static_cast<uint32_t>((gb >> 1) & 1), abort_flag, status, kDevTimeoutEpilogue)) break;
+    const uint32_t d1 = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + grp * 128 + uh * 32;
+    uint32_t ph = 0;
+    for (int gb = grp; gb < total; gb += G, ph ^= 1u) {
+      if (!mbar_wait_warp(d1_full(grp), ph, abort_flag, status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
-      uint32_t va[2][16], vb[2][16], o[16];
+      uint32_t o[16];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        tmem_ld16(t_d1 + c * 16, va[c]);
-        tmem_ld16(t_d1 + 64 + c * 16, vb[c]);
-      }
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_leader(d1_empty(grp), rank);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+        uint32_t va[16], vb[16];
+        tmem_ld16(d1 + c * 16, va);
+        tmem_ld16(d1 + 64 + c * 16, vb);
+        tmem_ld_wait();
         float h[16];
-        ff_gate16(va[c], vb[c], ACT, h);
+        ff_gate16(va, vb, ACT, h);
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[8 * c + j] = ff_pack<F16>(h[2 * j], h[2 * j + 1]);
       }
-      // these columns are free once G2 of block gb - 4 is complete (block gb + 1, the next one in its weight stage, comes later), and,
-      // before the first h of a tile, once the output warps have read tile t - 1 out of the D2 buffer that h borrows
-      if (gb >= 4 && !mbar_wait_warp(blk_done((gb - 4) % WS), static_cast<uint32_t>(((gb - 4) / WS) & 1), abort_flag, status, kDevTimeoutEpilogue)) break;
-      if (t >= 1 && read_tile != t) {
-        if (!mbar_wait_warp(d2_read((t + 1) & 1), static_cast<uint32_t>(((t - 1) >> 1) & 1), abort_flag, status, kDevTimeoutEpilogue)) break;
-        read_tile = t;
-      }
-      tc_fence_after();
-      tmem_st16(tmem + lanes + kNwColD2 + ((t + 1) & 1) * 128 + ((gb >> 1) & 1) * 64 + grp * 32 + uh * 16, o);
+      tmem_st16(d1, o);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -240,22 +234,19 @@ ff_narrow_kernel(const __grid_constant__ FfMaps maps, const FfNarrowParams p) {
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     for (int t = 0; t < my_tiles; ++t) {
       const long long row = static_cast<long long>(pair + t * num_pairs) * 256 + static_cast<int>(rank) * 128 + (warp & 3) * 32 + lane;
-      if (!mbar_wait_warp(d2_full(t & 1), (t >> 1) & 1, abort_flag, status, kDevTimeoutEpilogue)) break;
+      if (!mbar_wait_warp(d2_full(d2_of(t)), d2_use(t) & 1, abort_flag, status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
       uint16_t* out = static_cast<uint16_t*>(p.y) + row * p.d;
 #pragma unroll
       for (int c = 0; c < kN2; c += 32) {
         uint32_t v[2][16];
-        tmem_ld16(tmem + lanes + kNwColD2 + (t & 1) * 128 + c, v[0]);
-        tmem_ld16(tmem + lanes + kNwColD2 + (t & 1) * 128 + c + 16, v[1]);
+        tmem_ld16(tmem + lanes + d2_col(t) + c, v[0]);
+        tmem_ld16(tmem + lanes + d2_col(t) + c + 16, v[1]);
         tmem_ld_wait();
         if (c + 32 == kN2) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(d2_read(t & 1));
-            mbar_arrive_leader(d2_empty(t & 1), rank);
-          }
+          if (lane == 0) mbar_arrive_leader(d2_empty(d2_of(t)), rank);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {

@@ -823,12 +823,14 @@ __global__ void __launch_bounds__(1024) join_tile_gate_kernel(const JoinTilePara
   const int c = blockIdx.x * 32 + x;  // element of the teams' order
   float a = 0.f;
   if (c < 8 * team) {
-    const long long step = static_cast<long long>(8) * team;
-    for (int block = b0; block <= b1; ++block) {
-      const long long slot = group - block * block_rows / j.gate_rows;
-      const float* from = j.gate_part + ((static_cast<long long>(block) * p.group_slots + slot) * teams) * step + c;
-      // (teams of a block and chains: block after block continues where the last one stopped)
-      for (int k = (chain + 32 - (block - b0) * teams % 32) % 32; k < teams; k += 32) a += __ldcg(from + k * step);
+    // (the first block's rows may begin in an earlier gate row; every later block begins in this one)
+    const int slot = static_cast<int>(group - b0 * block_rows / j.gate_rows);
+    const int places = (b1 - b0 + 1) * teams;
+#pragma unroll 4
+    for (int k = chain; k < places; k += 32) {
+      const int block = k / teams;
+      const int place = ((b0 + block) * p.group_slots + (block == 0 ? slot : 0)) * teams + k - block * teams;
+      a += __ldcg(j.gate_part + static_cast<long long>(place) * (8 * team) + c);
     }
   }
   part[chain][x] = a;
