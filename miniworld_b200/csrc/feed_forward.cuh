@@ -33,6 +33,7 @@ enum FfAct : int { kFfSilu = 0, kFfGelu = 1 };
 struct FfMaps {
   CUtensorMap a[3];
   CUtensorMap b[3];
+  CUtensorMap out[3];  // FfParams::staged: boxes of 32 columns by 32 rows, 64-byte swizzle
 };
 
 struct FfParams {
@@ -44,16 +45,18 @@ struct FfParams {
   int kb, kb_second;   // 64-deep k blocks of the first and of the second segment
   int bn;              // accumulator columns of an output tile (kFfUp and kFfHidden: of its a | b part)
   int splits, kb_split;  // kFfWeights, SPLIT: parts of the k range, k blocks of each
-  const void* kept[2]; // kFfGrad: a and b of the forward, fp16, rows `ld` apart
+  int staged;          // outputs leave through shared memory
+  const void* kept[2]; // kFfGrad: a and b of the forward, fp16: see ff_kept_at
   void* keep[2];       // kFfUp: where to leave them, or null
   int type;            // kFfWeights: of `out`, 0 bf16, 1 fp32, 2 fp16
 };
 
-constexpr int kFfStages = 6;
+constexpr int kFfStages = 5;
 constexpr int kFfStageBytes = 32768;  // 128 rows of the first operand, up to 128 of the second, 64 deep
 constexpr int kFfEpilogueWarps = 16;
 constexpr int kFfThreads = 64 + 32 * kFfEpilogueWarps;
-constexpr int kFfSmemBytes = kFfStages * kFfStageBytes + 256 + 1024;
+constexpr int kFfBoxBytes = 2048;     // 32 x 32 values of an output; two for each epilogue warp
+constexpr int kFfSmemBytes = kFfStages * kFfStageBytes + kFfEpilogueWarps * 2 * kFfBoxBytes + 256 + 1024;
 
 template <bool F16>
 __device__ __forceinline__ uint32_t ff_pack(float a, float b) {
@@ -170,6 +173,16 @@ __device__ __forceinline__ void ff_put16(void* out, size_t i, const float (&v)[1
   }
 }
 
+// Where the forward leaves a row's 16 neighbours of a or b for the backward: a warp's 32 rows of them lie together (1 KB), since the
+// same threads hold them in both passes and no product reads them.
+__device__ __forceinline__ size_t ff_kept_at(int row, int col, long long ld) {
+  return (static_cast<size_t>(row >> 5) * (ld >> 4) + (col >> 4)) * 512 + (row & 31) * 16;
+}
+template <bool F16>
+__device__ __forceinline__ void ff_pack16(const float (&v)[16], uint32_t (&w)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = ff_pack<F16>(v[2 * j], v[2 * j + 1]);
+}
 // 16 values as fp16, saturating; p on a 32-byte boundary
 __device__ __forceinline__ void ff_keep16(__half* p, const uint32_t (&v)[16]) {
   uint32_t w[8];
@@ -205,7 +218,8 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bar_base = base + S * kFfStageBytes;
+  const uint32_t box_base = base + S * kFfStageBytes;
+  const uint32_t bar_base = box_base + kFfEpilogueWarps * 2 * kFfBoxBytes;
   auto full = [&](int s) { return bar_base + 8u * s; };
   auto empty = [&](int s) { return bar_base + 8u * (S + s); };
   auto acc_full = [&](int a) { return bar_base + 8u * (2 * S + a); };
@@ -235,7 +249,8 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     fence_mbar_init();
     for (int i = 0; i < 3; ++i) {
       if (i == 0 || OP == kFfWeights || (i == 1 && SECOND)) prefetch_tmap(&maps.a[i]);
-      if (i == 0 || OP == kFfHidden || (i == 1 && OP != kFfDown)) prefetch_tmap(&maps.b[i]);
+      if (i == 0 || OP == kFfHidden || (i == 1 && OP != kFfDown && OP != kFfGrad)) prefetch_tmap(&maps.b[i]);
+      if (p.staged && (i == 0 || OP == kFfHidden || (i == 1 && OP == kFfGrad))) prefetch_tmap(&maps.out[i]);
     }
   }
   if (warp == 1) {
@@ -428,7 +443,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     // of a and b, of which there is one set; dh has two).
     const int q = warp & 3, part = (warp - 2) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    int it = 0;
+    int it = 0, boxes = 0;
     for (int i = first; i < tiles; i += step, ++it) {
       const Tile t = tile_at(i);
       const int acc = it & 1;
@@ -439,7 +454,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
       auto kept = [&](int col) {
         ka[0] = ka[1] = kb[0] = kb[1] = make_uint4(0u, 0u, 0u, 0u);
         if (!in || col >= p.cols) return;
-        const size_t at = (static_cast<size_t>(row) * p.ld + col) * 2;
+        const size_t at = ff_kept_at(row, col, p.ld) * 2;
         ld_gpu_chunks(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.kept[0]) + at), true, ka);
         ld_gpu_chunks(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.kept[1]) + at), true, kb);
       };
@@ -451,13 +466,31 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
         __syncwarp();
         if (lane == 0) arrive(bar);
       };
-      // 16 neighbours of a row of the output (multiples of 8 of them within the width)
-      auto store16 = [&](void* out, int col, const float (&v)[16]) {
+      // 16 neighbours of a row of output `which` (multiples of 8 of them within the width). Through a box in shared memory, two calls
+      // to a box: a store of 32 lanes to 32 rows takes the load-store unit two cycles a sector, which bounds a tile of three outputs.
+      auto store16 = [&](int which, int col, const uint32_t (&w)[8]) {
+        if (p.staged) {
+          const uint32_t box = box_base + ((warp - 2) * 2 + (boxes & 1)) * kFfBoxBytes, mine = box + lane * 64;
+          const uint32_t c = (col >> 3) & 2, swap = (lane >> 1) & 3;  // 16-byte piece of the row's 64 bytes
+          if (c == 0) {  // the box before the last one has been read
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((c ^ swap) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (((c + 1) ^ swap) << 4)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+          if (c == 0) return;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row < p.rows && col - 16 < p.cols) tma_store_2d(&maps.out[which], box, col - 16, row);  // (lane 0: the box's first row)
+            bulk_commit();
+          }
+          ++boxes;
+          return;
+        }
         if (!in || col >= p.cols) return;
+        void* out = which == 0 ? p.out[0] : which == 1 ? p.out[1] : p.out[2];
         uint16_t* o = static_cast<uint16_t*>(out) + static_cast<size_t>(row) * p.ld + col;
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = ff_pack<F16>(v[2 * j], v[2 * j + 1]);
         if (col + 16 <= p.cols)
           ff_store32(o, w);
         else
@@ -475,32 +508,68 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
         }
         tmem_ld_wait();
         release(OP == kFfUp ? acc_empty(acc) : ab_empty);
+        const int col = t.n * kUnits + part * N;
+        if constexpr (OP == kFfUp) {
 #pragma unroll
-        for (int c = 0; c < N / 16; ++c) {
-          const int col = t.n * kUnits + part * N + c * 16;
-          if constexpr (OP == kFfUp) {
+          for (int c = 0; c < N / 16; ++c) {
             float v[16];
+            uint32_t w[8];
             ff_gate16(va[c], vb[c], ACT, v);
-            store16(p.out[0], col, v);
-            if (p.keep[0] != nullptr && in && col < p.cols) {
-              const size_t at = static_cast<size_t>(row) * p.ld + col;  // (rows of the buffer are whole lines: past the width there is room)
+            ff_pack16<F16>(v, w);
+            store16(0, col + c * 16, w);
+            if (p.keep[0] != nullptr && in && col + c * 16 < p.cols) {
+              const size_t at = ff_kept_at(row, col + c * 16, p.ld);
               ff_keep16(static_cast<__half*>(p.keep[0]) + at, va[c]);
               ff_keep16(static_cast<__half*>(p.keep[1]) + at, vb[c]);
             }
-          } else {
+          }
+        } else {
+          uint32_t w[3][N / 16][8];  // da, db, h: formed together, leaving one after the other
+#pragma unroll
+          for (int c = 0; c < N / 16; ++c) {
             uint32_t vd[16];
             tmem_ld16(d + part * N + c * 16, vd);
             tmem_ld_wait();
             if (c == N / 16 - 1) release(acc_empty(acc));
             float da[16], db[16], h[16];
             ff_gate_back16(va[c], vb[c], vd, ACT, da, db, h);
-            store16(p.out[0], col, da);
-            store16(p.out[1], col, db);
-            store16(p.out[2], col, h);
+            ff_pack16<F16>(da, w[0][c]);
+            ff_pack16<F16>(db, w[1][c]);
+            ff_pack16<F16>(h, w[2][c]);
           }
+#pragma unroll
+          for (int o = 0; o < 3; ++o)
+#pragma unroll
+            for (int c = 0; c < N / 16; ++c) store16(o, col + c * 16, w[o][c]);
         }
       } else {
         const int n = p.bn / 4;
+        if constexpr (OP == kFfGrad) {
+          // 32 columns at a time: da of both halves leaves, then db
+#pragma unroll 1
+          for (int c = 0; c < n; c += 32) {
+            const int col = t.n * p.bn + part * n + c;
+            uint32_t wb[2][8];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint32_t va[16], vb[16], v[16], wa[8];
+              tmem_ld16(d + part * n + c + 16 * k, v);
+              tmem_ld_wait();
+              if (k == 1 && c + 32 >= n) release(acc_empty(acc));
+              ff_kept16(ka, va);
+              ff_kept16(kb, vb);
+              if (k == 0 || c + 32 < n) kept(col + 16 * (k + 1));
+              float da[16], db[16], h[16];
+              ff_gate_back16(va, vb, v, ACT, da, db, h);  // (h is the forward's)
+              ff_pack16<F16>(da, wa);
+              ff_pack16<F16>(db, wb[k]);
+              store16(0, col + 16 * k, wa);
+            }
+            store16(1, col, wb[0]);
+            store16(1, col + 16, wb[1]);
+          }
+          continue;
+        }
 #pragma unroll 1
         for (int c = 0; c < n; c += 16) {
           uint32_t v[16];
@@ -522,17 +591,10 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
           float f[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]);
-          if constexpr (OP == kFfGrad) {
-            uint32_t va[16], vb[16];
-            ff_kept16(ka, va);
-            ff_kept16(kb, vb);
-            if (c + 16 < n) kept(col + 16);
-            float da[16], db[16];
-            ff_gate_back16(va, vb, v, ACT, da, db, f);  // (h is the forward's)
-            store16(p.out[0], col, da);
-            store16(p.out[1], col, db);
-          } else if constexpr (OP != kFfWeights) {
-            store16(p.out[0], col, f);
+          if constexpr (OP != kFfWeights) {
+            uint32_t w[8];
+            ff_pack16<F16>(f, w);
+            store16(0, col, w);
           } else if (in && col < p.cols) {
             const int left = p.cols - col;
             if (p.partial != nullptr) {
@@ -552,6 +614,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     }
   }
 
+  if (warp >= 2 && lane == 0) bulk_wait<0>();  // the boxes have been read and their stores performed
   if constexpr (SPLIT) {
     __syncwarp();
     cluster_sync_all();  // every CTA's tile is in its shared memory
@@ -585,6 +648,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     }
   }
 
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if constexpr (PAIR || SPLIT) cluster_sync_all();  // no CTA leaves while another may still signal its barriers or read its memory
