@@ -34,18 +34,27 @@ class Norm(NamedTuple):
     eps: float = 1e-5
 
 
+_ABSENT = (0, None, None, 0.0)
+
+
+def _kind(kind: str) -> int:
+    code = _KINDS.get(kind)
+    if code is None:
+        raise ValueError(f"norm kind must be one of {sorted(_KINDS)}, got {kind!r}")
+    return code
+
+
 def _spread(norm: Optional[Norm]) -> tuple:
     if norm is None:
-        return 0, None, None, 0.0
-    if norm.kind not in _KINDS:
-        raise ValueError(f"norm kind must be one of {sorted(_KINDS)}, got {norm.kind!r}")
-    return _KINDS[norm.kind], norm.weight, norm.bias, float(norm.eps)
+        return _ABSENT
+    kind, weight, bias, eps = norm
+    return _kind(kind), weight, bias, eps
 
 
 def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *, kind: str = "layer",
                eps: float = 1e-5) -> torch.Tensor:
     """``norm(x)`` over the last dimension, ``x`` bf16, fp16 or fp32 (differentiable)."""
-    return _lib.native().block_join(x, None, None, None, None, *_spread(None), *_spread(Norm(kind, weight, bias, eps)))[1]
+    return _lib.native().block_join(x, None, None, None, None, *_ABSENT, _kind(kind), weight, bias, eps)[1]
 
 
 def block_join(x: torch.Tensor, u: torch.Tensor, *, gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
@@ -66,9 +75,10 @@ def gated_feed_forward(x: torch.Tensor, w_a: torch.Tensor, w_b: torch.Tensor, w_
 
     bf16 and fp16 run as they are, other float types of ``x`` through bf16. The weights are of the type that the products run in, or
     fp32 (rounded to it in each call; their gradients are fp32)."""
-    if activation not in _ACTIVATIONS:
+    code = _ACTIVATIONS.get(activation)
+    if code is None:
         raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
-    return _lib.native().gated_feed_forward(x, w_a, w_b, w_s, _ACTIVATIONS[activation])
+    return _lib.native().gated_feed_forward(x, w_a, w_b, w_s, code)
 
 
 def read_status(device=None) -> int:

@@ -252,20 +252,6 @@ struct FfProblem {
   cudaStream_t stream;
 };
 
-// Output tensors of pairs' tiles: their epilogue warps have 32 columns or more
-static int ff_out_maps(FfMaps* maps, FfParams* p, bool pair, int outs) {
-  if (!pair || p->bn < 128) return 0;
-  p->staged = 1;
-  for (int i = 0; i < outs; ++i) {
-    const uint64_t dims[2] = {static_cast<uint64_t>(p->cols), static_cast<uint64_t>(p->rows)};
-    const uint64_t strides[1] = {static_cast<uint64_t>(p->ld) * 2};
-    const uint32_t box[2] = {32, 32};
-    const int rc = make_map(&maps->out[i], p->out[i], 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
-    if (rc != 0) return rc;
-  }
-  return 0;
-}
-
 template <int OP, bool PAIR, bool F16, int ACT, bool SPLIT>
 static int ff_launch_kernel(const FfMaps& maps, const FfParams& p, const DeviceInfo& info, cudaStream_t stream) {
   const auto kernel = ff_kernel<OP, PAIR, F16, ACT, SPLIT>;
@@ -330,8 +316,6 @@ static int ff_hidden(const FfProblem& f, const void* x, const void* dy, void* co
   p.kb = p.kb_second = blocks_of(f.d, 64);
   p.bn = 2 * units;
   p.splits = 1;
-  rc = ff_out_maps(&maps, &p, pair, dy != nullptr ? 3 : 1);
-  if (rc != 0) return rc;
   return dy != nullptr ? ff_launch<kFfHidden>(maps, p, pair, f) : ff_launch<kFfUp>(maps, p, pair, f);
 }
 
@@ -356,8 +340,7 @@ static int ff_grad(const FfProblem& f, const void* dy, const void* const kept[2]
   p.kb = blocks_of(f.d, 64);
   p.bn = bn;
   p.splits = 1;
-  rc = ff_out_maps(&maps, &p, pair, 2);
-  return rc != 0 ? rc : ff_launch<kFfGrad>(maps, p, pair, f);
+  return ff_launch<kFfGrad>(maps, p, pair, f);
 }
 
 // Tiles of y = h W_s^T or dx = da W_a + db W_b (`input`): k blocks are far more than tiles where there are few rows. Pairs (tiles of 256
@@ -427,8 +410,6 @@ static int ff_project(const FfProblem& f, const void* first, const void* second,
   p.bn = bn;
   p.splits = plan.splits;
   p.kb_split = plan.kb_split;
-  if (p.splits == 1) rc = ff_out_maps(&maps, &p, pair, 1);
-  if (rc != 0) return rc;
   return input ? ff_launch<kFfInput>(maps, p, pair, f) : ff_launch<kFfDown>(maps, p, pair, f);
 }
 

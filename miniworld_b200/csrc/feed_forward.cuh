@@ -33,7 +33,6 @@ enum FfAct : int { kFfSilu = 0, kFfGelu = 1 };
 struct FfMaps {
   CUtensorMap a[3];
   CUtensorMap b[3];
-  CUtensorMap out[3];  // FfParams::staged: boxes of 32 columns by 32 rows, 64-byte swizzle
 };
 
 struct FfParams {
@@ -45,18 +44,17 @@ struct FfParams {
   int kb, kb_second;   // 64-deep k blocks of the first and of the second segment
   int bn;              // accumulator columns of an output tile (kFfUp and kFfHidden: of its a | b part)
   int splits, kb_split;  // kFfWeights, SPLIT: parts of the k range, k blocks of each
-  int staged;          // outputs leave through shared memory
   const void* kept[2]; // kFfGrad: a and b of the forward, fp16: see ff_kept_at
   void* keep[2];       // kFfUp: where to leave them, or null
   int type;            // kFfWeights: of `out`, 0 bf16, 1 fp32, 2 fp16
 };
 
-constexpr int kFfStages = 5;
+constexpr int kFfStages = 6;
 constexpr int kFfStageBytes = 32768;  // 128 rows of the first operand, up to 128 of the second, 64 deep
 constexpr int kFfEpilogueWarps = 16;
 constexpr int kFfThreads = 64 + 32 * kFfEpilogueWarps;
-constexpr int kFfBoxBytes = 2048;     // 32 x 32 values of an output; two for each epilogue warp
-constexpr int kFfSmemBytes = kFfStages * kFfStageBytes + kFfEpilogueWarps * 2 * kFfBoxBytes + 256 + 1024;
+constexpr int kFfBoxBytes = 2048;     // 32 x 32 values of an output; one for each epilogue warp
+constexpr int kFfSmemBytes = kFfStages * kFfStageBytes + kFfEpilogueWarps * kFfBoxBytes + 256 + 1024;
 
 template <bool F16>
 __device__ __forceinline__ uint32_t ff_pack(float a, float b) {
@@ -219,7 +217,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t box_base = base + S * kFfStageBytes;
-  const uint32_t bar_base = box_base + kFfEpilogueWarps * 2 * kFfBoxBytes;
+  const uint32_t bar_base = box_base + kFfEpilogueWarps * kFfBoxBytes;
   auto full = [&](int s) { return bar_base + 8u * s; };
   auto empty = [&](int s) { return bar_base + 8u * (S + s); };
   auto acc_full = [&](int a) { return bar_base + 8u * (2 * S + a); };
@@ -250,7 +248,6 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     for (int i = 0; i < 3; ++i) {
       if (i == 0 || OP == kFfWeights || (i == 1 && SECOND)) prefetch_tmap(&maps.a[i]);
       if (i == 0 || OP == kFfHidden || (i == 1 && OP != kFfDown && OP != kFfGrad)) prefetch_tmap(&maps.b[i]);
-      if (p.staged && (i == 0 || OP == kFfHidden || (i == 1 && OP == kFfGrad))) prefetch_tmap(&maps.out[i]);
     }
   }
   if (warp == 1) {
@@ -441,9 +438,10 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     // ------------------------------------------------------------ epilogue: a row per thread, a quarter of the tile's columns per
     // group of four warps. All of a thread's accumulators are read at once and handed back before the arithmetic (kFfHidden: those
     // of a and b, of which there is one set; dh has two).
+    const bool boxes = OP == kFfUp || OP == kFfHidden ? PAIR : p.bn >= 128;  // 32 columns a warp and more
     const int q = warp & 3, part = (warp - 2) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    int it = 0, boxes = 0;
+    int it = 0;
     for (int i = first; i < tiles; i += step, ++it) {
       const Tile t = tile_at(i);
       const int acc = it & 1;
@@ -466,30 +464,32 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
         __syncwarp();
         if (lane == 0) arrive(bar);
       };
-      // 16 neighbours of a row of output `which` (multiples of 8 of them within the width). Through a box in shared memory, two calls
-      // to a box: a store of 32 lanes to 32 rows takes the load-store unit two cycles a sector, which bounds a tile of three outputs.
+      // 16 neighbours of a row of output `which` (multiples of 8 of them within the width). Where a warp has 32 columns and more, two calls
+      // fill a box of 32 rows x 32 columns in shared memory, and the warp stores it eight rows of 64 bytes at a time: 32 lanes that
+      // store to 32 rows take the load-store unit two cycles a sector, and copies of such boxes by TMA take it from the loads, whose
+      // rows of 128 bytes it moves in 2.7 cycles each (that is what bounds the wide products).
       auto store16 = [&](int which, int col, const uint32_t (&w)[8]) {
-        if (p.staged) {
-          const uint32_t box = box_base + ((warp - 2) * 2 + (boxes & 1)) * kFfBoxBytes, mine = box + lane * 64;
+        void* const out = which == 0 ? p.out[0] : which == 1 ? p.out[1] : p.out[2];
+        if (boxes) {
+          const uint32_t box = box_base + (warp - 2) * kFfBoxBytes, mine = box + lane * 64;
           const uint32_t c = (col >> 3) & 2, swap = (lane >> 1) & 3;  // 16-byte piece of the row's 64 bytes
-          if (c == 0) {  // the box before the last one has been read
-            if (lane == 0) bulk_wait_read<1>();
-            __syncwarp();
-          }
+          if (c == 0) __syncwarp();                                     // the box before has been read
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((c ^ swap) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (((c + 1) ^ swap) << 4)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
           if (c == 0) return;
-          fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
-            if (row < p.rows && col - 16 < p.cols) tma_store_2d(&maps.out[which], box, col - 16, row);  // (lane 0: the box's first row)
-            bulk_commit();
+          const int row0 = row - lane, piece = lane & 3, at = col - 16 + piece * 8;
+          uint16_t* o = static_cast<uint16_t*>(out) + static_cast<size_t>(row0) * p.ld + at;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = j * 8 + (lane >> 2);
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(box + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4)) : "memory");
+            if (row0 + r < p.rows && at < p.cols) *reinterpret_cast<uint4*>(o + static_cast<size_t>(r) * p.ld) = v;
           }
-          ++boxes;
           return;
         }
         if (!in || col >= p.cols) return;
-        void* out = which == 0 ? p.out[0] : which == 1 ? p.out[1] : p.out[2];
         uint16_t* o = static_cast<uint16_t*>(out) + static_cast<size_t>(row) * p.ld + col;
         if (col + 16 <= p.cols)
           ff_store32(o, w);
@@ -614,7 +614,6 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     }
   }
 
-  if (warp >= 2 && lane == 0) bulk_wait<0>();  // the boxes have been read and their stores performed
   if constexpr (SPLIT) {
     __syncwarp();
     cluster_sync_all();  // every CTA's tile is in its shared memory
@@ -648,7 +647,6 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
     }
   }
 
-  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if constexpr (PAIR || SPLIT) cluster_sync_all();  // no CTA leaves while another may still signal its barriers or read its memory

@@ -38,10 +38,10 @@ inline EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-// bf16 tensor map, with 128-byte swizzle if no other is asked for. dims[0] is the contiguous dimension; strides (bytes) are for
+// bf16 tensor map with 128-byte swizzle. dims[0] is the contiguous dimension; strides (bytes) are for
 // dims[1..rank-1].
 inline int make_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
-                    const uint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+                    const uint32_t* box) {
   EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr) {
     tl_last_cuda_error = static_cast<int>(cudaErrorNotSupported);
@@ -58,7 +58,7 @@ inline int make_map(CUtensorMap* m, const void* base, int rank, const uint64_t* 
     if (i > 0) s[i - 1] = strides[i - 1];
   }
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s,
-                  b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     tl_last_cuda_error = 100000 + static_cast<int>(r);
