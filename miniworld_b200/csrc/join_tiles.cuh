@@ -380,11 +380,12 @@ struct TileSum {
   }
 };
 
-// mean and 1 / sigma of a row
+// mean and 1 / sigma of a row. (With eight elements a thread, where two blocks share an SM, the merged form's instructions cost more
+// than the second exchange's latency.)
 template <int VEC, int NV, bool EXACT>
 __device__ __forceinline__ float2 tile_stats(const float2 (&v)[4 * NV], int kind, float eps, int d, float inv, int t, int team, TileSum& sum) {
   float mean = 0.f, dev;
-  if (EXACT && kind == kNormLayer) {
+  if (EXACT && NV > 1 && kind == kNormLayer) {
     float2 a = v[0], q = f2(0.f);
 #pragma unroll
     for (int i = 1; i < 4 * NV; ++i) a = __fadd2_rn(a, v[i]);
@@ -464,11 +465,13 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
   const float inv = 1.0f / static_cast<float>(d);
   const int row_bytes = d * static_cast<int>(sizeof(T));
   const int n = ring.count();
+  const uint32_t stage_bytes = p.slots * p.slot, ring_at = smem_u32(ring.stage0);
+  const long long tile_step = static_cast<long long>(ring.step()) * p.tile_rows;
+  long long r0 = static_cast<long long>(ring.first()) * p.tile_rows;
+  int s = 0;
+  uint32_t ph = 0, stage = ring_at;
   for (int k = 0; k < n; ++k) {
-    const int s = k % p.stages;
-    if (!mbar_wait_warp(ring.full(s), (k / p.stages) & 1, abort_flag, &blocks_status, kDevTimeoutStats)) break;
-    const uint32_t stage = smem_u32(ring.stage(s));
-    const long long r0 = static_cast<long long>(ring.first() + k * ring.step()) * p.tile_rows;
+    if (!mbar_wait_warp(ring.full(s), ph, abort_flag, &blocks_status, kDevTimeoutStats)) break;
     const int rows = j.rows - r0 < p.tile_rows ? static_cast<int>(j.rows - r0) : p.tile_rows;
     for (int r = id; r - id < p.tile_rows; r += teams) {
       const long long row = r0 + r;
@@ -530,6 +533,13 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(ring.done(s));
+    r0 += tile_step;
+    stage += stage_bytes;
+    if (++s == p.stages) {
+      s = 0;
+      ph ^= 1u;
+      stage = ring_at;
+    }
   }
 }
 
@@ -597,32 +607,34 @@ __global__ void __launch_bounds__(kTileThreads, JOIN ? 1 : 2) join_tile_backward
         sg_sum[i] = f2(0.f);
       }
     };
+    const uint32_t stage_bytes = p.slots * p.slot, ring_at = smem_u32(ring.stage0);
+    const long long tile_step = static_cast<long long>(ring.step()) * p.tile_rows;
+    long long r0 = first_row;
+    int s = 0;
+    uint32_t ph = 0, stage = ring_at;
     // statistics and mask of the team's next row, asked for while this one is worked on
     float2 next_post = f2(0.f), next_pre = f2(0.f);
     int next_valid = 0;
-    auto row_facts = [&](int k, int r) {
-      const long long row = static_cast<long long>(ring.first() + k * ring.step()) * p.tile_rows + r;
+    auto row_facts = [&](long long tile_row, int r) {
+      const long long row = tile_row + r;
       next_valid = 0;
-      if (k >= n || r >= p.tile_rows || row >= j.rows) return;
+      if (r >= p.tile_rows || row >= j.rows) return;
       if (JOIN) next_valid = j.mask == nullptr ? 1 : __ldcg(j.mask + row);
       if (JOIN && j.post_kind != kNormNone) next_post = __ldcg(j.post_stats + row);
       if (j.pre_kind != kNormNone) next_pre = __ldcg(j.pre_stats + row);
     };
-    row_facts(0, id);
+    if (n > 0) row_facts(r0, id);
     for (int k = 0; k < n; ++k) {
-      const int s = k % p.stages;
-      const long long r0 = static_cast<long long>(ring.first() + k * ring.step()) * p.tile_rows;
       const int rows = j.rows - r0 < p.tile_rows ? static_cast<int>(j.rows - r0) : p.tile_rows;
-      if (!mbar_wait_warp(ring.full(s), (k / p.stages) & 1, abort_flag, &blocks_status, kDevTimeoutStats)) break;
-      const uint32_t stage = smem_u32(ring.stage(s));
+      if (!mbar_wait_warp(ring.full(s), ph, abort_flag, &blocks_status, kDevTimeoutStats)) break;
       for (int r = id; r - id < p.tile_rows; r += teams) {
         const bool on = r < rows;
         const bool valid = next_valid != 0;
         const float2 post = next_post, pre = next_pre;
         if (r - id + teams < p.tile_rows)
-          row_facts(k, r + teams);
-        else
-          row_facts(k + 1, id);
+          row_facts(r0, r + teams);
+        else if (k + 1 < n)
+          row_facts(r0 + tile_step, id);
         const long long row = r0 + r;
         const int off = on ? r * row_bytes : 0;
         float2 x[4], e[4], q[4], u[4], g[4], w[4];
@@ -733,6 +745,13 @@ __global__ void __launch_bounds__(kTileThreads, JOIN ? 1 : 2) join_tile_backward
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(ring.done(s));
+      r0 += tile_step;
+      stage += stage_bytes;
+      if (++s == p.stages) {
+        s = 0;
+        ph ^= 1u;
+        stage = ring_at;
+      }
     }
     if (shared_gate && j.dgate != nullptr && n > 0) {
       long long last = first_row + static_cast<long long>(n) * p.tile_rows;
