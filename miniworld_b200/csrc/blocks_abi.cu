@@ -455,7 +455,7 @@ static int ff_vec_rows_up(long long rows) { return rows <= 1 ? 1 : rows <= 2 ? 2
 static bool ff_vec(long long rows, int d) { return rows <= kFfVecRows && ff_vec_rows_up(rows) * static_cast<long long>(d) * 4 <= kFfVecSmem; }
 template <bool F16>
 static int ff_vec_forward(const FfProblem& f, const void* x, void* h, void* y) {
-  const FfVec v = {x, f.w_a, f.w_b, f.w_s, h, y, static_cast<int>(f.rows), f.d, f.hidden, f.act, 0};
+  const FfVec v = {x, f.w_a, f.w_b, f.w_s, static_cast<float*>(h), y, static_cast<int>(f.rows), f.d, f.hidden, f.act, 0};
   switch (ff_vec_rows_up(f.rows)) {
     case 1: return ff_vec_launch<F16, 1>(f, v);
     case 2: return ff_vec_launch<F16, 2>(f, v);
@@ -552,7 +552,7 @@ static FfRegions ff_regions(long long rows, int d, int hidden, int weight_dtype,
   if (weight_dtype == B200_BLOCKS_F32) at += up(static_cast<size_t>(3) * hidden * d * 2, 1024);
   for (int i = 0; i < (backward ? 3 : 1); ++i) {
     r.hidden[i] = at;
-    at += up(static_cast<size_t>(rows) * ff_ld(hidden) * 2, 1024);
+    at += up(static_cast<size_t>(rows) * ff_ld(hidden) * (rows <= kFfVecRows ? 4 : 2), 1024);  // (fp32 where tensor cores take no part)
   }
   r.partial = at;
   const int parts = backward ? ff_split(rows, d, hidden, kMaxSms).most : 0;

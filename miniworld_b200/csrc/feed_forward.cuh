@@ -763,7 +763,8 @@ __device__ __forceinline__ float ff_warp_sum(float2 v) {
 
 struct FfVec {
   const void *x, *w_a, *w_b, *w_s;
-  void *h, *y;  // h [rows][hidden]
+  float* h;     // [rows][hidden]: no product of tensor cores asks for 16 bits here
+  void* y;
   int rows, d, hidden, act;
   int part;     // columns of h that are in shared memory at a time
 };
@@ -790,9 +791,9 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_up_kernel(const FfVec p)
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float sa = ff_warp_sum(a[r]), sb = ff_warp_sum(b[r]);
-    if (lane == r % 32 && r < p.rows) {
+    if (lane == r && r < p.rows) {
       const float f = p.act == kFfSilu ? __fdividef(sa, 1.0f + __expf(-sa)) : 0.5f * sa * (1.0f + erff(sa * 0.70710678f));
-      static_cast<uint16_t*>(p.h)[static_cast<size_t>(r) * p.hidden + unit] = static_cast<uint16_t>(ff_pack<F16>(f * sb, 0.f));
+      p.h[static_cast<size_t>(r) * p.hidden + unit] = f * sb;
     }
   }
 }
@@ -809,7 +810,11 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_down_kernel(const FfVec 
   for (int k0 = 0; k0 < p.hidden; k0 += p.part) {
     const int n = min(p.part, p.hidden - k0);
     if (k0 != 0) __syncthreads();
-    ff_vec_rows<F16, R>(vec_rows, p.h, p.rows, p.hidden, k0, n);
+    for (int e = threadIdx.x; e < R * (n / 4); e += kFfVecThreads) {
+      const int r = e / (n / 4), c = (e - r * (n / 4)) * 4;
+      const float4 v = r < p.rows ? __ldcg(reinterpret_cast<const float4*>(p.h + static_cast<size_t>(r) * p.hidden + k0 + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(vec_rows + r * n + (c & 4) / 4 * (n / 2) + c / 8 * 4) = v;  // (the order of ff_vec_rows)
+    }
     __syncthreads();
 #pragma unroll 4
     for (int c = lane * 8; c < n; c += 256) {
@@ -821,7 +826,7 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_down_kernel(const FfVec 
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float s = ff_warp_sum(acc[r]);
-    if (lane == r % 32 && r < p.rows) static_cast<uint16_t*>(p.y)[static_cast<size_t>(r) * p.d + col] = static_cast<uint16_t>(ff_pack<F16>(s, 0.f));
+    if (lane == r && r < p.rows) static_cast<uint16_t*>(p.y)[static_cast<size_t>(r) * p.d + col] = static_cast<uint16_t>(ff_pack<F16>(s, 0.f));
   }
 }
 
