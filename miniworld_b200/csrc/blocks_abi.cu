@@ -107,6 +107,8 @@ static int tile_smem(const JoinTileParams& p, int params) {
   return params * p.params * 4 + kTileScratch + std::max(p.stages * p.slots * p.slot, params == 3 ? p.workers * 8 * 4 : 0);
 }
 using TileKernel = void (*)(JoinTileParams);
+template <typename T>
+constexpr int kOdd = sizeof(T) == 2 ? 3 : 1;
 template <typename T, int VEC, bool EXACT>
 static TileKernel tile_forward_kernel(int nv) {
   switch (nv) {
@@ -119,10 +121,10 @@ static TileKernel tile_forward_kernel(int nv) {
 template <typename T, bool JOIN>
 static TileKernel tile_backward_kernel(int vec, bool exact) {
   if (exact) return join_tile_backward_kernel<T, 8, true, JOIN>;
-  return vec == 8 ? join_tile_backward_kernel<T, 8, false, JOIN> : vec == 2 ? join_tile_backward_kernel<T, 2, false, JOIN> : join_tile_backward_kernel<T, 1, false, JOIN>;
+  return vec == 8 ? join_tile_backward_kernel<T, 8, false, JOIN> : vec == 2 ? join_tile_backward_kernel<T, 2, false, JOIN> : join_tile_backward_kernel<T, kOdd<T>, false, JOIN>;
 }
 // elements of a row that a thread reads at once
-static int join_vec(int d) { return d % 8 == 0 ? 8 : d % 2 == 0 ? 2 : 1; }
+static int join_vec(int d, size_t size) { return d % 8 == 0 ? 8 : d % 2 == 0 ? 2 : size == 2 ? 3 : 1; }  // (see tile_col)
 
 template <typename T>
 static int launch_join_forward(const JoinParams& p0, bool wide, const DeviceInfo& info, cudaStream_t stream) {
@@ -137,14 +139,14 @@ static int launch_join_forward(const JoinParams& p0, bool wide, const DeviceInfo
   q.out_slot[0] = p0.y != nullptr ? 0 : -1;
   q.out_slot[1] = p0.h != nullptr ? (p0.u != nullptr ? 1 : 0) : -1;
   q.out_slot[2] = -1;
-  const void* tensors[] = {p0.x, p0.u, q.slot_of[2] >= 0 ? p0.gate : nullptr, p0.y, p0.h};
+  const void* tensors[] = {p0.x, p0.u, p0.gate, p0.y, p0.h};
   const int per_sm = s.nv == 1 ? 2 : 1;
   if (plan_tiles(&q, tensors, 5, sizeof(T), s.nv, 4, per_sm * info.sms, per_sm == 2 ? kTileSmemHalf : kTileSmem)) {
-    const int vec = join_vec(p0.d);
+    const int vec = join_vec(p0.d, sizeof(T));
     const TileKernel kernel = p0.d == 8 * s.nv * s.team ? tile_forward_kernel<T, 8, true>(s.nv)
                               : vec == 8                ? tile_forward_kernel<T, 8, false>(s.nv)
                               : vec == 2                ? tile_forward_kernel<T, 2, false>(s.nv)
-                                                        : tile_forward_kernel<T, 1, false>(s.nv);
+                                                        : tile_forward_kernel<T, kOdd<T>, false>(s.nv);
     const int rc = set_smem(kernel, kTileSmem, info.device);
     if (rc != 0) return rc;
     TRIMUL_CUDA(launch_overlapped(kernel, dim3(std::min(per_sm * info.sms, q.tiles)), q.workers + 32, tile_smem(q, 4), stream, q));
@@ -183,14 +185,14 @@ static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& 
   q.out_slot[2] = p.dgate != nullptr && !shared_gate ? q.slot_of[2] : -1;
   const bool join = p.u != nullptr;
   const int most = std::min(info.sms, kMaxSms) * (join ? 1 : 2);
-  const void* tensors[] = {p.x, p.u, q.slot_of[2] >= 0 ? p.gate : nullptr, p.dy, p.dh, p.dx, p.du, q.out_slot[2] >= 0 ? p.dgate : nullptr};
+  const void* tensors[] = {p.x, p.u, p.gate, p.dy, p.dh, p.dx, p.du, q.out_slot[2] >= 0 ? p.dgate : nullptr};
   if (q.slots > 0 && (!shared_gate || p.gate_rows >= kSharedGateRows) && plan_tiles(&q, tensors, 8, sizeof(T), 1, 3, most, join ? kTileSmem : kTileSmemHalf)) {
     const int blocks = std::min(most, q.tiles);
     if (shared_gate) {
       q.block_tiles = (q.tiles + blocks - 1) / blocks;
       q.group_slots = static_cast<int>(static_cast<long long>(q.block_tiles) * q.tile_rows / p.gate_rows) + 2;
     }
-    const int vec = join_vec(p.d);
+    const int vec = join_vec(p.d, sizeof(T));
     const TileKernel kernel = join ? tile_backward_kernel<T, true>(vec, p.d == 8 * p.team) : tile_backward_kernel<T, false>(vec, p.d == 8 * p.team);
     const int rc = set_smem(kernel, kTileSmem, info.device);
     if (rc != 0) return rc;
@@ -201,7 +203,7 @@ static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& 
       TRIMUL_CUDA(launch_overlapped(join_tile_sums_kernel, dim3((p.d + 31) / 32, 2), 1024, 0, stream, t));
     }
     if (p.dgate != nullptr && shared_gate) {
-      auto last = vec == 8 ? join_tile_gate_kernel<T, 8> : vec == 2 ? join_tile_gate_kernel<T, 2> : join_tile_gate_kernel<T, 1>;
+      auto last = vec == 8 ? join_tile_gate_kernel<T, 8> : vec == 2 ? join_tile_gate_kernel<T, 2> : join_tile_gate_kernel<T, kOdd<T>>;
       const long long groups = p.rows / p.gate_rows;
       if (groups > 65535) return B200_TRIMUL_E_SHAPE;
       TRIMUL_CUDA(launch_overlapped(last, dim3((8 * p.team + 31) / 32, static_cast<unsigned>(groups)), 1024, 0, stream, q));

@@ -58,9 +58,12 @@ template <int VEC>
 __device__ __forceinline__ int tile_param(int c, int params) {
   return VEC == 8 ? ((c >> 2) & 1) * (params >> 1) + (c >> 3) * 4 + (c & 3) : c;
 }
+// Column of element i of thread t. VEC neighbours are read at once: 8 (widths that are a multiple of eight), 2 (even ones), 3: two of a
+// 16-bit type in rows of an odd width, of which every other one starts in the middle of a 32-bit word; 1 (fp32 rows of an odd width).
 template <int VEC>
 __device__ __forceinline__ int tile_col(int i, int t, int team) {
-  return ((i / VEC) * team + t) * VEC + i % VEC;
+  constexpr int N = VEC == 3 ? 2 : VEC;
+  return ((i / N) * team + t) * N + i % N;
 }
 template <int VEC, int NV>
 __device__ __forceinline__ void tile_params(uint32_t w, int params, int t, int team, float2 (&v)[4 * NV]) {
@@ -77,7 +80,7 @@ __device__ __forceinline__ void tile_params(uint32_t w, int params, int t, int t
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NV; ++i) {
-      if constexpr (VEC == 2) {
+      if constexpr (VEC == 2 || VEC == 3) {
         asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[i].x), "=f"(v[i].y) : "r"(w + (i * team + t) * 8) : "memory");
       } else {
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i].x) : "r"(w + (2 * i * team + t) * 4) : "memory");
@@ -148,6 +151,22 @@ __device__ __forceinline__ void tile_load(uint32_t p, int d, int t, int team, fl
         }
       }
     }
+  } else if constexpr (VEC == 3) {
+    // the two words that the pair may lie in, and the halves of them that it does
+    const uint32_t word = p & ~3u, pick = (p & 2u) != 0 ? 0x5432u : 0x3210u;
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) {
+      const int c = (i * team + t) * 2;
+      uint32_t w = 0;
+      if (c < d) {
+        uint32_t lo, hi;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(lo) : "r"(word + c * 2) : "memory");
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(hi) : "r"(word + c * 2 + 4) : "memory");
+        w = __byte_perm(lo, hi, pick);
+        if (c + 1 == d) w &= 0xFFFFu;  // (the other half is the next row's)
+      }
+      v[i] = Io<T>::two(w);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NV; ++i) {
@@ -183,6 +202,20 @@ __device__ __forceinline__ void tile_store(uint32_t p, int d, int t, int team, c
       else
         asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(p + c * 4), "f"(v[i].x), "f"(v[i].y) : "memory");
     }
+  } else if constexpr (VEC == 3) {
+    const bool odd = (p & 2u) != 0;
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) {
+      const int c = (i * team + t) * 2;
+      if (c >= d) continue;
+      const uint32_t w = Io<T>::pack(v[i].x, v[i].y);
+      if (!odd && c + 1 < d) {
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(p + c * 2), "r"(w) : "memory");
+      } else {
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(p + c * 2), "h"(static_cast<unsigned short>(w)) : "memory");
+        if (c + 1 < d) asm volatile("st.shared.u16 [%0], %1;" ::"r"(p + c * 2 + 2), "h"(static_cast<unsigned short>(w >> 16)) : "memory");
+      }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * NV; ++i) {
@@ -192,12 +225,38 @@ __device__ __forceinline__ void tile_store(uint32_t p, int d, int t, int team, c
     }
   }
 }
-// (global memory, a gate row that many rows share: in L2)
-template <typename T, int VEC>
-__device__ __forceinline__ void tile_gate(const void* gate, long long row, int d, int t, int team, int i, float2& v) {
+// A gate row that many rows share, from L2
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void tile_gate(const void* gate, long long row, int d, int t, int team, float2 (&v)[4 * NV]) {
   const T* p = static_cast<const T*>(gate) + row * d;
-  const int a = tile_col<VEC>(2 * i, t, team), b = tile_col<VEC>(2 * i + 1, t, team);
-  v = make_float2(a < d ? Io<T>::get(p + a) : 0.f, b < d ? Io<T>::get(p + b) : 0.f);
+  if constexpr (VEC == 8) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * team + t) * 8;
+      uint4 w = make_uint4(0u, 0u, 0u, 0u), u = w;
+      if (c < d) {
+        w = __ldcg(reinterpret_cast<const uint4*>(p + c));
+        if (sizeof(T) == 4) u = __ldcg(reinterpret_cast<const uint4*>(p + c) + 1);
+      }
+      if constexpr (sizeof(T) == 2) {
+        v[4 * j] = Io<T>::two(w.x);
+        v[4 * j + 1] = Io<T>::two(w.y);
+        v[4 * j + 2] = Io<T>::two(w.z);
+        v[4 * j + 3] = Io<T>::two(w.w);
+      } else {
+        v[4 * j] = as_f2(w.x, w.y);
+        v[4 * j + 1] = as_f2(w.z, w.w);
+        v[4 * j + 2] = as_f2(u.x, u.y);
+        v[4 * j + 3] = as_f2(u.z, u.w);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) {
+      const int a = tile_col<VEC>(2 * i, t, team), b = tile_col<VEC>(2 * i + 1, t, team);
+      v[i] = make_float2(a < d ? Io<T>::get(p + a) : 0.f, b < d ? Io<T>::get(p + b) : 0.f);
+    }
+  }
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -503,9 +562,7 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
           if (p.slot_of[2] >= 0) {
             tile_load<T, VEC, NV, EXACT>(stage + p.slot_of[2] * p.slot + off, d, t, team, w);
           } else {
-            const long long g = on ? row / j.gate_rows : 0;
-#pragma unroll
-            for (int i = 0; i < 4 * NV; ++i) tile_gate<T, VEC>(j.gate, g, d, t, team, i, w[i]);
+            tile_gate<T, VEC, NV>(j.gate, on ? row / j.gate_rows : 0, d, t, team, w);
           }
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) u[i] = __fmul2_rn(u[i], sigmoid2(w[i]));
@@ -648,8 +705,7 @@ __global__ void __launch_bounds__(kTileThreads, JOIN ? 1 : 2) join_tile_backward
             if (!shared_gate) {
               tile_load<T, VEC, 1, EXACT>(stage + p.slot_of[2] * p.slot + off, d, t, team, g);
             } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) tile_gate<T, VEC>(j.gate, row / j.gate_rows, d, t, team, i, g[i]);
+              tile_gate<T, VEC, 1>(j.gate, row / j.gate_rows, d, t, team, g);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) g[i] = sigmoid2(g[i]);
