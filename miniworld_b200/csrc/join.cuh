@@ -63,7 +63,6 @@ struct Io<__nv_bfloat16> {
   static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
   static __device__ __forceinline__ float2 two(uint32_t w) { return bf16x2_to_float2(w); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
-  static __device__ __forceinline__ float one(unsigned short w) { return __uint_as_float(static_cast<uint32_t>(w) << 16); }
 };
 template <>
 struct Io<__half> {
@@ -74,7 +73,6 @@ struct Io<__half> {
   static __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
   static __device__ __forceinline__ float2 two(uint32_t w) { return f16x2_to_float2(w); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_f16x2(make_float2(a, b)); }
-  static __device__ __forceinline__ float one(unsigned short w) { return __half2float(__ushort_as_half(w)); }
 };
 template <>
 struct Io<float> {
