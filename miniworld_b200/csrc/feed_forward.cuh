@@ -79,26 +79,67 @@ __device__ __forceinline__ void ff_sigmoid4(float2 a, float2 b, float2& sa, floa
   sa = __fmul2_rn(ff_f2(r * py), make_float2(x.y, x.x));
   sb = __fmul2_rn(ff_f2(r * px), make_float2(y.y, y.x));
 }
-__device__ __forceinline__ float2 ff_at(const uint32_t (&v)[16], int j) { return make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); }
-// Values of 16 neighbouring units: act(a) b
-__device__ __forceinline__ void ff_gate16(const uint32_t (&a)[16], const uint32_t (&b)[16], int act, float (&h)[16]) {
-  if (act == kFfSilu) {
+// The normal distribution's function and e^(-a^2 / 2) of four values: with z = |a| / sqrt 2 and t = 1 / (1 + 0.3275911 z),
+// erfc(z) = (c1 t + ... + c5 t^5) e^(-z^2) to 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26), the
+// reciprocals from one as above. z is held below 16, where erfc is zero in fp32.
+__device__ __forceinline__ void ff_normal4(const float2 (&a)[2], float2 (&cdf)[2], float2 (&bell)[2]) {
+  float2 x[2], z[2];
 #pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      const float2 u = ff_at(a, j), v = ff_at(a, j + 2);
-      float2 su, sv;
-      ff_sigmoid4(u, v, su, sv);
-      const float2 r = __fmul2_rn(__fmul2_rn(u, su), ff_at(b, j)), q = __fmul2_rn(__fmul2_rn(v, sv), ff_at(b, j + 2));
-      h[j] = r.x;
-      h[j + 1] = r.y;
-      h[j + 2] = q.x;
-      h[j + 3] = q.y;
+  for (int k = 0; k < 2; ++k) {
+    z[k] = make_float2(fminf(fabsf(a[k].x) * 0.70710678f, 16.f), fminf(fabsf(a[k].y) * 0.70710678f, 16.f));
+    x[k] = __ffma2_rn(z[k], ff_f2(0.3275911f), ff_f2(1.f));
+    const float2 n = __fmul2_rn(__fmul2_rn(z[k], z[k]), ff_f2(-1.44269504f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(bell[k].x) : "f"(n.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(bell[k].y) : "f"(n.y));
+  }
+  const float p0 = x[0].x * x[0].y, p1 = x[1].x * x[1].y;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p0 * p1));
+  const float2 t[2] = {__fmul2_rn(ff_f2(r * p1), make_float2(x[0].y, x[0].x)), __fmul2_rn(ff_f2(r * p0), make_float2(x[1].y, x[1].x))};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float2 q = __ffma2_rn(t[k], ff_f2(0.5f * 1.061405429f), ff_f2(0.5f * -1.453152027f));
+    q = __ffma2_rn(q, t[k], ff_f2(0.5f * 1.421413741f));
+    q = __ffma2_rn(q, t[k], ff_f2(0.5f * -0.284496736f));
+    q = __ffma2_rn(q, t[k], ff_f2(0.5f * 0.254829592f));
+    q = __fmul2_rn(__fmul2_rn(q, t[k]), bell[k]);  // erfc(z) / 2
+    cdf[k] = make_float2(a[k].x < 0.f ? q.x : 1.f - q.x, a[k].y < 0.f ? q.y : 1.f - q.y);
+  }
+}
+__device__ __forceinline__ float2 ff_at(const uint32_t (&v)[16], int j) { return make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); }
+// act(a) and (where asked for) act'(a) of four values
+template <bool SLOPE>
+__device__ __forceinline__ void ff_act4(const float2 (&a)[2], int act, float2 (&f)[2], float2 (&slope)[2]) {
+  float2 s[2];
+  if (act == kFfSilu) {
+    ff_sigmoid4(a[0], a[1], s[0], s[1]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      f[k] = __fmul2_rn(a[k], s[k]);
+      if (SLOPE) slope[k] = __ffma2_rn(f[k], __fadd2_rn(ff_f2(1.f), make_float2(-s[k].x, -s[k].y)), s[k]);  // s (1 + a (1 - s))
     }
   } else {
+    float2 bell[2];
+    ff_normal4(a, s, bell);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float v = __uint_as_float(a[j]);
-      h[j] = 0.5f * v * (1.0f + erff(v * 0.70710678f)) * __uint_as_float(b[j]);
+    for (int k = 0; k < 2; ++k) {
+      f[k] = __fmul2_rn(a[k], s[k]);
+      if (SLOPE) slope[k] = __ffma2_rn(__fmul2_rn(a[k], ff_f2(0.39894228f)), bell[k], s[k]);  // cdf + a / sqrt(2 pi) e^(-a^2 / 2)
+    }
+  }
+}
+// Values of 16 neighbouring units: act(a) b
+__device__ __forceinline__ void ff_gate16(const uint32_t (&a)[16], const uint32_t (&b)[16], int act, float (&h)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 4) {
+    const float2 v[2] = {ff_at(a, j), ff_at(a, j + 2)};
+    float2 f[2], none[2];
+    ff_act4<false>(v, act, f, none);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float2 r = __fmul2_rn(f[k], ff_at(b, j + 2 * k));
+      h[j + 2 * k] = r.x;
+      h[j + 2 * k + 1] = r.y;
     }
   }
 }
@@ -107,22 +148,14 @@ __device__ __forceinline__ void ff_gate_back16(const uint32_t (&a)[16], const ui
                                                float (&db)[16], float (&h)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; i += 4) {
-    float2 s[2];
-    if (act == kFfSilu) ff_sigmoid4(ff_at(a, i), ff_at(a, i + 2), s[0], s[1]);
+    const float2 v[2] = {ff_at(a, i), ff_at(a, i + 2)};
+    float2 f[2], slope[2];
+    ff_act4<true>(v, act, f, slope);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int j = i + 2 * k;
-      const float2 va = ff_at(a, j), vb = ff_at(b, j), vd = ff_at(d, j);
-      float2 f, slope;
-      if (act == kFfSilu) {
-        f = __fmul2_rn(va, s[k]);
-        slope = __ffma2_rn(f, __fadd2_rn(ff_f2(1.f), make_float2(-s[k].x, -s[k].y)), s[k]);  // s (1 + a (1 - s))
-      } else {
-        const float2 cdf = make_float2(0.5f * (1.0f + erff(va.x * 0.70710678f)), 0.5f * (1.0f + erff(va.y * 0.70710678f)));
-        f = __fmul2_rn(va, cdf);
-        slope = make_float2(fmaf(va.x * 0.39894228f, __expf(-0.5f * va.x * va.x), cdf.x), fmaf(va.y * 0.39894228f, __expf(-0.5f * va.y * va.y), cdf.y));
-      }
-      const float2 x = __fmul2_rn(__fmul2_rn(vd, vb), slope), y = __fmul2_rn(vd, f), z = __fmul2_rn(f, vb);
+      const float2 vb = ff_at(b, j), vd = ff_at(d, j);
+      const float2 x = __fmul2_rn(__fmul2_rn(vd, vb), slope[k]), y = __fmul2_rn(vd, f[k]), z = __fmul2_rn(f[k], vb);
       da[j] = x.x;
       da[j + 1] = x.y;
       db[j] = y.x;
