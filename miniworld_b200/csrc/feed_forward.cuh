@@ -5,8 +5,9 @@
 //
 // The backward forms a and b again from x (16 M D H multiply-adds in all instead of 12), or, where that costs more than writing and
 // reading them (D >= 512 and many rows: the caller then keeps a buffer), takes them from the forward, as fp16 for either type of x
-// (11 bits of their values, saturating: kept in bf16 they would add more to the gradients' error than all other roundings). Products on the tensor cores (fp32 accumulators in tensor memory), by
-// one kernel template; what is between two products of a row is done in the first one's epilogue, on the accumulators:
+// (11 bits of their values, saturating: kept in bf16 they would add more to the gradients' error than all other roundings). The
+// products run on the tensor cores (fp32 accumulators in tensor memory), by one kernel template; what is between two products of a row
+// is done in the first one's epilogue, on the accumulators:
 //
 //   kFfUp       a | b side by side in one accumulator, h leaves              K = D
 //   kFfDown     y = h W_s^T                                                   K = H
@@ -20,6 +21,9 @@
 // The structure is the contraction's: persistent CTAs (pairs for large products: 256-row tiles, each CTA supplies its rows of the
 // first operand and half of the second), one warp loads through TMA, one issues the MMAs, the others are the epilogue of the tile
 // before. All waits are bounded; one that gives up leaves a code in blocks_status.
+// M, D, H = 16384, 1024, 4096, bf16, each alone: up 168 us (200 with a and b kept), down 97, grad 136, input 190, weights 298, that is 1.64,
+// 1.42, 1.01, 1.45 and 1.38 PFLOP/s (cuBLAS 8192^3: 1.64); forming a and b again (kFfHidden) 395 instead of grad's 136. The 256 x 256
+// tiles wait for their loads (stamps: 610 to 730 cycles for a k block of 512 cycles of products).
 #pragma once
 
 #include "blocks_status.cuh"

@@ -595,8 +595,8 @@ class SandwichTransition(nn.Module):
 
         update = mask * scale * sigmoid(gate) * norm_out(squeeze(act(expand_a h) * expand_b h)),   h = ln_in(x)
 
-    the :class:`Transition` of token and alignment tensors (``kind_out`` None, ``scale`` None and no gate: the same operator; its
-    parameters then have the same names, ``ln_in``, ``feed_forward.expand_a`` ... under ``feed_forward``)."""
+    the :class:`Transition` of token and alignment tensors (with ``kind_out`` None, ``scale`` None and no gate the same operator, whose
+    linears here lie under ``feed_forward``)."""
 
     def __init__(self, d: int, n: int = 4, hidden: Optional[int] = None, activation: str = "silu", kind: str = "layer",
                  kind_out: Optional[str] = "layer", scale: Optional[float] = None, implementation=None, check_status: bool = False):
