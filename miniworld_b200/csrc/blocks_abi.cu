@@ -207,9 +207,8 @@ static int launch_join_backward(const JoinParams& p, bool wide, const JoinGrid& 
     }
     if (p.dgate != nullptr && shared_gate) {
       auto last = vec == 8 ? join_tile_gate_kernel<T, 8> : vec == 2 ? join_tile_gate_kernel<T, 2> : join_tile_gate_kernel<T, kOdd<T>>;
-      const long long groups = p.rows / p.gate_rows;
-      if (groups > 65535) return B200_TRIMUL_E_SHAPE;
-      TRIMUL_CUDA(launch_overlapped(last, dim3((8 * p.team + 31) / 32, static_cast<unsigned>(groups)), 1024, 0, stream, q));
+      // (kSharedGateRows rows a gate row and more: memory ends long before the grid does)
+      TRIMUL_CUDA(launch_overlapped(last, dim3(static_cast<unsigned>(p.rows / p.gate_rows), (8 * p.team + 31) / 32), 1024, 0, stream, q));
     }
     return B200_TRIMUL_OK;
   }

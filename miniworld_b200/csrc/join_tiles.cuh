@@ -871,9 +871,9 @@ __global__ void __launch_bounds__(1024) join_tile_gate_kernel(const JoinTilePara
   const int x = threadIdx.x & 31, chain = threadIdx.x >> 5;
   const int team = j.team, teams = p.workers / team;
   const long long block_rows = static_cast<long long>(p.block_tiles) * p.tile_rows;
-  const long long group = blockIdx.y, begin = group * j.gate_rows, end = begin + j.gate_rows;
+  const long long group = blockIdx.x, begin = group * j.gate_rows, end = begin + j.gate_rows;
   const int b0 = static_cast<int>(begin / block_rows), b1 = static_cast<int>((end - 1) / block_rows);
-  const int c = blockIdx.x * 32 + x;  // element of the teams' order
+  const int c = blockIdx.y * 32 + x;  // element of the teams' order
   float a = 0.f;
   if (c < 8 * team) {
     // (the first block's rows may begin in an earlier gate row; every later block begins in this one)
@@ -882,8 +882,8 @@ __global__ void __launch_bounds__(1024) join_tile_gate_kernel(const JoinTilePara
 #pragma unroll 4
     for (int k = chain; k < places; k += 32) {
       const int block = k / teams;
-      const int place = ((b0 + block) * p.group_slots + (block == 0 ? slot : 0)) * teams + k - block * teams;
-      a += __ldcg(j.gate_part + static_cast<long long>(place) * (8 * team) + c);
+      const long long place = (static_cast<long long>(b0 + block) * p.group_slots + (block == 0 ? slot : 0)) * teams + k - block * teams;
+      a += __ldcg(j.gate_part + place * (8 * team) + c);
     }
   }
   part[chain][x] = a;

@@ -185,6 +185,20 @@ def test_gate_rows_inside_one_team():
     _compare(_run(t, None, "rms"), _want(t, None, "rms"), "parts")
 
 
+def test_many_gate_rows():
+    """More gate rows than one dimension of a grid may have blocks (65535), each of many rows."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    n, m, d = 66000, 257, 8
+    x, u, dy = (torch.randn(n, m, d, generator=g, device=DEV, dtype=torch.float32).bfloat16() for _ in range(3))
+    gate = torch.randn(n, 1, d, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    (got,) = torch.autograd.grad(blocks.block_join(x, u, gate=gate), gate, dy)
+    s = torch.sigmoid(gate.detach().double())
+    terms = dy.double() * u.double()
+    slope = s * (1 - s)
+    ref, amp = terms.sum(1, keepdim=True) * slope, terms.abs().sum(1, keepdim=True) * slope
+    assert float(((got.double() - ref).abs() / (2.0**-16 * amp + 2.0**-8 * ref.abs() + 1e-30)).max()) <= 1.0
+
+
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 @pytest.mark.parametrize("type", TYPES)
 @pytest.mark.parametrize("rows,d", [(1, 64), (1000, 64), (24, 384), (7, 33), (200, 1536)])
