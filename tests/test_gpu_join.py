@@ -270,6 +270,16 @@ def test_no_rows(rows):
         assert not got[k].any(), k
 
 
+@pytest.mark.parametrize("shape,gate", [((4, 0), (4, 1)), ((0, 5), (1, 1)), ((0,), ())])
+def test_gate_rows_of_no_rows(shape, gate):
+    """The gradient of a gate row that no row shares is zero, whatever the memory held."""
+    x = torch.zeros(*shape, 64, dtype=torch.bfloat16, device=DEV)
+    g = torch.zeros(*gate, 64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    torch.full((4 * 64,), float("nan"), dtype=torch.bfloat16, device=DEV)  # (freed: what the next allocation finds)
+    (got,) = torch.autograd.grad(blocks.block_join(x, x, gate=g), g, x)
+    assert got.shape == g.shape and not got.any()
+
+
 def test_layouts_and_types_are_converted():
     t = _make(60, 64, torch.bfloat16, (60,), True, False, "layer", "layer")
     want = _run(t, "layer", "layer")
