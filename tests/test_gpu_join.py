@@ -326,6 +326,39 @@ def test_refusals():
         torch.func.vmap(lambda r: blocks.block_norm(r))(x)
 
 
+def test_what_changes_before_the_backward_is_noticed():
+    x = torch.randn(6, 64, device=DEV).bfloat16().requires_grad_(True)
+    mask = torch.ones(6, dtype=torch.bool, device=DEV)
+    y = blocks.block_join(x, x, mask=mask)
+    mask[2] = False
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(torch.ones_like(y))
+    # hooks that give back other tensors than were saved
+    f = torch.randn(6, 64, device=DEV).requires_grad_(True)
+    for unpack in (lambda t: t.bfloat16(), lambda t: t[:3], lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = blocks.block_join(f, f * 2, scale=torch.ones(64, device=DEV), mask=torch.ones(6, dtype=torch.bool, device=DEV))
+        with pytest.raises(RuntimeError, match="came back with another"):
+            y.backward(torch.ones_like(y))
+
+
+def test_no_gradient_arrives():
+    class Cut(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, a):
+            return a * 1
+
+        @staticmethod
+        def backward(ctx, g):
+            return None
+
+    x = torch.randn(6, 64, device=DEV).bfloat16().requires_grad_(True)
+    u = torch.randn(6, 64, device=DEV).bfloat16().requires_grad_(True)
+    y, h = blocks.block_join(x, u, post=blocks.Norm(), pre=blocks.Norm())
+    g = torch.autograd.grad(Cut.apply(y).sum() + Cut.apply(h).sum(), [x, u], allow_unused=True)
+    assert all(i is None or not i.any() for i in g)
+
+
 def test_gradients_against_differences():
     """fp32, directional: (f(x + e v) - f(x - e v)) / 2e in double steps of the fp32 forward is off by 2^-24 |f| / e + e^2."""
     t = _make(16, 48, torch.float32, (16,), True, True, "layer", "rms")
