@@ -305,3 +305,34 @@ def test_refused_under_transforms():
     with FakeTensorMode() as mode:
         with pytest.raises(RuntimeError):
             blocks.block_norm(mode.from_tensor(x))
+
+
+def test_second_derivatives_are_refused():
+    """A gradient under ``create_graph`` is right and raises an error where it would be differentiated again."""
+    x = torch.randn(5, 64, device=DEV).bfloat16().requires_grad_(True)
+    w = [torch.randn(*s, device=DEV).mul_(0.1).requires_grad_(True) for s in ((72, 64), (72, 64), (64, 72))]
+    for f, leaves in ((lambda: blocks.block_join(x, x * 2, post=blocks.Norm(), pre=blocks.Norm())[1], [x]),
+                      (lambda: blocks.gated_feed_forward(x, *w), [x, *w])):
+        y = f()
+        dy = torch.randn_like(y)
+        want = torch.autograd.grad(f(), leaves, dy)
+        got = torch.autograd.grad(y, leaves, dy, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            sum(g.float().square().sum() for g in got).backward()
+
+
+def test_forward_mode_and_lazy_negation_are_refused():
+    import torch.autograd.forward_ad as fwad
+
+    x = torch.randn(5, 64, device=DEV).bfloat16()
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        blocks.block_norm(fwad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(RuntimeError, match="plain dense"):
+        blocks.block_norm(torch._neg_view(x))
+    # a gradient that arrives so is taken for what it stands for
+    x.requires_grad_(True)
+    dy = torch.randn(5, 64, device=DEV).bfloat16()
+    (want,) = torch.autograd.grad(blocks.block_norm(x), x, -dy)
+    (got,) = torch.autograd.grad(blocks.block_norm(x), x, torch._neg_view(dy))
+    assert torch.equal(got, want)
