@@ -90,7 +90,7 @@ static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count,
   long long rows = std::min<long long>(teams, share);
   rows = static_cast<long long>(up(static_cast<size_t>(rows), unit));
   p->params = 8 * nv * j.team;
-  const int fixed = params * p->params * 4 + kTileScratch;
+  const int fixed = params * p->params * 4 + kTileScratch + kTileTail;
   while (true) {
     p->slot = static_cast<int>(up(static_cast<size_t>(rows) * j.d * size, 128));
     p->stages = std::min(kTileMaxStages, (smem - fixed) / (p->slot * p->slots));
@@ -107,7 +107,7 @@ static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count,
 }
 static int tile_smem(const JoinTileParams& p, int params) {
   // (the backward's sums pass through the stages)
-  return params * p.params * 4 + kTileScratch + std::max(p.stages * p.slots * p.slot, params == 3 ? p.workers * 8 * 4 : 0);
+  return params * p.params * 4 + kTileScratch + kTileTail + std::max(p.stages * p.slots * p.slot, params == 3 ? p.workers * 8 * 4 : 0);
 }
 using TileKernel = void (*)(JoinTileParams);
 template <typename T>
@@ -232,6 +232,7 @@ static size_t join_sums_bytes(int d) { return up(static_cast<size_t>(kMaxSms) * 
 static int ff_device(DeviceInfo* info) {
   const int rc = device_info(info);
   if (rc != 0) return rc;
+  info->sms = std::min(info->sms, kMaxSms);  // (workspaces are sized for these)
   TRIMUL_CUDA(cudaSetDevice(info->device));
   return B200_TRIMUL_OK;
 }

@@ -291,7 +291,8 @@ struct TileRing {
     };
     auto store = [&](int k) -> bool {
       const int tile = first() + k * step(), s = k % S;
-      if (!mbar_wait(done(s), (k / S) & 1, abort_flag, &blocks_status, kDevTimeoutProducer)) return false;
+      const bool got = mbar_wait_thread(done(s), (k / S) & 1, abort_flag, &blocks_status, kDevTimeoutProducer);
+      if (!__all_sync(0xFFFFFFFFu, got && *abort_flag == 0)) return false;
       const size_t at = static_cast<size_t>(tile) * p.tile_rows * row_bytes;
       const uint32_t bytes = bytes_of(tile), whole = bytes & ~15u;
 #pragma unroll
@@ -455,8 +456,9 @@ __device__ __forceinline__ float2 tile_stats(const float2 (&v)[4 * NV], int kind
   return make_float2(mean, rsqrtf(fmaf(dev, inv, eps)));
 }
 
-// Shared memory: parameters | scratch of the sums | barriers | stages
+// Shared memory: parameters | scratch of the sums | barriers | stages | what the last row's words reach past its end (odd widths)
 constexpr int kTileScratch = kTileTeams * 32 * 8 + 2 * kTileMaxStages * 8 + 16;
+constexpr int kTileTail = 16;
 
 template <typename T, int VEC, int NV, bool EXACT>
 __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forward_kernel(const JoinTileParams p) {
@@ -508,7 +510,8 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
   int s = 0;
   uint32_t ph = 0, stage = ring_at;
   for (int k = 0; k < n; ++k) {
-    if (!mbar_wait_warp(ring.full(s), ph, abort_flag, &blocks_status, kDevTimeoutStats)) break;
+    // (a wait that gave up: the warps go on over what there is, every later wait returns at once, and none is missing at a barrier)
+    mbar_wait_warp(ring.full(s), ph, abort_flag, &blocks_status, kDevTimeoutStats);
     const int rows = j.rows - r0 < p.tile_rows ? static_cast<int>(j.rows - r0) : p.tile_rows;
     for (int r = id; r - id < p.tile_rows; r += teams) {
       const long long row = r0 + r;
@@ -661,7 +664,7 @@ __global__ void __launch_bounds__(kTileThreads, JOIN ? 1 : 2) join_tile_backward
     if (n > 0) row_facts(r0, id);
     for (int k = 0; k < n; ++k) {
       const int rows = j.rows - r0 < p.tile_rows ? static_cast<int>(j.rows - r0) : p.tile_rows;
-      if (!mbar_wait_warp(ring.full(s), ph, abort_flag, &blocks_status, kDevTimeoutStats)) break;
+      mbar_wait_warp(ring.full(s), ph, abort_flag, &blocks_status, kDevTimeoutStats);  // (as in the forward)
       for (int r = id; r - id < p.tile_rows; r += teams) {
         const bool on = r < rows;
         const bool valid = next_valid != 0;
