@@ -77,7 +77,8 @@ static bool all_aligned16(std::initializer_list<const void*> ps) {
 
 // Tiles of a call (see join_tiles.cuh): rows to a tile, stages and their places. False where the tensors do not start on 16 bytes
 // or a row takes more warps than there are or two stages do not fit: the kernels of join.cuh
-// then run. As many rows to a tile as the block works on at a time, fewer where that would leave SMs without one.
+// then run.
+constexpr int kTileRounds = 4;  // most rounds of a tile
 static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count, int size, int nv, int params, int blocks_most, int smem) {
   for (int i = 0; i < count; ++i)
     if (!aligned(tensors[i], 16)) return false;
@@ -86,19 +87,27 @@ static bool plan_tiles(JoinTileParams* p, const void* const* tensors, int count,
   const int unit = 16 / static_cast<int>(std::gcd(16, j.d * size));  // rows whose bytes are a multiple of 16
   const int teams = j.team > 32 ? std::min(kTileTeams, kTileWarps * 32 / j.team) : kTileWarps * 32 / j.team;
   p->workers = teams * j.team;
-  const long long share = (j.rows + blocks_most - 1) / blocks_most;
-  long long rows = std::min<long long>(teams, share);
-  rows = static_cast<long long>(up(static_cast<size_t>(rows), unit));
   p->params = 8 * nv * j.team;
   const int fixed = params * p->params * 4 + kTileScratch + kTileTail;
-  while (true) {
+  auto place = [&](int rows) {
     p->slot = static_cast<int>(up(static_cast<size_t>(rows) * j.d * size, 128));
     p->stages = std::min(kTileMaxStages, (smem - fixed) / (p->slot * p->slots));
-    if (p->stages >= 2) break;
-    if (rows <= unit) return false;
-    rows = static_cast<long long>(up(static_cast<size_t>(rows / 2), unit));
+    return p->stages;
+  };
+  // The fewest rounds of the teams in all, then the smallest tile: the rows of a tile are a multiple of `unit`, so that where that does not
+  // divide the teams the last round of a tile leaves some idle, and tiles of several rounds leave fewer (while four stages fit).
+  const long long share = (j.rows + blocks_most - 1) / blocks_most;
+  const int most = static_cast<int>(up(static_cast<size_t>(std::min<long long>(kTileRounds * teams, share)), unit));
+  int rows = 0;
+  long long best = 0;
+  for (int r = unit; r <= most; r += unit) {
+    if (place(r) < (r > teams ? 4 : 2)) break;
+    const long long tiles = (j.rows + r - 1) / r, rounds = (tiles + blocks_most - 1) / blocks_most * ((r + teams - 1) / teams);
+    if (rows == 0 || rounds < best) best = rounds, rows = r;
   }
-  p->tile_rows = static_cast<int>(rows);
+  if (rows == 0) return false;
+  place(rows);
+  p->tile_rows = rows;
   const long long tiles = (j.rows + rows - 1) / rows;
   if (tiles > 0x7FFFFFFF) return false;
   p->tiles = static_cast<int>(tiles);
@@ -650,7 +659,7 @@ int b200_block_join_workspace_bytes(long long rows, int d, long long gate_rows, 
     const int team = join_backward_team(d);
     // the kernels of join.cuh: two gate rows a team; on tiles: the gate rows that the blocks' rows touch (see launch_join_backward)
     const size_t plain = static_cast<size_t>(kMaxSms) * (kJoinBackwardThreads / team) * 2 * 8 * team * 4;
-    const long long most = gate_rows >= kSharedGateRows ? 2 * (rows + kTileWarps * 32 + 16) / gate_rows + 3 * kMaxSms : 0;
+    const long long most = gate_rows >= kSharedGateRows ? 2 * (rows + kTileRounds * kTileWarps * 32 + 16) / gate_rows + 3 * kMaxSms : 0;
     *out_bytes += std::max(plain, static_cast<size_t>(most) * (kTileWarps * 32 / team) * 8 * team * 4);
   }
   return B200_TRIMUL_OK;

@@ -359,11 +359,15 @@ struct TileSum {
   int team, warps, id, half, warp_in_team;
   template <typename F>
   __device__ __forceinline__ void steps(F f) const {
-    if (team >= 32) f(16);
-    if (team >= 16) f(8);
-    if (team >= 8) f(4);
-    if (team >= 4) f(2);
-    if (team >= 2) f(1);
+    if (team >= 32) {
+      f(16), f(8), f(4), f(2), f(1);
+    } else if (team == 16) {
+      f(8), f(4), f(2), f(1);
+    } else {
+      if (team >= 8) f(4);
+      if (team >= 4) f(2);
+      if (team >= 2) f(1);
+    }
   }
   // every warp's value in shared memory, ready to be read
   __device__ __forceinline__ const float2* exchange(float2 v) {
