@@ -810,17 +810,34 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_up_kernel(const FfVec p)
   extern __shared__ __align__(16) float vec_rows[];
   grid_dependency_wait();
   grid_dependents_launch();
+  const int unit = blockIdx.x * (kFfVecThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const size_t row = static_cast<size_t>(min(unit, p.hidden - 1)) * p.d;
+  const uint16_t* wa = static_cast<const uint16_t*>(p.w_a) + row;
+  const uint16_t* wb = static_cast<const uint16_t*>(p.w_b) + row;
+  // the first weights are on their way while the rows come in
+  constexpr int kFirst = 4;
+  uint4 fa[kFirst], fb[kFirst];
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i) {
+    const int c = lane * 8 + i * 256;
+    fa[i] = c < p.d ? __ldcg(reinterpret_cast<const uint4*>(wa + c)) : make_uint4(0, 0, 0, 0);
+    fb[i] = c < p.d ? __ldcg(reinterpret_cast<const uint4*>(wb + c)) : make_uint4(0, 0, 0, 0);
+  }
   ff_vec_rows<F16, R>(vec_rows, p.x, p.rows, p.d, 0, p.d);
   __syncthreads();
-  const int unit = blockIdx.x * (kFfVecThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (unit >= p.hidden) return;
-  const uint16_t* wa = static_cast<const uint16_t*>(p.w_a) + static_cast<size_t>(unit) * p.d;
-  const uint16_t* wb = static_cast<const uint16_t*>(p.w_b) + static_cast<size_t>(unit) * p.d;
   float2 a[R], b[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) a[r] = b[r] = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i) {
+    const int c = lane * 8 + i * 256;
+    if (c >= p.d) break;
+    ff_vec_step<F16, R>(a, vec_rows, p.d, c, fa[i]);
+    ff_vec_step<F16, R>(b, vec_rows, p.d, c, fb[i]);
+  }
 #pragma unroll 2
-  for (int c = lane * 8; c < p.d; c += 256) {
+  for (int c = lane * 8 + kFirst * 256; c < p.d; c += 256) {
     const uint4 va = __ldcg(reinterpret_cast<const uint4*>(wa + c)), vb = __ldcg(reinterpret_cast<const uint4*>(wb + c));
     ff_vec_step<F16, R>(a, vec_rows, p.d, c, va);
     ff_vec_step<F16, R>(b, vec_rows, p.d, c, vb);
@@ -837,10 +854,19 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_up_kernel(const FfVec p)
 template <bool F16, int R>
 __global__ void __launch_bounds__(kFfVecThreads) ff_vec_down_kernel(const FfVec p) {
   extern __shared__ __align__(16) float vec_rows[];
-  grid_dependency_wait();
-  grid_dependents_launch();
   const int col = blockIdx.x * (kFfVecThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint16_t* w = static_cast<const uint16_t*>(p.w_s) + static_cast<size_t>(col < p.d ? col : 0) * p.hidden;
+  // The first weights before the wait: the launch before is ff_vec_up_kernel, which writes h alone and has itself waited for what wrote
+  // the weights before it let this kernel begin.
+  constexpr int kFirst = 8;
+  uint4 first[kFirst];
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i) {
+    const int c = lane * 8 + i * 256;
+    first[i] = c < p.hidden ? __ldcg(reinterpret_cast<const uint4*>(w + c)) : make_uint4(0, 0, 0, 0);
+  }
+  grid_dependency_wait();
+  grid_dependents_launch();
   float2 acc[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) acc[r] = make_float2(0.f, 0.f);
@@ -853,8 +879,17 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_down_kernel(const FfVec 
       *reinterpret_cast<float4*>(vec_rows + r * n + (c & 4) / 4 * (n / 2) + c / 8 * 4) = v;  // (the order of ff_vec_rows)
     }
     __syncthreads();
+    int start = lane * 8;
+    if (k0 == 0) {
+#pragma unroll
+      for (int i = 0; i < kFirst; ++i) {
+        if (start >= n) break;
+        ff_vec_step<F16, R>(acc, vec_rows, n, start, first[i]);
+        start += 256;
+      }
+    }
 #pragma unroll 4
-    for (int c = lane * 8; c < n; c += 256) {
+    for (int c = start; c < n; c += 256) {
       const uint4 v = __ldcg(reinterpret_cast<const uint4*>(w + k0 + c));
       ff_vec_step<F16, R>(acc, vec_rows, n, c, v);
     }
