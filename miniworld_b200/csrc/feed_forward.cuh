@@ -763,18 +763,22 @@ template <bool F16>
 __device__ __forceinline__ float2 ff_two(uint32_t w) {
   return F16 ? f16x2_to_float2(w) : bf16x2_to_float2(w);
 }
-// rows [0, R) x columns [k0, k0 + n) of a 16-bit matrix to fp32 [R][n], the halves of each piece of eight n / 2 apart (16-byte reads of
+// rows [0, R) of n columns of a 16-bit matrix to fp32 [R][n], the halves of each piece of eight n / 2 apart (16-byte reads of
 // a warp without bank conflicts); rows past `rows` are zero
 template <bool F16, int R>
-__device__ __forceinline__ void ff_vec_rows(float* to, const void* from, int rows, int ld, int k0, int n) {
-  const int pieces = n / 8;
-  for (int e = threadIdx.x; e < R * pieces; e += kFfVecThreads) {
-    const int r = e / pieces, c = (e - r * pieces) * 8;
-    const uint4 w = r < rows ? __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(from) + static_cast<size_t>(r) * ld + k0 + c)) : make_uint4(0, 0, 0, 0);
-    const float2 a = ff_two<F16>(w.x), b = ff_two<F16>(w.y), d = ff_two<F16>(w.z), f = ff_two<F16>(w.w);
-    float* o = to + r * n + c / 2;
-    *reinterpret_cast<float4*>(o) = make_float4(a.x, a.y, b.x, b.y);
-    *reinterpret_cast<float4*>(o + n / 2) = make_float4(d.x, d.y, f.x, f.y);
+__device__ __forceinline__ void ff_vec_rows(float* to, const void* from, int rows, int ld, int n) {
+  for (int c = threadIdx.x * 8; c < n; c += kFfVecThreads * 8) {
+    uint4 w[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      w[r] = r < rows ? __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(from) + static_cast<size_t>(r) * ld + c)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float2 a = ff_two<F16>(w[r].x), b = ff_two<F16>(w[r].y), d = ff_two<F16>(w[r].z), f = ff_two<F16>(w[r].w);
+      float* o = to + r * n + c / 2;
+      *reinterpret_cast<float4*>(o) = make_float4(a.x, a.y, b.x, b.y);
+      *reinterpret_cast<float4*>(o + n / 2) = make_float4(d.x, d.y, f.x, f.y);
+    }
   }
 }
 // acc[r] += the products of eight weights with the rows' eight values
@@ -823,7 +827,7 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_up_kernel(const FfVec p)
     fa[i] = c < p.d ? __ldcg(reinterpret_cast<const uint4*>(wa + c)) : make_uint4(0, 0, 0, 0);
     fb[i] = c < p.d ? __ldcg(reinterpret_cast<const uint4*>(wb + c)) : make_uint4(0, 0, 0, 0);
   }
-  ff_vec_rows<F16, R>(vec_rows, p.x, p.rows, p.d, 0, p.d);
+  ff_vec_rows<F16, R>(vec_rows, p.x, p.rows, p.d, p.d);
   __syncthreads();
   if (unit >= p.hidden) return;
   float2 a[R], b[R];
@@ -873,10 +877,14 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_down_kernel(const FfVec 
   for (int k0 = 0; k0 < p.hidden; k0 += p.part) {
     const int n = min(p.part, p.hidden - k0);
     if (k0 != 0) __syncthreads();
-    for (int e = threadIdx.x; e < R * (n / 4); e += kFfVecThreads) {
-      const int r = e / (n / 4), c = (e - r * (n / 4)) * 4;
-      const float4 v = r < p.rows ? __ldcg(reinterpret_cast<const float4*>(p.h + static_cast<size_t>(r) * p.hidden + k0 + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<float4*>(vec_rows + r * n + (c & 4) / 4 * (n / 2) + c / 8 * 4) = v;  // (the order of ff_vec_rows)
+#pragma unroll 2
+    for (int c = threadIdx.x * 4; c < n; c += kFfVecThreads * 4) {
+      float4 v[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        v[r] = r < p.rows ? __ldcg(reinterpret_cast<const float4*>(p.h + static_cast<size_t>(r) * p.hidden + k0 + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int r = 0; r < R; ++r) *reinterpret_cast<float4*>(vec_rows + r * n + (c & 4) / 4 * (n / 2) + c / 8 * 4) = v[r];  // (the order of ff_vec_rows)
     }
     __syncthreads();
     int start = lane * 8;
