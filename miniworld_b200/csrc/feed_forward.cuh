@@ -755,7 +755,9 @@ __global__ void __launch_bounds__(1024) ff_reduce_kernel(const FfReduce p) {
 // A few rows (the single tokens of serving): every weight is read once and meets all rows, so the bytes of the weights bound it and
 // tensor cores would idle on tiles of 128 rows. A warp takes a hidden unit (its rows of W_a and W_b) or a column of y (a row of W_s), a
 // lane every 32nd piece of eight weights; the rows lie in shared memory in fp32. R: rows, rounded up to a power of two.
-constexpr int kFfVecRows = 4;  // (768 x 2048, both kernels: one row 6.0 us, four 8.8, eight 18.9; tiles of tensor cores 15.7)
+// (us a call, calls in a graph, this and tiles of tensor cores: 768 x 2048 one row 4.6, four 7.7, eight 11.6 and 12.8; 384 x 1536 eight
+// 9.3 and 9.7; 1024 x 4096 two 11.0, eight 23.9 and 17.6)
+constexpr int kFfVecRows = 4;
 constexpr int kFfVecThreads = 256;
 constexpr int kFfVecSmem = 96 * 1024;  // rows of the second product pass through it in parts
 
