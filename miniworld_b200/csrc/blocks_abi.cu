@@ -20,17 +20,16 @@ constexpr int kMaxSms = 160;
 
 // ---------------------------------------------------------------- join
 // Threads of a row (up to 32 reduce by shuffles alone; wider rows take four warps) and 8-element pieces of each: the fewest idle lanes,
-// then what measured fastest (us, forward of 2^24 elements with every part, NV = 1, 2, 4): pieces read at once, 16 bits: 64 wide 42.9,
-// 38.8, 45.1, 256 wide 44.9, 38.9, 42.9, fp32 61.3, 61.4, 88; 16-bit rows read in pairs (other widths): 101 wide 119, 117, 88, 250 wide
-// 82, 76, 53, 203 wide 121, 118, 117; fp32 203 wide 127, 107, 131. Three pieces only where they leave fewer lanes idle: 384 wide 36.7.
+// then two pieces (us, forward of 2^24 elements with every part, one, two and four pieces: 16 bits, 64 wide 42.6, 40.7, 42.8, 256 wide
+// 41.7, 39.1, 39.3, 200 wide 55, 53, 50, 250 wide 57, 50, 50, 101 wide 84, 77, 85, 203 wide 119, 83, 87; fp32, 256 wide 57, 61, 95, 203
+// wide 84, 69, 111). Three pieces only where they leave fewer lanes idle: 384 wide 36.7.
 struct JoinShape {
   int team, nv;
 };
-static JoinShape join_forward_shape(int d, int size) {
-  const bool pairs = size == 2 && d % 8 != 0;
+static JoinShape join_forward_shape(int d) {
   JoinShape best{0, 0};
   int waste = 0;
-  for (int nv : {pairs ? 4 : 2, pairs ? 2 : 1, pairs ? 1 : 4, 3})
+  for (int nv : {2, 1, 4, 3})
     for (int team : {1, 2, 4, 8, 16, 32, 64, 128}) {
       const int have = team * nv * 8;
       if (have < d || (team > 32 && nv < 4)) continue;
@@ -142,7 +141,7 @@ template <typename T>
 static int launch_join_forward(const JoinParams& p0, bool wide, const DeviceInfo& info, cudaStream_t stream) {
   JoinTileParams q = {};
   q.j = p0;
-  const JoinShape s = join_forward_shape(p0.d, sizeof(T));
+  const JoinShape s = join_forward_shape(p0.d);
   q.j.team = s.team;
   q.slot_of[0] = q.slots++;
   q.slot_of[1] = p0.u != nullptr ? q.slots++ : -1;

@@ -53,7 +53,8 @@ __device__ __forceinline__ uint4 lds4(uint32_t a) {
 __device__ __forceinline__ void sts4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// Single words under a predicate: a branch for each would cost more than the access (82646 rows of 203, forward: 129 against 121 us)
+// Single words under a predicate: a branch for each would cost more than the access (82646 rows of 203, forward on tiles of one round: 129
+// against 121 us)
 __device__ __forceinline__ uint32_t lds_if(uint32_t a, bool on) {
   uint32_t v;
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.shared.b32 %0, [%1];\n\t}" : "=r"(v) : "r"(a), "r"(static_cast<uint32_t>(on)) : "memory");
