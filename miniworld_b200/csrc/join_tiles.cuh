@@ -842,10 +842,17 @@ __global__ void __launch_bounds__(1024) join_tile_sums_kernel(const JoinTileSums
   const int pair = blockIdx.y;  // S1 and S2, or S3 and S4
   float a = 0.f, b = 0.f;
   if (c < p.d)
-    for (int k = chain; k < p.blocks; k += 32) {
-      const float* s = p.sums + (static_cast<size_t>(k) * 4 + pair * 2) * p.d + c;
-      a += __ldcg(s);
-      b += __ldcg(s + p.d);
+    for (int k0 = chain; k0 < p.blocks; k0 += 5 * 32) {  // (ten loads in flight, all that one block an SM leaves: 6.5 -> 5 us)
+      float va[5], vb[5];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) {
+        const int k = k0 + i * 32;
+        const float* s = p.sums + (static_cast<size_t>(k) * 4 + pair * 2) * p.d + c;
+        va[i] = k < p.blocks ? __ldcg(s) : 0.f;
+        vb[i] = k < p.blocks ? __ldcg(s + p.d) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 5; ++i) a += va[i], b += vb[i];
     }
   part[0][chain][x] = a;
   part[1][chain][x] = b;
