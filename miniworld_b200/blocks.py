@@ -10,7 +10,7 @@ operators: token and alignment tensors of other widths (the reference builds its
     x = block_join(x, f(h), gate=..., scale=..., post=Norm(...))
 
 Inputs are CUDA tensors; nothing here falls back to PyTorch arithmetic. Layouts and, where it says so, float types are converted;
-everything else is refused with a ``RuntimeError``.
+everything else is refused with a ``RuntimeError``, forward-mode derivatives and second derivatives among it.
 """
 
 from __future__ import annotations
@@ -62,8 +62,8 @@ def block_join(x: torch.Tensor, u: torch.Tensor, *, gate: Optional[torch.Tensor]
     """``y = x + mask * scale * sigmoid(gate) * post(u)`` and, with ``pre``, ``(y, pre(y))`` (differentiable).
 
     ``x`` bf16, fp16 or fp32 [..., d]; ``u`` of its shape; ``gate`` logits [..., d] of ``x``'s leading dimensions and then
-    ones (a row each, one for the rows of a sample, one for all); ``scale`` fp32 [d]; ``mask`` over the rows, zero: ``y = x`` there whatever ``u`` and
-    ``gate`` hold. ``u`` and ``gate`` of another float type are converted. ``pre`` sees ``y`` before it is rounded to ``x``'s type.
+    ones (a row each, one for the rows of a sample, one for all); ``scale`` fp32 [d]; ``mask`` over the rows, zero: ``y = x`` there
+    whatever ``u`` and ``gate`` hold. ``u`` and ``gate`` of another float type are converted. ``pre`` sees ``y`` before it is rounded to ``x``'s type.
     """
     y, h = _lib.native().block_join(x, u, gate, scale, mask, *_spread(post), *_spread(pre))
     return y if pre is None else (y, h)
