@@ -534,7 +534,9 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 2 : 1) join_tile_forwa
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) u[i] = __fmul2_rn(__fadd2_rn(u[i], f2(-st.x)), f2(st.y));
         }
-        if (j.post_w != nullptr || j.scale != nullptr) {
+        // (without weight and scale too where a layer norm has left -mean / sigma past the width: the zeros that stand there keep it out of
+        // the next norm's mean; selects in that mean would cost every call of such widths 3 %)
+        if (j.post_w != nullptr || j.scale != nullptr || (!EXACT && j.post_kind == kNormLayer)) {
           tile_params<VEC, NV>(par_at, p.params, t, team, w);
 #pragma unroll
           for (int i = 0; i < 4 * NV; ++i) u[i] = __fmul2_rn(u[i], w[i]);

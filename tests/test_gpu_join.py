@@ -397,3 +397,17 @@ def test_stack_of_modules():
     for i in range(3):
         b = joins[i](b, torch.tanh(norms[i](b)))
     assert float((a - b).abs().max()) <= 64 * 2.0**-24 * float(a.abs().max())
+
+
+@pytest.mark.parametrize("d", [100, 130, 200, 203, 250, 1000])
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("gate,bias", [(None, False), ("row", False), ("one", True), (None, True)])
+def test_norms_without_weights(gate, bias, type, d):
+    """No weight after the block and no scale: nothing but the width keeps the registers past it out of the next norm's mean."""
+    rows = 70
+    t = _make(rows, d, type, {None: None, "row": (rows,), "one": (1,)}[gate], False, True, "layer", "layer", bias)
+    t["u"] += 1  # (a mean, which those registers take with its sign turned)
+    ones = torch.ones(d, device=DEV)
+    want = _want({**t, "post_w": ones, "pre_w": ones}, "layer", "layer")
+    del t["post_w"], t["pre_w"], want["post_w"], want["pre_w"]
+    _compare(_run(t, "layer", "layer"), want, (gate, bias, type, d))
