@@ -68,8 +68,9 @@ int b200_block_join_backward(const void* dy, const void* dh, const void* x, cons
  * in each call). Workspaces: 1024-byte aligned, b200_ff_workspace_bytes of the same sizes (backward 0 or 1).
  */
 int b200_ff_workspace_bytes(long long rows, int d, int hidden, int weight_dtype, int backward, size_t* out_bytes);
-/* For a backward: bytes that the forward of these sizes keeps (h, and a = x w_a^T and b = x w_b^T in fp16, saturating at 65504), 0 where the backward forms them
- * again faster. A forward and its backward get the same buffer as `kept` (1024-byte aligned), or both null. */
+/* For a backward: bytes that the forward of these sizes keeps (h, and a = x w_a^T and b = x w_b^T to 10 bits and more with a power of
+ * two for 16 neighbouring units of a row: what is below 2^-25 of the largest of them loses bits), 0 where the backward forms them again
+ * faster. A forward and its backward get the same buffer as `kept` (1024-byte aligned), or both null. */
 int b200_ff_kept_bytes(long long rows, int d, int hidden, size_t* out_bytes);
 int b200_ff_forward(const void* x, const void* w_a, const void* w_b, const void* w_s, void* y, void* kept, void* workspace,
                     size_t workspace_bytes, long long rows, int d, int hidden, int dtype, int weight_dtype, int activation,

@@ -4,10 +4,11 @@
 //   dh = dy W_s,  da = dh b act'(a),  db = dh act(a),  dx = da W_a + db W_b,  dW_a = da^T x,  dW_b = db^T x,  dW_s = dy^T h
 //
 // The backward forms a and b again from x (16 M D H multiply-adds in all instead of 12), or, where that costs more than writing and
-// reading them (D >= 512 and many rows: the caller then keeps a buffer), takes them from the forward, as fp16 for either type of x
-// (11 bits of their values, saturating: kept in bf16 they would add more to the gradients' error than all other roundings). The
-// products run on the tensor cores (fp32 accumulators in tensor memory), by one kernel template; what is between two products of a row
-// is done in the first one's epilogue, on the accumulators:
+// reading them (D >= 512 and many rows: the caller then keeps a buffer), takes them from the forward, as fp16 values with a power of two
+// for 16 neighbours (10 to 11 bits of their values over fp32's range, see ff_keep16: kept in bf16 they would add more to the gradients'
+// error than all other roundings, and plain fp16 loses what lies beyond its range). The products run on the tensor cores (fp32
+// accumulators in tensor memory), by one kernel template; what is between two products of a row is done in the first one's epilogue, on
+// the accumulators:
 //
 //   kFfUp       a | b side by side in one accumulator, h leaves              K = D
 //   kFfDown     y = h W_s^T                                                   K = H
@@ -218,23 +219,49 @@ __device__ __forceinline__ void ff_pack16(const float (&v)[16], uint32_t (&w)[8]
 #pragma unroll
   for (int j = 0; j < 8; ++j) w[j] = ff_pack<F16>(v[2 * j], v[2 * j + 1]);
 }
-// 16 values as fp16, saturating; p on a 32-byte boundary
+// 16 values in 32 bytes (p on such a boundary) that keep the range of fp32: fp16 values times 2^(138 - 4 q), q = E / 4 (at least 3) for the
+// exponent field E of the largest finite one, which so lies in [2^11, 2^15). The six bits of q are the last bits of the first six
+// values, which are rounded to 10 bits for it (Veltkamp's splitting: x C - (x C - x) with C = 2^14 + 1; Dekker, Numerische Mathematik 18,
+// 1971); the others have 11. Both hold down to 2^-25 of the largest of the 16; what is smaller is a multiple of 2^-35 of it (2^-34 among
+// the first six). An infinite value stays infinite or becomes a NaN.
 __device__ __forceinline__ void ff_keep16(__half* p, const uint32_t (&v)[16]) {
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(__uint_as_float(v[j])));  // (a NaN is left out)
+  if (__float_as_uint(most) == 0x7F800000u) {
+    most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) most = fmaxf(most, (v[j] & 0x7FFFFFFFu) == 0x7F800000u ? 0.f : fabsf(__uint_as_float(v[j])));
+  }
+  const uint32_t q = max(__float_as_uint(most) >> 25, 3u);
+  const float2 scale = ff_f2(__uint_as_float((265u - 4u * q) << 23));
   uint32_t w[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = pack_f16x2_sat(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])));
+  for (int j = 0; j < 8; ++j) {
+    float2 x = __fmul2_rn(ff_at(v, 2 * j), scale);
+    if (j < 3) {
+      const float2 c = __fmul2_rn(x, ff_f2(16385.f)), n = make_float2(-c.x, -c.y);
+      x = __fadd2_rn(c, __fadd2_rn(x, n));
+    }
+    w[j] = pack_f16x2(x);
+    if (j < 3) w[j] = (w[j] & 0xFFFEFFFEu) | (q >> 2 * j & 1u) | (q >> (2 * j + 1) & 1u) << 16;
+  }
   ff_store32(p, w);
 }
 __device__ __forceinline__ void ff_kept16(const uint4 (&w)[2], uint32_t (&v)[16]) {
+  uint32_t h[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+  uint32_t q = 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const uint32_t q[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+  for (int j = 0; j < 3; ++j) {
+    q |= (h[j] & 1u) << 2 * j | (h[j] >> 16 & 1u) << (2 * j + 1);
+    h[j] &= 0xFFFEFFFEu;
+  }
+  const float2 scale = ff_f2(__uint_as_float((4u * q - 11u) << 23));  // 2^(4 q - 138)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = f16x2_to_float2(q[k]);
-      v[8 * j + 2 * k] = __float_as_uint(f.x);
-      v[8 * j + 2 * k + 1] = __float_as_uint(f.y);
-    }
+  for (int j = 0; j < 8; ++j) {
+    const float2 f = __fmul2_rn(f16x2_to_float2(h[j]), scale);
+    v[2 * j] = __float_as_uint(f.x);
+    v[2 * j + 1] = __float_as_uint(f.y);
   }
 }
 

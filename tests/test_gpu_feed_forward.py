@@ -244,3 +244,69 @@ def test_module_matches_the_function():
     assert torch.equal(y, want)
     y.float().square().sum().backward()
     assert all(p.grad is not None and p.grad.dtype == torch.float32 and bool(p.grad.any()) for p in m.parameters())
+
+
+@pytest.mark.parametrize("rows,d,hidden", [(2048, 512, 2048), (1025, 520, 72)])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("scale_a,scale_b", [(1e-3, 1e-3), (1e-6, 1e-6), (1e-8, 1e-8), (1.0, 1e-12), (2.0**18, 1.0), (1.0, 2.0**40), (1e-25, 1e25)])
+def test_expanded_inputs_of_any_magnitude(rows, d, hidden, act, scale_a, scale_b):
+    """Widths and rows for which the forward leaves its expanded inputs for the backward: they keep their precision over bf16's range."""
+    t = _make(rows, d, hidden, torch.bfloat16)
+    t["w_a"] *= scale_a
+    t["w_b"] *= scale_b
+    _compare(_run(t, act), _want(t, act, torch.bfloat16), (rows, d, hidden, act, scale_a, scale_b))
+
+
+def _with_kept(want, t, type):
+    """Bounds of a backward that takes a and b from the forward, which keeps them to a relative e of 2^-11 at most (uniform within it, of
+    either sign): db = dh f(a) is off by dh a f'(a) e, da = dh b f'(a) by dh b f'(a) e and dh b a f''(a) e. |f'| <= 1.13 and |a f''| <= 0.32
+    for SiLU and GELU (sqrt(1.13^2 + 0.32^2) < 1.2): standard deviations of 1.2 * 2^-11 / sqrt(3) of |dh a| and |dh b|, six of them as above."""
+    d = t["x"].shape[-1]
+    x, dy = t["x"].double().reshape(-1, d), t["dy"].double().reshape(-1, d)
+    wa, wb, ws = (t[k].to(type).double() for k in ("w_a", "w_b", "w_s"))
+    dh, six = dy @ ws, 6 * 1.2 * 2.0**-11 / 3**0.5
+    da, db = (dh * (x @ wb.t())).square(), (dh * (x @ wa.t())).square()
+    more = {"x": ((da @ wa.square()).sqrt() + (db @ wb.square()).sqrt()).reshape(t["x"].shape), "w_a": (da.t() @ x.square()).sqrt(),
+            "w_b": (db.t() @ x.square()).sqrt()}
+    return {k: (v, bound + six * more[k] if k in more else bound) for k, (v, bound) in want.items()}
+
+
+@pytest.mark.parametrize("rows,d,hidden", [(2048, 512, 2048), (1025, 520, 72)])
+def test_expanded_inputs_beyond_fp16(rows, d, hidden):
+    """fp16, |a| up to 2^19 with h, da and db within the type. The subnormal ones among these are rounded to multiples of 2^-24: the
+    products get 2^-25 of the other operand's magnitudes more."""
+    t = _make(rows, d, hidden, torch.float16, torch.float32)
+    t["w_a"] *= 2.0**17
+    t["w_b"] *= 2.0**-6
+    t["dy"] *= 2.0**-4
+    want = _with_kept(_want(t, "silu", torch.float16), t, torch.float16)
+    half = 2.0**-25
+    wa, wb, ws = (t[k].half().double().abs() for k in ("w_a", "w_b", "w_s"))
+    x, dy = t["x"].double().abs(), t["dy"].double().abs()
+    more = {"y": half * ws.sum(1).expand(rows, d), "x": half * (wa.sum(0) + wb.sum(0)).expand(rows, d), "w_a": half * x.sum(0).expand(hidden, d),
+            "w_b": half * x.sum(0).expand(hidden, d), "w_s": half * dy.sum(0)[:, None].expand(d, hidden)}
+    _compare(_run(t, "silu"), {k: (v, b + more[k]) for k, (v, b) in want.items()}, (rows, d, hidden))
+
+
+@pytest.mark.parametrize("rows,hidden", [(2048, 2048), (1025, 72)])
+def test_expanded_inputs_of_neighbours_that_differ(rows, hidden):
+    """Neighbouring units of which one is 2^20 times the other: each unit's own gradients keep their precision."""
+    t = _make(rows, 512, hidden, torch.bfloat16)
+    t["w_b"][::2] *= 2.0**-20
+    t["w_a"][1::3] *= 2.0**-20
+    _compare(_run(t, "silu"), _want(t, "silu", torch.bfloat16), (rows, hidden))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_expanded_inputs_that_are_not_finite(bad):
+    """An infinite or undefined weight of one unit: its gradients are not finite, its neighbours' are what they are without it."""
+    t = _make(1100, 512, 128, torch.bfloat16)
+    want = _run(t, "silu")
+    dirty = {k: v.clone() for k, v in t.items()}
+    dirty["w_b"][37, 5] = bad
+    leaves = {k: v.requires_grad_(True) for k, v in dirty.items() if k != "dy"}
+    got = dict(zip(leaves, torch.autograd.grad(blocks.gated_feed_forward(*leaves.values()), list(leaves.values()), dirty["dy"])))
+    keep = torch.arange(128, device=DEV) != 37
+    for k in ("w_a", "w_b"):
+        assert torch.equal(got[k][keep], want[k][keep]), k
+    assert not torch.isfinite(got["w_a"][37]).any()
