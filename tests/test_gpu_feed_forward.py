@@ -310,3 +310,13 @@ def test_expanded_inputs_that_are_not_finite(bad):
     for k in ("w_a", "w_b"):
         assert torch.equal(got[k][keep], want[k][keep]), k
     assert not torch.isfinite(got["w_a"][37]).any()
+
+
+@pytest.mark.parametrize("rows,d,hidden", [(1025, 512, 72), (4100, 520, 1544)])
+@pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("weights", ["same", "fp32"])
+def test_expanded_inputs_that_the_forward_keeps(rows, d, hidden, type, act, weights):
+    """Single CTAs and pairs of the backward that takes a and b from the forward."""
+    t = _make(rows, d, hidden, type, torch.float32 if weights == "fp32" else None)
+    _compare(_run(t, act), _with_kept(_want(t, act, type), t, type), (rows, d, hidden, type, act, weights))
