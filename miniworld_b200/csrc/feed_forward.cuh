@@ -68,14 +68,20 @@ __device__ __forceinline__ uint32_t ff_pack(float a, float b) {
 
 __device__ __forceinline__ float2 ff_f2(float v) { return make_float2(v, v); }
 // 1 / (1 + 2^(-a log2 e)) of four values with one reciprocal, of the product of the four denominators (the special-function unit, four
-// lanes a clock and scheduler, is what an epilogue of few products waits for). The exponent is held below 31, so that the product stays
-// finite: sigmoid(a) is 2^-31 for a < -21, off by less than 5e-10.
+// lanes a clock and scheduler, is what an epilogue of few products waits for). OPEN: all are numbers from kFfOpen on, and the product is
+// finite. Otherwise the exponents are held below 31 for it, and where they were beyond, a < -21.5, the result is zero (it is less than
+// 5e-10 there: a sigmoid(a) is off by 1e-8 at most, for any a). Which of the two is settled for 16 values of a warp's rows at a time:
+// with the limits in every value 196608 x 64 x 256 took 33.2 us and the hidden gradients of 119736 x 120 x 320 20 us more.
+constexpr float kFfOpen = -21.f;
+template <bool OPEN>
 __device__ __forceinline__ void ff_sigmoid4(float2 a, float2 b, float2& sa, float2& sb) {
-  float2 x = __fmul2_rn(a, ff_f2(-1.44269504f)), y = __fmul2_rn(b, ff_f2(-1.44269504f));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.x) : "f"(fminf(x.x, 31.f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.y) : "f"(fminf(x.y, 31.f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(fminf(y.x, 31.f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(fminf(y.y, 31.f)));
+  const float2 m = __fmul2_rn(a, ff_f2(-1.44269504f)), n = __fmul2_rn(b, ff_f2(-1.44269504f));
+  const auto held = [](float v) { return OPEN ? v : fminf(v, 31.f); };
+  float2 x, y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.x) : "f"(held(m.x)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x.y) : "f"(held(m.y)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(held(n.x)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(held(n.y)));
   x = __fadd2_rn(x, ff_f2(1.f));
   y = __fadd2_rn(y, ff_f2(1.f));
   const float px = x.x * x.y, py = y.x * y.y;
@@ -83,6 +89,25 @@ __device__ __forceinline__ void ff_sigmoid4(float2 a, float2 b, float2& sa, floa
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(px * py));
   sa = __fmul2_rn(ff_f2(r * py), make_float2(x.y, x.x));
   sb = __fmul2_rn(ff_f2(r * px), make_float2(y.y, y.x));
+  if (!OPEN) {
+    sa = make_float2(m.x >= 31.f ? 0.f : sa.x, m.y >= 31.f ? 0.f : sa.y);
+    sb = make_float2(n.x >= 31.f ? 0.f : sb.x, n.y >= 31.f ? 0.f : sb.y);
+  }
+}
+// The least of three, NaN if one of them is
+__device__ __forceinline__ float ff_least(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Whether the whole warp's values are open (GELU asks for nothing)
+__device__ __forceinline__ bool ff_open(const uint32_t (&a)[16], int act) {
+  if (act != kFfSilu) return true;
+  float v = __uint_as_float(a[0]);
+#pragma unroll
+  for (int j = 1; j < 15; j += 2) v = ff_least(v, __uint_as_float(a[j]), __uint_as_float(a[j + 1]));
+  v = ff_least(v, __uint_as_float(a[15]), 0.f);
+  return __all_sync(0xFFFFFFFFu, v >= kFfOpen);
 }
 // The normal distribution's function and e^(-a^2 / 2) of four values: with z = |a| / sqrt 2 and t = 1 / (1 + 0.3275911 z),
 // erfc(z) = (c1 t + ... + c5 t^5) e^(-z^2) to 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26), the
@@ -113,11 +138,11 @@ __device__ __forceinline__ void ff_normal4(const float2 (&a)[2], float2 (&cdf)[2
 }
 __device__ __forceinline__ float2 ff_at(const uint32_t (&v)[16], int j) { return make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); }
 // act(a) and (where asked for) act'(a) of four values
-template <bool SLOPE>
+template <bool SLOPE, bool OPEN>
 __device__ __forceinline__ void ff_act4(const float2 (&a)[2], int act, float2 (&f)[2], float2 (&slope)[2]) {
   float2 s[2];
   if (act == kFfSilu) {
-    ff_sigmoid4(a[0], a[1], s[0], s[1]);
+    ff_sigmoid4<OPEN>(a[0], a[1], s[0], s[1]);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       f[k] = __fmul2_rn(a[k], s[k]);
@@ -134,12 +159,13 @@ __device__ __forceinline__ void ff_act4(const float2 (&a)[2], int act, float2 (&
   }
 }
 // Values of 16 neighbouring units: act(a) b
-__device__ __forceinline__ void ff_gate16(const uint32_t (&a)[16], const uint32_t (&b)[16], int act, float (&h)[16]) {
+template <bool OPEN>
+__device__ __forceinline__ void ff_gate16_of(const uint32_t (&a)[16], const uint32_t (&b)[16], int act, float (&h)[16]) {
 #pragma unroll
   for (int j = 0; j < 16; j += 4) {
     const float2 v[2] = {ff_at(a, j), ff_at(a, j + 2)};
     float2 f[2], none[2];
-    ff_act4<false>(v, act, f, none);
+    ff_act4<false, OPEN>(v, act, f, none);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float2 r = __fmul2_rn(f[k], ff_at(b, j + 2 * k));
@@ -148,14 +174,21 @@ __device__ __forceinline__ void ff_gate16(const uint32_t (&a)[16], const uint32_
     }
   }
 }
+__device__ __forceinline__ void ff_gate16(const uint32_t (&a)[16], const uint32_t (&b)[16], int act, float (&h)[16]) {
+  if (ff_open(a, act))
+    ff_gate16_of<true>(a, b, act, h);
+  else
+    ff_gate16_of<false>(a, b, act, h);
+}
 // ... and of the backward: dh b act'(a), dh act(a), act(a) b
-__device__ __forceinline__ void ff_gate_back16(const uint32_t (&a)[16], const uint32_t (&b)[16], const uint32_t (&d)[16], int act, float (&da)[16],
+template <bool OPEN>
+__device__ __forceinline__ void ff_gate_back16_of(const uint32_t (&a)[16], const uint32_t (&b)[16], const uint32_t (&d)[16], int act, float (&da)[16],
                                                float (&db)[16], float (&h)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; i += 4) {
     const float2 v[2] = {ff_at(a, i), ff_at(a, i + 2)};
     float2 f[2], slope[2];
-    ff_act4<true>(v, act, f, slope);
+    ff_act4<true, OPEN>(v, act, f, slope);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int j = i + 2 * k;
@@ -169,6 +202,13 @@ __device__ __forceinline__ void ff_gate_back16(const uint32_t (&a)[16], const ui
       h[j + 1] = z.y;
     }
   }
+}
+__device__ __forceinline__ void ff_gate_back16(const uint32_t (&a)[16], const uint32_t (&b)[16], const uint32_t (&d)[16], int act, float (&da)[16],
+                                               float (&db)[16], float (&h)[16]) {
+  if (ff_open(a, act))
+    ff_gate_back16_of<true>(a, b, d, act, da, db, h);
+  else
+    ff_gate_back16_of<false>(a, b, d, act, da, db, h);
 }
 
 // 32 bytes in one request where the address allows: whole sectors of L2 (in halves a tile's stores took twice as long)

@@ -320,3 +320,16 @@ def test_expanded_inputs_that_the_forward_keeps(rows, d, hidden, type, act, weig
     """Single CTAs and pairs of the backward that takes a and b from the forward."""
     t = _make(rows, d, hidden, type, torch.float32 if weights == "fp32" else None)
     _compare(_run(t, act), _with_kept(_want(t, act, type), t, type), (rows, d, hidden, type, act, weights))
+
+
+@pytest.mark.parametrize("rows,d", [(3, 64), (200, 64), (9500, 64), (1100, 512)])
+@pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
+def test_closed_units(rows, d, type):
+    """a = -4096: act(a) and its slope are zero in any precision, and so are the output and every gradient."""
+    make = lambda *s, v: torch.full(s, v, dtype=type, device=DEV, requires_grad=True)  # noqa: E731
+    t = [make(rows, d, v=1.0), make(128, d, v=-4096.0 / d), make(128, d, v=64.0 / d), make(d, 128, v=1.0)]
+    for act in ("silu", "gelu"):
+        y = blocks.gated_feed_forward(*t, activation=act)
+        assert not y.any(), act
+        for g in torch.autograd.grad(y, t, torch.ones_like(y)):
+            assert not g.any(), act
