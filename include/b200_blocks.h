@@ -7,7 +7,9 @@
  *    graph. The caller owns every buffer; the library allocates nothing.
  *  - dtype of the activations: B200_BLOCKS_BF16, _F32 or _F16. Norm parameters and the residual scale are fp32.
  *  - Results are deterministic (fixed orders of summation). All arithmetic is fp32, each output is rounded once; the feed-forward also
- *    rounds h, da and db to the activations' type (operands of 16-bit products; fp16 saturates there; h of up to four rows stays fp32).
+ *    rounds h, da and db to the activations' type (operands of 16-bit products; h of up to four rows stays fp32). In fp16 a finite h,
+ *    and a finite y of up to four rows, beyond 65504 become that; da, db and every other result become infinite there, and what is
+ *    infinite or NaN on the way is never made finite.
  *  - The feed-forward's device-side waits are bounded: one that gives up lets the kernel finish and leaves a positive code that
  *    b200_blocks_read_status returns (and clears).
  */

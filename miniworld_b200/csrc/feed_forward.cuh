@@ -18,7 +18,8 @@
 //   kFfWeights  dW_a, dW_b and dW_s^T = h^T dy: three products of one shape, the rows (K = M) split over the CTAs; fp32 partials
 //
 // Operands as they lie in memory: the weights' other orientation and the rows-as-K operands are read MN-major, so nothing is
-// transposed. h, da and db are rounded to the type of x (saturating for fp16), each once, as operands of 16-bit products have to be.
+// transposed. h, da and db are rounded to the type of x, each once, as operands of 16-bit products have to be (a finite h stays within fp16;
+// da, db and the results go to infinity beyond it).
 // The structure is the contraction's: persistent CTAs (pairs for large products: 256-row tiles, each CTA supplies its rows of the
 // first operand and half of the second), one warp loads through TMA, one issues the MMAs, the others are the epilogue of the tile
 // before. All waits are bounded; one that gives up leaves a code in blocks_status.
@@ -61,9 +62,20 @@ constexpr int kFfThreads = 64 + 32 * kFfEpilogueWarps;
 constexpr int kFfBoxBytes = 2048;     // 32 x 32 values of an output; one for each epilogue warp
 constexpr int kFfSmemBytes = kFfStages * kFfStageBytes + kFfEpilogueWarps * kFfBoxBytes + 256 + 1024;
 
+// Two values of a result, or of da and db: beyond fp16 they are infinite, so that gradients formed from them say so
 template <bool F16>
 __device__ __forceinline__ uint32_t ff_pack(float a, float b) {
-  return F16 ? pack_f16x2_sat(make_float2(a, b)) : pack_bf16x2(a, b);
+  return F16 ? pack_f16x2(make_float2(a, b)) : pack_bf16x2(a, b);
+}
+// Two values of h, an operand whose finite ones stay within fp16: those beyond become +-65504, infinite ones stay. (v 2^-112 is below the
+// half of a step there for a finite h, |h| < 2^104: 2^52 for each of a and b from fp16 rows of 2^20 elements.)
+template <bool F16>
+__device__ __forceinline__ uint32_t ff_pack_held(float a, float b) {
+  if (!F16) return pack_bf16x2(a, b);
+  const float2 v = make_float2(a, b);
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(pack_f16x2_sat(v)), "r"(pack_f16x2(__fmul2_rn(v, make_float2(0x1p-112f, 0x1p-112f)))));
+  return r;
 }
 
 __device__ __forceinline__ float2 ff_f2(float v) { return make_float2(v, v); }
@@ -258,6 +270,20 @@ template <bool F16>
 __device__ __forceinline__ void ff_pack16(const float (&v)[16], uint32_t (&w)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) w[j] = ff_pack<F16>(v[2 * j], v[2 * j + 1]);
+}
+// ... of h. (0 times each value adds up to a NaN where one is not finite: half an instruction a value instead of ff_pack_held's three a pair)
+template <bool F16>
+__device__ __forceinline__ void ff_pack16_held(const float (&v)[16], uint32_t (&w)[8]) {
+  ff_pack16<F16>(v, w);
+  if constexpr (F16) {
+    uint32_t z = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(z) : "r"(w[j]), "r"(0u));
+    if ((z & 0x7FFF7FFFu) != 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = ff_pack_held<true>(v[2 * j], v[2 * j + 1]);
+    }
+  }
 }
 // 16 values in 32 bytes (p on such a boundary) that keep the range of fp32: fp16 values times 2^(138 - 4 q), q = E / 4 (at least 3) for the
 // exponent field E of the largest finite one, which so lies in [2^11, 2^15). The six bits of q are the last bits of the first six
@@ -619,7 +645,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
             float v[16];
             uint32_t w[8];
             ff_gate16(va[c], vb[c], ACT, v);
-            ff_pack16<F16>(v, w);
+            ff_pack16_held<F16>(v, w);
             store16(0, col + c * 16, w);
             if (p.keep[0] != nullptr && in && col + c * 16 < p.cols) {
               const size_t at = ff_kept_at(row, col + c * 16, p.ld);
@@ -639,7 +665,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_kernel(const __grid_constant
             ff_gate_back16(va[c], vb[c], vd, ACT, da, db, h);
             ff_pack16<F16>(da, w[0][c]);
             ff_pack16<F16>(db, w[1][c]);
-            ff_pack16<F16>(h, w[2][c]);
+            ff_pack16_held<F16>(h, w[2][c]);
           }
 #pragma unroll
           for (int o = 0; o < 3; ++o)
@@ -975,11 +1001,11 @@ __global__ void __launch_bounds__(kFfVecThreads) ff_vec_down_kernel(const FfVec 
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float s = ff_warp_sum(acc[r]);
-    if (lane == r && r < p.rows) static_cast<uint16_t*>(p.y)[static_cast<size_t>(r) * p.d + col] = static_cast<uint16_t>(ff_pack<F16>(s, 0.f));
+    if (lane == r && r < p.rows) static_cast<uint16_t*>(p.y)[static_cast<size_t>(r) * p.d + col] = static_cast<uint16_t>(ff_pack_held<F16>(s, 0.f));
   }
 }
 
-// fp32 master weights as operands (the type of x, saturating for fp16)
+// fp32 master weights as operands: rounded to the type of x
 __global__ void __launch_bounds__(256) ff_cast_kernel(const float* a, const float* b, const float* s, uint4* out, long long n8, int f16) {
   grid_dependency_wait();
   grid_dependents_launch();

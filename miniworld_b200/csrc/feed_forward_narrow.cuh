@@ -212,6 +212,7 @@ ff_narrow_kernel(const __grid_constant__ FfMaps maps, const FfNarrowParams p) {
       if (!mbar_wait_warp(d1_full(grp), ph, abort_flag, status, kDevTimeoutEpilogue)) break;
       tc_fence_after();
       uint32_t o[16];
+      float most = 0.f;  // of |h|, NaN where one of them is
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t va[16], vb[16];
@@ -221,8 +222,16 @@ ff_narrow_kernel(const __grid_constant__ FfMaps maps, const FfNarrowParams p) {
         float h[16];
         ff_gate16(va, vb, ACT, h);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[8 * c + j] = ff_pack<F16>(h[2 * j], h[2 * j + 1]);
+        for (int j = 0; j < 8; ++j) {
+          const float2 v = make_float2(h[2 * j], h[2 * j + 1]);
+          if (F16) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(v.x), "f"(v.y));
+          o[8 * c + j] = F16 ? pack_f16x2_sat(v) : pack_bf16x2(v.x, v.y);
+        }
       }
+      // fp16: a finite h beyond the range becomes +-65504, and so would an infinite one. It makes the whole row of y infinite or NaN in any
+      // case, so two NaN in the place of two of the row's values say the same (one instruction for two values; with each value's own
+      // infinity 34.1 us, GELU 48, against 32.8 and 45)
+      if (F16 && !(most < INFINITY)) o[0] = 0x7FFF7FFFu;
       tmem_st16(d1, o);
       tmem_st_wait();
       tc_fence_before();

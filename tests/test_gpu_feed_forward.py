@@ -333,3 +333,51 @@ def test_closed_units(rows, d, type):
         assert not y.any(), act
         for g in torch.autograd.grad(y, t, torch.ones_like(y)):
             assert not g.any(), act
+
+
+@pytest.mark.parametrize("rows,d", [(3, 64), (150, 64), (20000, 64), (1100, 512)])
+def test_fp16_rows_that_are_not_finite(rows, d):
+    """An infinite element of a row: nothing finite comes out of that row, the others are what they are without it."""
+    t = _make(rows, d, 256, torch.float16)
+    w = [t[k] for k in ("w_a", "w_b", "w_s")]
+    keep = torch.arange(rows, device=DEV) != 1
+    want = blocks.gated_feed_forward(t["x"], *w)
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        x = t["x"].clone()
+        x[1, 3] = bad
+        for act in ("silu", "gelu"):
+            got = blocks.gated_feed_forward(x, *w, activation=act)
+            assert not torch.isfinite(got[1]).any(), (bad, act)
+            assert act == "gelu" or torch.equal(got[keep], want[keep]), bad
+
+
+@pytest.mark.parametrize("rows,d", [(8, 64), (150, 64), (20000, 64), (1100, 512), (5000, 1024)])
+def test_fp16_results_overflow_to_infinity(rows, d):
+    """Results beyond the type are infinite, as a loss scaler expects, with operands (h, da, db) inside it."""
+    full = lambda *s, v: torch.full(s, v, dtype=torch.float16, device=DEV, requires_grad=True)  # noqa: E731
+    # a = b = 32, h = 1024, y = 128 * 1024 = 2^17;  dh = d, da = db = 32 d, dx = 128 * 2 * 32 d * 32 / d = 2^18
+    x, w_a, w_b, w_s = full(rows, d, v=1.0), full(128, d, v=32.0 / d), full(128, d, v=32.0 / d), full(d, 128, v=1.0)
+    y = blocks.gated_feed_forward(x, w_a, w_b, w_s)
+    assert (y == float("inf")).all()
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert (dx == float("inf")).all()
+
+
+@pytest.mark.parametrize("rows,d", [(3, 64), (150, 64), (20000, 64), (1100, 512), (5000, 1024)])
+def test_fp16_gradients_of_units_overflow(rows, d):
+    """da and db beyond the type: every gradient formed from them says so."""
+    full = lambda *s, v: torch.full(s, v, dtype=torch.float16, device=DEV, requires_grad=True)  # noqa: E731
+    # a = b = 64, dh = 2048: da = db = 2^17
+    t = [full(rows, d, v=1.0), full(64, d, v=64.0 / d), full(64, d, v=64.0 / d), full(d, 64, v=2048.0 / d)]
+    y = blocks.gated_feed_forward(*t)
+    g = torch.autograd.grad(y, t[:3], torch.ones_like(y))
+    assert not any(torch.isfinite(v).any() for v in g)
+
+
+@pytest.mark.parametrize("rows", [2, 100])
+def test_fp32_weights_beyond_fp16(rows):
+    """A master weight that the type of the products cannot hold is infinite there, as a conversion makes it."""
+    t = _make(rows, 64, 64, torch.float16, torch.float32)
+    t["w_a"][3, 2] = 1e6
+    got = blocks.gated_feed_forward(t["x"], t["w_a"], t["w_b"], t["w_s"])
+    assert not torch.isfinite(got).any()
