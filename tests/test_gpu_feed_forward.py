@@ -381,3 +381,24 @@ def test_fp32_weights_beyond_fp16(rows):
     t["w_a"][3, 2] = 1e6
     got = blocks.gated_feed_forward(t["x"], t["w_a"], t["w_b"], t["w_s"])
     assert not torch.isfinite(got).any()
+
+
+@pytest.mark.parametrize("rows,d,hidden", [(1100, 512, 128), (50, 64, 128)])
+def test_saved_tensors_that_come_back_as_others(rows, d, hidden):
+    """Saved-tensor hooks that give back tensors which fit one another, but not the forward: refused before anything is launched."""
+    t = _make(rows, d, hidden, torch.bfloat16)
+    shapes = {(hidden, d): (2 * hidden, d), (d, hidden): (d, 2 * hidden)}
+    leaves = [t[k].clone().requires_grad_(True) for k in ("x", "w_a", "w_b", "w_s")]
+
+    def wider(v):
+        return torch.zeros(shapes.get(tuple(v.shape), tuple(v.shape)), dtype=v.dtype, device=DEV)
+
+    def narrower(v):
+        return v[:hidden // 2].contiguous() if tuple(v.shape) == (hidden, d) else v[:, :hidden // 2].contiguous() if tuple(v.shape) == (d, hidden) else v
+
+    for unpack in (wider, narrower, lambda v: v.half(), lambda v: v.float(), lambda v: v[: v.shape[0] // 2], lambda v: v.cpu(),
+                   lambda v: v.t().contiguous().t(), lambda v: v.flatten()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v, unpack):
+            y = blocks.gated_feed_forward(*leaves)
+        with pytest.raises(RuntimeError, match="came back with another|must be"):
+            torch.autograd.grad(y, leaves, t["dy"])
