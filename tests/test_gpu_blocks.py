@@ -336,3 +336,87 @@ def test_forward_mode_and_lazy_negation_are_refused():
     (want,) = torch.autograd.grad(blocks.block_norm(x), x, -dy)
     (got,) = torch.autograd.grad(blocks.block_norm(x), x, torch._neg_view(dy))
     assert torch.equal(got, want)
+
+
+def _allocated():
+    torch.cuda.synchronize()
+    return torch.cuda.memory_allocated()
+
+
+def _wide():
+    """A feed-forward that keeps 6 bytes a hidden value for its backward, and what it keeps."""
+    m = mw.GatedFeedForward(512, n=4).to(DEV).bfloat16()
+    torch.nn.init.normal_(m.squeeze.weight, std=0.02)
+    return m, torch.randn(4096, 512, device=DEV).bfloat16().requires_grad_(True), 6 * 4096 * 2048
+
+
+def test_what_is_kept_goes_with_the_backward():
+    """... although the output (a logged loss) still holds the node."""
+    m, x, kept = _wide()
+    before = _allocated()
+    y = m(x)
+    assert _allocated() - before >= kept
+    torch.autograd.grad(y, [x, *m.parameters()], torch.ones_like(y))
+    assert _allocated() - before <= y.numel() * 2 + 4096
+    x = torch.randn(1 << 18, 16, device=DEV).bfloat16().requires_grad_(True)
+    before = _allocated()
+    y, h = blocks.block_join(x, x, post=blocks.Norm(), pre=blocks.Norm())
+    torch.autograd.grad([y, h], [x], [y.detach(), h.detach()])
+    assert _allocated() - before <= 4 * y.numel() + 8192  # (not the statistics, 8 bytes a row of each norm)
+
+
+def test_checkpoints_hold_nothing_of_a_block():
+    from torch.utils.checkpoint import checkpoint
+
+    m, x, kept = _wide()
+    norm = blocks.Norm("rms")
+
+    def f(x):
+        y, h = blocks.block_join(x, m(x), post=norm, pre=norm)
+        return y + h
+
+    dy = torch.randn(4096, 512, device=DEV).bfloat16()
+    leaves = [x, *m.parameters()]
+    want = torch.autograd.grad(f(x), leaves, dy)
+    before = _allocated()
+    y = checkpoint(f, x, use_reentrant=False)
+    assert _allocated() - before <= y.numel() * 2 + 4096
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(a, b)
+
+
+def test_what_is_kept_may_be_moved():
+    """Saved-tensor hooks that copy to the host and back, to memory that begins at any 16-byte boundary."""
+    m, x, kept = _wide()
+    norm = blocks.Norm("layer")
+
+    def f():
+        return blocks.block_join(x, m(x), post=norm, pre=norm)
+
+    dy, dh = torch.randn(4096, 512, device=DEV).bfloat16(), torch.randn(4096, 512, device=DEV).bfloat16()
+    leaves = [x, *m.parameters()]
+    want = torch.autograd.grad(f(), leaves, [dy, dh])
+
+    def moved(t):
+        room = torch.empty(t.numel() * t.element_size() + 16, dtype=torch.uint8, device=DEV)
+        return room[16:].view(t.dtype).view(t.shape).copy_(t)
+
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t, moved)):
+        with hooks:
+            out = f()
+        for a, b in zip(torch.autograd.grad(out, leaves, [dy, dh]), want):
+            assert torch.equal(a, b)
+
+
+def test_what_is_kept_comes_back_as_something_else():
+    m, x, _ = _wide()
+    f = torch.randn(6, 64, device=DEV).requires_grad_(True)
+    for make, leaf, unpack in (
+            (lambda: m(x), x, lambda t: t[:1024] if t.dtype == torch.uint8 else t),
+            (lambda: m(x), x, lambda t: t.cpu() if t.dtype == torch.uint8 else t),
+            (lambda: blocks.block_norm(f), f, lambda t: t[:5] if t.shape == (6, 2) else t),
+            (lambda: blocks.block_join(f, f, post=blocks.Norm()), f, lambda t: t.double() if t.shape == (6, 2) else t)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = make()
+        with pytest.raises(RuntimeError, match="came back with another"):
+            torch.autograd.grad(y, leaf, torch.ones_like(y))
