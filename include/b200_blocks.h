@@ -41,8 +41,8 @@ extern "C" {
  *   t = norm_post(u);  y = x + valid * scale * sigmoid(gate) * t;  h = norm_pre(y)
  * x, u, y, h: [rows, d]. gate: logits [rows / gate_rows, d], row r of x uses gate row r / gate_rows (1: a row each; rows: one for
  * all), null: no gate. mask: uint8 [rows], 0: y = x there, whatever u and gate hold. scale, post_w, post_b, pre_w, pre_b: fp32 [d],
- * null: 1 or 0. post_kind B200_NORM_NONE: t = u; pre_kind B200_NORM_NONE: no h. h is the norm of the unrounded y. y may be x and h
- * may be u (a thread reads its row's elements before it writes them).
+ * null: 1 or 0. post_kind B200_NORM_NONE: t = u; pre_kind B200_NORM_NONE: no h (the parameters of a norm that is not there are not
+ * read). h is the norm of the unrounded y. y may be x and h may be u (a thread reads its row's elements before it writes them).
  * post_stats, pre_stats: fp32 [rows, 2], mean and 1 / sigma, for the backward (null: not kept).
  */
 int b200_block_join_forward(const void* x, const void* u, const void* gate, const uint8_t* mask, const float* scale,

@@ -623,10 +623,10 @@ int b200_block_join_forward(const void* x, const void* u, const void* gate, cons
   p.gate = gate;
   p.mask = mask;
   p.scale = scale;
-  p.post_w = post_w;
-  p.post_b = post_b;
-  p.pre_w = pre_w;
-  p.pre_b = pre_b;
+  p.post_w = post_kind != kNormNone ? post_w : nullptr;  // (parameters of a norm that is not there are not read)
+  p.post_b = post_kind != kNormNone ? post_b : nullptr;
+  p.pre_w = pre_kind != kNormNone ? pre_w : nullptr;
+  p.pre_b = pre_kind != kNormNone ? pre_b : nullptr;
   p.y = y;
   p.h = h;
   p.post_stats = reinterpret_cast<float2*>(post_stats);
@@ -698,10 +698,10 @@ int b200_block_join_backward(const void* dy, const void* dh, const void* x, cons
   p.gate = gate;
   p.mask = mask;
   p.scale = scale;
-  p.post_w = post_w;
-  p.post_b = post_b;
-  p.pre_w = pre_w;
-  p.pre_b = pre_b;
+  p.post_w = post_kind != kNormNone ? post_w : nullptr;  // (parameters of a norm that is not there are not read)
+  p.post_b = post_kind != kNormNone ? post_b : nullptr;
+  p.pre_w = pre_kind != kNormNone ? pre_w : nullptr;
+  p.pre_b = pre_kind != kNormNone ? pre_b : nullptr;
   p.post_stats = reinterpret_cast<float2*>(const_cast<float*>(post_stats));
   p.pre_stats = reinterpret_cast<float2*>(const_cast<float*>(pre_stats));
   p.dy = dy;

@@ -411,3 +411,40 @@ def test_norms_without_weights(gate, bias, type, d):
     want = _want({**t, "post_w": ones, "pre_w": ones}, "layer", "layer")
     del t["post_w"], t["pre_w"], want["post_w"], want["pre_w"]
     _compare(_run(t, "layer", "layer"), want, (gate, bias, type, d))
+
+
+def test_c_calls_without_a_norm_do_not_read_its_parameters():
+    """post_kind 0: t = u, whatever post_w and post_b point to, on tiles and (one element off a boundary) on the first kernels."""
+    import ctypes
+
+    from miniworld_b200 import _lib
+
+    lib = _lib.load()
+    t = _make(50, 100, torch.bfloat16, None, True, False, None, "layer")
+    w, b = torch.full((100,), 3.0, device=DEV), torch.full((100,), 5.0, device=DEV)
+    need = ctypes.c_size_t(0)
+    assert lib.b200_block_join_workspace_bytes(50, 100, 1, ctypes.byref(need)) == 0
+    ws = torch.empty(need.value + 1024, dtype=torch.uint8, device=DEV)
+    at = (ws.data_ptr() + 1023) // 1024 * 1024
+    p = lambda v: None if v is None else v.data_ptr()  # noqa: E731
+
+    def run(post_w, post_b, off):
+        def place(v):
+            room = torch.zeros(v.numel() + 8, dtype=v.dtype, device=DEV)[off:off + v.numel()].view(v.shape)
+            return room.copy_(v)
+
+        x, u, dy, dh = (place(t[k]) for k in ("x", "u", "dy", "dh"))
+        y, h, dx, du = (place(torch.zeros_like(x)) for _ in range(4))
+        stats, dscale = torch.zeros(50, 2, device=DEV), torch.zeros(100, device=DEV)
+        stream = torch.cuda.current_stream().cuda_stream
+        assert lib.b200_block_join_forward(p(x), p(u), None, None, p(t["scale"]), p(post_w), p(post_b), p(t["pre_w"]), p(t["pre_b"]), p(y), p(h), None,
+                                           p(stats), 50, 100, 1, 0, 0, 1, 1e-5, 1e-5, stream) == 0
+        assert lib.b200_block_join_backward(p(dy), p(dh), p(x), p(u), None, None, p(t["scale"]), p(post_w), p(post_b), p(t["pre_w"]), p(t["pre_b"]), None,
+                                            p(stats), p(dx), p(du), None, p(dscale), None, None, None, None, at, need.value, 50, 100, 1, 0, 0, 1,
+                                            stream) == 0
+        torch.cuda.synchronize()
+        return [v.clone() for v in (y, h, stats, dx, du, dscale)]
+
+    for off in (0, 1):
+        for a, b_ in zip(run(w, b, off), run(None, None, off)):
+            assert torch.equal(a, b_), off
