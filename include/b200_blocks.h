@@ -53,7 +53,8 @@ int b200_block_join_forward(const void* x, const void* u, const void* gate, cons
 /*
  * Gradients of the above from dy and dh (either may be null: zero), the forward's inputs and statistics. Outputs that are null are
  * left out: dx, du [rows, d], dgate [rows / gate_rows, d] in the activations' type, d_scale, d_post_w, d_post_b, d_pre_w, d_pre_b
- * fp32 [d]. Every output is overwritten. In rows that the mask leaves out du and dgate are zero and nothing is added to the sums.
+ * fp32 [d] (d_scale, d_post_w and d_post_b need u, the last two a norm after the block). Every output is overwritten. In rows that the
+ * mask leaves out du and dgate are zero and nothing is added to the sums.
  * Workspace: b200_block_join_workspace_bytes, 1024-byte aligned.
  */
 int b200_block_join_workspace_bytes(long long rows, int d, long long gate_rows, size_t* out_bytes);

@@ -681,6 +681,10 @@ int b200_block_join_backward(const void* dy, const void* dh, const void* x, cons
     return B200_TRIMUL_E_NULL;
   if (u == nullptr && (pre_kind == kNormNone || post_kind != kNormNone || gate != nullptr || mask != nullptr || scale != nullptr))
     return B200_TRIMUL_E_NULL;
+  // (sums of a block's output or of a norm that is not there: no kernel forms them)
+  if ((u == nullptr && (d_scale != nullptr || d_post_w != nullptr || d_post_b != nullptr)) ||
+      (post_kind == kNormNone && (d_post_w != nullptr || d_post_b != nullptr)))
+    return B200_TRIMUL_E_NULL;
   if ((pre_kind == kNormNone && dh != nullptr) || (u == nullptr && (dy != nullptr || du != nullptr)) || (gate == nullptr && dgate != nullptr))
     return B200_TRIMUL_E_NULL;
   if (!aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;

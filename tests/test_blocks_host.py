@@ -138,3 +138,13 @@ def test_parameters_of_the_modules():
     }
     assert mw.BlockNorm(64, "rms").bias is None and mw.BlockNorm(64, "rms", bias=True).bias is not None
     assert mw.BlockJoin(64, None).norm_out is None and mw.BlockJoin(64).scale is None
+
+
+@pytest.mark.parametrize("names,post", [(("d_scale",), 0), (("d_post_w",), 0), (("d_post_b",), 0), (("d_post_w",), None), (("d_post_b",), None)])
+def test_join_backward_refuses_sums_of_what_is_not_there(lib, p, names, post):
+    """Gradients of the scale and of the norm after the block without the block's output (``post`` 0: a plain norm), or without that norm."""
+    u = None if post == 0 else p
+    d = [p if n in names else None for n in ("d_scale", "d_post_w", "d_post_b", "d_pre_w", "d_pre_b")]
+    code = lib.b200_block_join_backward(None if u is None else p, p, p, u, None, None, None, None, None, None, None, None, p, p, u, None, *d, p, 1 << 40,
+                                        4, 64, 1, 0, 0, 1, None)
+    assert code == -1
