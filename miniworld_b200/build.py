@@ -93,16 +93,26 @@ def build_native(force: bool = False) -> Path:
     return NATIVE_PATH
 
 
+def _compiler_tag() -> str:
+    """What an object file is made with: objects of different compilers or flags are not linked together."""
+    nvcc = find_nvcc()
+    return "\n".join([nvcc, *NVCC_FLAGS, _run([nvcc, "--version"]).stdout])
+
+
 def _compile(source: Path, force: bool, verbose: bool) -> Path:
-    """Object file of one ``.cu`` file, kept beside the package and made again when a file that it includes is newer."""
-    obj, deps = PKG_DIR / f"{source.stem}.o", PKG_DIR / f"{source.stem}.tag"
-    if not force and obj.exists() and deps.exists():
-        used = [Path(w) for w in deps.read_text().replace("\\\n", " ").split()[1:]]
+    """Object file of one ``.cu`` file, kept beside the package and made again when a file that it includes is newer or the compiler
+    or its flags have changed."""
+    obj, deps, made_with = (PKG_DIR / f"{source.stem}{end}" for end in (".o", ".tag", ".flags.tag"))
+    tag = _compiler_tag()
+    if not force and obj.exists() and deps.exists() and made_with.exists() and made_with.read_text() == tag:
+        used = [Path(w) for w in deps.read_text().replace("\\\n", " ").split(" : ", 1)[-1].split()]
         built = obj.stat().st_mtime
         if used and all(p.exists() and p.stat().st_mtime <= built for p in used):
             return obj
     cmd = [find_nvcc(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-MD", "-MF", str(deps)]
+    made_with.unlink(missing_ok=True)
     proc = _run(cmd + ["-c", "-o", str(obj), str(source)])
+    made_with.write_text(tag)
     if verbose:
         print(proc.stderr)
     return obj

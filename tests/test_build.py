@@ -45,3 +45,30 @@ def test_no_knobs_in_the_kernels():
     once) would compile and give wrong results: the sources have no such switches."""
     for source in sorted(build.CSRC.iterdir()):
         assert not [line for line in source.read_text().splitlines() if line.lstrip().startswith(("#if", "#ifdef", "#ifndef"))], source.name
+
+
+def test_an_object_of_other_flags_or_another_compiler_is_made_again(tmp_path, monkeypatch):
+    source, compiled, version = tmp_path / "a.cu", [], ["12.9"]
+    source.write_text("")
+
+    def run(cmd):
+        if "--version" in cmd:
+            return build.subprocess.CompletedProcess(cmd, 0, stdout=version[0], stderr="")
+        compiled.append(cmd)
+        (tmp_path / "a.o").write_bytes(b"")
+        (tmp_path / "a.tag").write_text(f"a.o : {source}\n")
+        return build.subprocess.CompletedProcess(cmd, 0, stdout="", stderr="")
+
+    monkeypatch.setattr(build, "PKG_DIR", tmp_path)
+    monkeypatch.setattr(build, "_run", run)
+
+    def made():
+        compiled.clear()
+        build._compile(source, False, False)
+        return len(compiled)
+
+    assert made() == 1 and made() == 0
+    monkeypatch.setattr(build, "NVCC_FLAGS", [*build.NVCC_FLAGS, "-G"])
+    assert made() == 1 and made() == 0
+    version[0] = "13.0"
+    assert made() == 1 and made() == 0
