@@ -22,7 +22,8 @@ constexpr int kMaxSms = 160;
 // Threads of a row (up to 32 reduce by shuffles alone; wider rows take four warps) and 8-element pieces of each: the fewest idle lanes,
 // then two pieces (us, forward of 2^24 elements with every part, one, two and four pieces: 16 bits, 64 wide 42.6, 40.7, 42.8, 256 wide
 // 41.7, 39.1, 39.3, 200 wide 55, 53, 50, 250 wide 57, 50, 50, 101 wide 84, 77, 85, 203 wide 119, 83, 87; fp32, 256 wide 57, 61, 95, 203
-// wide 84, 69, 111). Three pieces only where they leave fewer lanes idle: 384 wide 36.7.
+// wide 84, 69, 111). Three pieces only where they leave fewer lanes idle: 384 wide 36.7. One piece is left to rows of up to eight elements,
+// whatever the type (fp32 of 256 would gain 4 us with one, of 203 lose 15).
 struct JoinShape {
   int team, nv;
 };
@@ -122,8 +123,9 @@ template <typename T>
 constexpr int kOdd = sizeof(T) == 2 ? 3 : 1;
 template <typename T, int VEC, bool EXACT>
 static TileKernel tile_forward_kernel(int nv) {
+  if constexpr (VEC != 8 || EXACT)  // (one piece: widths of up to eight, of which eight is exact)
+    if (nv == 1) return join_tile_forward_kernel<T, VEC, 1, EXACT>;
   switch (nv) {
-    case 1: return join_tile_forward_kernel<T, VEC, 1, EXACT>;
     case 2: return join_tile_forward_kernel<T, VEC, 2, EXACT>;
     case 3: return join_tile_forward_kernel<T, VEC, 3, EXACT>;
     default: return join_tile_forward_kernel<T, VEC, 4, EXACT>;
@@ -138,7 +140,7 @@ static TileKernel tile_backward_kernel(int vec, bool exact) {
 static int join_vec(int d, size_t size) { return d % 8 == 0 ? 8 : d % 2 == 0 ? 2 : size == 2 ? 3 : 1; }  // (see tile_col)
 
 template <typename T>
-static int launch_join_forward(const JoinParams& p0, bool wide, const DeviceInfo& info, cudaStream_t stream) {
+static int launch_join_forward(const JoinParams& p0, const DeviceInfo& info, cudaStream_t stream) {
   JoinTileParams q = {};
   q.j = p0;
   const JoinShape s = join_forward_shape(p0.d);
@@ -169,10 +171,10 @@ static int launch_join_forward(const JoinParams& p0, bool wide, const DeviceInfo
   const int blocks = static_cast<int>(std::min<long long>((p.rows + teams - 1) / teams, 8ll * info.sms));
   void (*kernel)(JoinParams) = nullptr;
   switch (s.nv) {
-    case 1: kernel = wide ? join_forward_kernel<T, true, 1> : join_forward_kernel<T, false, 1>; break;
-    case 2: kernel = wide ? join_forward_kernel<T, true, 2> : join_forward_kernel<T, false, 2>; break;
-    case 3: kernel = wide ? join_forward_kernel<T, true, 3> : join_forward_kernel<T, false, 3>; break;
-    default: kernel = wide ? join_forward_kernel<T, true, 4> : join_forward_kernel<T, false, 4>; break;
+    case 1: kernel = join_forward_kernel<T, 1>; break;
+    case 2: kernel = join_forward_kernel<T, 2>; break;
+    case 3: kernel = join_forward_kernel<T, 3>; break;
+    default: kernel = join_forward_kernel<T, 4>; break;
   }
   TRIMUL_CUDA(launch_overlapped(kernel, dim3(blocks), kJoinForwardThreads, 0, stream, p));
   return B200_TRIMUL_OK;
@@ -642,11 +644,10 @@ int b200_block_join_forward(const void* x, const void* u, const void* gate, cons
   if (!aligned(x, size) || !aligned(u, size) || !aligned(gate, size) || !aligned(y, size) || !aligned(h, size) ||
       !aligned(post_stats, 8) || !aligned(pre_stats, 8))
     return B200_TRIMUL_E_ALIGN;
-  const bool wide = d % 8 == 0 && all_aligned16({x, u, gate, y, h});
   const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  if (dtype == B200_BLOCKS_BF16) return launch_join_forward<__nv_bfloat16>(p, wide, info, stream);
-  if (dtype == B200_BLOCKS_F16) return launch_join_forward<__half>(p, wide, info, stream);
-  return launch_join_forward<float>(p, wide, info, stream);
+  if (dtype == B200_BLOCKS_BF16) return launch_join_forward<__nv_bfloat16>(p, info, stream);
+  if (dtype == B200_BLOCKS_F16) return launch_join_forward<__half>(p, info, stream);
+  return launch_join_forward<float>(p, info, stream);
 }
 
 int b200_block_join_workspace_bytes(long long rows, int d, long long gate_rows, size_t* out_bytes) {

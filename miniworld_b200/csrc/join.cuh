@@ -220,7 +220,8 @@ __device__ __forceinline__ float sigmoid_fast(float g) { return __fdividef(1.0f,
 constexpr int kJoinForwardThreads = 256;
 constexpr int kJoinBackwardThreads = 512;
 
-template <typename T, bool WIDE, int NV>
+// (single elements only: rows on 16-byte boundaries always fit the tiles of join_tiles.cuh)
+template <typename T, int NV>
 __global__ void __launch_bounds__(kJoinForwardThreads) join_forward_kernel(const JoinParams p) {
   __shared__ float2 scratch[kJoinForwardThreads / 64 * 32];
   const int team = p.team, t = threadIdx.x % team, id = threadIdx.x / team, teams = blockDim.x / team;
@@ -232,43 +233,43 @@ __global__ void __launch_bounds__(kJoinForwardThreads) join_forward_kernel(const
     const long long row = first + id;
     const bool on = row < p.rows;
     float x[8 * NV];
-    load_row<T, WIDE, NV>(p.x, row, d, t, team, on, x);
+    load_row<T, false, NV>(p.x, row, d, t, team, on, x);
     if (p.u != nullptr) {
       const bool valid = on && (p.mask == nullptr || __ldcg(p.mask + row) != 0);
       float u[8 * NV], g[8 * NV], w[8 * NV];
-      load_row<T, WIDE, NV>(p.u, row, d, t, team, valid, u);
-      if (p.gate != nullptr) load_row<T, WIDE, NV>(p.gate, p.gate_rows == 1 ? row : row / p.gate_rows, d, t, team, valid, g);
+      load_row<T, false, NV>(p.u, row, d, t, team, valid, u);
+      if (p.gate != nullptr) load_row<T, false, NV>(p.gate, p.gate_rows == 1 ? row : row / p.gate_rows, d, t, team, valid, g);
       if (p.post_kind != kNormNone) {
-        const float2 st = row_stats<WIDE, NV>(u, p.post_kind, p.post_eps, d, t, team, sum);
+        const float2 st = row_stats<false, NV>(u, p.post_kind, p.post_eps, d, t, team, sum);
         if (on && t == 0 && p.post_stats != nullptr) p.post_stats[row] = st;
 #pragma unroll
         for (int i = 0; i < 8 * NV; ++i) u[i] = (u[i] - st.x) * st.y;
-        load_param<WIDE, NV>(p.post_w, d, t, team, 1.f, w);
+        load_param<false, NV>(p.post_w, d, t, team, 1.f, w);
 #pragma unroll
         for (int i = 0; i < 8 * NV; ++i) u[i] *= w[i];
-        load_param<WIDE, NV>(p.post_b, d, t, team, 0.f, w);
+        load_param<false, NV>(p.post_b, d, t, team, 0.f, w);
 #pragma unroll
         for (int i = 0; i < 8 * NV; ++i) u[i] += w[i];
       }
       if (p.gate != nullptr)
 #pragma unroll
         for (int i = 0; i < 8 * NV; ++i) u[i] *= sigmoid_fast(g[i]);
-      load_param<WIDE, NV>(p.scale, d, t, team, 1.f, w);
+      load_param<false, NV>(p.scale, d, t, team, 1.f, w);
       if (valid)
 #pragma unroll
         for (int i = 0; i < 8 * NV; ++i)
-          if (join_col<WIDE>(i, t, team) < d) x[i] = fmaf(u[i], w[i], x[i]);
-      if (on) store_row<T, WIDE, NV>(p.y, row, d, t, team, x);
+          if (join_col<false>(i, t, team) < d) x[i] = fmaf(u[i], w[i], x[i]);
+      if (on) store_row<T, false, NV>(p.y, row, d, t, team, x);
     }
     if (p.pre_kind != kNormNone) {
-      const float2 st = row_stats<WIDE, NV>(x, p.pre_kind, p.pre_eps, d, t, team, sum);
+      const float2 st = row_stats<false, NV>(x, p.pre_kind, p.pre_eps, d, t, team, sum);
       if (on && t == 0 && p.pre_stats != nullptr) p.pre_stats[row] = st;
       float w[8 * NV], b[8 * NV];
-      load_param<WIDE, NV>(p.pre_w, d, t, team, 1.f, w);
-      load_param<WIDE, NV>(p.pre_b, d, t, team, 0.f, b);
+      load_param<false, NV>(p.pre_w, d, t, team, 1.f, w);
+      load_param<false, NV>(p.pre_b, d, t, team, 0.f, b);
 #pragma unroll
       for (int i = 0; i < 8 * NV; ++i) x[i] = fmaf((x[i] - st.x) * st.y, w[i], b[i]);
-      if (on) store_row<T, WIDE, NV>(p.h, row, d, t, team, x);
+      if (on) store_row<T, false, NV>(p.h, row, d, t, team, x);
     }
   }
 }

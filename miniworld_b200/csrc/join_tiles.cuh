@@ -21,13 +21,13 @@
 namespace trimul {
 
 // Warps that compute; one more copies: four to a scheduler with 128 registers a thread, or two such blocks an SM with 64 (the
-// forward with eight elements of a row a thread, the backward of a norm alone).
+// backward of a norm alone, and the forward with eight elements of a row a thread, which rows of up to eight elements have).
 constexpr int kTileWarps = 15;
 constexpr int kTileThreads = kTileWarps * 32 + 32;
 constexpr int kTileTeams = 7;                          // most teams of several warps
 constexpr int kTileMaxStages = 8;
 constexpr int kTileSmem = 224 * 1024;                  // of the 227 KB a block may have (the 228 KB of an SM)
-constexpr int kTileSmemHalf = 112 * 1024;              // two blocks an SM: forward, eight elements of a row a thread
+constexpr int kTileSmemHalf = 112 * 1024;              // two blocks an SM: see above
 
 struct JoinTileParams {
   JoinParams j;
@@ -423,8 +423,8 @@ struct TileSum {
   }
 };
 
-// mean and 1 / sigma of a row. (With eight elements a thread, where two blocks share an SM, the merged form's instructions cost more
-// than the second exchange's latency.)
+// mean and 1 / sigma of a row. (With eight elements a thread, rows of eight, where two blocks share an SM, the merged form's
+// instructions cost more than the second exchange's latency.)
 template <int VEC, int NV, bool EXACT>
 __device__ __forceinline__ float2 tile_stats(const float2 (&v)[4 * NV], int kind, float eps, int d, float inv, int t, int team, TileSum& sum) {
   float mean = 0.f, dev;
