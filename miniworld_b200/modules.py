@@ -124,6 +124,18 @@ class _Kept:
         self.module.__dict__[self.name] = self.kept
 
 
+def _pinned(fn):
+    """``fn`` of a module's ``_apply`` that follows the device but leaves float types (and so the values, bit for bit) alone."""
+
+    def pinned(t):
+        out = fn(t)
+        if t.is_floating_point() and out.dtype != t.dtype:
+            return t.to(device=out.device)
+        return out
+
+    return pinned
+
+
 class Fp32LayerNorm(nn.LayerNorm):
     """LayerNorm parameter holder whose affine parameters are pinned to fp32: ``module.to(torch.bfloat16)`` moves them
     between devices but never changes (or rounds) their values, like the reference's fp32-pinned LayerNorm
@@ -131,13 +143,7 @@ class Fp32LayerNorm(nn.LayerNorm):
     normalisation itself runs inside the fused kernels."""
 
     def _apply(self, fn, recurse=True):
-        def pinned(t):
-            out = fn(t)
-            if t.is_floating_point() and out.dtype != t.dtype:
-                return t.to(device=out.device)  # follow the device, keep the fp32 values bit for bit
-            return out
-
-        return super()._apply(pinned, recurse)
+        return super()._apply(_pinned(fn), recurse)
 
 
 _TRI_NAMES = tuple(tuple(k.split(".")) for k in (
@@ -547,11 +553,7 @@ class BlockJoin(nn.Module):
         self.scale = None if scale is None else nn.Parameter(torch.full((d,), float(scale)))
 
     def _apply(self, fn, recurse=True):
-        kept = None if self.scale is None else self.scale.data
-        super()._apply(fn, recurse)
-        if kept is not None and self.scale.dtype != kept.dtype:  # pinned to fp32 like the norms' parameters
-            self.scale.data = kept.to(self.scale.device)
-        return self
+        return super()._apply(_pinned(fn), recurse)  # the scale and its gradient stay fp32 like the norms' parameters
 
     def forward(self, x: torch.Tensor, u: torch.Tensor, gate: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                 next_norm: Optional[BlockNorm] = None):

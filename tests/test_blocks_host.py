@@ -148,3 +148,21 @@ def test_join_backward_refuses_sums_of_what_is_not_there(lib, p, names, post):
     code = lib.b200_block_join_backward(None if u is None else p, p, p, u, None, None, None, None, None, None, None, None, p, p, u, None, *d, p, 1 << 40,
                                         4, 64, 1, 0, 0, 1, None)
     assert code == -1
+
+
+@pytest.mark.parametrize("type", [torch.bfloat16, torch.float16, torch.float64])
+def test_conversions_leave_the_fp32_parameters_and_their_gradients(type):
+    """``.to(type)`` between steps: values and accumulated gradients of norms and scale stay as they are, bit for bit."""
+    m = mw.SandwichTransition(64, n=2, scale=0.1)
+    for p in m.parameters():
+        torch.nn.init.normal_(p)
+        p.grad = torch.randn_like(p)
+    want = {k: (p.detach().clone(), p.grad.clone()) for k, p in m.named_parameters()}
+    m.to(type)
+    for k, p in m.named_parameters():
+        kept = not k.startswith("feed_forward")
+        assert p.dtype == p.grad.dtype == (torch.float32 if kept else type), k
+        assert not kept or (torch.equal(p, want[k][0]) and torch.equal(p.grad, want[k][1])), k
+    moved = m.to("meta")
+    assert moved.join.scale.is_meta and moved.join.scale.dtype == torch.float32
+    assert moved.to_empty(device="cpu").join.scale.device.type == "cpu"
