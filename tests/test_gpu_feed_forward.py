@@ -402,3 +402,27 @@ def test_saved_tensors_that_come_back_as_others(rows, d, hidden):
             y = blocks.gated_feed_forward(*leaves)
         with pytest.raises(RuntimeError, match="came back with another|must be"):
             torch.autograd.grad(y, leaves, t["dy"])
+
+
+@pytest.mark.parametrize("rows,d", [(200, 64), (9500, 64), (1100, 512), (5000, 1024)])
+@pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_units_that_are_not_finite_do_not_touch_their_neighbours(rows, d, type, act):
+    """Units share powers of two and reciprocals (of a product, whose rounding and so whose last bits depend on all four factors): one
+    whose a is infinite or a NaN leaves the others' gradients within the bounds that they have without it, since a sigmoid's relative
+    error is the same few units of 2^-24 for any factors of the product."""
+    t = _make(rows, d, 128, type)
+    want = _want(t, act, type)
+    if d >= 512:
+        want = _with_kept(want, t, type)
+    keep = torch.arange(128, device=DEV) != 37
+    want = {"w_a": tuple(v[keep] for v in want["w_a"]), "w_b": tuple(v[keep] for v in want["w_b"]), "w_s": tuple(v[:, keep] for v in want["w_s"])}
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        leaves = {k: v.clone() for k, v in t.items() if k != "dy"}
+        leaves["w_a"][37, 5] = bad
+        for v in leaves.values():
+            v.requires_grad_(True)
+        y = blocks.gated_feed_forward(*leaves.values(), activation=act)
+        got = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), t["dy"])))
+        assert not torch.isfinite(y).any() and not torch.isfinite(got["w_a"][37]).any(), bad
+        _compare({"w_a": got["w_a"][keep], "w_b": got["w_b"][keep], "w_s": got["w_s"][:, keep]}, want, (rows, d, type, act, bad))
