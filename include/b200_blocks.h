@@ -10,7 +10,7 @@
  *    rounds h, da and db to the activations' type (operands of 16-bit products; h of up to four rows stays fp32). In fp16 a finite h,
  *    and a finite y of up to four rows, beyond 65504 become that; da, db and every other result become infinite there, and what is
  *    infinite or NaN on the way is never made finite.
- *  - The feed-forward's device-side waits are bounded: one that gives up lets the kernel finish and leaves a positive code that
+ *  - Device-side waits are bounded: one that gives up lets the kernel finish and leaves a positive code that
  *    b200_blocks_read_status returns (and clears).
  */
 #ifndef B200_BLOCKS_H_
@@ -85,7 +85,7 @@ int b200_ff_backward(const void* dy, const void* x, const void* w_a, const void*
                      void* dw_a, void* dw_b, void* dw_s, void* workspace, size_t workspace_bytes, long long rows, int d, int hidden, int dtype,
                      int weight_dtype, int activation, void* cuda_stream);
 
-/* Synchronises `cuda_stream`; *code: 0, or the code of the first wait of a feed-forward kernel on the current device that gave up
+/* Synchronises `cuda_stream`; *code: 0, or the code of the first wait of one of these kernels on the current device that gave up
  * since the last call (then cleared). */
 int b200_blocks_read_status(void* cuda_stream, int* code);
 

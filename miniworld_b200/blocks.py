@@ -82,7 +82,7 @@ def gated_feed_forward(x: torch.Tensor, w_a: torch.Tensor, w_b: torch.Tensor, w_
 
 
 def read_status(device=None) -> int:
-    """Synchronises the current stream; 0, or the code of the first device-side wait of a feed-forward on ``device`` that gave up
+    """Synchronises the current stream; 0, or the code of the first device-side wait of a block operator on ``device`` that gave up
     since the last call."""
     import ctypes
 

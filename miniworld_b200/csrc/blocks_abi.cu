@@ -548,10 +548,10 @@ static int check_ff(long long rows, int d, int hidden, int weight_dtype, int dty
   return B200_TRIMUL_OK;
 }
 
-// What the forward keeps for the backward: h in x's type, a and b in fp16, [rows][ld] each; nothing where forming a and b again is
+// What the forward keeps for the backward: h in x's type, a and b as ff_keep16 packs them, [rows][ld] values of 16 bits each; nothing where forming a and b again is
 // cheaper. Writing and reading them costs 8 bytes a value, forming them 4 D operations: 0.0012 against 0.0027 D picoseconds at
 // 6.5 TB/s and 1.5 PFLOP/s, equal at D = 460; calls of few rows are bound by latency either way and keep nothing.
-// (16384 x 1024 x 4096: training step 1207 -> 1122 us, kernels alone 1151 -> 921.)
+// (16384 x 1024 x 4096: kernels of a training step, each alone, 1151 -> 938 us.)
 static size_t ff_kept_bytes(long long rows, int d, int hidden) {
   if (d < 512 || rows < 1024) return 0;
   return 3 * up(up(static_cast<size_t>(rows), 32) * ff_ld(hidden) * 2, 1024);

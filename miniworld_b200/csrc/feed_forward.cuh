@@ -23,8 +23,8 @@
 // The structure is the contraction's: persistent CTAs (pairs for large products: 256-row tiles, each CTA supplies its rows of the
 // first operand and half of the second), one warp loads through TMA, one issues the MMAs, the others are the epilogue of the tile
 // before. All waits are bounded; one that gives up leaves a code in blocks_status.
-// M, D, H = 16384, 1024, 4096, bf16, each alone: up 168 us (200 with a and b kept), down 97, grad 136, input 190, weights 298, that is 1.64,
-// 1.42, 1.01, 1.45 and 1.38 PFLOP/s (cuBLAS 8192^3: 1.64); forming a and b again (kFfHidden) 395 instead of grad's 136. The 256 x 256
+// M, D, H = 16384, 1024, 4096, bf16, each alone: up 168 us (204 with a and b kept), down 98, grad 145, input 191, weights 300, that is 1.64,
+// 1.40, 0.95, 1.44 and 1.37 PFLOP/s (cuBLAS 8192^3: 1.64); forming a and b again (kFfHidden) 395 instead of grad's 145. The 256 x 256
 // tiles wait for their loads (stamps: 610 to 730 cycles for a k block of 512 cycles of products).
 #pragma once
 

@@ -13,7 +13,8 @@
 // D1 into registers and leaves h in the same columns, which are free again once G2 of the block is complete.
 // What bounds it is the special-function unit: an exponential a unit and a reciprocal for four, 1.25 x 64 x 128 / 16 = 640 cycles a
 // block and SM, so the groups are there to keep it busy while others wait for products, tensor memory and barriers: 196608 x 64 x 256
-// with two groups (h in the idle D2, a reciprocal for two) 42 us; now 33.6 us, of which that unit is busy half of the time.
+// with two groups (h in the idle D2, a reciprocal for two) 42 us; now 31.8 us in a graph of calls, of which that unit is busy half of
+// the time.
 // Warps: 0 weights, 1 G1, 2 input tiles, 3 G2, 4-27 the gate's groups, 28-31 output. All waits are bounded.
 #pragma once
 
