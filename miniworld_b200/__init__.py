@@ -3,16 +3,19 @@ module in :mod:`miniworld_b200.training`).
 
 Public surface: the module classes (drop-in for ``miniworld_engine.modules.TriangleMultiplication`` as
 MiniWorld's blocks use it), the functional entry points over the C ABI, the
-block operators of any width (:mod:`miniworld_b200.blocks` and their modules), and the row-sharded /
+block and token operators of any width (:mod:`miniworld_b200.blocks` and their modules), and the row-sharded /
 batch-parallel multi-GPU wrappers.
 """
 
 from .modules import (  # noqa: F401
     BidirectionalTriangleMultiplication,
+    BlockDropout,
     BlockJoin,
     BlockNorm,
     GatedFeedForward,
+    RelativePosition,
     SandwichTransition,
+    TokenAttention,
     Transition,
     TriangleMultiplication,
     TriangleMultiplicationIncoming,
@@ -29,6 +32,9 @@ __all__ = [
     "BlockJoin",
     "GatedFeedForward",
     "SandwichTransition",
+    "TokenAttention",
+    "RelativePosition",
+    "BlockDropout",
     "TriangleMultiplicationOutgoing",
     "TriangleMultiplicationIncoming",
     "to_openfold_state_dict",

@@ -1,4 +1,5 @@
-"""ctypes binding of ``libb200_trimul.so`` (the C ABI declared in ``include/b200_trimul.h`` and ``include/b200_blocks.h``).
+"""ctypes binding of ``libb200_trimul.so`` (the C ABI declared in ``include/b200_trimul.h``, ``b200_blocks.h`` and
+``b200_tokens.h``).
 
 There is no fallback: if the library is missing or a call fails, a ``RuntimeError`` is raised.
 """
@@ -154,6 +155,35 @@ BLOCKS_SIGNATURES = {
     "b200_blocks_read_status": (c_int, [c_void_p, POINTER(c_int)]),
 }
 
+
+
+class AttentionTensor(ctypes.Structure):
+    """``b200_attention_tensor`` of include/b200_tokens.h."""
+
+    _fields_ = [("data", c_void_p), ("row_stride", _L), ("head_stride", _L)]
+
+
+class AttentionCall(ctypes.Structure):
+    """``b200_attention_call`` of include/b200_tokens.h."""
+
+    _fields_ = [("rows", _L), ("sequences", c_int), ("length", c_int), ("heads", c_int), ("kv_heads", c_int), ("d", c_int), ("dtype", c_int),
+                ("causal", c_int), ("scale", c_float), ("offsets", c_void_p), ("mask", c_void_p), ("table", c_void_p), ("table_dtype", c_int),
+                ("bucket_of", c_void_p), ("buckets", c_int), ("reach", c_int)]
+
+
+# name -> (restype, argtypes) of include/b200_tokens.h
+_TENSOR, _CALL = POINTER(AttentionTensor), POINTER(AttentionCall)
+TOKENS_SIGNATURES = {
+    "b200_token_attention_forward": (c_int, [_CALL, _TENSOR, _TENSOR, _TENSOR, c_void_p, c_void_p, c_void_p]),
+    "b200_token_attention_workspace_bytes": (c_int, [_CALL, POINTER(c_size_t)]),
+    "b200_token_attention_backward": (c_int, [_CALL, _TENSOR, _TENSOR, _TENSOR, c_void_p, c_void_p, _TENSOR] + [c_void_p] * 5 + [c_size_t, c_void_p]),
+    "b200_relative_position_forward": (c_int, [c_void_p] * 6 + [c_int] * 7 + [c_void_p]),
+    "b200_relative_position_workspace_bytes": (c_int, [c_int] * 4 + [POINTER(c_size_t)]),
+    "b200_relative_position_backward": (c_int, [c_void_p] * 6 + [c_size_t] + [c_int] * 7 + [c_void_p]),
+    "b200_block_dropout": (c_int, [c_void_p] * 3 + [ctypes.c_ulonglong, c_void_p, _L, _L, _L, c_int, c_int, c_void_p]),
+    "b200_tokens_read_status": (c_int, [c_void_p, POINTER(c_int)]),
+}
+
 _lib = None
 
 
@@ -168,7 +198,7 @@ def load() -> ctypes.CDLL:
             "(there is no CPU or PyTorch fallback for this path)"
         )
     lib = ctypes.CDLL(str(LIB_PATH))
-    for name, (restype, argtypes) in {**SIGNATURES, **BLOCKS_SIGNATURES}.items():
+    for name, (restype, argtypes) in {**SIGNATURES, **BLOCKS_SIGNATURES, **TOKENS_SIGNATURES}.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is not exported
         fn.restype = restype
         fn.argtypes = argtypes

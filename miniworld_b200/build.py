@@ -18,7 +18,9 @@ NATIVE_TAG_PATH = PKG_DIR / "_native.tag"  # what NATIVE_PATH was built against
 HOST_SOURCE = CSRC / "host.cpp"
 HEADER = PKG_DIR.parent / "include" / "b200_trimul.h"
 BLOCKS_HEADER = PKG_DIR.parent / "include" / "b200_blocks.h"
-BLOCKS_HOST = CSRC / "host_blocks.inc"  # part of HOST_SOURCE
+TOKENS_HEADER = PKG_DIR.parent / "include" / "b200_tokens.h"
+BLOCKS_HOST = CSRC / "host_blocks.inc"  # parts of HOST_SOURCE
+TOKENS_HOST = CSRC / "host_tokens.inc"
 
 NVCC_FLAGS = [
     "-gencode",
@@ -32,7 +34,7 @@ NVCC_FLAGS = [
 
 
 def _sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [p for p in sorted(CSRC.glob("*.inc")) if p != BLOCKS_HOST] + [HEADER, BLOCKS_HEADER]
+    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [p for p in sorted(CSRC.glob("*.inc")) if p not in (BLOCKS_HOST, TOKENS_HOST)] + [HEADER, BLOCKS_HEADER, TOKENS_HEADER]
 
 
 def is_stale() -> bool:
@@ -55,7 +57,7 @@ def native_is_stale() -> bool:
     if not NATIVE_PATH.exists() or not NATIVE_TAG_PATH.exists() or NATIVE_TAG_PATH.read_text() != native_tag():
         return True
     built = NATIVE_PATH.stat().st_mtime
-    return any(src.stat().st_mtime > built for src in (HOST_SOURCE, HEADER, BLOCKS_HOST, BLOCKS_HEADER, Path(__file__)))
+    return any(src.stat().st_mtime > built for src in (HOST_SOURCE, HEADER, BLOCKS_HOST, BLOCKS_HEADER, TOKENS_HOST, TOKENS_HEADER, Path(__file__)))
 
 
 def find_nvcc() -> str:

@@ -19,12 +19,14 @@
 #include <torch/extension.h>
 
 #include <array>
+#include <cmath>
 #include <optional>
 #include <string>
 #include <tuple>
 #include <vector>
 
 #include "../../include/b200_blocks.h"
+#include "../../include/b200_tokens.h"
 #include "../../include/b200_trimul.h"
 
 // The parameters of a call, in Python a list of tensors or a pair (a module's _modules, ((child, name), ...)) that names the
@@ -382,6 +384,7 @@ OptTensor transition_train(const Tensor& x, const CallParams& call, double eps, 
 }
 
 #include "host_blocks.inc"
+#include "host_tokens.inc"
 
 }  // namespace
 
@@ -426,4 +429,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("transition_train", torch::wrap_pybind_function_no_gil(transition_train));
   m.def("block_join", torch::wrap_pybind_function_no_gil(block_join));
   m.def("gated_feed_forward", torch::wrap_pybind_function_no_gil(gated_feed_forward));
+  m.def("token_attention", torch::wrap_pybind_function_no_gil(token_attention));
+  m.def("relative_position", torch::wrap_pybind_function_no_gil(relative_position));
+  m.def("block_dropout", torch::wrap_pybind_function_no_gil(block_dropout));
 }

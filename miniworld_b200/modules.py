@@ -609,3 +609,68 @@ class SandwichTransition(nn.Module):
 
     def forward(self, x: torch.Tensor, gate: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         return self.join(x, self.feed_forward(self.ln_in(x)), gate, mask)
+
+
+class TokenAttention(nn.Module):
+    """Attention among the tokens of a sequence, ``forward(q, k, v, mask=None, offsets=None)``
+    (:func:`miniworld_b200.blocks.token_attention`), with a learned bias of the relative position: ``table`` [buckets, heads], kept in
+    fp32, for distances up to ``reach`` (``exact`` as in :func:`miniworld_b200.blocks.relative_buckets`; ``reach`` None: no bias)."""
+
+    def __init__(self, heads: int, reach: Optional[int] = 32, exact: Optional[int] = None, causal: bool = False, scale: Optional[float] = None,
+                 check_status: bool = False):
+        super().__init__()
+        self.heads, self.causal, self.scale, self.check_status = heads, bool(causal), scale, bool(check_status)
+        bucket_of = None if reach is None else blocks.relative_buckets(reach, exact)
+        self.register_buffer("bucket_of", bucket_of, persistent=False)
+        self.table = None if bucket_of is None else nn.Parameter(torch.zeros(int(bucket_of.max()) + 1, heads))
+
+    def _apply(self, fn, recurse=True):
+        return super()._apply(_pinned(fn), recurse)
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        o = blocks.token_attention(q, k, v, offsets=offsets, mask=mask, causal=self.causal, scale=self.scale, table=self.table,
+                                   bucket_of=self.bucket_of)
+        if self.check_status:
+            blocks.check_status(q.device, "token_attention")
+        return o
+
+
+class RelativePosition(nn.Module):
+    """The relative position of its two tokens added to every cell of a pair tensor, ``forward(z, index, chain=None)``
+    (:func:`miniworld_b200.blocks.relative_position`): ``table`` [buckets + 1, d_pair], kept in fp32, its last row for the pairs of
+    different chains."""
+
+    def __init__(self, d_pair: int, reach: int = 32, exact: Optional[int] = None):
+        super().__init__()
+        bucket_of = blocks.relative_buckets(reach, exact)
+        self.register_buffer("bucket_of", bucket_of, persistent=False)
+        self.table = nn.Parameter(torch.empty(int(bucket_of.max()) + 2, d_pair))
+        nn.init.normal_(self.table, std=0.02)
+
+    def _apply(self, fn, recurse=True):
+        return super()._apply(_pinned(fn), recurse)
+
+    def forward(self, z: torch.Tensor, index: torch.Tensor, chain: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return blocks.relative_position(z, self.table, index, bucket_of=self.bucket_of, chain=chain)
+
+
+class BlockDropout(nn.Module):
+    """The residual add of a block's output with dropout, ``forward(x, u, key=None) -> x + keep * u / (1 - p)`` in training and ``x + u``
+    otherwise (:func:`miniworld_b200.blocks.block_dropout`). ``shared`` names a dimension whose rows use one mask; ``key`` defaults to
+    a new one from PyTorch's generator."""
+
+    def __init__(self, p: float, shared: Optional[int] = None):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be from 0 to 1, got {p}")
+        self.p, self.shared = float(p), shared
+
+    def forward(self, x: torch.Tensor, u: torch.Tensor, key: Optional[torch.Tensor] = None) -> torch.Tensor:
+        p = self.p if self.training else 0.0
+        if p == 0.0:
+            return x + u
+        return blocks.block_dropout(x, u, blocks.dropout_key(u.device) if key is None else key, p=p, shared=self.shared)
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}, shared={self.shared}"
