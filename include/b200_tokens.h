@@ -51,18 +51,20 @@ typedef struct {
 
 /*
  * o_i = sum_j softmax_j(scale q_i . k_j + bias) v_j, o [rows, heads, d] contiguous. Rows without a key (masked ones, rows of no
- * sequence) are zero, and what masked rows hold is never used. lse: fp32 [heads, rows], for the backward (null: not kept).
+ * sequence) are zero, and what masked rows hold is never used. For a backward (both null: not kept): rest, of o's type and shape, what
+ * rounding o took away (2^11 times as much in fp16), and lse, fp32 [heads, rows], log2 of the softmax's denominators.
  */
 int b200_token_attention_forward(const b200_attention_call* call, const b200_attention_tensor* q, const b200_attention_tensor* k,
-                                 const b200_attention_tensor* v, void* o, float* lse, void* cuda_stream);
+                                 const b200_attention_tensor* v, void* o, void* rest, float* lse, void* cuda_stream);
 
 /*
- * Gradients from dO (strides as for q), the forward's inputs, o and lse: dq [rows, heads, d], dk and dv [rows, kv_heads, d], contiguous,
+ * Gradients from dO (strides as for q), the forward's inputs, o, rest and lse: dq [rows, heads, d], dk and dv [rows, kv_heads, d], contiguous,
  * and, where it is not null, dtable (table_dtype). Workspace: 1024-byte aligned, b200_token_attention_workspace_bytes of the same call.
  */
 int b200_token_attention_workspace_bytes(const b200_attention_call* call, size_t* out_bytes);
 int b200_token_attention_backward(const b200_attention_call* call, const b200_attention_tensor* q, const b200_attention_tensor* k,
-                                  const b200_attention_tensor* v, const void* o, const float* lse, const b200_attention_tensor* d_o, void* dq,
+                                  const b200_attention_tensor* v, const void* o, const void* rest, const float* lse,
+                                  const b200_attention_tensor* d_o, void* dq,
                                   void* dk, void* dv, void* dtable, void* workspace, size_t workspace_bytes, void* cuda_stream);
 
 /*

@@ -174,9 +174,9 @@ class AttentionCall(ctypes.Structure):
 # name -> (restype, argtypes) of include/b200_tokens.h
 _TENSOR, _CALL = POINTER(AttentionTensor), POINTER(AttentionCall)
 TOKENS_SIGNATURES = {
-    "b200_token_attention_forward": (c_int, [_CALL, _TENSOR, _TENSOR, _TENSOR, c_void_p, c_void_p, c_void_p]),
+    "b200_token_attention_forward": (c_int, [_CALL, _TENSOR, _TENSOR, _TENSOR] + [c_void_p] * 4),
     "b200_token_attention_workspace_bytes": (c_int, [_CALL, POINTER(c_size_t)]),
-    "b200_token_attention_backward": (c_int, [_CALL, _TENSOR, _TENSOR, _TENSOR, c_void_p, c_void_p, _TENSOR] + [c_void_p] * 5 + [c_size_t, c_void_p]),
+    "b200_token_attention_backward": (c_int, [_CALL, _TENSOR, _TENSOR, _TENSOR] + [c_void_p] * 3 + [_TENSOR] + [c_void_p] * 5 + [c_size_t, c_void_p]),
     "b200_relative_position_forward": (c_int, [c_void_p] * 6 + [c_int] * 7 + [c_void_p]),
     "b200_relative_position_workspace_bytes": (c_int, [c_int] * 4 + [POINTER(c_size_t)]),
     "b200_relative_position_backward": (c_int, [c_void_p] * 6 + [c_size_t] + [c_int] * 7 + [c_void_p]),

@@ -22,7 +22,7 @@ struct AttentionParams {
   const uint8_t* mask;            // [rows]
   const void* table;              // [buckets, heads]
   const int* bucket_of;           // [2 reach + 1]
-  void *o, *dq, *dk, *dv;         // [rows, heads, d]
+  void *o, *rest, *dq, *dk, *dv;  // [rows, heads, d]; rest: what rounding o took away
   float* lse;                     // [heads][rows]: log2 of the softmax's denominator, +inf where a row has no key
   float* delta;                   // [heads][rows]
   float* partial;                 // [heads][blocks][2 reach + 1]: sums of ds by distance
@@ -82,53 +82,6 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// A warp a query row and head: 32 keys at a time, a key a lane for the scores, channels over the lanes for the sums.
-template <typename T>
-__global__ void __launch_bounds__(kAttentionWarps * 32) attention_forward_kernel(const AttentionParams p) {
-  __shared__ float row_q[kAttentionWarps][kAttentionMostWidth];
-  constexpr bool f16 = sizeof(T) == 2 && __is_same(T, __half);
-  grid_dependency_wait();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y, kv_head = head / (p.heads / p.kv_heads);
-  float* q = row_q[warp];
-  for (long long row = static_cast<long long>(blockIdx.x) * kAttentionWarps + warp; row < p.rows; row += static_cast<long long>(gridDim.x) * kAttentionWarps) {
-    const AttentionRow r = attention_row(p, row);
-    T* out = static_cast<T*>(p.o) + (row * p.heads + head) * p.d;
-    float most = -INFINITY, total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r.there) {
-      __syncwarp();
-      for (int c = lane; c < p.d; c += 32) q[c] = static_cast<float>(__ldcg(attention_at<T>(p.q, row, head) + c));
-      __syncwarp();
-      const long long last = p.causal ? row + 1 : r.last;
-      for (long long j0 = r.first; j0 < last; j0 += 32) {
-        const long long j = j0 + lane;
-        const bool counts = j < last && (p.mask == nullptr || __ldcg(p.mask + j) != 0);
-        float s = -INFINITY;
-        if (counts)
-          s = (attention_dot(q, attention_at<T>(p.k, j, kv_head), p.d) * p.scale + attention_bias(p, static_cast<int>(j - row), head, f16)) * kLog2e;
-        const float next = fmaxf(most, warp_max(s));
-        if (__all_sync(0xFFFFFFFFu, !counts)) continue;
-        const float shrink = most == -INFINITY ? 0.f : exp2f(most - next), e = counts ? exp2f(s - next) : 0.f;
-        total = total * shrink + warp_sum(e);
-        most = next;
-        for (int a = 0; a < 4; ++a) acc[a] *= shrink;
-        uint32_t left = __ballot_sync(0xFFFFFFFFu, counts);
-        while (left != 0) {
-          const int i = __ffs(left) - 1;
-          left &= left - 1;
-          const float w = __shfl_sync(0xFFFFFFFFu, e, i);
-          const T* v = attention_at<T>(p.v, j0 + i, kv_head);
-          for (int a = 0; a < 4; ++a)
-            if (lane + 32 * a < p.d) acc[a] = fmaf(w, static_cast<float>(__ldcg(v + lane + 32 * a)), acc[a]);
-        }
-      }
-    }
-    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-    for (int a = 0; a < 4; ++a)
-      if (lane + 32 * a < p.d) out[lane + 32 * a] = static_cast<T>(acc[a] * inv);
-    if (p.lse != nullptr && lane == 0) p.lse[head * p.rows + row] = inv == 0.f && total == 0.f ? INFINITY : most + log2f(total);
-  }
-}
-
 // delta, dq and the sums of ds by distance: a warp a query row
 template <typename T>
 __global__ void __launch_bounds__(kAttentionWarps * 32) attention_dq_kernel(const AttentionParams p) {
@@ -150,10 +103,11 @@ __global__ void __launch_bounds__(kAttentionWarps * 32) attention_dq_kernel(cons
     if (r.there && lse != INFINITY) {
       __syncwarp();
       const T* o = static_cast<const T*>(p.o) + (row * p.heads + head) * p.d;
+      const T* rest = static_cast<const T*>(p.rest) + (row * p.heads + head) * p.d;
       for (int c = lane; c < p.d; c += 32) {
         q[c] = static_cast<float>(__ldcg(attention_at<T>(p.q, row, head) + c));
         g[c] = static_cast<float>(__ldcg(attention_at<T>(p.dout, row, head) + c));
-        delta = fmaf(g[c], static_cast<float>(__ldcg(o + c)), delta);
+        delta = fmaf(g[c], static_cast<float>(__ldcg(o + c)) + static_cast<float>(__ldcg(rest + c)) * (f16 ? 1.f / 2048.f : 1.f), delta);
       }
       delta = warp_sum(delta);
       __syncwarp();

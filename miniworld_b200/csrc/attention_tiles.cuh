@@ -1,0 +1,133 @@
+// What the attention's kernels on the tensor cores share: which rows a block works on, operands in shared and tensor memory, the bias.
+//
+// Tiles are 128 queries by 128 keys. Scores and their gradients are products into tensor memory, a row a lane; threads take them into
+// registers, and what comes of them (probabilities, gradients of scores) goes back into tensor memory in 16 bits as the first operand
+// of the next product: neither of the two ever passes through shared memory.
+#pragma once
+
+#include "attention.cuh"
+
+namespace trimul {
+
+constexpr int kAtTile = 128;
+constexpr int kAtTileBytes = 128 * 128;  // 128 rows of 64 elements
+// what a result's rounding error is multiplied by before it is rounded itself
+template <bool F16>
+constexpr float kAtRest = F16 ? 2048.f : 1.f;
+
+struct AttentionMaps {
+  CUtensorMap q, k, v, dout;  // [rows][heads][d], boxes of 128 rows of 64 elements
+};
+
+__device__ __forceinline__ void umma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_pair(float2 v) {
+  if constexpr (F16)
+    return pack_f16x2(v);
+  else
+    return pack_bf16x2(v);
+}
+template <bool F16>
+__device__ __forceinline__ float2 unpack_pair(uint32_t v) {
+  if constexpr (F16)
+    return f16x2_to_float2(v);
+  else
+    return bf16x2_to_float2(v);
+}
+template <int REGS>
+__device__ __forceinline__ void registers_more() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void registers_fewer() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+// The rows of a block. Sequences of equal lengths are cut into tiles one after the other. Packed ones get, for sequence s, the places
+// from floor(offsets[s] / rows of a tile) + s on: at least as many as it has tiles, and found by looking for the greatest s whose first
+// place is not beyond the block's, without any table. What is left at most is one place a sequence. Place `sequences` stands for the
+// rows behind the last one.
+struct AttentionPlace {
+  long long first, last;  // the sequence's rows
+  int tile;               // of `tile_rows` rows of it; beyond its end: nothing to do
+  int behind;             // rows of no sequence
+};
+__host__ __device__ inline long long attention_places(const int* offsets, long long rows, int sequences, int length, int tile_rows) {
+  if (offsets == nullptr) return static_cast<long long>(sequences) * ((length + tile_rows - 1) / tile_rows);
+  return rows / tile_rows + sequences + 1;
+}
+// by a whole warp
+__device__ __forceinline__ AttentionPlace attention_place(const AttentionParams& p, long long place, int tile_rows) {
+  AttentionPlace r;
+  if (p.offsets == nullptr) {
+    const int tiles = (p.length + tile_rows - 1) / tile_rows;
+    const long long s = place / tiles;
+    r.first = s * p.length;
+    r.last = r.first + p.length;
+    r.tile = static_cast<int>(place - s * tiles);
+    r.behind = 0;
+    return r;
+  }
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = p.sequences + 1;  // the sequence is one of lo .. lo + n - 1
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lane * step;
+    const bool before = at < n && attention_offset(p, lo + at) / tile_rows + lo + at <= place;
+    const int at_most = max(__popc(__ballot_sync(0xFFFFFFFFu, before)) - 1, 0) * step;
+    lo += at_most;
+    n = min(step, n - at_most);
+  }
+  r.first = attention_offset(p, lo);
+  r.last = lo < p.sequences ? attention_offset(p, lo + 1) : p.rows;
+  r.tile = static_cast<int>(max(place - (r.first / tile_rows + lo), 0ll));
+  r.behind = lo == p.sequences;
+  return r;
+}
+
+// Biases of all distances that tiles near the diagonal meet, in units of log2: entry i is that of the distance i - (reach + 255).
+__host__ __device__ constexpr int attention_bias_entries(int reach) { return 2 * (reach + 255) + 1; }
+__device__ __forceinline__ void attention_bias_fill(const AttentionParams& p, float* bias, int head, bool f16, int thread, int threads) {
+  const int entries = attention_bias_entries(p.reach);
+  for (int i = thread; i < entries; i += threads) bias[i] = attention_bias(p, i - (p.reach + 255), head, f16) * kLog2e;
+}
+
+// Keys first .. first + 127 that the mask leaves, a bit each (mask null: all); those at or beyond `limit` are the caller's business.
+__device__ __forceinline__ void attention_mask_bits(const AttentionParams& p, long long first, long long last, uint32_t (&bits)[4]) {
+  const int lane = threadIdx.x & 31;
+  bool there[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long row = first + 32 * i + lane;
+    there[i] = row < last && __ldcg(p.mask + row) != 0;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bits[i] = __ballot_sync(0xFFFFFFFFu, there[i]);
+}
+
+// Zeroes the rows of a tile in shared memory that are not among the `bits` (whole warp): an operand's rows that belong to other
+// sequences or are masked must not meet the zeros that stand for them in the other operand as infinities or NaN.
+__device__ __forceinline__ void attention_clean_rows(uint32_t tile, int halves, const uint32_t (&bits)[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int h = 0; h < halves; ++h)
+#pragma unroll 1
+    for (int r = lane / 8; r < 128; r += 4)
+      if (!(bits[r >> 5] >> (r & 31) & 1u))
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + h * kAtTileBytes + r * 128 + (lane & 7) * 16), "r"(0) : "memory");
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+}  // namespace trimul

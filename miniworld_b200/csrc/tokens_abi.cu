@@ -6,13 +6,12 @@
 #include <initializer_list>
 
 #include "attention.cuh"
+#include "attention_forward.cuh"
 #include "dropout.cuh"
 #include "host_util.cuh"
 #include "position.cuh"
 
 namespace trimul {
-
-static __device__ int tokens_status;  // 0, or the code of the first bounded wait that gave up (it stays until the host has read it)
 
 static size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 static long long blocks_for(long long n, long long b) { return (n + b - 1) / b; }
@@ -81,6 +80,23 @@ static AttentionParams attention_params(const b200_attention_call* c, const b200
 }
 constexpr int kAttentionBlocks = 1024;  // blocks of a head
 static int attention_blocks(long long rows) { return static_cast<int>(std::min<long long>(blocks_for(rows, kAttentionWarps), kAttentionBlocks)); }
+// [rows][heads][d] in boxes of 128 rows of 64 elements
+static int attention_map(CUtensorMap* m, const AttentionTensor& t, long long rows, int heads, int d) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(heads), static_cast<uint64_t>(rows)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(heads == 1 ? d : t.head) * 2, static_cast<uint64_t>(rows == 1 ? static_cast<long long>(heads) * d : t.row) * 2};
+  const uint32_t box[3] = {64, 1, kAtTile};
+  return make_map(m, t.base, 3, dims, strides, box);
+}
+template <bool F16, int HALVES>
+static int launch_attention_forward(const AttentionMaps& maps, const AttentionParams& p, const DeviceInfo& info, cudaStream_t stream) {
+  using C = AtForward<HALVES>;
+  const auto kernel = attention_forward_kernel<F16, HALVES>;
+  const int rc = set_smem(kernel, C::smem(B200_POSITION_MAX_REACH), info.device);
+  if (rc != 0) return rc;
+  const long long places = attention_places(p.offsets, p.rows, p.sequences, p.length, C::kTiles * kAtTile);
+  TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(places), p.heads), C::kThreads, C::smem(p.reach), stream, maps, p));
+  return B200_TRIMUL_OK;
+}
 struct AttentionRegions {
   size_t delta, partial, total;
 };
@@ -164,23 +180,28 @@ using namespace trimul;
 extern "C" {
 
 int b200_token_attention_forward(const b200_attention_call* call, const b200_attention_tensor* q, const b200_attention_tensor* k,
-                                 const b200_attention_tensor* v, void* o, float* lse, void* cuda_stream) {
+                                 const b200_attention_tensor* v, void* o, void* rest, float* lse, void* cuda_stream) {
   int rc = check_attention(call);
   if (rc != 0) return rc;
   if (call->rows == 0) return B200_TRIMUL_OK;
   for (const b200_attention_tensor* t : {q, k, v})
     if ((rc = check_attention_tensor(t)) != 0) return rc;
-  if (o == nullptr) return B200_TRIMUL_E_NULL;
-  if (!aligned(o, 16)) return B200_TRIMUL_E_ALIGN;
+  if (o == nullptr || (rest == nullptr) != (lse == nullptr)) return B200_TRIMUL_E_NULL;
+  if (!all_aligned16({o, rest})) return B200_TRIMUL_E_ALIGN;
   DeviceInfo info;
   if ((rc = tokens_device(&info)) != 0) return rc;
   AttentionParams p = attention_params(call, q, k, v);
   p.o = o;
+  p.rest = rest;
   p.lse = lse;
-  p.blocks = attention_blocks(p.rows);
-  const auto kernel = call->dtype == B200_BLOCKS_F16 ? attention_forward_kernel<__half> : attention_forward_kernel<__nv_bfloat16>;
-  TRIMUL_CUDA(launch_overlapped(kernel, dim3(p.blocks, p.heads), kAttentionWarps * 32, 0, static_cast<cudaStream_t>(cuda_stream), p));
-  return B200_TRIMUL_OK;
+  AttentionMaps maps = {};
+  rc = attention_map(&maps.q, p.q, p.rows, p.heads, p.d);
+  if (rc == 0) rc = attention_map(&maps.k, p.k, p.rows, p.kv_heads, p.d);
+  if (rc == 0) rc = attention_map(&maps.v, p.v, p.rows, p.kv_heads, p.d);
+  if (rc != 0) return rc;
+  const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  if (call->dtype == B200_BLOCKS_F16) return p.d <= 64 ? launch_attention_forward<true, 1>(maps, p, info, stream) : launch_attention_forward<true, 2>(maps, p, info, stream);
+  return p.d <= 64 ? launch_attention_forward<false, 1>(maps, p, info, stream) : launch_attention_forward<false, 2>(maps, p, info, stream);
 }
 
 int b200_token_attention_workspace_bytes(const b200_attention_call* call, size_t* out_bytes) {
@@ -192,7 +213,8 @@ int b200_token_attention_workspace_bytes(const b200_attention_call* call, size_t
 }
 
 int b200_token_attention_backward(const b200_attention_call* call, const b200_attention_tensor* q, const b200_attention_tensor* k,
-                                  const b200_attention_tensor* v, const void* o, const float* lse, const b200_attention_tensor* d_o, void* dq,
+                                  const b200_attention_tensor* v, const void* o, const void* rest, const float* lse,
+                                  const b200_attention_tensor* d_o, void* dq,
                                   void* dk, void* dv, void* dtable, void* workspace, size_t workspace_bytes, void* cuda_stream) {
   int rc = check_attention(call);
   if (rc != 0) return rc;
@@ -205,8 +227,8 @@ int b200_token_attention_backward(const b200_attention_call* call, const b200_at
   }
   for (const b200_attention_tensor* t : {q, k, v, d_o})
     if ((rc = check_attention_tensor(t)) != 0) return rc;
-  if (o == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || workspace == nullptr) return B200_TRIMUL_E_NULL;
-  if (!all_aligned16({o, dq, dk, dv}) || !aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;
+  if (o == nullptr || rest == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || workspace == nullptr) return B200_TRIMUL_E_NULL;
+  if (!all_aligned16({o, rest, dq, dk, dv}) || !aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;
   const AttentionRegions regions = attention_regions(call);
   if (workspace_bytes < regions.total) return B200_TRIMUL_E_WORKSPACE;
   DeviceInfo info;
@@ -214,6 +236,7 @@ int b200_token_attention_backward(const b200_attention_call* call, const b200_at
   AttentionParams p = attention_params(call, q, k, v);
   p.dout = attention_tensor(d_o);
   p.o = const_cast<void*>(o);
+  p.rest = const_cast<void*>(rest);
   p.lse = const_cast<float*>(lse);
   p.dq = dq;
   p.dk = dk;

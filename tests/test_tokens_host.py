@@ -55,9 +55,9 @@ REFUSED_CALLS = [
 def test_attention_refuses_calls(lib, p, kw, code):
     c, t = _call(p, **kw), _lib.AttentionTensor(p, 128, 32)
     need = ctypes.c_size_t(0)
-    assert lib.b200_token_attention_forward(c, t, t, t, p, None, None) == code
+    assert lib.b200_token_attention_forward(c, t, t, t, p, None, None, None) == code
     assert lib.b200_token_attention_workspace_bytes(c, ctypes.byref(need)) == code
-    assert lib.b200_token_attention_backward(c, t, t, t, p, p, t, p, p, p, None, p, 1 << 40, None) == code
+    assert lib.b200_token_attention_backward(c, t, t, t, p, p, p, t, p, p, p, None, p, 1 << 40, None) == code
 
 
 def test_attention_refuses_tensors(lib, p):
@@ -68,19 +68,21 @@ def test_attention_refuses_tensors(lib, p):
         for at in range(4):
             four = [t if i == at else good for i in range(4)]
             if at < 3:
-                assert lib.b200_token_attention_forward(c, *four[:3], p, None, None) == code
-            assert lib.b200_token_attention_backward(c, *four[:3], p, p, four[3], p, p, p, None, p, 1 << 40, None) == code
-    assert lib.b200_token_attention_forward(None, good, good, good, p, None, None) == -1
-    assert lib.b200_token_attention_forward(c, good, good, good, None, None, None) == -1
-    assert lib.b200_token_attention_forward(c, good, good, good, p + 2, None, None) == -4
-    assert lib.b200_token_attention_forward(_call(p, rows=0, sequences=0), None, None, None, None, None, None) == 0
+                assert lib.b200_token_attention_forward(c, *four[:3], p, None, None, None) == code
+            assert lib.b200_token_attention_backward(c, *four[:3], p, p, p, four[3], p, p, p, None, p, 1 << 40, None) == code
+    assert lib.b200_token_attention_forward(None, good, good, good, p, None, None, None) == -1
+    assert lib.b200_token_attention_forward(c, good, good, good, None, None, None, None) == -1
+    assert lib.b200_token_attention_forward(c, good, good, good, p, p, None, None) == -1  # both are kept, or none
+    assert lib.b200_token_attention_forward(c, good, good, good, p, p + 8, p, None) == -4
+    assert lib.b200_token_attention_forward(c, good, good, good, p + 2, None, None, None) == -4
+    assert lib.b200_token_attention_forward(_call(p, rows=0, sequences=0), None, None, None, None, None, None, None) == 0
 
-    def back(o=p, lse=p, dq=p, dk=p, dv=p, dtable=None, ws=p, n=1 << 40, call=c):
-        return lib.b200_token_attention_backward(call, good, good, good, o, lse, good, dq, dk, dv, dtable, ws, n, None)
+    def back(o=p, rest=p, lse=p, dq=p, dk=p, dv=p, dtable=None, ws=p, n=1 << 40, call=c):
+        return lib.b200_token_attention_backward(call, good, good, good, o, rest, lse, good, dq, dk, dv, dtable, ws, n, None)
 
-    assert back(o=None) == back(lse=None) == back(dq=None) == back(dk=None) == back(dv=None) == back(ws=None) == -1
+    assert back(o=None) == back(rest=None) == back(lse=None) == back(dq=None) == back(dk=None) == back(dv=None) == back(ws=None) == -1
     assert back(dtable=p) == -1  # the gradient of a table that is not there
-    assert back(o=p + 8) == back(dq=p + 8) == back(dk=p + 4) == back(dv=p + 2) == back(ws=p + 16) == -4
+    assert back(o=p + 8) == back(rest=p + 2) == back(dq=p + 8) == back(dk=p + 4) == back(dv=p + 2) == back(ws=p + 16) == -4
     assert back(n=8) == -5
     need = ctypes.c_size_t(0)
     assert lib.b200_token_attention_workspace_bytes(c, None) == -1
