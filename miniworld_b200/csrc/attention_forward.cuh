@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
           for (int h = 0; h < HALVES; ++h)
             tma_load_3d(q_s + (t * HALVES + h) * kAtTileBytes, &maps.q, q_ready, h * 64, head, static_cast<int>(place.first) + (place.tile * T + t) * kAtTile);
       int i = 0;
-      uint32_t through = 0, odd = 0;  // a bit a stage: its last copy went to landed(); parity of landed()'s current phase
+      AttentionRing state;
       for (; i < 2 * n; ++i) {
         // which tile is next
         bool value;
@@ -133,26 +133,13 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
         const int s = i % ST;
         if (i >= ST && !mbar_wait(empty(s), static_cast<uint32_t>((i / ST) & 1) ^ 1u, abort_flag, status, kDevTimeoutProducer)) break;
         const bool other = value && dirty(j);
-        if (other && (through >> (s + 16) & 1u)) odd ^= 1u << s;
-        through = (through & ~(1u << s)) | (other ? 0x10001u << s : 0u);
+        state.use(s, other);
         const uint32_t bar = other ? landed(s) : ready(s);
         mbar_arrive_expect_tx(bar, C::kStageBytes);
         for (int h = 0; h < HALVES; ++h)
           tma_load_3d(ring + s * C::kStageBytes + h * kAtTileBytes, value ? &maps.v : &maps.k, bar, h * 64, kv_head, static_cast<int>(place.first) + j * kAtTile);
       }
-      // copies that nothing has waited for (after a wait has given up) land before the block may exit
-      if (*abort_flag != 0) {
-        const long long t0 = clock64();
-        while (!mbar_try_wait(q_ready, 0) && clock64() - t0 < kWaitLimitCycles) {
-        }
-        for (int k = i > ST ? i - ST : 0; k < i; ++k) {
-          const int s = k % ST;
-          const bool other = through >> s & 1u;
-          const long long t1 = clock64();
-          while (!mbar_try_wait(other ? landed(s) : ready(s), other ? odd >> s & 1u : static_cast<uint32_t>((k / ST) & 1)) && clock64() - t1 < kWaitLimitCycles) {
-          }
-        }
-      }
+      if (*abort_flag != 0) state.drain<ST>(q_ready, landed, ready);
     } else if (warp == mma_warp && elect_one()) {
       constexpr uint32_t fmt = F16 ? kFmtF16 : kFmtBF16;
       constexpr uint32_t idesc_s = umma_idesc(128, 128, false, false, fmt, fmt);
@@ -209,14 +196,8 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
       for (int j = 0; j < n; ++j) {
         if (!dirty(j)) continue;
         const int i = value_place(j), s = i % ST;
-        uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-        const long long first = place.first + static_cast<long long>(j) * kAtTile;
-        if (p.mask != nullptr) attention_mask_bits(p, first, place.last, bits);
-        else
-          for (int w = 0; w < 4; ++w) {
-            const int left = length - j * kAtTile - 32 * w;
-            bits[w] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u;
-          }
+        uint32_t bits[4];
+        attention_rows_there(p, place, length, j, bits);
         if (!mbar_wait_warp(landed(s), odd >> s & 1u, abort_flag, status, kDevTimeoutStats)) break;
         odd ^= 1u << s;
         attention_clean_rows(ring + s * C::kStageBytes, HALVES, bits);

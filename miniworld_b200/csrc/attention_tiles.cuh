@@ -116,6 +116,47 @@ __device__ __forceinline__ void attention_mask_bits(const AttentionParams& p, lo
   for (int i = 0; i < 4; ++i) bits[i] = __ballot_sync(0xFFFFFFFFu, there[i]);
 }
 
+// The same of tile j of a sequence, with or without a mask, up to the sequence's end
+__device__ __forceinline__ void attention_rows_there(const AttentionParams& p, const AttentionPlace& place, int length, int j, uint32_t (&bits)[4]) {
+  if (p.mask != nullptr) {
+    attention_mask_bits(p, place.first + static_cast<long long>(j) * kAtTile, place.last, bits);
+    return;
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int left = length - j * kAtTile - 32 * w;
+    bits[w] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u;
+  }
+}
+
+// What the copying thread remembers of its ring, a bit a stage: whether it was used, the parity of that use, whether the copy went to
+// landed() and not to ready(), and the parity of landed(), which only such copies have.
+struct AttentionRing {
+  uint32_t used = 0, odd = 0, through = 0, landed = 0, landed_odd = 0;
+  __device__ __forceinline__ void use(int s, bool other) {
+    const uint32_t bit = 1u << s;
+    odd ^= used & bit;
+    used |= bit;
+    through = other ? through | bit : through & ~bit;
+    if (other) {
+      landed_odd ^= landed & bit;
+      landed |= bit;
+    }
+  }
+  // Copies that nothing has waited for (after a wait has given up) land before the block may exit.
+  template <int ST, typename Landed, typename Ready>
+  __device__ __forceinline__ void drain(uint32_t first, Landed landed_bar, Ready ready_bar) const {
+    auto land = [](uint32_t b, uint32_t phase) {
+      const long long t0 = clock64();
+      while (!mbar_try_wait(b, phase) && clock64() - t0 < kWaitLimitCycles) {
+      }
+    };
+    land(first, 0);
+    for (int s = 0; s < ST; ++s)
+      if (used >> s & 1u) land(through >> s & 1u ? landed_bar(s) : ready_bar(s), (through >> s & 1u ? landed_odd : odd) >> s & 1u);
+  }
+};
+
 // Zeroes the rows of a tile in shared memory that are not among the `bits` (whole warp): an operand's rows that belong to other
 // sequences or are masked must not meet the zeros that stand for them in the other operand as infinities or NaN.
 __device__ __forceinline__ void attention_clean_rows(uint32_t tile, int halves, const uint32_t (&bits)[4]) {

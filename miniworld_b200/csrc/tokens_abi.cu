@@ -4,8 +4,9 @@
 
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
-#include "attention.cuh"
+#include "attention_backward.cuh"
 #include "attention_forward.cuh"
 #include "dropout.cuh"
 #include "host_util.cuh"
@@ -78,8 +79,6 @@ static AttentionParams attention_params(const b200_attention_call* c, const b200
   p.scale = c->scale;
   return p;
 }
-constexpr int kAttentionBlocks = 1024;  // blocks of a head
-static int attention_blocks(long long rows) { return static_cast<int>(std::min<long long>(blocks_for(rows, kAttentionWarps), kAttentionBlocks)); }
 // [rows][heads][d] in boxes of 128 rows of 64 elements
 static int attention_map(CUtensorMap* m, const AttentionTensor& t, long long rows, int heads, int d) {
   const uint64_t dims[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(heads), static_cast<uint64_t>(rows)};
@@ -97,14 +96,37 @@ static int launch_attention_forward(const AttentionMaps& maps, const AttentionPa
   TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(places), p.heads), C::kThreads, C::smem(p.reach), stream, maps, p));
   return B200_TRIMUL_OK;
 }
+static int attention_delta_blocks(long long rows, int d) {
+  int team = 1;
+  while (team * 8 < d) team *= 2;
+  return static_cast<int>(std::min<long long>(kAtDeltaBlocks, blocks_for(rows, kAtDeltaThreads / team)));
+}
+template <bool F16, int HALVES>
+static int launch_attention_backward(const AttentionMaps& maps, const AttentionParams& p, const DeviceInfo& info, cudaStream_t stream) {
+  using T = std::conditional_t<F16, __half, __nv_bfloat16>;
+  const auto dq = attention_dq_kernel<F16, HALVES>;
+  const auto dkv = attention_dkv_kernel<F16, HALVES>;
+  int rc = set_smem(dq, AtDq<HALVES>::smem(true, B200_POSITION_MAX_REACH), info.device);
+  if (rc == 0) rc = set_smem(dkv, AtDkv<HALVES>::smem(true, B200_POSITION_MAX_REACH), info.device);
+  if (rc != 0) return rc;
+  const bool table = p.table != nullptr;
+  TRIMUL_CUDA(launch_overlapped(attention_delta_kernel<T>, dim3(p.delta_blocks, p.kv_heads), kAtDeltaThreads, 0, stream, p));
+  TRIMUL_CUDA(launch_overlapped(dq, dim3(static_cast<unsigned>(p.places), p.heads), kAtBackThreads, AtDq<HALVES>::smem(table, p.reach), stream, maps, p));
+  TRIMUL_CUDA(launch_overlapped(dkv, dim3(static_cast<unsigned>(p.places), p.kv_heads), kAtBackThreads, AtDkv<HALVES>::smem(table, p.reach), stream, maps, p));
+  if (p.partial != nullptr)
+    TRIMUL_CUDA(launch_overlapped(p.wide_table ? attention_table_kernel<float> : attention_table_kernel<T>, dim3(p.heads), 1024, 0, stream, p));
+  return B200_TRIMUL_OK;
+}
 struct AttentionRegions {
-  size_t delta, partial, total;
+  size_t delta, most, partial, total;
 };
 static AttentionRegions attention_regions(const b200_attention_call* c) {
   AttentionRegions r;
   r.delta = 0;
-  r.partial = up(static_cast<size_t>(c->rows) * c->heads * 4, 1024);
-  r.total = r.partial + (c->table != nullptr ? up(static_cast<size_t>(c->heads) * attention_blocks(c->rows) * (2 * c->reach + 1) * 4, 1024) : 0);
+  r.most = up(static_cast<size_t>(c->rows) * c->heads * 4, 1024);
+  r.partial = r.most + up(static_cast<size_t>(c->kv_heads) * attention_delta_blocks(c->rows, c->d) * 8, 1024);
+  const size_t places = static_cast<size_t>(attention_places(c->offsets, c->rows, c->sequences, c->length, kAtTile));
+  r.total = r.partial + (c->table != nullptr ? up(places * c->heads * (2 * c->reach + 1) * 4, 1024) : 0);
   return r;
 }
 
@@ -242,18 +264,20 @@ int b200_token_attention_backward(const b200_attention_call* call, const b200_at
   p.dk = dk;
   p.dv = dv;
   p.dtable = dtable;
-  p.delta = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + regions.delta);
-  p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + regions.partial);
-  p.blocks = attention_blocks(p.rows);
-  const bool f16 = call->dtype == B200_BLOCKS_F16;
-  const int distances = (2 * p.reach + 1) * 4, warps = kAttentionWarps * 32;
-  const auto kernel = f16 ? attention_dq_kernel<__half> : attention_dq_kernel<__nv_bfloat16>;
-  TRIMUL_CUDA(launch_overlapped(kernel, dim3(p.blocks, p.heads), warps, p.table != nullptr ? kAttentionWarps * distances : 0, stream, p));
-  TRIMUL_CUDA(launch_overlapped(f16 ? attention_dkv_kernel<__half> : attention_dkv_kernel<__nv_bfloat16>, dim3(p.blocks, p.kv_heads), warps, 0, stream, p));
-  if (dtable != nullptr)
-    TRIMUL_CUDA(launch_overlapped(p.wide_table ? attention_table_kernel<float> : f16 ? attention_table_kernel<__half> : attention_table_kernel<__nv_bfloat16>,
-                                  dim3(p.heads), 256, distances, stream, p));
-  return B200_TRIMUL_OK;
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  p.delta = reinterpret_cast<float*>(ws + regions.delta);
+  p.most = reinterpret_cast<float*>(ws + regions.most);
+  p.partial = dtable != nullptr ? reinterpret_cast<float*>(ws + regions.partial) : nullptr;
+  p.places = attention_places(p.offsets, p.rows, p.sequences, p.length, kAtTile);
+  p.delta_blocks = attention_delta_blocks(p.rows, p.d);
+  AttentionMaps maps = {};
+  rc = attention_map(&maps.q, p.q, p.rows, p.heads, p.d);
+  if (rc == 0) rc = attention_map(&maps.k, p.k, p.rows, p.kv_heads, p.d);
+  if (rc == 0) rc = attention_map(&maps.v, p.v, p.rows, p.kv_heads, p.d);
+  if (rc == 0) rc = attention_map(&maps.dout, p.dout, p.rows, p.heads, p.d);
+  if (rc != 0) return rc;
+  if (call->dtype == B200_BLOCKS_F16) return p.d <= 64 ? launch_attention_backward<true, 1>(maps, p, info, stream) : launch_attention_backward<true, 2>(maps, p, info, stream);
+  return p.d <= 64 ? launch_attention_backward<false, 1>(maps, p, info, stream) : launch_attention_backward<false, 2>(maps, p, info, stream);
 }
 
 int b200_relative_position_forward(const void* z, const float* table, const void* index, const void* chain, const int* bucket_of, void* y,

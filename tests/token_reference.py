@@ -22,11 +22,12 @@ def attention(q, k, v, lengths, mask=None, causal=False, scale=None, table=None,
     dq is off by u |dq| + scale sum (u |ds| + p e) |k|, likewise dk; dv by u |dv| + u sum p |dO|; dtable by the sum of p e (and u |dtable|
     in 16 bits). What fp32 adds: scores are sums of d products and exponents of up to a few hundred, each to 2^-24 of their magnitude, so
     a probability to a relative (d + 8) 2^-24 (scale |q| . |k| + |bias| + 8); sums to (rows + d) 2^-24 of the sum of their magnitudes.
+    Below 2^-126 fp32 has no normal numbers and exp2 gives 0: a probability may be off by that much, and so may a product of it.
     """
     type, rows, heads, d = q.dtype, q.shape[0], q.shape[1], q.shape[2]
     group = heads // k.shape[1]
     scale = d**-0.5 if scale is None else scale
-    u, tiny, f32 = half_step(type), smallest(type), 2.0**-24
+    u, tiny, f32, lost = half_step(type), smallest(type), 2.0**-24, 2.0**-126
     r = {n: torch.zeros(t.shape, dtype=torch.float64, device=q.device) for n, t in (("o", q), ("q", q), ("k", k), ("v", v))}
     e = {n: torch.zeros_like(t) for n, t in r.items()}
     if table is not None:
@@ -59,7 +60,7 @@ def attention(q, k, v, lengths, mask=None, causal=False, scale=None, table=None,
         loss = (d + 8) * f32 * (size.masked_fill(~counts, 0.0) + 8)
         loss = loss + (loss * p).sum(-1, keepdim=True)
         o = p @ vs
-        p_off = p * (u + loss + m * f32)
+        p_off = p * (u + loss + m * f32) + lost
         r["o"][at] = o.transpose(0, 1)
         o_off = u * o.abs() + p_off @ vs.abs() * (1 + u) + m * f32 * (p @ vs.abs()) + tiny
         e["o"][at] = o_off.transpose(0, 1)
@@ -70,7 +71,7 @@ def attention(q, k, v, lengths, mask=None, causal=False, scale=None, table=None,
         dp_size = g.abs() @ vs.abs().transpose(1, 2)
         ds = p * (dp - delta)
         delta_off = (g.abs() * o_off).sum(-1, keepdim=True) + d * f32 * (g.abs() * o.abs()).sum(-1, keepdim=True)
-        exact_off = p * (delta_off + d * f32 * dp_size) + ds.abs() * (loss + m * f32)  # before ds is rounded
+        exact_off = p * (delta_off + d * f32 * dp_size) + ds.abs() * (loss + m * f32) + lost * (dp_size + delta.abs() + 1)  # before ds is rounded
         ds_off = exact_off * (1 + u) + u * ds.abs()
         sums = (m + 16) * f32
 
