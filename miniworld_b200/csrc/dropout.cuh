@@ -84,10 +84,18 @@ __device__ __forceinline__ T dropped(T x, T u, bool keep, float scale, bool resi
 }
 
 constexpr int kDropoutThreads = 256;
-constexpr int kDropoutRows = 4;  // rows in flight
+constexpr int kDropoutFlight = 4;  // pieces of eight elements that a thread loads at once
 
-// Eight mask elements a thread and, where rows share a mask, `chunk` rows under them: HBM bound, and near the issue limit where no
-// row shares (about 13 instructions an element, 5 of them the generator).
+// Eight elements under one mask group: y from x and u
+template <typename T, bool RESIDUAL>
+__device__ __forceinline__ void drop_eight(const DropoutParams& p, uint4 r, Eight<T>& x, Eight<T>& u, T* y) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u.at(i) = dropped(x.at(i), u.at(i), half_of(r, i) >= p.threshold, p.scale, RESIDUAL);
+  u.store(y);
+}
+
+// No rows share: a thread takes a few groups of eight elements and draws their numbers while the elements are on their way. HBM bound;
+// about 10 instructions an element, 5 of them the generator.
 template <typename T, bool RESIDUAL>
 __global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const DropoutParams p) {
   grid_dependency_wait();
@@ -96,34 +104,67 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const DropoutP
   const T* u = static_cast<const T*>(p.u);
   T* y = static_cast<T*>(p.y);
   const DropoutKey key(p);
-  const long long n = p.outer * p.inner, groups = (n + 7) / 8;
-  const long long first_row = static_cast<long long>(blockIdx.y) * p.chunk, last_row = min(p.shared, first_row + p.chunk);
-  for (long long g = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; g < groups; g += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const uint4 r = key.numbers(g);
-    const long long o = p.shared == 1 ? 0 : g * 8 / p.inner, base = g * 8 + o * (p.shared - 1) * p.inner;
-    if (g * 8 + 8 > n) {  // (one row under the mask: rows that share one come here with whole groups)
-      for (int i = 0; g * 8 + i < n; ++i)
-        y[g * 8 + i] = dropped(RESIDUAL ? __ldcg(x + g * 8 + i) : T(0.f), __ldcg(u + g * 8 + i), half_of(r, i) >= p.threshold, p.scale, RESIDUAL);
-      continue;
+  const long long n = p.outer * p.inner;
+  const long long first = static_cast<long long>(blockIdx.x) * (kDropoutThreads * kDropoutFlight) + threadIdx.x;
+  Eight<T> a[kDropoutFlight], b[kDropoutFlight];
+#pragma unroll
+  for (int q = 0; q < kDropoutFlight; ++q) {
+    const long long at = (first + q * kDropoutThreads) * 8;
+    if (at + 8 <= n) {
+      b[q].load(u + at);
+      if (RESIDUAL) a[q].load(x + at);
     }
-    for (long long s = first_row; s < last_row; s += kDropoutRows) {
-      Eight<T> a[kDropoutRows], b[kDropoutRows];
+  }
 #pragma unroll
-      for (int q = 0; q < kDropoutRows; ++q)
-        if (s + q < last_row) {
-          b[q].load(u + base + (s + q) * p.inner);
-          if (RESIDUAL) a[q].load(x + base + (s + q) * p.inner);
-        }
-#pragma unroll
-      for (int q = 0; q < kDropoutRows; ++q)
-        if (s + q < last_row) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) b[q].at(i) = dropped(a[q].at(i), b[q].at(i), half_of(r, i) >= p.threshold, p.scale, RESIDUAL);
-          b[q].store(y + base + (s + q) * p.inner);
-        }
+  for (int q = 0; q < kDropoutFlight; ++q) {
+    const long long g = first + q * kDropoutThreads, at = g * 8;
+    if (at >= n) break;
+    const uint4 r = key.numbers(g);
+    if (at + 8 <= n) {
+      drop_eight<T, RESIDUAL>(p, r, a[q], b[q], y + at);
+    } else {
+      for (int i = 0; at + i < n; ++i)
+        y[at + i] = dropped(RESIDUAL ? __ldcg(x + at + i) : T(0.f), __ldcg(u + at + i), half_of(r, i) >= p.threshold, p.scale, RESIDUAL);
     }
   }
 }
+
+// Rows share a mask and have whole groups of eight: a thread draws a group's numbers once for `chunk` rows.
+template <typename T, bool RESIDUAL>
+__global__ void __launch_bounds__(kDropoutThreads) dropout_shared_kernel(const DropoutParams p) {
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const T* x = static_cast<const T*>(p.x);
+  const T* u = static_cast<const T*>(p.u);
+  T* y = static_cast<T*>(p.y);
+  const DropoutKey key(p);
+  const long long g = static_cast<long long>(blockIdx.x) * kDropoutThreads + threadIdx.x;
+  if (g * 8 >= p.outer * p.inner) return;
+  const long long base = g * 8 + g * 8 / p.inner * (p.shared - 1) * p.inner;
+  long long s = static_cast<long long>(blockIdx.y) * p.chunk;
+  const long long last = min(p.shared, s + p.chunk);
+  Eight<T> a[kDropoutFlight], b[kDropoutFlight];
+  auto fetch = [&]() {
+#pragma unroll
+    for (int q = 0; q < kDropoutFlight; ++q)
+      if (s + q < last) {
+        b[q].load(u + base + (s + q) * p.inner);
+        if (RESIDUAL) a[q].load(x + base + (s + q) * p.inner);
+      }
+  };
+  fetch();
+  const uint4 r = key.numbers(g);
+  while (true) {
+#pragma unroll
+    for (int q = 0; q < kDropoutFlight; ++q)
+      if (s + q < last) drop_eight<T, RESIDUAL>(p, r, a[q], b[q], y + base + (s + q) * p.inner);
+    s += kDropoutFlight;
+    if (s >= last) break;
+    fetch();
+  }
+}
+
+constexpr int kDropoutSingles = 8;  // rows in flight
 
 // The same where rows of an odd width share a mask or a tensor does not start on 16 bytes: one mask element a thread.
 template <typename T, bool RESIDUAL>
@@ -139,16 +180,16 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_single_kernel(const D
   for (long long e = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; e < n; e += static_cast<long long>(gridDim.x) * blockDim.x) {
     const bool keep = half_of(key.numbers(e / 8), static_cast<int>(e & 7)) >= p.threshold;
     const long long base = e + e / p.inner * (p.shared - 1) * p.inner;
-    for (long long s = first_row; s < last_row; s += 2 * kDropoutRows) {
-      T a[2 * kDropoutRows], b[2 * kDropoutRows];
+    for (long long s = first_row; s < last_row; s += kDropoutSingles) {
+      T a[kDropoutSingles], b[kDropoutSingles];
 #pragma unroll
-      for (int q = 0; q < 2 * kDropoutRows; ++q)
+      for (int q = 0; q < kDropoutSingles; ++q)
         if (s + q < last_row) {
           b[q] = __ldcg(u + base + (s + q) * p.inner);
           a[q] = RESIDUAL ? __ldcg(x + base + (s + q) * p.inner) : T(0.f);
         }
 #pragma unroll
-      for (int q = 0; q < 2 * kDropoutRows; ++q)
+      for (int q = 0; q < kDropoutSingles; ++q)
         if (s + q < last_row) y[base + (s + q) * p.inner] = dropped(a[q], b[q], keep, p.scale, RESIDUAL);
     }
   }

@@ -3,6 +3,9 @@
 // Gradient of the table: the sum of dy over the pairs of each bucket; dz is dy.
 #pragma once
 
+#include <type_traits>
+
+#include "../../include/b200_tokens.h"
 #include "ptx.cuh"
 
 namespace trimul {
@@ -19,6 +22,9 @@ struct PositionParams {
   int b, n, c, buckets, reach;
   bool wide;            // index and chain are 64-bit
   int chunks, blocks;   // backward: pieces of kPositionChunk channels, blocks of each
+  int cells;            // forward: cells of a tile
+  uint32_t magic;       // ceil(2^32 / pieces of a cell)
+  bool table_in_smem;
 };
 
 // index and chain of token j of sample b
@@ -33,7 +39,7 @@ __device__ __forceinline__ longlong2 position_token(const PositionParams& p, lon
   }
   return t;
 }
-__device__ __forceinline__ int position_bucket(const PositionParams& p, longlong2 i, longlong2 j) {
+__device__ __forceinline__ int position_bucket(const PositionParams& p, const int* bucket_of, longlong2 i, longlong2 j) {
   if (i.y != j.y) return p.buckets - 1;
   // (the difference of any two 64-bit indices: compared before it could wrap)
   const long long reach = p.reach;
@@ -42,7 +48,11 @@ __device__ __forceinline__ int position_bucket(const PositionParams& p, longlong
     d = static_cast<unsigned long long>(j.x) - static_cast<unsigned long long>(i.x) > static_cast<unsigned long long>(reach) ? reach : j.x - i.x;
   else
     d = static_cast<unsigned long long>(i.x) - static_cast<unsigned long long>(j.x) > static_cast<unsigned long long>(reach) ? -reach : j.x - i.x;
-  return min(max(__ldcg(p.bucket_of + d + reach), 0), p.buckets - 1);
+  return bucket_of[d + reach];
+}
+// the buckets of all distances, brought into the table's range
+__device__ __forceinline__ void position_buckets(const PositionParams& p, int* bucket_of) {
+  for (int i = threadIdx.x; i < 2 * p.reach + 1; i += blockDim.x) bucket_of[i] = min(max(__ldcg(p.bucket_of + i), 0), p.buckets - 1);
 }
 
 template <typename T, int V>
@@ -64,53 +74,133 @@ __device__ __forceinline__ Piece<T, V> load_piece(const T* p) {
   return r;
 }
 
-constexpr int kPositionThreads = 256;
+// v += t, rounded once
+template <typename T, int Q>
+__device__ __forceinline__ void add_piece(T* v, const Piece<float, Q>& t) {
+  if constexpr (sizeof(T) == 2 && Q >= 2) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+    for (int e = 0; e < Q; e += 2) {
+      constexpr bool f16 = std::is_same_v<T, __half>;
+      const float2 s = __fadd2_rn(f16 ? f16x2_to_float2(w[e / 2]) : bf16x2_to_float2(w[e / 2]), make_float2(t.v[e], t.v[e + 1]));
+      w[e / 2] = f16 ? pack_f16x2(s) : pack_bf16x2(s);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < Q; ++e) v[e] = static_cast<T>(static_cast<float>(v[e]) + t.v[e]);
+  }
+}
 
-// HBM bound. A block walks rows (b, i); threads take pieces of V channels of neighbouring cells.
+constexpr int kPositionThreads = 256;
+constexpr int kPositionMostCells = 512;
+constexpr int kPositionFlight = 4;  // pieces of V channels that a thread loads at once
+
+// HBM bound. A block takes tiles of consecutive cells (b, i, j), whatever rows they are of: the buckets of a tile first (a thread a cell,
+// loads for the next tile while this one streams), then its pieces of V channels. The table lies in shared memory, the floats of a piece
+// a quarter-warp's stride apart, so that neighbouring lanes read neighbouring words.
 template <typename T, int V>
 __global__ void __launch_bounds__(kPositionThreads) position_forward_kernel(const PositionParams p) {
+  extern __shared__ float4 table_smem[];
+  __shared__ int bucket_of[2 * B200_POSITION_MAX_REACH + 1];
+  __shared__ int buckets[2][kPositionMostCells];
   grid_dependency_wait();
   grid_dependents_launch();
   const T* z = static_cast<const T*>(p.z);
   T* y = static_cast<T*>(p.y);
+  float* const table = reinterpret_cast<float*>(table_smem);
+  constexpr int Q = V < 4 ? V : 4, QUADS = V / Q;  // floats read at once, and how often for a piece
   const int pieces = p.c / V;
-  const long long rows = static_cast<long long>(p.b) * p.n, row_pieces = static_cast<long long>(p.n) * pieces;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const longlong2 ti = position_token(p, row);
-    const long long sample = row / p.n * p.n;
-    for (long long q = static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x; q < row_pieces; q += static_cast<long long>(gridDim.y) * blockDim.x) {
-      const int j = static_cast<int>(q / pieces), c = static_cast<int>(q - static_cast<long long>(j) * pieces) * V;
-      Piece<T, V> v = load_piece<T, V>(z + (row * p.n + j) * p.c + c);
-      const float* t = p.table + static_cast<long long>(position_bucket(p, ti, position_token(p, sample + j))) * p.c + c;
+  position_buckets(p, bucket_of);
+  if (p.table_in_smem) {
+    const int row_quads = pieces * QUADS;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.buckets * row_quads; i += kPositionThreads) {
+      const int row = i / row_quads, at = i - row * row_quads, d = at / pieces, piece = at - d * pieces;
+      *reinterpret_cast<Piece<float, Q>*>(table + static_cast<long long>(i) * Q) = load_piece<float, Q>(p.table + row * p.c + piece * V + d * Q);
+    }
+  }
+  __syncthreads();
+  const long long cells = static_cast<long long>(p.b) * p.n * p.n, tiles = (cells + p.cells - 1) / p.cells;
+  auto bucket_at = [&](long long cell) {
+    const long long row = cell / p.n;  // (b, i)
+    const long long j = cell - row * p.n, sample = row / p.n;
+    return position_bucket(p, bucket_of, position_token(p, row), position_token(p, sample * p.n + j));
+  };
+  int next[2];
+  auto look = [&](long long tile) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) v.v[e] = static_cast<T>(static_cast<float>(v.v[e]) + __ldcg(t + e));
-      *reinterpret_cast<Piece<T, V>*>(y + (row * p.n + j) * p.c + c) = v;
+    for (int k = 0; k < 2; ++k) {
+      const int i = threadIdx.x + k * kPositionThreads;
+      const long long cell = tile * p.cells + i;
+      next[k] = i < p.cells && cell < cells ? bucket_at(cell) : 0;
+    }
+  };
+  look(blockIdx.x);
+  int turn = 0;
+  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (threadIdx.x + k * kPositionThreads < p.cells) buckets[turn][threadIdx.x + k * kPositionThreads] = next[k];
+    __syncthreads();  // (the other buffer was read before the barrier of the tile before)
+    const int count = static_cast<int>(min(static_cast<long long>(p.cells), cells - tile * p.cells)) * pieces;
+    const T* from = z + tile * p.cells * p.c;
+    T* to = y + tile * p.cells * p.c;
+    bool looked = false;
+    for (int q0 = threadIdx.x; q0 < count || !looked; q0 += kPositionFlight * kPositionThreads) {
+      Piece<T, V> v[kPositionFlight];
+#pragma unroll
+      for (int k = 0; k < kPositionFlight; ++k)
+        if (q0 + k * kPositionThreads < count) v[k] = load_piece<T, V>(from + static_cast<long long>(q0 + k * kPositionThreads) * V);
+      if (!looked) {
+        if (tile + gridDim.x < tiles) look(tile + gridDim.x);
+        looked = true;
+      }
+#pragma unroll
+      for (int k = 0; k < kPositionFlight; ++k) {
+        const int q = q0 + k * kPositionThreads;
+        if (q >= count) break;
+        const int cell = p.magic == 0 ? q : static_cast<int>(__umulhi(static_cast<uint32_t>(q), p.magic)), piece = q - cell * pieces;
+        const int row = buckets[turn][cell];
+#pragma unroll
+        for (int d = 0; d < QUADS; ++d) {
+          const Piece<float, Q> t = p.table_in_smem ? *reinterpret_cast<const Piece<float, Q>*>(table + row * p.c + (d * pieces + piece) * Q)
+                                                    : load_piece<float, Q>(p.table + row * p.c + piece * V + d * Q);
+          add_piece<T, Q>(v[k].v + d * Q, t);
+        }
+        *reinterpret_cast<Piece<T, V>*>(to + static_cast<long long>(q) * V) = v[k];
+      }
     }
   }
 }
 
 constexpr int kPositionChunk = 64;  // channels of a warp: two a lane
-constexpr int kPositionRun = 32;    // positions that a warp looks at together
+constexpr int kPositionWarps = 13;  // tables of sums of 66 buckets that fit into shared memory
 
-// Sums over the buckets, in fixed orders: a warp owns 64 channels of a run of positions and a table of sums in shared memory; it adds
-// up neighbouring positions of one bucket in registers (most pairs are far apart and share the outer two). The block adds its warps'
-// tables up, and position_sums_kernel the blocks'.
+// Sums over the buckets, in fixed orders: a warp owns 64 channels and a run of positions, of which it has 32 (fp32: 16) on their way while
+// it adds up as many before them. Neighbouring positions of one bucket are added up in registers (most pairs are far apart and share the
+// outer two), others in the warp's table in shared memory. The block adds its warps' tables up, and position_sums_kernel the blocks'.
 template <typename T, int V>
-__global__ void position_backward_kernel(const PositionParams p) {
-  extern __shared__ float sums[];  // [warps][buckets][kPositionChunk]
+__global__ void __launch_bounds__(kPositionWarps * 32, 1) position_backward_kernel(const PositionParams p) {
+  constexpr int R = sizeof(T) == 2 ? 32 : 16;  // positions that a warp looks at together
+  extern __shared__ float4 sums_smem[];
+  __shared__ int bucket_of[2 * B200_POSITION_MAX_REACH + 1];
+  float* const sums = reinterpret_cast<float*>(sums_smem);  // [warps][buckets][kPositionChunk]
   grid_dependency_wait();
   grid_dependents_launch();
   const T* dy = static_cast<const T*>(p.dy);
   const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int table = p.buckets * kPositionChunk;
-  for (int i = threadIdx.x; i < warps * table; i += blockDim.x) sums[i] = 0.f;
+  for (int i = threadIdx.x; i < warps * table / 4; i += blockDim.x) sums_smem[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  position_buckets(p, bucket_of);
   __syncthreads();
   const int chunk = blockIdx.x % p.chunks, block = blockIdx.x / p.chunks;
-  float* own = sums + warp * table + lane * 2;
-  const int c = chunk * kPositionChunk + lane * 2;
-  const int runs = (p.n + kPositionRun - 1) / kPositionRun;  // of a row
+  float* const own = sums + warp * table + lane * 2;
+  // a lane without a channel of its own (or with one) reads the last ones again and writes them to columns that nobody reads
+  const int c = min(chunk * kPositionChunk + lane * 2, p.c - V);
+  const bool second = V == 1 && c + 1 < p.c;
+  const int runs = (p.n + R - 1) / R;  // of a row
   const long long units = static_cast<long long>(p.b) * p.n * runs, teams = static_cast<long long>(p.blocks) * warps;
-  const long long team = static_cast<long long>(block) * warps + warp;
+  const long long team = static_cast<long long>(block) * warps + warp, last = units * (team + 1) / teams;
   float2 sum = make_float2(0.f, 0.f);
   int run = -1;
   auto flush = [&]() {
@@ -121,41 +211,90 @@ __global__ void position_backward_kernel(const PositionParams p) {
     }
     sum = make_float2(0.f, 0.f);
   };
-  auto value = [&](const T* at) {  // two channels of a position
-    float2 v = make_float2(0.f, 0.f);
-    if constexpr (V == 2) {
-      if (c < p.c) {
-        const Piece<T, 2> w = load_piece<T, 2>(at + c);
-        v = make_float2(static_cast<float>(w.v[0]), static_cast<float>(w.v[1]));
-      }
-    } else {
-      if (c < p.c) v.x = static_cast<float>(load_piece<T, 1>(at + c).v[0]);
-      if (c + 1 < p.c) v.y = static_cast<float>(load_piece<T, 1>(at + c + 1).v[0]);
-    }
-    return v;
+  using Word = std::conditional_t<sizeof(T) == 2, uint32_t, uint2>;  // two channels of a position
+  struct Unit {
+    Word v[R];
+    int bucket;
   };
-  const long long last = units * (team + 1) / teams;
-  for (long long unit = units * team / teams; unit < last; ++unit) {
+  auto values = [](Word w) {
+    if constexpr (sizeof(T) == 4)
+      return make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+    else if constexpr (std::is_same_v<T, __half>)
+      return f16x2_to_float2(w);
+    else
+      return bf16x2_to_float2(w);
+  };
+  auto fetch = [&](long long unit, Unit& u) {
     const long long row = unit / runs;
-    const int j0 = static_cast<int>(unit - row * runs) * kPositionRun, count = min(kPositionRun, p.n - j0);
-    int bucket = -1;
-    if (lane < count) bucket = position_bucket(p, position_token(p, row), position_token(p, row / p.n * p.n + j0 + lane));
-    const T* at = dy + (row * p.n + j0) * p.c;
-    float2 v[kPositionRun];
+    const int j0 = static_cast<int>(unit - row * runs) * R, most = p.n - 1 - j0;
+    const T* at = dy + (row * p.n + j0) * p.c + c;
 #pragma unroll
-    for (int i = 0; i < kPositionRun; ++i)
-      if (i < count) v[i] = value(at + static_cast<long long>(i) * p.c);
+    for (int i = 0; i < R; ++i) {
+      const T* from = at + static_cast<long long>(min(i, most)) * p.c;  // (positions past the row's end: its last, not added)
+      if constexpr (V == 2) {
+        u.v[i] = __ldcg(reinterpret_cast<const Word*>(from));
+      } else if constexpr (sizeof(T) == 4) {
+        u.v[i] = make_uint2(__ldcg(reinterpret_cast<const uint32_t*>(from)), second ? __ldcg(reinterpret_cast<const uint32_t*>(from) + 1) : 0u);
+      } else {
+        const unsigned short* at16 = reinterpret_cast<const unsigned short*>(from);
+        u.v[i] = __ldcg(at16) | (second ? static_cast<uint32_t>(__ldcg(at16 + 1)) << 16 : 0u);
+      }
+    }
+  };
+  // its tokens, a lane a position, are asked for a unit before that, and their buckets found after the work on the unit between
+  longlong2 mine, other;
+  auto ask = [&](long long unit) {
+    const long long row = unit / runs;
+    const int j0 = static_cast<int>(unit - row * runs) * R;
+    mine = position_token(p, row);
+    other = position_token(p, row / p.n * p.n + min(j0 + lane, p.n - 1));
+  };
+  auto find = [&](long long unit) {
+    const int j = static_cast<int>(unit % runs) * R + lane;
+    return lane < R && j < p.n ? position_bucket(p, bucket_of, mine, other) : -1;
+  };
+  auto add = [&](const Unit& u) {
+    const int bucket = __shfl_sync(0xFFFFFFFFu, u.bucket, 0);
+    if (__all_sync(0xFFFFFFFFu, u.bucket == bucket || lane >= R)) {
+      if (bucket != run) {
+        flush();
+        run = bucket;
+      }
 #pragma unroll
-    for (int i = 0; i < kPositionRun; ++i) {
-      if (i >= count) break;
-      const int b = __shfl_sync(0xFFFFFFFFu, bucket, i);
+      for (int i = 0; i < R; ++i) {
+        sum = __fadd2_rn(sum, values(u.v[i]));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int b = __shfl_sync(0xFFFFFFFFu, u.bucket, i);
       if (b != run) {
         flush();
         run = b;
       }
-      sum.x += v[i].x;
-      sum.y += v[i].y;
+      // (run -1: past the row's end; the sum is dropped)
+      sum = __fadd2_rn(sum, values(u.v[i]));
     }
+  };
+  const long long begin = units * team / teams;
+  Unit a, b;
+  if (begin < last) {
+    fetch(begin, a);
+    ask(begin);
+    a.bucket = find(begin);
+    if (begin + 1 < last) ask(begin + 1), b.bucket = find(begin + 1);
+  }
+  auto step = [&](long long unit, Unit& now, Unit& next) {
+    if (unit + 1 < last) fetch(unit + 1, next);
+    const bool more = unit + 2 < last;
+    if (more) ask(unit + 2);
+    add(now);
+    if (more) now.bucket = find(unit + 2);
+  };
+  for (long long unit = begin; unit < last; unit += 2) {
+    step(unit, a, b);
+    if (unit + 1 < last) step(unit + 1, b, a);
   }
   flush();
   __syncthreads();

@@ -136,17 +136,17 @@ static int check_position(int b, int n, int c, int buckets) {
   if (buckets > B200_POSITION_MAX_BUCKETS || c > B200_NORM_MAX_WIDTH) return B200_TRIMUL_E_UNSUPPORTED;
   return static_cast<long long>(b) * n > 0x7FFFFFFFll || static_cast<double>(b) * n * n * c > 0x1p40 ? B200_TRIMUL_E_SHAPE : B200_TRIMUL_OK;
 }
-constexpr size_t kPositionSmem = 200 * 1024;
+constexpr size_t kPositionSmem = 220 * 1024;
 struct PositionGrid {
   int warps, chunks, blocks;
 };
-// As many warps to a block as tables of sums fit into shared memory, up to 13 (two blocks of less do not hold more); blocks: one an SM
-// in all chunks together, and no more than there is work for.
+// As many warps to a block as tables of sums fit into shared memory, up to 13; blocks: one an SM in all chunks together, and no more than
+// there is work for.
 static PositionGrid position_grid(int b, int n, int c, int buckets, int sms) {
   PositionGrid g;
-  g.warps = static_cast<int>(std::min<size_t>(13, kPositionSmem / (static_cast<size_t>(buckets) * kPositionChunk * 4)));
+  g.warps = static_cast<int>(std::min<size_t>(kPositionWarps, kPositionSmem / (static_cast<size_t>(buckets) * kPositionChunk * 4)));
   g.chunks = static_cast<int>(blocks_for(c, kPositionChunk));
-  const long long units = static_cast<long long>(b) * n * blocks_for(n, kPositionRun);
+  const long long units = static_cast<long long>(b) * n * blocks_for(n, 32);
   g.blocks = static_cast<int>(std::max<long long>(1, std::min<long long>(std::max(1, sms / g.chunks), blocks_for(units, g.warps))));
   return g;
 }
@@ -155,17 +155,33 @@ static size_t position_bytes(const PositionGrid& g, int buckets) {
 }
 
 template <typename T, int V>
-static int launch_position_forward(const PositionParams& p, const DeviceInfo& info, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(p.b) * p.n, pieces = static_cast<long long>(p.n) * (p.c / V);
-  const int y = static_cast<int>(std::min<long long>(blocks_for(pieces, kPositionThreads), 64));
-  const int x = static_cast<int>(std::min<long long>(rows, std::max<long long>(1, 64ll * info.sms / y)));
-  TRIMUL_CUDA(launch_overlapped(position_forward_kernel<T, V>, dim3(x, y), kPositionThreads, 0, stream, p));
+static int launch_position_forward(PositionParams p, const DeviceInfo& info, cudaStream_t stream) {
+  const long long cells = static_cast<long long>(p.b) * p.n * p.n;
+  const int pieces = p.c / V;
+  // tiles of about 64 KB, smaller where that leaves SMs without one
+  long long tile = std::max<long long>(1, std::min<long long>(kPositionMostCells, 65536 / (static_cast<long long>(p.c) * sizeof(T))));
+  while (tile > 8 && blocks_for(cells, tile) < 4ll * info.sms) tile /= 2;
+  p.cells = static_cast<int>(tile);
+  p.magic = pieces == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + pieces - 1) / pieces);
+  // the table in shared memory where a block reads it often enough to have it copied
+  const size_t table = static_cast<size_t>(p.buckets) * p.c * 4;
+  p.table_in_smem = table <= 100 * 1024 && cells / (4 * info.sms) > 2 * p.buckets;
+  const int smem = p.table_in_smem ? static_cast<int>(table) : 0;
+  const int per_sm = table <= 50 * 1024 || !p.table_in_smem ? 4 : 2;
+  const auto kernel = position_forward_kernel<T, V>;
+  const int rc = set_smem(kernel, 100 * 1024, info.device);
+  if (rc != 0) return rc;
+  TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(std::min<long long>(blocks_for(cells, tile), per_sm * info.sms))), kPositionThreads, smem, stream, p));
   return B200_TRIMUL_OK;
 }
 template <typename T>
 static int position_forward(const PositionParams& p, const DeviceInfo& info, cudaStream_t stream) {
   constexpr int kWhole = 16 / sizeof(T);
-  if (p.c % kWhole == 0 && all_aligned16({p.z, p.y})) return launch_position_forward<T, kWhole>(p, info, stream);
+  auto fits = [&](int v) { return p.c % v == 0 && aligned(p.z, v * sizeof(T)) && aligned(p.y, v * sizeof(T)) && aligned(p.table, std::min(v, 4) * 4); };
+  if (fits(kWhole)) return launch_position_forward<T, kWhole>(p, info, stream);
+  if (fits(kWhole / 2)) return launch_position_forward<T, kWhole / 2>(p, info, stream);
+  if constexpr (kWhole / 4 > 1)
+    if (fits(kWhole / 4)) return launch_position_forward<T, kWhole / 4>(p, info, stream);
   return launch_position_forward<T, 1>(p, info, stream);
 }
 template <typename T>
@@ -182,15 +198,21 @@ static int position_backward(const PositionParams& p, const PositionGrid& g, con
 // ---------------------------------------------------------------- dropout
 template <typename T>
 static int dropout(DropoutParams p, const DeviceInfo& info, cudaStream_t stream) {
-  const bool whole = all_aligned16({p.x, p.u, p.y}) && (p.shared == 1 || p.inner % 8 == 0);
-  const long long threads = whole ? blocks_for(p.outer * p.inner, 8) : p.outer * p.inner;
-  // rows that share a mask are cut into runs until there are enough threads to fill the GPU
-  const long long want = 2048ll * info.sms;
-  p.chunk = std::max<long long>(std::min<long long>(p.shared, 8), blocks_for(p.shared * threads, want));
+  const bool residual = p.x != nullptr, whole = all_aligned16({p.x, p.u, p.y});
+  const long long n = p.outer * p.inner, groups = blocks_for(n, 8);
+  if (whole && p.shared == 1) {
+    const auto kernel = residual ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+    TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks_for(groups, kDropoutThreads * kDropoutFlight))), kDropoutThreads, 0, stream, p));
+    return B200_TRIMUL_OK;
+  }
+  const bool eights = whole && p.inner % 8 == 0;
+  const long long threads = eights ? groups : n;
+  // rows that share a mask are cut into runs, as long as there are enough threads to fill the GPU
+  p.chunk = std::max<long long>(std::min<long long>(p.shared, 8), blocks_for(p.shared * threads, 2048ll * info.sms));
   p.chunk = std::max(p.chunk, blocks_for(p.shared, 65535));
   const dim3 grid(static_cast<unsigned>(std::min<long long>(blocks_for(threads, kDropoutThreads), 1 << 30)), static_cast<unsigned>(blocks_for(p.shared, p.chunk)));
-  void (*kernel)(DropoutParams) = whole ? (p.x != nullptr ? dropout_kernel<T, true> : dropout_kernel<T, false>)
-                                        : (p.x != nullptr ? dropout_single_kernel<T, true> : dropout_single_kernel<T, false>);
+  void (*kernel)(DropoutParams) = eights ? (residual ? dropout_shared_kernel<T, true> : dropout_shared_kernel<T, false>)
+                                         : (residual ? dropout_single_kernel<T, true> : dropout_single_kernel<T, false>);
   TRIMUL_CUDA(launch_overlapped(kernel, grid, kDropoutThreads, 0, stream, p));
   return B200_TRIMUL_OK;
 }
