@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
         if (!dirty(j)) continue;
         const int s = C::key_stage(j);
         uint32_t bits[4];
-        attention_rows_there(p, place, length, j, bits);
+        attention_rows_there(p, place, length, j * kAtTile, bits);
         if (!mbar_wait_warp(landed(s), odd >> s & 1u, abort_flag, status, kDevTimeoutStats)) break;
         odd ^= 1u << s;
         attention_clean_rows(ring + s * C::kStageBytes, HALVES, bits);
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int col0 = half * 64 + i * 32, left = limit - col0;
-        const uint32_t counts = bits[half * 2 + i] & (left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u);
+        const uint32_t counts = bits[half * 2 + i] & first_bits(left);
         uint32_t w[16];
         float2 total = make_float2(0.f, 0.f), mass = make_float2(0.f, 0.f);
 #pragma unroll
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
         const int tile = first_tile + u % tiles;
         if (!dirty(tile)) continue;
         uint32_t bits[4];
-        attention_rows_there(p, place, length, tile, bits);
+        attention_rows_there(p, place, length, tile * kAtTile, bits);
         bool ok = true;
         for (int i = 2 * u; i < 2 * u + 2 && ok; ++i) {
           const int s = i % ST;

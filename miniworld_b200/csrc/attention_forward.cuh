@@ -20,15 +20,17 @@ struct AtForward {
   static constexpr int kTiles = HALVES;                 // query tiles of a block
   static constexpr bool kOver = HALVES == 2;            // probabilities over the scores
   static constexpr int kStages = HALVES == 1 ? 5 : 4;   // of key and value tiles
-  static constexpr int kSoftmaxWarps = 4 * kTiles;
+  static constexpr int kSoftmaxWarps = 8 * kTiles;
   static constexpr int kThreads = kSoftmaxWarps * 32 + 128;
   static constexpr int kBlocks = HALVES == 1 ? 2 : 1;   // an SM
-  // registers: the launch's are kThreads * 128 or 168; the softmax's warps take from the others
-  static constexpr int kMany = HALVES == 1 ? 200 : 208, kFew = HALVES == 1 ? 56 : 88;
+  // registers: the launch's are 80 or 96; the softmax's warps take from the others (2 x 104 + 32 = 3 x 80, 4 x 104 + 64 = 5 x 96)
+  static constexpr int kMany = 104, kFew = HALVES == 1 ? 32 : 64;
   static constexpr uint32_t kColumns = HALVES == 1 ? 256 : 512;
   static constexpr int kStageBytes = HALVES * kAtTileBytes;
-  static constexpr int kFixed = kTiles * HALVES * kAtTileBytes + kStages * kStageBytes + 256 /* barriers */ + 64 /* place */;
-  static int smem(int reach) { return 1024 + kFixed + attention_bias_entries(reach) * 4; }
+  static constexpr int kBars = kTiles * HALVES * kAtTileBytes + kStages * kStageBytes;
+  static constexpr int kSwap = kBars + 320;             // what the two threads of a row tell each other
+  static constexpr int kBias = kSwap + kTiles * 2 * kAtTile * 4;
+  static int smem(bool table, int reach) { return 1024 + kBias + (table ? attention_bias_entries(reach) * 4 : 0); }
   __host__ __device__ static constexpr uint32_t scores(int t) { return static_cast<uint32_t>(t) * 128; }
   __host__ __device__ static constexpr uint32_t probabilities(int t) { return kOver ? static_cast<uint32_t>(t) * 128 : 128u; }
   __host__ __device__ static constexpr uint32_t out(int t) { return kOver ? 256u + static_cast<uint32_t>(t) * 128 : 192u; }
@@ -42,7 +44,7 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t q_s = base, ring = q_s + T * HALVES * kAtTileBytes, bars = ring + ST * C::kStageBytes;
+  const uint32_t q_s = base, ring = q_s + T * HALVES * kAtTileBytes, bars = base + C::kBars;
   auto landed = [&](int s) { return bars + 8u * s; };          // a copy has landed, rows of it are still to be zeroed
   auto ready = [&](int s) { return bars + 8u * (ST + s); };    // the tile can be used
   auto empty = [&](int s) { return bars + 8u * (2 * ST + s); };
@@ -53,11 +55,12 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
   auto probs_ready = [&](int t) { return bars + 8u * (B0 + 1 + 2 * T + t); };
   auto out_done = [&](int t) { return bars + 8u * (B0 + 1 + 3 * T + t); };
   static_assert(8 * (B0 + 1 + 4 * T) <= 240, "barriers");
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + (bars - base) + 240);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBars + 240);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* const status = &tokens_status;
-  AttentionPlace* const place_s = reinterpret_cast<AttentionPlace*>(smem + (bars - base) + 256);
-  float* const bias = reinterpret_cast<float*>(smem + (bars - base) + 320);
+  AttentionPlace* const place_s = reinterpret_cast<AttentionPlace*>(smem + C::kBars + 256);
+  float* const swap = reinterpret_cast<float*>(smem + C::kSwap);  // [query tile][half][row]
+  float* const bias = reinterpret_cast<float*>(smem + C::kBias);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int load_warp = C::kSoftmaxWarps, mma_warp = load_warp + 1, clean_warp = load_warp + 2;
@@ -70,8 +73,8 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
     mbar_init(q_ready, 1);
     for (int t = 0; t < T; ++t) {
       mbar_init(scores_ready(t), 1);
-      mbar_init(scores_read(t), 4);
-      mbar_init(probs_ready(t), 4);
+      mbar_init(scores_read(t), 8);
+      mbar_init(probs_ready(t), 8);
       mbar_init(out_done(t), 1);
     }
     *abort_flag = 0;
@@ -100,8 +103,8 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
   auto tiles_of = [&](int t) {
     const long long q0 = (static_cast<long long>(place.tile) * T + t) * kAtTile;
     if (place.behind || q0 >= length) return 0;
-    const int all = (length + kAtTile - 1) / kAtTile;
-    return p.causal ? static_cast<int>(min(q0 / kAtTile + 1, static_cast<long long>(all))) : all;
+    const int keys = p.causal ? static_cast<int>(min(q0 + kAtTile, static_cast<long long>(length))) : length;
+    return (keys + kAtTile - 1) / kAtTile;
   };
   const int n0 = tiles_of(0), n1 = T == 2 ? tiles_of(T - 1) : 0, n = max(n0, n1);
   // places in the order of use: scores of the next tile come before the sum of this one where they have columns of their own
@@ -117,9 +120,8 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
         if ((t == 0 ? n0 : n1) > 0)
           for (int h = 0; h < HALVES; ++h)
             tma_load_3d(q_s + (t * HALVES + h) * kAtTileBytes, &maps.q, q_ready, h * 64, head, static_cast<int>(place.first) + (place.tile * T + t) * kAtTile);
-      int i = 0;
       AttentionRing state;
-      for (; i < 2 * n; ++i) {
+      for (int i = 0; i < 2 * n; ++i) {
         // which tile is next
         bool value;
         int j;
@@ -147,6 +149,7 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
       const uint32_t idesc_o = umma_idesc(128, steps * 16, false, true, fmt, fmt);
       bool ok = n > 0 && mbar_wait(q_ready, 0, abort_flag, status, kDevTimeoutMma);
       auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && mbar_wait(bar, parity & 1u, abort_flag, status, kDevTimeoutMma); };
+      // (products are carried out in the order of their issue: scores go over the last tile's probabilities after these have been used)
       auto form_scores = [&](int t, int j, bool first, bool last) {
         const int i = key_place(j), s = i % ST;
         if (first) wait(ready(s), i / ST);
@@ -165,39 +168,29 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
         wait(probs_ready(t), j);
         if (!ok) return;
         tc_fence_after();
-        const int keys = min(kAtTile, length - j * kAtTile), key_steps = 2 * ((keys + 31) / 32);  // (probabilities come in pieces of 32)
+        const int key_steps = 2 * ((min(kAtTile, length - j * kAtTile) + 31) / 32);  // (probabilities come in pieces of 32)
         for (int ks = 0; ks < key_steps; ++ks)
           umma_ta(tmem + C::out(t), tmem + C::probabilities(t) + ks * 8, umma_desc_mnmajor(ring + s * C::kStageBytes + ks * 2048, kAtTileBytes), idesc_o,
                   (j | ks) != 0 ? 1u : 0u);
         umma_commit(out_done(t));
         if (last) umma_commit(empty(s));
       };
-      if (T == 1) {
-        if (ok) form_scores(0, 0, true, true);
-        for (int j = 0; j < n && ok; ++j) {
-          if (j + 1 < n) form_scores(0, j + 1, true, true);
-          if (ok) add_values(0, j, true, true);
-        }
-      } else {
-        const bool two = n1 > 0;
-        if (ok) form_scores(0, 0, true, !two);
-        if (ok && two) form_scores(1, 0, false, true);
-        for (int j = 0; j < n && ok; ++j) {
-          // (the second tile has at least as many key tiles as the first, or none)
-          const bool a = j < n0, b = j < n1, next_a = j + 1 < n0, next_b = j + 1 < n1;
-          if (a) add_values(0, j, true, !b);
-          if (next_a && ok) form_scores(0, j + 1, true, !next_b);
-          if (b && ok) add_values(1, j, !a, true);
-          if (next_b && ok) form_scores(1, j + 1, !next_a, true);
-        }
+      // (the second query tile has at least as many key tiles as the first, or none)
+      for (int j = -1; j < n && ok; ++j) {
+        const bool a = j >= 0 && j < n0, b = j >= 0 && j < n1, next_a = j + 1 < n0, next_b = j + 1 < n1;
+        if (!C::kOver && next_a) form_scores(0, j + 1, true, true);
+        if (a && ok) add_values(0, j, true, !b);
+        if (C::kOver && next_a && ok) form_scores(0, j + 1, true, !next_b);
+        if (b && ok) add_values(1, j, !a, true);
+        if (next_b && ok) form_scores(1, j + 1, !next_a, true);
       }
     } else if (warp == clean_warp) {
       uint32_t odd = 0;  // a bit a stage: parity of landed()'s next phase
       for (int j = 0; j < n; ++j) {
         if (!dirty(j)) continue;
-        const int i = value_place(j), s = i % ST;
+        const int s = value_place(j) % ST;
         uint32_t bits[4];
-        attention_rows_there(p, place, length, j, bits);
+        attention_rows_there(p, place, length, j * kAtTile, bits);
         if (!mbar_wait_warp(landed(s), odd >> s & 1u, abort_flag, status, kDevTimeoutStats)) break;
         odd ^= 1u << s;
         attention_clean_rows(ring + s * C::kStageBytes, HALVES, bits);
@@ -206,11 +199,14 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
     }
   } else {
     registers_more<C::kMany>();
-    const int t = warp >> 2, nt = t == 0 ? n0 : n1, row = (warp & 3) * 32 + lane;
+    // two threads a row: columns 0 .. 63 and 64 .. 127 of the scores, every other 16 columns of the sums
+    const int t = warp >> 3, half = warp >> 2 & 1, nt = t == 0 ? n0 : n1, row = (warp & 3) * 32 + lane, pair = 2 + t * 4 + (warp & 3);
     const uint32_t own = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's lanes
     const int q0 = (place.tile * T + t) * kAtTile, q_row = q0 + row;
     const bool inside = q_row < length;
     const bool there = inside && !place.behind && (p.mask == nullptr || __ldcg(p.mask + place.first + q_row) != 0);
+    float* const mine = swap + (t * 2 + half) * kAtTile + row;
+    const float* const other = swap + (t * 2 + (half ^ 1)) * kAtTile + row;
     float low = 0.f, high = 0.f;  // the outer buckets
     if (p.table != nullptr && n > 0) {
       attention_bias_fill(p, bias, head, F16, threadIdx.x, C::kSoftmaxWarps * 32);
@@ -222,118 +218,121 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
     constexpr float kGrowth = 8.f;
     const float scale = p.scale * kLog2e;
     float m = -INFINITY;
-    float2 sum = make_float2(0.f, 0.f);
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     bool ok = true;
+    // (every thread comes to every barrier of its pair: after a wait has given up the others return at once)
     for (int j = 0; j < nt; ++j) {
-      const int key0 = j * kAtTile, d0 = key0 - q0;
-      const bool near = p.table != nullptr && d0 + 127 > -p.reach && d0 - 127 < p.reach;
+      const int key0 = j * kAtTile + half * 64, d0 = key0 - q0;
+      const bool near = p.table != nullptr && d0 + 63 > -p.reach && d0 - 127 < p.reach;
       const float add = p.table == nullptr || near ? 0.f : d0 > 0 ? high : low;
-      const int keys = min(kAtTile, length - key0), pieces = (keys + 31) / 32;
-      const int limit = p.causal ? min(keys, q_row - key0 + 1) : keys;
-      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+      const int keys = length - key0, limit = p.causal ? min(keys, q_row - key0 + 1) : keys;
+      uint32_t bits[2] = {~0u, ~0u};
       if (p.mask != nullptr) attention_mask_bits(p, place.first + key0, place.last, bits);
       ok = mbar_wait_warp(scores_ready(t), j & 1, abort_flag, status, kDevTimeoutEpilogue);
-      if (!ok) break;
       tc_fence_after();
-      uint32_t v[4][32];
+      uint32_t v[2][32];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(own + C::scores(t) + i * 32, v[i]);
+      for (int i = 0; i < 2; ++i) tmem_ld32(own + C::scores(t) + half * 64 + i * 32, v[i]);
       tmem_ld_wait();
-      tc_fence_before();
       if (!C::kOver) {
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(scores_read(t));
       }
       float factor = scale;
-      if (near) {
+      if (near || scale <= 0.f) {
         const float* b = bias + (p.reach + 255) + d0 - row;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[i][c] = __float_as_uint(fmaf(__uint_as_float(v[i][c]), scale, b[i * 32 + c]));
-        factor = 1.f;
-      } else if (scale <= 0.f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int c = 0; c < 32; ++c) v[i][c] = __float_as_uint(__uint_as_float(v[i][c]) * scale);
+          for (int c = 0; c < 32; ++c) v[i][c] = __float_as_uint(fmaf(__uint_as_float(v[i][c]), scale, near ? b[i * 32 + c] : 0.f));
         factor = 1.f;
       }
-      float most = -INFINITY;
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (a chain of dependent instructions costs more than they have)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int left = limit - 32 * i;
-        const uint32_t counts = bits[i] & (left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u);
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t counts = bits[i] & first_bits(limit - 32 * i);
         if (counts != ~0u) {
 #pragma unroll
           for (int c = 0; c < 32; ++c)
             if (!(counts >> c & 1u)) v[i][c] = 0xFF800000u;
         }
 #pragma unroll
-        for (int c = 0; c < 32; ++c) most = fmaxf(most, __uint_as_float(v[i][c]));
+        for (int c = 0; c < 32; c += 2) top[c / 2 % 4] = max3(top[c / 2 % 4], __uint_as_float(v[i][c]), __uint_as_float(v[i][c + 1]));
       }
-      most = fmaf(most, factor, add);
-      // a new maximum only where it grew by much, or where there was none
-      const bool grew = most > m + kGrowth || (m == -INFINITY && most > m);
-      const bool any = __any_sync(0xFFFFFFFFu, grew);
-      float shrink = 1.f;
-      if (grew) {
-        shrink = exp2_approx(m - most);
-        m = most;
-        sum.x *= shrink;
-        sum.y *= shrink;
+      const float most = fmaf(max3(fmaxf(top[0], top[1]), top[2], top[3]), factor, add);
+      // A new maximum only where it grew by much, or where there was none; only then do the two threads of a row compare theirs. (Both
+      // have read their scores when one writes probabilities over them.)
+      if (named_bar_or(pair, 64, most > m + kGrowth || (m == -INFINITY && most > m))) {
+        *mine = most;
+        named_bar_sync(pair, 64);
+        const float both = fmaxf(most, *other);
+        float shrink = 1.f;
+        if (both > m + kGrowth || (m == -INFINITY && both > m)) {
+          shrink = exp2_approx(m - both);
+          m = both;
+          sum[0] = make_float2(sum[0].x * shrink, sum[0].y * shrink);
+          sum[1] = make_float2(sum[1].x * shrink, sum[1].y * shrink);
+        }
+        if (j > 0) {
+          // (no product is adding to the accumulator after that: the next one waits for these probabilities)
+          ok = ok && mbar_wait_warp(out_done(t), (j - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
+          tc_fence_after();
+          const float2 shrink2 = make_float2(shrink, shrink);
+          for (int c0 = half * 16; c0 < p.d; c0 += 32) {
+            uint32_t o[16];
+            tmem_ld16(own + C::out(t) + c0, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              const float2 s = __fmul2_rn(make_float2(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), shrink2);
+              o[c] = __float_as_uint(s.x);
+              o[c + 1] = __float_as_uint(s.y);
+            }
+            tmem_st16(own + C::out(t) + c0, o);
+          }
+        }
       }
       const float shift = add + kOffset - (m == -INFINITY ? 0.f : m);
       const float2 factor2 = make_float2(factor, factor), shift2 = make_float2(shift, shift);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i < pieces) {
+      for (int i = 0; i < 2; ++i) {
+        if (i * 32 < keys) {
           uint32_t w[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             float2 e = __ffma2_rn(make_float2(__uint_as_float(v[i][2 * c]), __uint_as_float(v[i][2 * c + 1])), factor2, shift2);
             e.x = exp2_approx(e.x);
             e.y = exp2_approx(e.y);
-            sum = __fadd2_rn(sum, e);
+            sum[c & 1] = __fadd2_rn(sum[c & 1], e);
             w[c] = pack_pair<F16>(e);
           }
-          if (i == 0 && j > 0) {
-            // the products with the last tile's probabilities are done: their columns and the sums can be written
+          if (!C::kOver && i == 0 && j > 0 && ok) {
+            // the products with the last tile's probabilities are done: their columns can be written
             ok = mbar_wait_warp(out_done(t), (j - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
             tc_fence_after();
-            if (any && ok) {
-              const float2 shrink2 = make_float2(shrink, shrink);
-              for (int c0 = 0; c0 < p.d; c0 += 16) {
-                uint32_t o[16];
-                tmem_ld16(own + C::out(t) + c0, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int c = 0; c < 16; c += 2) {
-                  const float2 s = __fmul2_rn(make_float2(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), shrink2);
-                  o[c] = __float_as_uint(s.x);
-                  o[c + 1] = __float_as_uint(s.y);
-                }
-                tmem_st16(own + C::out(t) + c0, o);
-              }
-            }
           }
-          tmem_st16(own + C::probabilities(t) + i * 16, w);
+          tmem_st16(own + C::probabilities(t) + half * 32 + i * 16, w);
         }
       }
-      if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(probs_ready(t));
     }
-    if (nt > 0 && ok) ok = mbar_wait_warp(out_done(t), (nt - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
+    if (nt > 0) {
+      ok = ok && mbar_wait_warp(out_done(t), (nt - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
+      named_bar_sync(pair, 64);  // (the other has read this one's maximum)
+      *mine = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      named_bar_sync(pair, 64);
+    }
     if (ok) {
       tc_fence_after();
-      const float total = sum.x + sum.y;
+      const float total = nt > 0 ? swap[t * 2 * kAtTile + row] + swap[(t * 2 + 1) * kAtTile + row] : 0.f;
       const bool some = there && total != 0.f;  // (NaN: some)
       const float inverse = some ? 1.f / total : 0.f;
       const long long at = ((place.first + q_row) * p.heads + head) * p.d;
-      for (int c0 = 0; c0 < p.d; c0 += 16) {
+      for (int c0 = half * 16; c0 < p.d; c0 += 32) {
         uint32_t o[16], w[8], rest[8];
         if (nt > 0) {
           tmem_ld16(own + C::out(t) + c0, o);
@@ -349,16 +348,15 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
         }
         if (inside) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-            if (c0 + half * 8 < p.d) {
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + at + c0 + half * 8) = make_uint4(w[half * 4], w[half * 4 + 1], w[half * 4 + 2], w[half * 4 + 3]);
+          for (int q = 0; q < 2; ++q)
+            if (c0 + q * 8 < p.d) {
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + at + c0 + q * 8) = make_uint4(w[q * 4], w[q * 4 + 1], w[q * 4 + 2], w[q * 4 + 3]);
               if (p.rest != nullptr)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.rest) + at + c0 + half * 8) =
-                    make_uint4(rest[half * 4], rest[half * 4 + 1], rest[half * 4 + 2], rest[half * 4 + 3]);
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.rest) + at + c0 + q * 8) = make_uint4(rest[q * 4], rest[q * 4 + 1], rest[q * 4 + 2], rest[q * 4 + 3]);
             }
         }
       }
-      if (inside && p.lse != nullptr) p.lse[head * p.rows + place.first + q_row] = some ? m - kOffset + log2f(total) : INFINITY;
+      if (half == 0 && inside && p.lse != nullptr) p.lse[head * p.rows + place.first + q_row] = some ? m - kOffset + log2f(total) : INFINITY;
     }
   }
   __syncthreads();

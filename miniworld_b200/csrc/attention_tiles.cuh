@@ -32,6 +32,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // (NaN: the greatest of the others)
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 template <bool F16>
 __device__ __forceinline__ uint32_t pack_pair(float2 v) {
   if constexpr (F16)
@@ -103,30 +108,30 @@ __device__ __forceinline__ void attention_bias_fill(const AttentionParams& p, fl
   for (int i = thread; i < entries; i += threads) bias[i] = attention_bias(p, i - (p.reach + 255), head, f16) * kLog2e;
 }
 
-// Keys first .. first + 127 that the mask leaves, a bit each (mask null: all); those at or beyond `limit` are the caller's business.
-__device__ __forceinline__ void attention_mask_bits(const AttentionParams& p, long long first, long long last, uint32_t (&bits)[4]) {
+// Rows first .. first + 32 W - 1 that lie before `last` and that the mask leaves, a bit each (whole warp)
+template <int W>
+__device__ __forceinline__ void attention_mask_bits(const AttentionParams& p, long long first, long long last, uint32_t (&bits)[W]) {
   const int lane = threadIdx.x & 31;
-  bool there[4];
+  bool there[W];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < W; ++i) {
     const long long row = first + 32 * i + lane;
     there[i] = row < last && __ldcg(p.mask + row) != 0;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bits[i] = __ballot_sync(0xFFFFFFFFu, there[i]);
+  for (int i = 0; i < W; ++i) bits[i] = __ballot_sync(0xFFFFFFFFu, there[i]);
 }
-
-// The same of tile j of a sequence, with or without a mask, up to the sequence's end
-__device__ __forceinline__ void attention_rows_there(const AttentionParams& p, const AttentionPlace& place, int length, int j, uint32_t (&bits)[4]) {
+// The first `count` of 32 as bits
+__device__ __forceinline__ uint32_t first_bits(int count) { return count >= 32 ? ~0u : count > 0 ? (1u << count) - 1u : 0u; }
+// The same of the rows from row0 of a sequence on, with or without a mask
+template <int W>
+__device__ __forceinline__ void attention_rows_there(const AttentionParams& p, const AttentionPlace& place, int length, int row0, uint32_t (&bits)[W]) {
   if (p.mask != nullptr) {
-    attention_mask_bits(p, place.first + static_cast<long long>(j) * kAtTile, place.last, bits);
+    attention_mask_bits(p, place.first + row0, place.last, bits);
     return;
   }
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const int left = length - j * kAtTile - 32 * w;
-    bits[w] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u;
-  }
+  for (int w = 0; w < W; ++w) bits[w] = first_bits(length - row0 - 32 * w);
 }
 
 // What the copying thread remembers of its ring, a bit a stage: whether it was used, the parity of that use, whether the copy went to
@@ -159,14 +164,19 @@ struct AttentionRing {
 
 // Zeroes the rows of a tile in shared memory that are not among the `bits` (whole warp): an operand's rows that belong to other
 // sequences or are masked must not meet the zeros that stand for them in the other operand as infinities or NaN.
-__device__ __forceinline__ void attention_clean_rows(uint32_t tile, int halves, const uint32_t (&bits)[4]) {
+template <int W>
+__device__ __forceinline__ void attention_clean_rows(uint32_t tile, int halves, const uint32_t (&bits)[W]) {
   const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (bits[w] == ~0u) continue;
 #pragma unroll 1
-  for (int h = 0; h < halves; ++h)
+    for (int h = 0; h < halves; ++h)
 #pragma unroll 1
-    for (int r = lane / 8; r < 128; r += 4)
-      if (!(bits[r >> 5] >> (r & 31) & 1u))
-        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + h * kAtTileBytes + r * 128 + (lane & 7) * 16), "r"(0) : "memory");
+      for (int r = lane / 8; r < 32; r += 4)
+        if (!(bits[w] >> r & 1u))
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + h * (W * 4096) + (w * 32 + r) * 128 + (lane & 7) * 16), "r"(0) : "memory");
+  }
   fence_proxy_async_smem();
   __syncwarp();
 }

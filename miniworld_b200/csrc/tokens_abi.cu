@@ -90,10 +90,10 @@ template <bool F16, int HALVES>
 static int launch_attention_forward(const AttentionMaps& maps, const AttentionParams& p, const DeviceInfo& info, cudaStream_t stream) {
   using C = AtForward<HALVES>;
   const auto kernel = attention_forward_kernel<F16, HALVES>;
-  const int rc = set_smem(kernel, C::smem(B200_POSITION_MAX_REACH), info.device);
+  const int rc = set_smem(kernel, C::smem(true, B200_POSITION_MAX_REACH), info.device);
   if (rc != 0) return rc;
   const long long places = attention_places(p.offsets, p.rows, p.sequences, p.length, C::kTiles * kAtTile);
-  TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(places), p.heads), C::kThreads, C::smem(p.reach), stream, maps, p));
+  TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(places), p.heads), C::kThreads, C::smem(p.table != nullptr, p.reach), stream, maps, p));
   return B200_TRIMUL_OK;
 }
 static int attention_delta_blocks(long long rows, int d) {
