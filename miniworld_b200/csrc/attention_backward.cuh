@@ -3,7 +3,7 @@
 // the queries of all heads of the group). Scores and dO v^T are formed again in both of the latter: 7 products where 5 would do, against
 // adding dq up over blocks in whatever order they end.
 //
-// Eight warps do the arithmetic: a thread has a row and 64 columns of the scores and of dO v^T. Both are in registers while the next
+// Sixteen warps do the arithmetic: a thread has a row and 32 columns of the scores and of dO v^T. Both are in registers while the next
 // tile's are formed; probabilities and ds go back into tensor memory as the first operand of the sums.
 //
 // fp16: probabilities are held times 2^15, and ds times the power of two that brings its bound 2 max |dO| max |v| to 2^14 .. 2^15, so that
@@ -110,9 +110,9 @@ __device__ __forceinline__ float attention_ds_scale(const AttentionParams& p, in
   return bound > 0.f && bound < INFINITY ? exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -60), 60))) : 1.f;
 }
 
-constexpr int kAtBackWarps = 8;  // of the arithmetic
+constexpr int kAtBackWarps = 16;  // of the arithmetic: a thread has a row and 32 columns
 constexpr int kAtBackThreads = kAtBackWarps * 32 + 128;
-constexpr int kAtBackMany = 208, kAtBackFew = 88;  // registers: the launch's are 168, and 2 x 208 + 88 = 3 x 168
+constexpr int kAtBackMany = 104, kAtBackFew = 64;  // registers: the launch's are 96, and 4 x 104 + 64 = 5 x 96
 
 // ---------------------------------------------------------------- dq
 template <int HALVES>
@@ -126,11 +126,9 @@ struct AtDq {
   static constexpr int kBars = 2 * HALVES * kAtTileBytes + kStages * kStageBytes;
   static constexpr int kBias = kBars + 320;
   static int smem(bool table, int reach) {
-    // biases; diagonals: a square of 32 x 32 a warp; sums by distance of every warp
-    const int bias = up16(attention_bias_entries(reach) * 4);
-    return 1024 + kBias + (table ? bias + kAtBackWarps * 4096 + kAtBackWarps * (2 * reach + 1) * 4 + 128 * 8 : 0);
+    // biases; sums by distance of every warp; what the threads of a row tell each other
+    return 1024 + kBias + (table ? (attention_bias_entries(reach) + kAtBackWarps * (2 * reach + 1) + 4 * kAtTile) * 4 : 0);
   }
-  __host__ __device__ static constexpr int up16(int v) { return (v + 15) / 16 * 16; }
 };
 
 template <bool F16, int HALVES>
@@ -269,14 +267,14 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
     }
   } else {
     registers_more<kAtBackMany>();
-    const int half = warp >> 2, row0 = (warp & 3) * 32, row = row0 + lane, q_row = q0 + row;
+    const int quarter = warp >> 2, row0 = (warp & 3) * 32, row = row0 + lane, q_row = q0 + row;
     const uint32_t own = tmem + (static_cast<uint32_t>(warp & 3) << 21);
     const bool inside = q_row < length;
     const bool there = inside && !place.behind && (p.mask == nullptr || __ldcg(p.mask + place.first + q_row) != 0);
     const bool sums = p.partial != nullptr;
     const int distances = 2 * p.reach + 1;
-    float* const square = reinterpret_cast<float*>(smem + C::kBias + C::up16(attention_bias_entries(p.reach) * 4)) + warp * 1024;
-    float* const by_distance = square + (kAtBackWarps - warp) * 1024 + warp * distances;
+    float* const all_distances = bias + attention_bias_entries(p.reach);  // [warps][distances], then [4][128]
+    float* const by_distance = all_distances + warp * distances;
     float low = 0.f, high = 0.f;
     if (p.table != nullptr && n > 0) {
       attention_bias_fill(p, bias, head, F16, threadIdx.x, kAtBackWarps * 32);
@@ -294,112 +292,98 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
     float all = 0.f, sum_low = 0.f, sum_high = 0.f, mass_low = 0.f, mass_high = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      const int key0 = j * kAtTile, d0 = key0 - q0, keys = min(kAtTile, length - key0);
-      const bool near = p.table != nullptr && d0 + 127 > -p.reach && d0 - 127 < p.reach;
+      const int key0 = j * kAtTile + quarter * 32, d0 = key0 - q0, keys = length - key0;
+      const bool near = p.table != nullptr && d0 + 31 > -p.reach && d0 - 127 < p.reach;
       const float add = p.table == nullptr || near ? 0.f : d0 > 0 ? high : low;
       const int limit = !there ? 0 : p.causal ? min(keys, q_row - key0 + 1) : keys;
-      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+      uint32_t bits[1] = {~0u};
       if (p.mask != nullptr) attention_mask_bits(p, place.first + key0, place.last, bits);
+      const uint32_t counts = bits[0] & first_bits(limit);
       ok = mbar_wait_warp(formed, j & 1, abort_flag, status, kDevTimeoutEpilogue);
       if (!ok) break;
       tc_fence_after();
-      uint32_t v[2][32], g[2][32];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        tmem_ld32(own + C::kScores + half * 64 + i * 32, v[i]);
-        tmem_ld32(own + C::kGrad + half * 64 + i * 32, g[i]);
-      }
+      uint32_t v[32], g[32];
+      tmem_ld32(own + C::kScores + quarter * 32, v);
+      tmem_ld32(own + C::kGrad + quarter * 32, g);
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(read);
       const float factor = near ? 1.f : scale, shift = add - lse;
       if (near) {
-        const float* b = bias + (p.reach + 255) + d0 + half * 64 - row;
+        const float* b = bias + (p.reach + 255) + d0 - row;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[i][k] = __float_as_uint(fmaf(__uint_as_float(v[i][k]), scale, b[i * 32 + k]));
+        for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(fmaf(__uint_as_float(v[k]), scale, b[k]));
       }
       const float2 factor2 = make_float2(factor, factor), shift2 = make_float2(shift, shift);
+      uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int col0 = half * 64 + i * 32, left = limit - col0;
-        const uint32_t counts = bits[half * 2 + i] & first_bits(left);
-        uint32_t w[16];
-        float2 total = make_float2(0.f, 0.f), mass = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          float2 e = __ffma2_rn(make_float2(__uint_as_float(v[i][2 * k]), __uint_as_float(v[i][2 * k + 1])), factor2, shift2);
-          e.x = exp2_approx(e.x);
-          e.y = exp2_approx(e.y);
-          float2 ds = __fmul2_rn(e, __ffma2_rn(make_float2(__uint_as_float(g[i][2 * k]), __uint_as_float(g[i][2 * k + 1])), c2, minus_delta));
-          if (counts != ~0u) {
-            if (!(counts >> (2 * k) & 1u)) ds.x = e.x = 0.f;
-            if (!(counts >> (2 * k + 1) & 1u)) ds.y = e.y = 0.f;
-          }
-          w[k] = pack_pair<F16>(ds);
-          if (sums) {
-            total = __fadd2_rn(total, ds);
-            mass = __fadd2_rn(mass, e);
-            v[i][2 * k] = __float_as_uint(e.x), v[i][2 * k + 1] = __float_as_uint(e.y);
-            g[i][2 * k] = __float_as_uint(ds.x), g[i][2 * k + 1] = __float_as_uint(ds.y);
-          }
+      for (int k = 0; k < 16; ++k) {
+        float2 e = __ffma2_rn(make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), factor2, shift2);
+        e.x = exp2_approx(e.x);
+        e.y = exp2_approx(e.y);
+        float2 ds = __fmul2_rn(e, __ffma2_rn(make_float2(__uint_as_float(g[2 * k]), __uint_as_float(g[2 * k + 1])), c2, minus_delta));
+        if (counts != ~0u) {
+          if (!(counts >> (2 * k) & 1u)) ds.x = e.x = 0.f;
+          if (!(counts >> (2 * k + 1) & 1u)) ds.y = e.y = 0.f;
         }
-        if (i == 0 && j > 0) {
-          ok = mbar_wait_warp(ds_done, (j - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
-          tc_fence_after();
-        }
-        tmem_st16(own + C::kDs + half * 32 + i * 16, w);
-        if (sums) {
-          const float t = total.x + total.y, m = mass.x + mass.y;
-          all += t;
-          const int e0 = d0 + col0 - row0;  // distance of the square's first column from its first row
-          if (e0 + 31 <= -p.reach) {
-            sum_low += t;
-            mass_low += m;
-          } else if (e0 - 31 >= p.reach) {
-            sum_high += t;
-            mass_high += m;
-          } else {
-            // columns up to / from which on this row is in an outer bucket (a reach of 0 is one bucket: the lower)
-            const int last_low = -p.reach - e0 + lane, first_high = max(p.reach - e0 + lane, last_low + 1);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float ds = __uint_as_float(g[i][k]), e = __uint_as_float(v[i][k]);
-              if (k <= last_low) sum_low += ds, mass_low += e;
-              if (k >= first_high) sum_high += ds, mass_high += e;
-              square[lane * 32 + ((k - lane) & 31)] = ds;
-            }
-            __syncwarp();
-            // column x of the skewed square holds the diagonals x (from the rows above 32 - x) and x - 32
-            float upper = 0.f, lower = 0.f;
-#pragma unroll
-            for (int r = 0; r < 32; ++r) {
-              const float ds = square[r * 32 + lane];
-              if (r + lane < 32) upper += ds;
-              else lower += ds;
-            }
-            const int du = e0 + lane, dl = du - 32;
-            if (du > -p.reach && du < p.reach) by_distance[du + p.reach] += upper;
-            __syncwarp();
-            if (dl > -p.reach && dl < p.reach) by_distance[dl + p.reach] += lower;
-            __syncwarp();
-          }
-        }
+        w[k] = pack_pair<F16>(ds);
+        v[2 * k] = __float_as_uint(e.x), v[2 * k + 1] = __float_as_uint(e.y);
+        g[2 * k] = __float_as_uint(ds.x), g[2 * k + 1] = __float_as_uint(ds.y);
       }
-      if (!ok) break;
+      if (j > 0) {
+        ok = mbar_wait_warp(ds_done, (j - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      tmem_st16(own + C::kDs + quarter * 16, w);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_ready);
+      if (sums) {
+        float2 total = make_float2(0.f, 0.f), mass = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          total = __fadd2_rn(total, make_float2(__uint_as_float(g[k]), __uint_as_float(g[k + 1])));
+          mass = __fadd2_rn(mass, make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
+        }
+        const float t = total.x + total.y;
+        all += t;
+        const int e0 = d0 - row0;  // distance of this square's first column from its first row
+        if (e0 + 31 <= -p.reach) {
+          sum_low += t;
+          mass_low += mass.x + mass.y;
+        } else if (e0 - 31 >= p.reach) {
+          sum_high += t;
+          mass_high += mass.x + mass.y;
+        } else {
+          // columns up to / from which on this row is in an outer bucket (a reach of 0 is one bucket: the lower)
+          const int last_low = -p.reach - e0 + lane, first_high = max(p.reach - e0 + lane, last_low + 1);
+          // Lane x adds up the square's diagonals x (of the rows above 32 - x) and x - 32: column k of row r is in the one or the other.
+          float upper = 0.f, lower = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float ds = __uint_as_float(g[k]), e = __uint_as_float(v[k]);
+            if (k <= last_low) sum_low += ds, mass_low += e;
+            if (k >= first_high) sum_high += ds, mass_high += e;
+            const float turned = __shfl_sync(0xFFFFFFFFu, ds, k - lane);  // (of row k - lane modulo 32)
+            if (lane <= k) upper += turned;
+            else lower += turned;
+          }
+          const int du = e0 + lane, dl = du - 32;
+          if (du > -p.reach && du < p.reach) by_distance[du + p.reach] += upper;
+          if (dl > -p.reach && dl < p.reach) by_distance[dl + p.reach] += lower;
+          __syncwarp();
+        }
+      }
     }
     if (n > 0 && ok) ok = mbar_wait_warp(ds_done, (n - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
     if (ok) {
       tc_fence_after();
       const float back = p.scale / c;
       const long long at = ((place.first + q_row) * p.heads + head) * p.d;
-      for (int c0 = half * 16; c0 < p.d; c0 += 32) {
+      for (int c0 = quarter * 16; c0 < p.d; c0 += 64) {
         uint32_t o[16], w[8];
         if (n > 0) {
           tmem_ld16(own + C::kSum + c0, o);
@@ -418,29 +402,28 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
     if (sums) {
       // ds of a row adds up to nothing but what delta is off by: its share, by the probabilities' mass, comes off the outer buckets, of
       // whose terms most are of one sign otherwise
-      float* const rows = square + (kAtBackWarps - warp) * 1024 + kAtBackWarps * distances;  // [2][128], then the warps' sums
+      float* const rows = all_distances + kAtBackWarps * distances;
       float* const out = p.partial + (static_cast<long long>(head) * gridDim.x + place_index) * distances;
       if (n > 0) {
-        rows[half * 128 + row] = all;
+        rows[quarter * 128 + row] = all;
         named_bar_sync(1, kAtBackWarps * 32);
-        const float off = rows[row] + rows[128 + row];
+        const float off = (rows[row] + rows[128 + row]) + (rows[256 + row] + rows[384 + row]);
         const float l = warp_sum(sum_low - off * mass_low), h = warp_sum(sum_high - off * mass_high);
         named_bar_sync(1, kAtBackWarps * 32);
         if (lane == 0) {
           rows[warp] = l;
-          rows[8 + warp] = h;
+          rows[kAtBackWarps + warp] = h;
         }
         named_bar_sync(1, kAtBackWarps * 32);
       }
       for (int i = threadIdx.x; i < distances; i += kAtBackWarps * 32) {
         float s = 0.f;
         if (n > 0) {
-          const float* d = by_distance - warp * distances + i;
-          for (int k = 0; k < kAtBackWarps; ++k) s += d[k * distances];
+          for (int k = 0; k < kAtBackWarps; ++k) s += all_distances[k * distances + i];
           if (i == 0)
             for (int k = 0; k < kAtBackWarps; ++k) s += rows[k];
           if (i == distances - 1)
-            for (int k = 0; k < kAtBackWarps; ++k) s += rows[8 + k];
+            for (int k = 0; k < kAtBackWarps; ++k) s += rows[kAtBackWarps + k];
         }
         out[i] = s / c;
       }
@@ -475,7 +458,9 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
   auto ready = [&](int s) { return bars + 8u * (ST + s); };
   auto empty = [&](int s) { return bars + 8u * (2 * ST + s); };
   const uint32_t k_ready = bars + 8u * (3 * ST), formed = k_ready + 8, read = k_ready + 16, ds_ready = k_ready + 24, ds_done = k_ready + 32;
-  static_assert(8 * (3 * ST + 5) <= 240, "barriers");
+  auto rows_ready = [&](int b) { return k_ready + 40 + 8u * b; };
+  auto rows_free = [&](int b) { return k_ready + 56 + 8u * b; };
+  static_assert(8 * (3 * ST + 9) <= 240, "barriers");
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBars + 240);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* const ds_scale_s = reinterpret_cast<float*>(tmem_slot + 2);
@@ -485,7 +470,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
   float* const bias = reinterpret_cast<float*>(smem + C::kBias);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int load_warp = kAtBackWarps, mma_warp = load_warp + 1, clean_warp = load_warp + 2;
+  const int load_warp = kAtBackWarps, mma_warp = load_warp + 1, clean_warp = load_warp + 2, rows_warp = load_warp + 3;
   const int kv_head = blockIdx.y, group = p.heads / p.kv_heads;
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -498,6 +483,10 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
     mbar_init(read, kAtBackWarps);
     mbar_init(ds_ready, kAtBackWarps);
     mbar_init(ds_done, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(rows_ready(b), 1);
+      mbar_init(rows_free(b), kAtBackWarps);
+    }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -609,88 +598,101 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
         }
         if (!ok) break;
       }
+    } else if (warp == rows_warp) {
+      // what a tile's queries have: -lse (with the outer bucket's bias, where the whole tile is in one) and -delta, a buffer ahead
+      int head = kv_head * group, tile = first_tile;
+      float low = 0.f, high = 0.f;
+      const float held = F16 ? *ds_scale_s * (1.f / 32768.f) : 1.f;
+      for (int u = 0; u < n; ++u) {
+        if (p.table != nullptr && tile == first_tile) {
+          low = attention_bias(p, -p.reach, head, F16) * kLog2e;
+          high = attention_bias(p, p.reach, head, F16) * kLog2e;
+        }
+        const int q0 = tile * kAtTile, d0 = key0 - q0;
+        const float add = p.table == nullptr || attention_near(p, d0) ? 0.f : d0 > 0 ? high : low;
+        float l[4], d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int query = q0 + i * 32 + lane;
+          l[i] = -INFINITY;
+          d[i] = 0.f;
+          if (query < length) {
+            const long long at = head * p.rows + place.first + query;
+            l[i] = (F16 ? 15.f : 0.f) + add - __ldcg(p.lse + at);
+            d[i] = -__ldcg(p.delta + at) * held;
+          }
+        }
+        if (u >= 2 && !mbar_wait_warp(rows_free(u & 1), ((u >> 1) & 1) ^ 1, abort_flag, status, kDevTimeoutStats)) break;
+        float* const rows = of_rows + (u & 1) * 256;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          rows[i * 32 + lane] = l[i];
+          rows[128 + i * 32 + lane] = d[i];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(rows_ready(u & 1));
+        if (++tile == first_tile + tiles) tile = first_tile, ++head;
+      }
     }
   } else {
     registers_more<kAtBackMany>();
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane, k_row = key0 + row;
+    const int quarter = warp >> 2, row = (warp & 3) * 32 + lane, k_row = key0 + row;
     const uint32_t own = tmem + (static_cast<uint32_t>(warp & 3) << 21);
     const bool inside = k_row < length;
     const bool there = inside && !place.behind && (p.mask == nullptr || __ldcg(p.mask + place.first + k_row) != 0);
-    constexpr float kOffset = F16 ? 15.f : 0.f;
     const float c = F16 ? *ds_scale_s : 1.f, held = F16 ? c * (1.f / 32768.f) : 1.f, scale = p.scale * kLog2e;
     const float2 held2 = make_float2(held, held);
-    float low = 0.f, high = 0.f;
     int head = kv_head * group, tile = first_tile;
-    // this thread's share of what the tile's queries have: -lse of query threadIdx.x, or -delta of query threadIdx.x - 128
-    auto fetch = [&](int h, int t) {
-      const int query = t * kAtTile + (threadIdx.x & 127);
-      if (query >= length) return threadIdx.x < 128 ? -INFINITY : 0.f;
-      const float x = __ldcg((threadIdx.x < 128 ? p.lse : p.delta) + h * p.rows + place.first + query);
-      return threadIdx.x < 128 ? kOffset - x : -x * held;
-    };
-    float next = n > 0 ? fetch(head, tile) : 0.f;
     bool ok = true;
+    // (every thread comes to every barrier of its group: after a wait has given up the others return at once)
     for (int u = 0; u < n; ++u) {
       const int q0 = tile * kAtTile, d0 = key0 - q0;
       if (p.table != nullptr && tile == first_tile) {
-        // (no thread reads the last head's biases any more: see the barrier of the tile before, after which it had read them)
-        if (u > 0) named_bar_sync(1, kAtBackWarps * 32);
+        if (u > 0) named_bar_sync(1, kAtBackWarps * 32);  // no thread reads the last head's biases any more
         attention_bias_fill(p, bias, head, F16, threadIdx.x, kAtBackWarps * 32);
         named_bar_sync(1, kAtBackWarps * 32);
-        low = bias[0];
-        high = bias[2 * (p.reach + 255)];
       }
-      const bool near = p.table != nullptr && d0 + 127 > -p.reach && d0 - 127 < p.reach;
-      const float add = p.table == nullptr || near ? 0.f : d0 > 0 ? high : low;
-      float* const rows = of_rows + (u & 1) * 256;
-      rows[threadIdx.x] = threadIdx.x < 128 ? next + add : next;
-      named_bar_sync(1, kAtBackWarps * 32);
+      const bool near = p.table != nullptr && attention_near(p, d0);
       if (++tile == first_tile + tiles) tile = first_tile, ++head;
-      if (u + 1 < n) next = fetch(head, tile);
-      ok = mbar_wait_warp(formed, u & 1, abort_flag, status, kDevTimeoutEpilogue);
-      // (every thread comes to every barrier of its group: after a wait has given up the others return at once)
+      ok = mbar_wait_warp(rows_ready(u & 1), (u >> 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
+      ok = mbar_wait_warp(formed, u & 1, abort_flag, status, kDevTimeoutEpilogue) && ok;
       tc_fence_after();
-      uint32_t v[2][32], g[2][32];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        tmem_ld32(own + C::kScores + half * 64 + i * 32, v[i]);
-        tmem_ld32(own + C::kGrad + half * 64 + i * 32, g[i]);
-      }
+      uint32_t v[32], g[32];
+      tmem_ld32(own + C::kScores + quarter * 32, v);
+      tmem_ld32(own + C::kGrad + quarter * 32, g);
       tmem_ld_wait();
       tc_fence_before();
       if (!C::kOver) {
         __syncwarp();
         if (lane == 0) mbar_arrive(read);
+      } else {
+        named_bar_sync(2 + (warp & 3), 128);  // all of a row's columns have been read before results go over them
       }
       const float factor = near ? 1.f : scale;
       if (near) {
-        const float* b = bias + (p.reach + 255) + d0 + row - half * 64;
+        const float* b = bias + (p.reach + 255) + d0 + row - quarter * 32;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[i][k] = __float_as_uint(fmaf(__uint_as_float(v[i][k]), scale, b[-i * 32 - k]));
+        for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(fmaf(__uint_as_float(v[k]), scale, b[-k]));
       }
       const float2 factor2 = make_float2(factor, factor);
-      const int first = p.causal ? k_row - q0 - half * 64 : -1;  // the first of this thread's columns that counts
-      if (C::kOver) {
-        // both halves of a row's columns have been read before the other half's results go over them
-        named_bar_sync(2 + (warp & 3), 64);
-      }
+      const int first = p.causal ? k_row - q0 - quarter * 32 : -1;  // the first of this thread's columns that counts
+      const float* const rows = of_rows + (u & 1) * 256 + quarter * 32;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint32_t w[16], x[16];
+        uint32_t w[8], x[8];
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) {
-          const float4 l = *reinterpret_cast<const float4*>(rows + half * 64 + i * 32 + 2 * k), d = *reinterpret_cast<const float4*>(rows + 128 + half * 64 + i * 32 + 2 * k);
+        for (int k = 0; k < 8; k += 2) {
+          const int at = i * 16 + 2 * k;
+          const float4 l = *reinterpret_cast<const float4*>(rows + at), d = *reinterpret_cast<const float4*>(rows + 128 + at);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const int at = 2 * (k + q);
-            float2 e = __ffma2_rn(make_float2(__uint_as_float(v[i][at]), __uint_as_float(v[i][at + 1])), factor2, q == 0 ? make_float2(l.x, l.y) : make_float2(l.z, l.w));
+            const int col = at + 2 * q;
+            float2 e = __ffma2_rn(make_float2(__uint_as_float(v[col]), __uint_as_float(v[col + 1])), factor2, q == 0 ? make_float2(l.x, l.y) : make_float2(l.z, l.w));
             e.x = exp2_approx(e.x);
             e.y = exp2_approx(e.y);
-            float2 ds = __fmul2_rn(e, __ffma2_rn(make_float2(__uint_as_float(g[i][at]), __uint_as_float(g[i][at + 1])), held2, q == 0 ? make_float2(d.x, d.y) : make_float2(d.z, d.w)));
-            if (i * 32 + at < first) e.x = ds.x = 0.f;
-            if (i * 32 + at + 1 < first) e.y = ds.y = 0.f;
+            float2 ds = __fmul2_rn(e, __ffma2_rn(make_float2(__uint_as_float(g[col]), __uint_as_float(g[col + 1])), held2, q == 0 ? make_float2(d.x, d.y) : make_float2(d.z, d.w)));
+            if (col < first) e.x = ds.x = 0.f;
+            if (col + 1 < first) e.y = ds.y = 0.f;
             w[k + q] = pack_pair<F16>(e);
             x[k + q] = pack_pair<F16>(ds);
           }
@@ -699,24 +701,26 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
           ok = mbar_wait_warp(ds_done, (u - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
           tc_fence_after();
         }
-        tmem_st16(own + C::kProbs + half * 32 + i * 16, w);
-        tmem_st16(own + C::kDs + half * 32 + i * 16, x);
+        tmem_st8(own + C::kProbs + quarter * 16 + i * 8, w);
+        tmem_st8(own + C::kDs + quarter * 16 + i * 8, x);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_ready);
+      if (lane == 0) {
+        mbar_arrive(rows_free(u & 1));
+        mbar_arrive(ds_ready);
+      }
     }
     if (n > 0 && ok) ok = mbar_wait_warp(ds_done, (n - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
     if (ok) {
       tc_fence_after();
-      const float back_k = p.scale / c, back_v = F16 ? 1.f / 32768.f : 1.f;
       const long long at = ((place.first + k_row) * p.kv_heads + kv_head) * p.d;
-      // the two halves of the warps write one each
-      const uint32_t from = own + (half == 0 ? C::kDk : C::kDv);
-      const float back = half == 0 ? back_k : back_v;
-      uint16_t* const to = static_cast<uint16_t*>(half == 0 ? p.dk : p.dv);
-      for (int c0 = 0; c0 < p.d; c0 += 16) {
+      // two of a row's threads write dk, two dv
+      const uint32_t from = own + (quarter < 2 ? C::kDk : C::kDv);
+      const float back = quarter < 2 ? p.scale / c : F16 ? 1.f / 32768.f : 1.f;
+      uint16_t* const to = static_cast<uint16_t*>(quarter < 2 ? p.dk : p.dv);
+      for (int c0 = (quarter & 1) * 16; c0 < p.d; c0 += 32) {
         uint32_t o[16], w[8];
         if (n > 0) {
           tmem_ld16(from + c0, o);

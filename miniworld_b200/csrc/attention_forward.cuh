@@ -297,23 +297,22 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
       const float2 factor2 = make_float2(factor, factor), shift2 = make_float2(shift, shift);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (i * 32 < keys) {
-          uint32_t w[16];
+        uint32_t w[16];
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            float2 e = __ffma2_rn(make_float2(__uint_as_float(v[i][2 * c]), __uint_as_float(v[i][2 * c + 1])), factor2, shift2);
-            e.x = exp2_approx(e.x);
-            e.y = exp2_approx(e.y);
-            sum[c & 1] = __fadd2_rn(sum[c & 1], e);
-            w[c] = pack_pair<F16>(e);
-          }
-          if (!C::kOver && i == 0 && j > 0 && ok) {
-            // the products with the last tile's probabilities are done: their columns can be written
-            ok = mbar_wait_warp(out_done(t), (j - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
-            tc_fence_after();
-          }
-          tmem_st16(own + C::probabilities(t) + half * 32 + i * 16, w);
+        for (int c = 0; c < 16; ++c) {
+          float2 e = __ffma2_rn(make_float2(__uint_as_float(v[i][2 * c]), __uint_as_float(v[i][2 * c + 1])), factor2, shift2);
+          e.x = exp2_approx(e.x);
+          e.y = exp2_approx(e.y);
+          sum[c & 1] = __fadd2_rn(sum[c & 1], e);
+          w[c] = pack_pair<F16>(e);
         }
+        if (!C::kOver && i == 0 && j > 0 && ok) {
+          // The products with the last tile's probabilities are done: their columns can be written. (Every warp waits, whether or not it
+          // has columns with keys: one that went on would arrive for this tile while the others have yet to arrive for the last.)
+          ok = mbar_wait_warp(out_done(t), (j - 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
+          tc_fence_after();
+        }
+        if (i * 32 < keys) tmem_st16(own + C::probabilities(t) + half * 32 + i * 16, w);
       }
       tmem_st_wait();
       tc_fence_before();

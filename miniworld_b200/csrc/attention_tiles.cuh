@@ -51,6 +51,12 @@ __device__ __forceinline__ float2 unpack_pair(uint32_t v) {
   else
     return bf16x2_to_float2(v);
 }
+// 32 lanes x 8 consecutive 32-bit columns, registers -> TMEM
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 template <int REGS>
 __device__ __forceinline__ void registers_more() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
@@ -107,6 +113,9 @@ __device__ __forceinline__ void attention_bias_fill(const AttentionParams& p, fl
   const int entries = attention_bias_entries(p.reach);
   for (int i = thread; i < entries; i += threads) bias[i] = attention_bias(p, i - (p.reach + 255), head, f16) * kLog2e;
 }
+
+// Whether tiles of 128 keys and 128 queries, whose first ones are `d0` apart, have pairs within the reach
+__device__ __forceinline__ bool attention_near(const AttentionParams& p, int d0) { return d0 + 127 > -p.reach && d0 - 127 < p.reach; }
 
 // Rows first .. first + 32 W - 1 that lie before `last` and that the mask leaves, a bit each (whole warp)
 template <int W>

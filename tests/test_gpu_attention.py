@@ -119,6 +119,24 @@ def test_masks(kind, m, causal, fill):
         assert not got[n][~mask].any()
 
 
+@pytest.mark.parametrize("type,d", [(torch.float16, 64), (torch.bfloat16, 24), (torch.bfloat16, 96)])
+@pytest.mark.parametrize("left", [1, 44, 64, 65, 100])
+def test_many_blocks_with_short_last_tiles(type, d, left):
+    """Last tiles with keys for one half of the columns only, in more blocks than the GPU holds at once: warps that have nothing to do
+    for a tile keep step with those that have."""
+    lengths = [256 + left] * 40 + [left] * 40 + [384 + left] * 20
+    t = _inputs(sum(lengths), 8, 4, d, type, left, 32)
+    bucket_of = _bucket_of("log")
+    first = _run(t, lengths, True, None, False, bucket_of)
+    want, off = attention(t["q"], t["k"], t["v"], lengths, None, False, None, t["table"], bucket_of, t["do"])
+    for n, v in first.items():
+        check(v, want[n], off[n], n)
+    for _ in range(5):
+        for n, v in _run(t, lengths, True, None, False, bucket_of).items():
+            assert torch.equal(v, first[n]), n
+        assert blocks.read_status(DEV) == 0
+
+
 def test_a_masked_packed_batch():
     lengths = [200, 0, 77, 130]
     t = _inputs(sum(lengths) + 9, 4, 4, 48, torch.float16, 5, 65)
