@@ -240,12 +240,18 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
         if (lane == 0) mbar_arrive(scores_read(t));
       }
       float factor = scale;
-      if (near || scale <= 0.f) {
+      if (near) {
         const float* b = bias + (p.reach + 255) + d0 - row;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[i][c] = __float_as_uint(fmaf(__uint_as_float(v[i][c]), scale, near ? b[i * 32 + c] : 0.f));
+          for (int c = 0; c < 32; ++c) v[i][c] = __float_as_uint(fmaf(__uint_as_float(v[i][c]), scale, b[i * 32 + c]));
+        factor = 1.f;
+      } else if (scale <= 0.f) {  // (the greatest score is not that of the greatest product)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[i][c] = __float_as_uint(__uint_as_float(v[i][c]) * scale);
         factor = 1.f;
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (a chain of dependent instructions costs more than they have)
