@@ -309,11 +309,23 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(read);
-      const float factor = near ? 1.f : scale, shift = add - lse;
+      float factor = scale;
+      const float shift = add - lse;
       if (near) {
         const float* b = bias + (p.reach + 255) + d0 - row;
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(fmaf(__uint_as_float(v[k]), scale, b[k]));
+        factor = 1.f;
+      }
+      if (counts != ~0u) {
+        // (what does not count may be anything: the products are taken out before they meet numbers)
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const bool there_k = counts >> k & 1u;
+          v[k] = there_k ? __float_as_uint(__uint_as_float(v[k]) * factor) : 0xFF800000u;
+          g[k] = there_k ? g[k] : 0u;
+        }
+        factor = 1.f;
       }
       const float2 factor2 = make_float2(factor, factor), shift2 = make_float2(shift, shift);
       uint32_t w[16];
@@ -322,11 +334,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
         float2 e = __ffma2_rn(make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), factor2, shift2);
         e.x = exp2_approx(e.x);
         e.y = exp2_approx(e.y);
-        float2 ds = __fmul2_rn(e, __ffma2_rn(make_float2(__uint_as_float(g[2 * k]), __uint_as_float(g[2 * k + 1])), c2, minus_delta));
-        if (counts != ~0u) {
-          if (!(counts >> (2 * k) & 1u)) ds.x = e.x = 0.f;
-          if (!(counts >> (2 * k + 1) & 1u)) ds.y = e.y = 0.f;
-        }
+        const float2 ds = __fmul2_rn(e, __ffma2_rn(make_float2(__uint_as_float(g[2 * k]), __uint_as_float(g[2 * k + 1])), c2, minus_delta));
         w[k] = pack_pair<F16>(ds);
         v[2 * k] = __float_as_uint(e.x), v[2 * k + 1] = __float_as_uint(e.y);
         g[2 * k] = __float_as_uint(ds.x), g[2 * k + 1] = __float_as_uint(ds.y);
@@ -441,8 +449,9 @@ struct AtDkv {
   static constexpr int kStageBytes = HALVES * kAtTileBytes;
   static constexpr uint32_t kScores = 0, kGrad = 128, kProbs = kOver ? 0 : 256, kDs = kOver ? 128 : 320, kDv = kOver ? 256 : 384, kDk = kOver ? 384 : 448;
   static constexpr int kBars = 2 * HALVES * kAtTileBytes + kStages * kStageBytes;
-  static constexpr int kRows = kBars + 320;       // two buffers of what a tile's queries have: -lse, -delta
-  static constexpr int kBias = kRows + 2 * 2 * 128 * 4;
+  static constexpr int kRowBuffers = 4;
+  static constexpr int kRows = kBars + 320;       // of what a tile's queries have: -lse, -delta
+  static constexpr int kBias = kRows + kRowBuffers * 2 * 128 * 4;
   static int smem(bool table, int reach) { return 1024 + kBias + (table ? attention_bias_entries(reach) * 4 : 0); }
 };
 
@@ -459,9 +468,9 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
   auto empty = [&](int s) { return bars + 8u * (2 * ST + s); };
   const uint32_t k_ready = bars + 8u * (3 * ST), formed = k_ready + 8, read = k_ready + 16, ds_ready = k_ready + 24, ds_done = k_ready + 32;
   auto rows_ready = [&](int b) { return k_ready + 40 + 8u * b; };
-  auto rows_free = [&](int b) { return k_ready + 56 + 8u * b; };
-  static_assert(8 * (3 * ST + 9) <= 240, "barriers");
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBars + 240);
+  auto rows_free = [&](int b) { return k_ready + 40 + 8u * (C::kRowBuffers + b); };
+  static_assert(8 * (3 * ST + 5 + 2 * C::kRowBuffers) <= 256 && sizeof(AttentionPlace) + 12 <= 64, "barriers");
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBars + 256 + sizeof(AttentionPlace));
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* const ds_scale_s = reinterpret_cast<float*>(tmem_slot + 2);
   int* const status = &tokens_status;
@@ -483,7 +492,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
     mbar_init(read, kAtBackWarps);
     mbar_init(ds_ready, kAtBackWarps);
     mbar_init(ds_done, 1);
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < C::kRowBuffers; ++b) {
       mbar_init(rows_ready(b), 1);
       mbar_init(rows_free(b), kAtBackWarps);
     }
@@ -599,39 +608,39 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
         if (!ok) break;
       }
     } else if (warp == rows_warp) {
-      // what a tile's queries have: -lse (with the outer bucket's bias, where the whole tile is in one) and -delta, a buffer ahead
-      int head = kv_head * group, tile = first_tile;
-      float low = 0.f, high = 0.f;
+      // what a tile's queries have: -lse (with the outer bucket's bias, where the whole tile is in one) and -delta; the next tile's are on
+      // their way while this one's are written
       const float held = F16 ? *ds_scale_s * (1.f / 32768.f) : 1.f;
+      int head = kv_head * group, tile = first_tile;
+      float low = 0.f, high = 0.f, l[4], d[4];
+      auto fetch = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int query = tile * kAtTile + i * 32 + lane;
+          const long long at = head * p.rows + place.first + query;
+          l[i] = query < length ? __ldcg(p.lse + at) : INFINITY;
+          d[i] = query < length ? __ldcg(p.delta + at) : 0.f;
+        }
+      };
+      if (n > 0) fetch();
       for (int u = 0; u < n; ++u) {
         if (p.table != nullptr && tile == first_tile) {
           low = attention_bias(p, -p.reach, head, F16) * kLog2e;
           high = attention_bias(p, p.reach, head, F16) * kLog2e;
         }
-        const int q0 = tile * kAtTile, d0 = key0 - q0;
-        const float add = p.table == nullptr || attention_near(p, d0) ? 0.f : d0 > 0 ? high : low;
-        float l[4], d[4];
+        const int d0 = key0 - tile * kAtTile, buffer = u % C::kRowBuffers;
+        const float add = (F16 ? 15.f : 0.f) + (p.table == nullptr || attention_near(p, d0) ? 0.f : d0 > 0 ? high : low);
+        float* const rows = of_rows + buffer * 256;
+        if (u >= C::kRowBuffers && !mbar_wait_warp(rows_free(buffer), ((u / C::kRowBuffers) & 1) ^ 1, abort_flag, status, kDevTimeoutStats)) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int query = q0 + i * 32 + lane;
-          l[i] = -INFINITY;
-          d[i] = 0.f;
-          if (query < length) {
-            const long long at = head * p.rows + place.first + query;
-            l[i] = (F16 ? 15.f : 0.f) + add - __ldcg(p.lse + at);
-            d[i] = -__ldcg(p.delta + at) * held;
-          }
-        }
-        if (u >= 2 && !mbar_wait_warp(rows_free(u & 1), ((u >> 1) & 1) ^ 1, abort_flag, status, kDevTimeoutStats)) break;
-        float* const rows = of_rows + (u & 1) * 256;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          rows[i * 32 + lane] = l[i];
-          rows[128 + i * 32 + lane] = d[i];
+          rows[i * 32 + lane] = add - l[i];
+          rows[128 + i * 32 + lane] = -d[i] * held;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(rows_ready(u & 1));
+        if (lane == 0) mbar_arrive(rows_ready(buffer));
         if (++tile == first_tile + tiles) tile = first_tile, ++head;
+        if (u + 1 < n) fetch();
       }
     }
   } else {
@@ -653,8 +662,9 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
         named_bar_sync(1, kAtBackWarps * 32);
       }
       const bool near = p.table != nullptr && attention_near(p, d0);
+      const int buffer = u % C::kRowBuffers;
       if (++tile == first_tile + tiles) tile = first_tile, ++head;
-      ok = mbar_wait_warp(rows_ready(u & 1), (u >> 1) & 1, abort_flag, status, kDevTimeoutEpilogue);
+      ok = mbar_wait_warp(rows_ready(buffer), (u / C::kRowBuffers) & 1, abort_flag, status, kDevTimeoutEpilogue);
       ok = mbar_wait_warp(formed, u & 1, abort_flag, status, kDevTimeoutEpilogue) && ok;
       tc_fence_after();
       uint32_t v[32], g[32];
@@ -668,15 +678,24 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
       } else {
         named_bar_sync(2 + (warp & 3), 128);  // all of a row's columns have been read before results go over them
       }
-      const float factor = near ? 1.f : scale;
+      float factor = scale;
       if (near) {
         const float* b = bias + (p.reach + 255) + d0 + row - quarter * 32;
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(fmaf(__uint_as_float(v[k]), scale, b[-k]));
+        factor = 1.f;
+      }
+      if (p.causal && d0 == 0) {  // queries before the key do not count
+        const int first = row - quarter * 32;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          v[k] = k >= first ? __float_as_uint(__uint_as_float(v[k]) * factor) : 0xFF800000u;
+          g[k] = k >= first ? g[k] : 0u;
+        }
+        factor = 1.f;
       }
       const float2 factor2 = make_float2(factor, factor);
-      const int first = p.causal ? k_row - q0 - quarter * 32 : -1;  // the first of this thread's columns that counts
-      const float* const rows = of_rows + (u & 1) * 256 + quarter * 32;
+      const float* const rows = of_rows + buffer * 256 + quarter * 32;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t w[8], x[8];
@@ -690,9 +709,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
             float2 e = __ffma2_rn(make_float2(__uint_as_float(v[col]), __uint_as_float(v[col + 1])), factor2, q == 0 ? make_float2(l.x, l.y) : make_float2(l.z, l.w));
             e.x = exp2_approx(e.x);
             e.y = exp2_approx(e.y);
-            float2 ds = __fmul2_rn(e, __ffma2_rn(make_float2(__uint_as_float(g[col]), __uint_as_float(g[col + 1])), held2, q == 0 ? make_float2(d.x, d.y) : make_float2(d.z, d.w)));
-            if (col < first) e.x = ds.x = 0.f;
-            if (col + 1 < first) e.y = ds.y = 0.f;
+            const float2 ds = __fmul2_rn(e, __ffma2_rn(make_float2(__uint_as_float(g[col]), __uint_as_float(g[col + 1])), held2, q == 0 ? make_float2(d.x, d.y) : make_float2(d.z, d.w)));
             w[k + q] = pack_pair<F16>(e);
             x[k + q] = pack_pair<F16>(ds);
           }
@@ -708,7 +725,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(rows_free(u & 1));
+        mbar_arrive(rows_free(buffer));
         mbar_arrive(ds_ready);
       }
     }
