@@ -286,9 +286,9 @@ __global__ void __launch_bounds__(kPositionWarps * 32, 1) position_backward_kern
     if (begin + 1 < last) ask(begin + 1), b.bucket = find(begin + 1);
   }
   auto step = [&](long long unit, Unit& now, Unit& next) {
-    if (unit + 1 < last) fetch(unit + 1, next);
     const bool more = unit + 2 < last;
-    if (more) ask(unit + 2);
+    if (more) ask(unit + 2);  // (in front of the values: they come in the order they were asked for)
+    if (unit + 1 < last) fetch(unit + 1, next);
     add(now);
     if (more) now.bucket = find(unit + 2);
   };
