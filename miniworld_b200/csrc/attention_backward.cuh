@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int load_warp = kAtBackWarps, mma_warp = load_warp + 1, clean_warp = load_warp + 2;
-  const int head = blockIdx.y, kv_head = head / (p.heads / p.kv_heads);
+  const int head = attention_block_head(p.heads), kv_head = head / (p.heads / p.kv_heads);
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(landed(s), 1);
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
   }
   grid_dependency_wait();
   grid_dependents_launch();
-  const int place_index = static_cast<int>(p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  const long long place_index = attention_block_place(p, p.heads, p.causal);
   if (warp == 0) {
     const AttentionPlace r = attention_place(p, place_index, kAtTile);
     if (lane == 0) *place_s = r;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
       // ds of a row adds up to nothing but what delta is off by: its share, by the probabilities' mass, comes off the outer buckets, of
       // whose terms most are of one sign otherwise
       float* const rows = all_distances + kAtBackWarps * distances;
-      float* const out = p.partial + (static_cast<long long>(head) * gridDim.x + place_index) * distances;
+      float* const out = p.partial + (head * p.places + place_index) * distances;
       if (n > 0) {
         rows[quarter * 128 + row] = all;
         named_bar_sync(1, kAtBackWarps * 32);
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int load_warp = kAtBackWarps, mma_warp = load_warp + 1, clean_warp = load_warp + 2, rows_warp = load_warp + 3;
-  const int kv_head = blockIdx.y, group = p.heads / p.kv_heads;
+  const int kv_head = attention_block_head(p.kv_heads), group = p.heads / p.kv_heads;
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(landed(s), 1);
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
   grid_dependency_wait();
   grid_dependents_launch();
   if (warp == 0) {
-    const AttentionPlace r = attention_place(p, blockIdx.x, kAtTile);
+    const AttentionPlace r = attention_place(p, attention_block_place(p, p.kv_heads, false), kAtTile);
     if (lane == 0) *place_s = r;
   }
   if (F16 && warp == 1) {

@@ -86,8 +86,7 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
   }
   grid_dependency_wait();
   grid_dependents_launch();
-  // (the longest rows of a causal sequence first)
-  const long long place_index = p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const long long place_index = attention_block_place(p, p.heads, p.causal);
   if (warp == 0) {
     const AttentionPlace r = attention_place(p, place_index, T * kAtTile);
     if (lane == 0) *place_s = r;
@@ -97,7 +96,7 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const AttentionPlace place = *place_s;
-  const int head = blockIdx.y, kv_head = head / (p.heads / p.kv_heads);
+  const int head = attention_block_head(p.heads), kv_head = head / (p.heads / p.kv_heads);
   const int length = static_cast<int>(place.last - place.first);
   // key tiles of query tile t
   auto tiles_of = [&](int t) {

@@ -79,6 +79,13 @@ __host__ __device__ inline long long attention_places(const int* offsets, long l
   if (offsets == nullptr) return static_cast<long long>(sequences) * ((length + tile_rows - 1) / tile_rows);
   return rows / tile_rows + sequences + 1;
 }
+// The heads of a place one after the other: their rows lie side by side in memory (512 x 384 tokens, 8 heads of 32: see the forward), and
+// the longest rows of all heads of a causal sequence come first.
+__device__ __forceinline__ int attention_block_head(int heads) { return static_cast<int>(blockIdx.x % static_cast<unsigned>(heads)); }
+__device__ __forceinline__ long long attention_block_place(const AttentionParams& p, int heads, bool last_first) {
+  const long long at = blockIdx.x / static_cast<unsigned>(heads);
+  return last_first ? p.places - 1 - at : at;
+}
 // by a whole warp
 __device__ __forceinline__ AttentionPlace attention_place(const AttentionParams& p, long long place, int tile_rows) {
   AttentionPlace r;

@@ -41,6 +41,7 @@ static int check_attention(const b200_attention_call* c) {
   if (c->d < 8 || c->d > B200_ATTENTION_MAX_WIDTH || c->d % 8 != 0 || c->heads > 32768) return B200_TRIMUL_E_UNSUPPORTED;
   if (c->dtype != B200_BLOCKS_BF16 && c->dtype != B200_BLOCKS_F16) return B200_TRIMUL_E_UNSUPPORTED;
   if (c->rows * c->heads > (1ll << 40) / c->d) return B200_TRIMUL_E_SHAPE;
+  if (attention_places(c->offsets, c->rows, c->sequences, c->length, kAtTile) * c->heads > 0x7FFFFFFFll) return B200_TRIMUL_E_SHAPE;  // (blocks)
   if (!(c->scale == c->scale) || c->scale - c->scale != 0.f) return B200_TRIMUL_E_UNSUPPORTED;
   if (c->table != nullptr) {
     if (c->bucket_of == nullptr) return B200_TRIMUL_E_NULL;
@@ -87,13 +88,13 @@ static int attention_map(CUtensorMap* m, const AttentionTensor& t, long long row
   return make_map(m, t.base, 3, dims, strides, box);
 }
 template <bool F16, int HALVES>
-static int launch_attention_forward(const AttentionMaps& maps, const AttentionParams& p, const DeviceInfo& info, cudaStream_t stream) {
+static int launch_attention_forward(const AttentionMaps& maps, AttentionParams p, const DeviceInfo& info, cudaStream_t stream) {
   using C = AtForward<HALVES>;
   const auto kernel = attention_forward_kernel<F16, HALVES>;
   const int rc = set_smem(kernel, C::smem(true, B200_POSITION_MAX_REACH), info.device);
   if (rc != 0) return rc;
-  const long long places = attention_places(p.offsets, p.rows, p.sequences, p.length, C::kTiles * kAtTile);
-  TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(places), p.heads), C::kThreads, C::smem(p.table != nullptr, p.reach), stream, maps, p));
+  p.places = attention_places(p.offsets, p.rows, p.sequences, p.length, C::kTiles * kAtTile);
+  TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(p.places * p.heads)), C::kThreads, C::smem(p.table != nullptr, p.reach), stream, maps, p));
   return B200_TRIMUL_OK;
 }
 static int attention_delta_blocks(long long rows, int d) {
@@ -111,8 +112,8 @@ static int launch_attention_backward(const AttentionMaps& maps, const AttentionP
   if (rc != 0) return rc;
   const bool table = p.table != nullptr;
   TRIMUL_CUDA(launch_overlapped(attention_delta_kernel<T>, dim3(p.delta_blocks, p.kv_heads), kAtDeltaThreads, 0, stream, p));
-  TRIMUL_CUDA(launch_overlapped(dq, dim3(static_cast<unsigned>(p.places), p.heads), kAtBackThreads, AtDq<HALVES>::smem(table, p.reach), stream, maps, p));
-  TRIMUL_CUDA(launch_overlapped(dkv, dim3(static_cast<unsigned>(p.places), p.kv_heads), kAtBackThreads, AtDkv<HALVES>::smem(table, p.reach), stream, maps, p));
+  TRIMUL_CUDA(launch_overlapped(dq, dim3(static_cast<unsigned>(p.places * p.heads)), kAtBackThreads, AtDq<HALVES>::smem(table, p.reach), stream, maps, p));
+  TRIMUL_CUDA(launch_overlapped(dkv, dim3(static_cast<unsigned>(p.places * p.kv_heads)), kAtBackThreads, AtDkv<HALVES>::smem(table, p.reach), stream, maps, p));
   if (p.partial != nullptr)
     TRIMUL_CUDA(launch_overlapped(p.wide_table ? attention_table_kernel<float> : attention_table_kernel<T>, dim3(p.heads), 1024, 0, stream, p));
   return B200_TRIMUL_OK;
