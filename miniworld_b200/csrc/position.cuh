@@ -228,17 +228,22 @@ __global__ void __launch_bounds__(kPositionWarps * 32, 1) position_backward_kern
     const long long row = unit / runs;
     const int j0 = static_cast<int>(unit - row * runs) * R, most = p.n - 1 - j0;
     const T* at = dy + (row * p.n + j0) * p.c + c;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const T* from = at + static_cast<long long>(min(i, most)) * p.c;  // (positions past the row's end: its last, not added)
+    auto read = [&](const T* from) -> Word {
       if constexpr (V == 2) {
-        u.v[i] = __ldcg(reinterpret_cast<const Word*>(from));
+        return __ldcg(reinterpret_cast<const Word*>(from));
       } else if constexpr (sizeof(T) == 4) {
-        u.v[i] = make_uint2(__ldcg(reinterpret_cast<const uint32_t*>(from)), second ? __ldcg(reinterpret_cast<const uint32_t*>(from) + 1) : 0u);
+        return make_uint2(__ldcg(reinterpret_cast<const uint32_t*>(from)), second ? __ldcg(reinterpret_cast<const uint32_t*>(from) + 1) : 0u);
       } else {
         const unsigned short* at16 = reinterpret_cast<const unsigned short*>(from);
-        u.v[i] = __ldcg(at16) | (second ? static_cast<uint32_t>(__ldcg(at16 + 1)) << 16 : 0u);
+        return __ldcg(at16) | (second ? static_cast<uint32_t>(__ldcg(at16 + 1)) << 16 : 0u);
       }
+    };
+    if (most >= R - 1) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) u.v[i] = read(at + i * p.c);
+    } else {  // (positions past the row's end: its last, not added)
+#pragma unroll
+      for (int i = 0; i < R; ++i) u.v[i] = read(at + min(i, most) * p.c);
     }
   };
   // its tokens, a lane a position, are asked for a unit before that, and their buckets found after the work on the unit between
