@@ -79,8 +79,8 @@ __host__ __device__ inline long long attention_places(const int* offsets, long l
   if (offsets == nullptr) return static_cast<long long>(sequences) * ((length + tile_rows - 1) / tile_rows);
   return rows / tile_rows + sequences + 1;
 }
-// The heads of a place one after the other: their rows lie side by side in memory (512 x 384 tokens, 8 heads of 32: see the forward), and
-// the longest rows of all heads of a causal sequence come first.
+// The heads of a place one after the other: their rows lie side by side in memory, and the longest rows of all heads of a causal sequence come
+// first (38009 packed tokens, causal, 16 heads of 128: 847 -> 797 us against all places of a head first).
 __device__ __forceinline__ int attention_block_head(int heads) { return static_cast<int>(blockIdx.x % static_cast<unsigned>(heads)); }
 __device__ __forceinline__ long long attention_block_place(const AttentionParams& p, int heads, bool last_first) {
   const long long at = blockIdx.x / static_cast<unsigned>(heads);

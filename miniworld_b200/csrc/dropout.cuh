@@ -94,8 +94,9 @@ __device__ __forceinline__ void drop_eight(const DropoutParams& p, uint4 r, Eigh
   u.store(y);
 }
 
-// No rows share: a thread takes a few groups of eight elements and draws their numbers while the elements are on their way. HBM bound;
-// about 10 instructions an element, 5 of them the generator.
+// No rows share: a thread takes a few groups of eight elements and draws their numbers while the elements are on their way. HBM bound
+// (about 10 instructions an element, 5 of them the generator: issue 53 % busy): 16384 x 1024 fp16 23 us with the residual, 20 without,
+// where 100 and 67 MB have to move; with one group a thread whose numbers came first 55 and 36.
 template <typename T, bool RESIDUAL>
 __global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const DropoutParams p) {
   grid_dependency_wait();
@@ -129,7 +130,8 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const DropoutP
   }
 }
 
-// Rows share a mask and have whole groups of eight: a thread draws a group's numbers once for `chunk` rows.
+// Rows share a mask and have whole groups of eight: a thread draws a group's numbers once for `chunk` rows. 384 x 384 x 128 bf16, a
+// mask for 384 rows: 23 us with the residual (113 MB), 18 to 20 without (75 MB).
 template <typename T, bool RESIDUAL>
 __global__ void __launch_bounds__(kDropoutThreads) dropout_shared_kernel(const DropoutParams p) {
   grid_dependency_wait();
