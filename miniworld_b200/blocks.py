@@ -118,7 +118,7 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offset
     ``offsets`` (integers [sequences + 1], the first 0, non-decreasing) the tokens of ``q`` [tokens, heads, d] are packed sequences: the
     rows ``offsets[s] .. offsets[s + 1]`` are sequence ``s``, of any length; rows behind the last one come out zero. ``mask`` over the
     tokens: those with zero are not attended to and come out zero, whatever they hold, with zero gradients. ``causal``: a token attends
-    to itself and the ones before it. ``scale`` defaults to ``d ** -0.5``. ``table`` [buckets, heads] (q's type or fp32) with ``bucket_of``
+    to itself and the ones before it (a value that is not finite at a later token may reach earlier ones all the same). ``scale`` defaults to ``d ** -0.5``. ``table`` [buckets, heads] (q's type or fp32) with ``bucket_of``
     (:func:`relative_buckets`): ``table[bucket_of[clip(j - i, -reach, reach) + reach], head]`` is added to the score of query ``i`` and
     key ``j`` of a sequence.
 

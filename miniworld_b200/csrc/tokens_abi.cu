@@ -87,11 +87,22 @@ static int attention_map(CUtensorMap* m, const AttentionTensor& t, long long row
   const uint32_t box[3] = {64, 1, kAtTile};
   return make_map(m, t.base, 3, dims, strides, box);
 }
+// The warps that take registers wait until others have given them up: the sum of their shares must be what the block is launched with,
+// whatever the compiler has made of the launch bounds (asked once a kernel).
+template <auto KERNEL, int WARPGROUPS, int MANY, int FEW>
+static int check_registers() {
+  static const int registers = [] {
+    cudaFuncAttributes a = {};
+    return cudaFuncGetAttributes(&a, KERNEL) == cudaSuccess ? a.numRegs : 0;
+  }();
+  return registers * WARPGROUPS >= (WARPGROUPS - 1) * MANY + FEW ? B200_TRIMUL_OK : B200_TRIMUL_E_UNSUPPORTED;
+}
 template <bool F16, int HALVES>
 static int launch_attention_forward(const AttentionMaps& maps, AttentionParams p, const DeviceInfo& info, cudaStream_t stream) {
   using C = AtForward<HALVES>;
   const auto kernel = attention_forward_kernel<F16, HALVES>;
-  const int rc = set_smem(kernel, C::smem(true, B200_POSITION_MAX_REACH), info.device);
+  int rc = set_smem(kernel, C::smem(true, B200_POSITION_MAX_REACH), info.device);
+  if (rc == 0) rc = check_registers<attention_forward_kernel<F16, HALVES>, C::kThreads / 128, C::kMany, C::kFew>();
   if (rc != 0) return rc;
   p.places = attention_places(p.offsets, p.rows, p.sequences, p.length, C::kTiles * kAtTile);
   TRIMUL_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(p.places * p.heads)), C::kThreads, C::smem(p.table != nullptr, p.reach), stream, maps, p));
@@ -109,6 +120,8 @@ static int launch_attention_backward(const AttentionMaps& maps, const AttentionP
   const auto dkv = attention_dkv_kernel<F16, HALVES>;
   int rc = set_smem(dq, AtDq<HALVES>::smem(true, B200_POSITION_MAX_REACH), info.device);
   if (rc == 0) rc = set_smem(dkv, AtDkv<HALVES>::smem(true, B200_POSITION_MAX_REACH), info.device);
+  if (rc == 0) rc = check_registers<attention_dq_kernel<F16, HALVES>, kAtBackThreads / 128, kAtBackMany, kAtBackFew>();
+  if (rc == 0) rc = check_registers<attention_dkv_kernel<F16, HALVES>, kAtBackThreads / 128, kAtBackMany, kAtBackFew>();
   if (rc != 0) return rc;
   const bool table = p.table != nullptr;
   TRIMUL_CUDA(launch_overlapped(attention_delta_kernel<T>, dim3(p.delta_blocks, p.kv_heads), kAtDeltaThreads, 0, stream, p));
