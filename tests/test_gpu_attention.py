@@ -67,6 +67,31 @@ def test_lengths(m, causal):
     _compare(_inputs(2 * m, 2, 2, 32, torch.bfloat16, m, 65), [m] * 2, causal=causal, bias="near")
 
 
+@pytest.mark.parametrize("m", [1, 2, 63, 64, 65, 127, 128, 129, 192, 200, 255, 256, 257, 384, 385, 512, 640])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
+def test_lengths_of_wide_heads(m, causal, type):
+    """Widths beyond 64: two query tiles to a block, of which the second may be short or not there."""
+    _compare(_inputs(2 * m, 4, 2, 96, type, m, 65), [m] * 2, causal=causal, bias="near")
+
+
+@pytest.mark.parametrize("kind", ["tail", "holes", "first", "none"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d,type", [(128, torch.bfloat16), (72, torch.float16)])
+def test_masks_of_wide_heads_in_packed_sequences(kind, causal, d, type):
+    lengths = [300, 5, 0, 129, 256]
+    rows = sum(lengths) + 50
+    place = torch.arange(rows, device=DEV)
+    mask = {"tail": place % 300 < 220, "holes": torch.rand(rows, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV) > 0.3,
+            "first": place % 300 > 140, "none": place < 0}[kind]
+    t = _inputs(rows, 8, 2, d, type, 7, 32)
+    for n in ("q", "k", "v", "do"):
+        t[n][~mask] = float("nan")
+    got = _compare(t, lengths, packed=True, mask=mask, causal=causal, bias="log")
+    for n in ("o", "q", "k", "v"):
+        assert not got[n][~mask].any() and not got[n][sum(lengths):].any()
+
+
 @pytest.mark.parametrize("d", [8, 16, 24, 32, 40, 48, 56, 64, 72, 80, 96, 104, 120, 128])
 @pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
 def test_widths(d, type):
