@@ -100,17 +100,23 @@ __device__ __forceinline__ AttentionPlace attention_place(const AttentionParams&
   }
   const int lane = threadIdx.x & 31;
   int lo = 0, n = p.sequences + 1;  // the sequence is one of lo .. lo + n - 1
-  while (n > 1) {
+  while (n > 32) {
     const int step = (n + 31) / 32, at = lane * step;
     const bool before = at < n && attention_offset(p, lo + at) / tile_rows + lo + at <= place;
     const int at_most = max(__popc(__ballot_sync(0xFFFFFFFFu, before)) - 1, 0) * step;
     lo += at_most;
     n = min(step, n - at_most);
   }
-  r.first = attention_offset(p, lo);
-  r.last = lo < p.sequences ? attention_offset(p, lo + 1) : p.rows;
-  r.tile = static_cast<int>(max(place - (r.first / tile_rows + lo), 0ll));
-  r.behind = lo == p.sequences;
+  // (the offsets of the last candidates are those of the sequence found: no load follows another here)
+  const long long offset = attention_offset(p, min(lo + lane, p.sequences));
+  const bool before = lane < n && offset / tile_rows + lo + lane <= place;
+  const int found = max(__popc(__ballot_sync(0xFFFFFFFFu, before)) - 1, 0), s = lo + found;
+  r.first = __shfl_sync(0xFFFFFFFFu, offset, found);
+  r.last = __shfl_sync(0xFFFFFFFFu, offset, min(found + 1, 31));
+  if (s == p.sequences) r.last = p.rows;
+  else if (found == 31) r.last = attention_offset(p, s + 1);
+  r.tile = static_cast<int>(max(place - (r.first / tile_rows + s), 0ll));
+  r.behind = s == p.sequences;
   return r;
 }
 
