@@ -298,3 +298,34 @@ def test_bucket_numbers_beyond_the_table_stay_inside():
     o = blocks.token_attention(q, q, q, table=table, bucket_of=where)
     (g,) = torch.autograd.grad(o.float().sum(), table)
     assert torch.isfinite(o).all() and torch.isfinite(g).all()
+
+
+@pytest.mark.parametrize("shape", [(5, 0, 2, 16), (0, 2, 16), (2, 0, 3, 4, 128), (3, 2, 0, 1, 8)])
+def test_calls_without_tokens_in_any_dimension(shape):
+    q = torch.zeros(shape, device=DEV, dtype=torch.float16, requires_grad=True)
+    for mask in (None, torch.ones(shape[:-2], device=DEV)):
+        o = blocks.token_attention(q, q, q, mask=mask)
+        (g,) = torch.autograd.grad(o, q, torch.zeros_like(o))
+        assert o.shape == g.shape == shape
+
+
+@pytest.mark.parametrize("d", [32, 96])
+def test_backward_of_offsets_that_mean_nothing_stays_inside(d):
+    """As the forward's: in bounds whatever the offsets are, and tensors beside the inputs and the table keep their values."""
+    around = torch.zeros(3, 300, 2, d, dtype=torch.bfloat16, device=DEV)
+    q, table = around[1].requires_grad_(True), torch.zeros(9, 2, device=DEV, requires_grad=True)
+    where = blocks.relative_buckets(4, device=DEV)
+    many = torch.randint(-400, 700, (1200,), generator=torch.Generator().manual_seed(3)).tolist()
+    for ends in ([0, 150, 1000], [0, -7, 300], [0, 280, 20, 300], [5, 250, 300], [0, 2**31 - 1], [0, -(2**31), 30], many, many[:33], many[:32]):
+        o = blocks.token_attention(q, q, q, offsets=torch.tensor(ends, dtype=torch.int32, device=DEV), table=table, bucket_of=where)
+        g = torch.autograd.grad(o, [q, table], torch.ones_like(o))
+        assert g[0].shape == q.shape
+    torch.cuda.synchronize()
+    assert not around.detach().any() and not table.detach().any()
+
+
+def test_many_sequences_of_every_count():
+    """The search for a block's sequence in up to 32 candidates, and in rounds above: 31 to 34 and 1023 to 1026 sequences."""
+    for count in (31, 32, 33, 34, 63, 64, 1023, 1024, 1025, 1026):
+        lengths = [(7 * i) % 5 + (140 if i in (0, 30, 31, 32, count - 1) else 0) for i in range(count)]
+        _compare(_inputs(sum(lengths) + 3, 1, 1, 16, torch.bfloat16, count), lengths, packed=True)
