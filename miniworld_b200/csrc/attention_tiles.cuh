@@ -115,7 +115,8 @@ __device__ __forceinline__ AttentionPlace attention_place(const AttentionParams&
   r.last = __shfl_sync(0xFFFFFFFFu, offset, min(found + 1, 31));
   if (s == p.sequences) r.last = p.rows;
   else if (found == 31) r.last = attention_offset(p, s + 1);
-  r.tile = static_cast<int>(max(place - (r.first / tile_rows + s), 0ll));
+  // (offsets out of order may leave any number of places to a sequence: its rows are counted in 32 bits)
+  r.tile = static_cast<int>(min(max(place - (r.first / tile_rows + s), 0ll), p.rows / tile_rows + 1));
   r.behind = s == p.sequences;
   return r;
 }
