@@ -611,6 +611,13 @@ class SandwichTransition(nn.Module):
         return self.join(x, self.feed_forward(self.ln_in(x)), gate, mask)
 
 
+def _table_rows(bucket_of: torch.Tensor, more: int) -> int:
+    rows = int(bucket_of.max()) + 1 + more
+    if rows > 512:
+        raise ValueError(f"tables of up to 512 buckets are implemented, this reach needs {rows}")
+    return rows
+
+
 class TokenAttention(nn.Module):
     """Attention among the tokens of a sequence, ``forward(q, k, v, mask=None, offsets=None)``
     (:func:`miniworld_b200.blocks.token_attention`), with a learned bias of the relative position: ``table`` [buckets, heads], kept in
@@ -622,7 +629,7 @@ class TokenAttention(nn.Module):
         self.heads, self.causal, self.scale, self.check_status = heads, bool(causal), scale, bool(check_status)
         bucket_of = None if reach is None else blocks.relative_buckets(reach, exact)
         self.register_buffer("bucket_of", bucket_of, persistent=False)
-        self.table = None if bucket_of is None else nn.Parameter(torch.zeros(int(bucket_of.max()) + 1, heads))
+        self.table = None if bucket_of is None else nn.Parameter(torch.zeros(_table_rows(bucket_of, 0), heads))
 
     def _apply(self, fn, recurse=True):
         return super()._apply(_pinned(fn), recurse)
@@ -645,7 +652,7 @@ class RelativePosition(nn.Module):
         super().__init__()
         bucket_of = blocks.relative_buckets(reach, exact)
         self.register_buffer("bucket_of", bucket_of, persistent=False)
-        self.table = nn.Parameter(torch.empty(int(bucket_of.max()) + 2, d_pair))
+        self.table = nn.Parameter(torch.empty(_table_rows(bucket_of, 1), d_pair))
         nn.init.normal_(self.table, std=0.02)
 
     def _apply(self, fn, recurse=True):
@@ -657,8 +664,8 @@ class RelativePosition(nn.Module):
 
 class BlockDropout(nn.Module):
     """The residual add of a block's output with dropout, ``forward(x, u, key=None) -> x + keep * u / (1 - p)`` in training and ``x + u``
-    otherwise (:func:`miniworld_b200.blocks.block_dropout`). ``shared`` names a dimension whose rows use one mask; ``key`` defaults to
-    a new one from PyTorch's generator."""
+    otherwise, in ``x``'s type (``x`` None: without it; :func:`miniworld_b200.blocks.block_dropout`). ``shared`` names a dimension whose
+    rows use one mask; ``key`` defaults to a new one from PyTorch's generator."""
 
     def __init__(self, p: float, shared: Optional[int] = None):
         super().__init__()
@@ -666,10 +673,10 @@ class BlockDropout(nn.Module):
             raise ValueError(f"p must be from 0 to 1, got {p}")
         self.p, self.shared = float(p), shared
 
-    def forward(self, x: torch.Tensor, u: torch.Tensor, key: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, x: Optional[torch.Tensor], u: torch.Tensor, key: Optional[torch.Tensor] = None) -> torch.Tensor:
         p = self.p if self.training else 0.0
         if p == 0.0:
-            return x + u
+            return u if x is None else x + u.to(x.dtype)
         return blocks.block_dropout(x, u, blocks.dropout_key(u.device) if key is None else key, p=p, shared=self.shared)
 
     def extra_repr(self) -> str:

@@ -161,3 +161,19 @@ def test_parameters_of_the_modules():
     assert {k: (tuple(v.shape), v.dtype) for k, v in m.state_dict().items()} == {"a.table": ((65, 8), torch.float32), "c.table": ((34, 64), torch.float32)}
     assert m["a"].bucket_of.dtype == m["c"].bucket_of.dtype == torch.int32 and m["b"].bucket_of is None
     assert m.to("meta")["a"].bucket_of.is_meta
+
+
+@pytest.mark.parametrize("u", [torch.float32, torch.float16, torch.bfloat16])
+def test_dropout_that_drops_nothing_keeps_the_type_of_training(u):
+    x, u = torch.randn(3, 4).bfloat16(), torch.randn(3, 4).to(u)
+    for m in (mw.BlockDropout(0.3).eval(), mw.BlockDropout(0.0)):
+        y = m(x, u)
+        assert y.dtype == x.dtype and torch.equal(y, x + u.bfloat16()) and torch.equal(m(None, u), u)
+
+
+def test_tables_that_no_kernel_takes_are_refused_at_once():
+    assert mw.TokenAttention(2, reach=255).table.shape == (511, 2) and mw.RelativePosition(8, reach=255).table.shape == (512, 8)
+    assert mw.TokenAttention(2, reach=256, exact=128).table.shape == (512, 2)
+    for build in (lambda: mw.TokenAttention(2, reach=256), lambda: mw.RelativePosition(8, reach=256), lambda: mw.RelativePosition(8, reach=256, exact=128)):
+        with pytest.raises(ValueError, match="512 buckets"):
+            build()
