@@ -26,7 +26,8 @@ constexpr int kAtDeltaThreads = 256;
 constexpr int kAtDeltaBlocks = 256;  // at most, of a key head
 
 // delta[h][row] = dO . o, from o before it was rounded: the rounded one's error, times the probabilities' mass, would stand in the
-// biases' gradients, where the true sums nearly cancel (4096 tokens: 0.027 of their norm). In fp16 also the greatest |dO|^2 and |v|^2.
+// biases' gradients, where the true sums nearly cancel (4096 tokens: 0.027 of their norm). In fp16 also the greatest |dO|^2 of the rows
+// that have keys, and |v|^2 of those that are keys: the two differ where biases of -inf leave a row without a key that others attend to.
 template <typename T>
 __global__ void __launch_bounds__(kAtDeltaThreads) attention_delta_kernel(const AttentionParams p) {
   constexpr bool f16 = __is_same(T, __half);
@@ -47,14 +48,13 @@ __global__ void __launch_bounds__(kAtDeltaThreads) attention_delta_kernel(const 
     const uint4 w = own ? __ldcg(reinterpret_cast<const uint4*>(at + lane * 8)) : make_uint4(0, 0, 0, 0);
     v[0] = unpack_pair<f16>(w.x), v[1] = unpack_pair<f16>(w.y), v[2] = unpack_pair<f16>(w.z), v[3] = unpack_pair<f16>(w.w);
   };
-  const long long rounds = (p.rows + step - 1) / step;
+  const long long rounds = (p.rows + step - 1) / step, keys_end = f16 && p.offsets != nullptr ? attention_offset(p, p.sequences) : p.rows;
   for (long long k = 0; k < rounds; ++k) {
     const long long row = k * step + static_cast<long long>(blockIdx.x) * (kAtDeltaThreads / team) + threadIdx.x / team;
     const bool inside = row < p.rows;
     const long long r = inside ? row : 0;
-    bool there = false;
     for (int h = kv_head * group; h < (kv_head + 1) * group; ++h) {
-      there = inside && __ldcg(p.lse + h * p.rows + r) != INFINITY;
+      const bool there = inside && __ldcg(p.lse + h * p.rows + r) != INFINITY;
       float2 g[4], o[4], e[4];
       values(attention_at<T>(p.dout, r, h), g);
       const long long at = (r * p.heads + h) * p.d;
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kAtDeltaThreads) attention_delta_kernel(const 
       float2 v[4];
       values(attention_at<T>(p.v, r, kv_head), v);
       float square = 0.f;
-      if (there) {
+      if (inside && row < keys_end && (p.mask == nullptr || __ldcg(p.mask + r) != 0)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) square = fmaf(v[i].x, v[i].x, fmaf(v[i].y, v[i].y, square));
       }
