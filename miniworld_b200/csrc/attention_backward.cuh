@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dq_kernel(const _
         for (int h = 0; h < HALVES; ++h)
           tma_load_3d(ring + s * C::kStageBytes + h * kAtTileBytes, value ? &maps.v : &maps.k, bar, h * 64, kv_head, static_cast<int>(place.first) + j * kAtTile);
       }
-      if (*abort_flag != 0) state.drain<ST>(q_ready, landed, ready);
+      state.drain<ST>(q_ready, landed, ready);
     } else if (warp == mma_warp && elect_one()) {
       constexpr uint32_t fmt = F16 ? kFmtF16 : kFmtBF16;
       constexpr uint32_t idesc_s = umma_idesc(128, 128, false, false, fmt, fmt);
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
           tma_load_3d(ring + s * C::kStageBytes + h * kAtTileBytes, grad ? &maps.dout : &maps.q, bar, h * 64, head, static_cast<int>(place.first) + tile * kAtTile);
         if (grad && ++tile == first_tile + tiles) tile = first_tile, ++head;
       }
-      if (*abort_flag != 0) state.drain<ST>(k_ready, landed, ready);
+      state.drain<ST>(k_ready, landed, ready);
     } else if (warp == mma_warp && elect_one()) {
       constexpr uint32_t fmt = F16 ? kFmtF16 : kFmtBF16;
       constexpr uint32_t idesc_s = umma_idesc(128, 128, false, false, fmt, fmt);

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(AtForward<HALVES>::kThreads, AtForward<HALVES>
         for (int h = 0; h < HALVES; ++h)
           tma_load_3d(ring + s * C::kStageBytes + h * kAtTileBytes, value ? &maps.v : &maps.k, bar, h * 64, kv_head, static_cast<int>(place.first) + j * kAtTile);
       }
-      if (*abort_flag != 0) state.drain<ST>(q_ready, landed, ready);
+      state.drain<ST>(q_ready, landed, ready);
     } else if (warp == mma_warp && elect_one()) {
       constexpr uint32_t fmt = F16 ? kFmtF16 : kFmtBF16;
       constexpr uint32_t idesc_s = umma_idesc(128, 128, false, false, fmt, fmt);

@@ -171,7 +171,8 @@ struct AttentionRing {
       landed |= bit;
     }
   }
-  // Copies that nothing has waited for (after a wait has given up) land before the block may exit.
+  // Copies that nothing waits for any more (a wait may give up at any time, also after the last copy was started) land before the block may
+  // exit. Where all went well they have, or their readers are waiting too.
   template <int ST, typename Landed, typename Ready>
   __device__ __forceinline__ void drain(uint32_t first, Landed landed_bar, Ready ready_bar) const {
     auto land = [](uint32_t b, uint32_t phase) {
