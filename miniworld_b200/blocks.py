@@ -86,16 +86,12 @@ def gated_feed_forward(x: torch.Tensor, w_a: torch.Tensor, w_b: torch.Tensor, w_
     return _lib.native().gated_feed_forward(x, w_a, w_b, w_s, code)
 
 
-def relative_buckets(reach: int, exact: Optional[int] = None, device=None) -> torch.Tensor:
-    """Buckets of the distances ``-reach .. reach`` (of a key from its query, of the pair's second token from its first), int32
-    ``[2 reach + 1]``; greater distances count as the outermost. ``exact`` None: a bucket for each distance, ``distance + reach``.
-    Else two halves of ``2 exact`` buckets, for distances up to 0 and above: one bucket for each distance shorter than ``exact``, the
-    other ``exact`` of a half on a logarithmic scale that ends at ``reach``.
-    """
+def _bucket_list(reach: int, exact: Optional[int] = None) -> list[int]:
+    """The numbers of :func:`relative_buckets`."""
     if not 0 <= reach <= 256:
         raise ValueError(f"reach must be from 0 to 256, got {reach}")
     if exact is None:
-        return torch.arange(2 * reach + 1, dtype=torch.int32, device=device)
+        return list(range(2 * reach + 1))
     if not 1 <= exact < reach or 4 * exact > 512:
         raise ValueError(f"exact must be at least 1, less than reach = {reach} and at most 128, got {exact}")
 
@@ -105,7 +101,17 @@ def relative_buckets(reach: int, exact: Optional[int] = None, device=None) -> to
             far = min(2 * exact - 1, exact + int(math.log(far / exact) / math.log(reach / exact) * exact))
         return far + (2 * exact if distance > 0 else 0)
 
-    return torch.tensor([bucket(d) for d in range(-reach, reach + 1)], dtype=torch.int32, device=device)
+    return [bucket(d) for d in range(-reach, reach + 1)]
+
+
+def relative_buckets(reach: int, exact: Optional[int] = None, device=None) -> torch.Tensor:
+    """Buckets of the distances ``-reach .. reach`` (of a key from its query, of the pair's second token from its first), int32
+    ``[2 reach + 1]``; greater distances count as the outermost. ``exact`` None: a bucket for each distance, ``distance + reach``.
+    Else two halves of ``2 exact`` buckets, for distances up to 0 and above: one bucket for each distance shorter than ``exact``, the
+    other ``exact`` of a half on a logarithmic scale that ends at ``reach``.
+    """
+    numbers = _bucket_list(reach, exact)
+    return torch.arange(len(numbers), dtype=torch.int32, device=device) if exact is None else torch.tensor(numbers, dtype=torch.int32, device=device)
 
 
 def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: Optional[torch.Tensor] = None,

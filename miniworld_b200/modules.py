@@ -611,28 +611,45 @@ class SandwichTransition(nn.Module):
         return self.join(x, self.feed_forward(self.ln_in(x)), gate, mask)
 
 
-def _table_rows(bucket_of: torch.Tensor, more: int) -> int:
-    rows = int(bucket_of.max()) + 1 + more
-    if rows > 512:
-        raise ValueError(f"tables of up to 512 buckets are implemented, this reach needs {rows}")
-    return rows
+class _Buckets(nn.Module):
+    """A module with a map of relative positions to buckets, ``bucket_of`` (None without a reach), a buffer that is not part of the state: its
+    values follow from the arguments, whatever becomes of the module's memory (``to_empty``, construction on the meta device)."""
+
+    def __init__(self, reach: Optional[int], exact: Optional[int], more: int):
+        super().__init__()
+        self.reach, self.exact = reach, exact
+        self.rows = 0 if reach is None else max(blocks._bucket_list(reach, exact)) + 1 + more
+        if self.rows > 512:
+            raise ValueError(f"tables of up to 512 buckets are implemented, this reach needs {self.rows}")
+        self.register_buffer("bucket_of", None if reach is None else blocks.relative_buckets(reach, exact), persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        pinned, buckets = _pinned(fn), self.bucket_of
+
+        def kept(t):
+            out = pinned(t)
+            if t is not buckets or out is t or out.is_meta:
+                return out
+            return blocks.relative_buckets(self.reach, self.exact, out.device) if t.is_meta else t.to(out.device)
+
+        return super()._apply(kept, recurse)
 
 
-class TokenAttention(nn.Module):
+class TokenAttention(_Buckets):
     """Attention among the tokens of a sequence, ``forward(q, k, v, mask=None, offsets=None)``
     (:func:`miniworld_b200.blocks.token_attention`), with a learned bias of the relative position: ``table`` [buckets, heads], kept in
     fp32, for distances up to ``reach`` (``exact`` as in :func:`miniworld_b200.blocks.relative_buckets`; ``reach`` None: no bias)."""
 
     def __init__(self, heads: int, reach: Optional[int] = 32, exact: Optional[int] = None, causal: bool = False, scale: Optional[float] = None,
                  check_status: bool = False):
-        super().__init__()
+        super().__init__(reach, exact, 0)
         self.heads, self.causal, self.scale, self.check_status = heads, bool(causal), scale, bool(check_status)
-        bucket_of = None if reach is None else blocks.relative_buckets(reach, exact)
-        self.register_buffer("bucket_of", bucket_of, persistent=False)
-        self.table = None if bucket_of is None else nn.Parameter(torch.zeros(_table_rows(bucket_of, 0), heads))
+        self.table = None if reach is None else nn.Parameter(torch.empty(self.rows, heads))
+        self.reset_parameters()
 
-    def _apply(self, fn, recurse=True):
-        return super()._apply(_pinned(fn), recurse)
+    def reset_parameters(self) -> None:
+        if self.table is not None:
+            nn.init.zeros_(self.table)
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor] = None,
                 offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -643,20 +660,18 @@ class TokenAttention(nn.Module):
         return o
 
 
-class RelativePosition(nn.Module):
+class RelativePosition(_Buckets):
     """The relative position of its two tokens added to every cell of a pair tensor, ``forward(z, index, chain=None)``
     (:func:`miniworld_b200.blocks.relative_position`): ``table`` [buckets + 1, d_pair], kept in fp32, its last row for the pairs of
     different chains."""
 
     def __init__(self, d_pair: int, reach: int = 32, exact: Optional[int] = None):
-        super().__init__()
-        bucket_of = blocks.relative_buckets(reach, exact)
-        self.register_buffer("bucket_of", bucket_of, persistent=False)
-        self.table = nn.Parameter(torch.empty(_table_rows(bucket_of, 1), d_pair))
-        nn.init.normal_(self.table, std=0.02)
+        super().__init__(reach, exact, 1)
+        self.table = nn.Parameter(torch.empty(self.rows, d_pair))
+        self.reset_parameters()
 
-    def _apply(self, fn, recurse=True):
-        return super()._apply(_pinned(fn), recurse)
+    def reset_parameters(self) -> None:
+        nn.init.normal_(self.table, std=0.02)
 
     def forward(self, z: torch.Tensor, index: torch.Tensor, chain: Optional[torch.Tensor] = None) -> torch.Tensor:
         return blocks.relative_position(z, self.table, index, bucket_of=self.bucket_of, chain=chain)
