@@ -680,7 +680,8 @@ class RelativePosition(_Buckets):
 class BlockDropout(nn.Module):
     """The residual add of a block's output with dropout, ``forward(x, u, key=None) -> x + keep * u / (1 - p)`` in training and ``x + u``
     otherwise, in ``x``'s type (``x`` None: without it; :func:`miniworld_b200.blocks.block_dropout`). ``shared`` names a dimension whose
-    rows use one mask; ``key`` defaults to a new one from PyTorch's generator."""
+    rows use one mask; ``key`` defaults to a new one from PyTorch's generator. Where nothing is dropped the sum is PyTorch's, on any device;
+    shapes, types and ``shared`` are those of training all the same."""
 
     def __init__(self, p: float, shared: Optional[int] = None):
         super().__init__()
@@ -691,8 +692,18 @@ class BlockDropout(nn.Module):
     def forward(self, x: Optional[torch.Tensor], u: torch.Tensor, key: Optional[torch.Tensor] = None) -> torch.Tensor:
         p = self.p if self.training else 0.0
         if p == 0.0:
+            self._check(u if x is None else x, u)
             return u if x is None else x + u.to(x.dtype)
         return blocks.block_dropout(x, u, blocks.dropout_key(u.device) if key is None else key, p=p, shared=self.shared)
+
+    def _check(self, x: torch.Tensor, u: torch.Tensor) -> None:
+        """What training refuses"""
+        if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise RuntimeError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
+        if not u.is_floating_point() or u.shape != x.shape or u.device != x.device:
+            raise RuntimeError(f"u must be a float tensor of x's shape {list(x.shape)} and device, got {u.dtype} {list(u.shape)} on {u.device}")
+        if self.shared is not None and not -u.dim() <= self.shared < u.dim():
+            raise RuntimeError(f"shared must name one of the {u.dim()} dimensions, got {self.shared}")
 
     def extra_repr(self) -> str:
         return f"p={self.p}, shared={self.shared}"
