@@ -59,7 +59,9 @@ int b200_token_attention_forward(const b200_attention_call* call, const b200_att
 
 /*
  * Gradients from dO (strides as for q), the forward's inputs, o, rest and lse: dq [rows, heads, d], dk and dv [rows, kv_heads, d], contiguous,
- * and, where it is not null, dtable (table_dtype). Workspace: 1024-byte aligned, b200_token_attention_workspace_bytes of the same call.
+ * and, where it is not null, dtable (table_dtype). Workspace: 1024-byte aligned, b200_token_attention_workspace_bytes of the same call; where
+ * dtable is null, that of the call without a table is enough (the gradient of a table takes 4 (2 reach + 1) bytes a head and tile of
+ * 128 rows of a sequence, and one tile a sequence more).
  */
 int b200_token_attention_workspace_bytes(const b200_attention_call* call, size_t* out_bytes);
 int b200_token_attention_backward(const b200_attention_call* call, const b200_attention_tensor* q, const b200_attention_tensor* k,

@@ -288,7 +288,7 @@ int b200_token_attention_backward(const b200_attention_call* call, const b200_at
   if (o == nullptr || rest == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || workspace == nullptr) return B200_TRIMUL_E_NULL;
   if (!all_aligned16({o, rest, dq, dk, dv}) || !aligned(workspace, 1024)) return B200_TRIMUL_E_ALIGN;
   const AttentionRegions regions = attention_regions(call);
-  if (workspace_bytes < regions.total) return B200_TRIMUL_E_WORKSPACE;
+  if (workspace_bytes < (dtable != nullptr ? regions.total : regions.partial)) return B200_TRIMUL_E_WORKSPACE;
   DeviceInfo info;
   if ((rc = tokens_device(&info)) != 0) return rc;
   AttentionParams p = attention_params(call, q, k, v);
