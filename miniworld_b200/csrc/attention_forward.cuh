@@ -12,7 +12,7 @@
 // One B200, 2 x 4096 tokens, 16 heads: 218 us at d = 64 (the special function unit busy 56 % of the time over the launch, 82 % between
 // a block's first and last tile), 284 us at d = 128 (970 TFLOP/s, 0.62 of measured). With a thread a row 250 and 341: one warp a
 // scheduler and block waits out its own latencies. Tiles of 64 keys with four blocks an SM (d <= 64) or two buffers of scores (d > 64) 238
-// and 368: a product of 64 columns takes as long as one of 128, for the rows of q that it reads. Short sequences pay 4500 of a block's 14000
+// and 368: a product of 64 columns takes as long as one of 128, for the rows of q that it reads from shared memory. Short sequences pay 4500 of a block's 14000
 // clocks before its first scores and 2000 after its last (512 x 384 tokens, 8 heads of 32: 354 us). Blocks that stay and have the next
 // work's tiles on their way, or a copying warp that does not wait for the others' set-up, cost registers that the softmax needs: 415
 // and 430 us there.

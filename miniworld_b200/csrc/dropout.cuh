@@ -94,9 +94,10 @@ __device__ __forceinline__ void drop_eight(const DropoutParams& p, uint4 r, Eigh
   u.store(y);
 }
 
-// No rows share: a thread takes a few groups of eight elements and draws their numbers while the elements are on their way. HBM bound
-// (about 10 instructions an element, 5 of them the generator: issue 53 % busy): 16384 x 1024 fp16 23 us with the residual, 20 without,
-// where 100 and 67 MB have to move; with one group a thread whose numbers came first 55 and 36.
+// No rows share: a thread takes a few groups of eight elements and draws their numbers while the elements are on their way. 16384 x 1024
+// fp16 23 us with the residual, 20 without, where 100 and 67 MB have to move (0.67 and 0.51 of the measured rate): between memory and
+// instructions, about 26 an element (issue 53 and 61 % busy; halves, choices and conversions go one element at a time). With one group a
+// thread whose numbers came first 55 and 36.
 template <typename T, bool RESIDUAL>
 __global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const DropoutParams p) {
   grid_dependency_wait();
@@ -168,7 +169,9 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_shared_kernel(const D
 
 constexpr int kDropoutSingles = 8;  // rows in flight
 
-// The same where rows of an odd width share a mask or a tensor does not start on 16 bytes: one mask element a thread.
+// The same where rows of an odd width share a mask or a tensor does not start on 16 bytes: one mask element a thread, one element a load.
+// 384 x 384 x 101 bf16, a mask for 384 rows: 33 us for 89 MB; 16384 x 1024 bf16 without shared rows, where numbers for eight elements are drawn
+// for each: 409 us.
 template <typename T, bool RESIDUAL>
 __global__ void __launch_bounds__(kDropoutThreads) dropout_single_kernel(const DropoutParams p) {
   grid_dependency_wait();

@@ -180,8 +180,11 @@ constexpr int kPositionWarps = 13;  // tables of sums of 66 buckets that fit int
 // Sums over the buckets, in fixed orders: a warp owns 64 channels and a run of positions, of which it has 32 (fp32: 16) on their way while
 // it adds up as many before them. Neighbouring positions of one bucket are added up in registers (most pairs are far apart and share the
 // outer two), others in the warp's table in shared memory. The block adds its warps' tables up, and position_sums_kernel the blocks'.
-// 768 x 768 x 128 bf16: 53 us for 151 MB; each warp waits for one unit's 4 KB at a time, 53 KB an SM, and tables leave room for no more
-// warps. (Buckets found after the values they are for had been asked for: 75; values converted as they came: 398.)
+// 768 x 768 x 128 bf16: 53 us for 151 MB, with 13 warps and 53 KB on their way an SM. What bounds it is the work between the loads, of
+// 4 bytes a lane each, and in mixed runs a shuffle, a branch and a read and write of shared memory for a position (issue 49 % busy): two
+// units on their way in 12 warps were slower (step 111 -> 120 us). More rows leave fewer warps: 130, 258 and 512 take 152, 349 and 804 us for
+// a step's forward and backward where 66 take 104. (Buckets found after the values they are for had been asked for: 75; values
+// converted as they came: 398.)
 template <typename T, int V>
 __global__ void __launch_bounds__(kPositionWarps * 32, 1) position_backward_kernel(const PositionParams p) {
   constexpr int R = sizeof(T) == 2 ? 32 : 16;  // positions that a warp looks at together
