@@ -21,6 +21,7 @@ extern "C" {
 #endif
 
 #define B200_ATTENTION_MAX_WIDTH 128
+#define B200_ATTENTION_MAX_BIAS 65504.f
 #define B200_POSITION_MAX_REACH 256
 #define B200_POSITION_MAX_BUCKETS 512
 
@@ -42,7 +43,8 @@ typedef struct {
   float scale;         /* of the scores */
   const int* offsets;
   const uint8_t* mask; /* [rows], 0: the row neither attends nor is attended to; null: all do */
-  /* bias table[bucket_of[clip(j - i, -reach, reach) + reach], head] of key j and query i of a sequence; table null: none */
+  /* bias table[bucket_of[clip(j - i, -reach, reach) + reach], head] of key j and query i of a sequence; table null: none. -inf: the pair
+   * does not count; finite ones beyond +-B200_ATTENTION_MAX_BIAS count as that. */
   const void* table;    /* [buckets, heads] */
   int table_dtype;      /* dtype or B200_BLOCKS_F32 */
   const int* bucket_of; /* int32 [2 reach + 1] */

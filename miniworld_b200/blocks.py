@@ -126,7 +126,8 @@ def token_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offset
     tokens: those with zero are not attended to and come out zero, whatever they hold, with zero gradients. ``causal``: a token attends
     to itself and the ones before it (a value that is not finite at a later token may reach earlier ones all the same). ``scale`` defaults to ``d ** -0.5``. ``table`` [buckets, heads] (q's type or fp32) with ``bucket_of``
     (:func:`relative_buckets`): ``table[bucket_of[clip(j - i, -reach, reach) + reach], head]`` is added to the score of query ``i`` and
-    key ``j`` of a sequence.
+    key ``j`` of a sequence; where it is -inf the pair does not count (rows without any pair come out zero), and finite biases beyond
+    fp16's range (65504 either way) count as its ends.
 
     bf16 and fp16 run as they are, other float types through bf16; scores, their gradients and sums are fp32, the probabilities and
     the gradients of the scores are rounded to 16 bits as operands of the products."""

@@ -7,6 +7,7 @@
 // leaves out has none. Rows without a key, and rows of no sequence, are zero and have zero gradients.
 #pragma once
 
+#include "../../include/b200_tokens.h"
 #include "ptx.cuh"
 
 namespace trimul {
@@ -38,15 +39,20 @@ __device__ __forceinline__ long long attention_offset(const AttentionParams& p, 
   if (p.offsets == nullptr) return static_cast<long long>(s) * p.length;
   return s == 0 ? 0 : min(max(static_cast<long long>(__ldcg(p.offsets + s)), 0ll), p.rows);
 }
+constexpr float kLog2e = 1.4426950408889634f;
+
+// In units of log2. Finite biases beyond fp16's range count as its ends: next to greater ones fp32 would lose the scores, the powers of two
+// that fp16 probabilities are held times and the logarithm of a row's sum, and at the type's lowest value the unit's factor makes them infinite.
+// (Where a row has greater ones too, the probability of a pair that far below is zero either way.)
 __device__ __forceinline__ float attention_bias(const AttentionParams& p, int distance, int head, bool f16) {
   if (p.table == nullptr) return 0.f;
   const int b = min(max(__ldcg(p.bucket_of + min(max(distance, -p.reach), p.reach) + p.reach), 0), p.buckets - 1);
   const long long at = static_cast<long long>(b) * p.heads + head;
-  if (p.wide_table) return __ldcg(static_cast<const float*>(p.table) + at);
-  return f16 ? __half2float(__ldcg(static_cast<const __half*>(p.table) + at)) : __bfloat162float(__ldcg(static_cast<const __nv_bfloat16*>(p.table) + at));
+  const float v = p.wide_table ? __ldcg(static_cast<const float*>(p.table) + at)
+                  : f16        ? __half2float(__ldcg(static_cast<const __half*>(p.table) + at))
+                               : __bfloat162float(__ldcg(static_cast<const __nv_bfloat16*>(p.table) + at));
+  return (fabsf(v) > B200_ATTENTION_MAX_BIAS && fabsf(v) < INFINITY ? copysignf(B200_ATTENTION_MAX_BIAS, v) : v) * kLog2e;
 }
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 __device__ __forceinline__ const T* attention_at(const AttentionTensor& t, long long row, int head) {

@@ -631,8 +631,8 @@ __global__ void __launch_bounds__(kAtBackThreads, 1) attention_dkv_kernel(const 
       if (n > 0) fetch();
       for (int u = 0; u < n; ++u) {
         if (p.table != nullptr && tile == first_tile) {
-          low = attention_bias(p, -p.reach, head, F16) * kLog2e;
-          high = attention_bias(p, p.reach, head, F16) * kLog2e;
+          low = attention_bias(p, -p.reach, head, F16);
+          high = attention_bias(p, p.reach, head, F16);
         }
         const int d0 = key0 - tile * kAtTile, buffer = u % C::kRowBuffers;
         const float add = (F16 ? 15.f : 0.f) + (p.table == nullptr || attention_near(p, d0) ? 0.f : d0 > 0 ? high : low);

@@ -125,7 +125,7 @@ __device__ __forceinline__ AttentionPlace attention_place(const AttentionParams&
 __host__ __device__ constexpr int attention_bias_entries(int reach) { return 2 * (reach + 255) + 1; }
 __device__ __forceinline__ void attention_bias_fill(const AttentionParams& p, float* bias, int head, bool f16, int thread, int threads) {
   const int entries = attention_bias_entries(p.reach);
-  for (int i = thread; i < entries; i += threads) bias[i] = attention_bias(p, i - (p.reach + 255), head, f16) * kLog2e;
+  for (int i = thread; i < entries; i += threads) bias[i] = attention_bias(p, i - (p.reach + 255), head, f16);
 }
 
 // Whether tiles of 128 keys and 128 queries, whose first ones are `d0` apart, have pairs within the reach
